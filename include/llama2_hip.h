@@ -299,6 +299,99 @@ int llama2_sample_top_p(const llama2_half* logits, const int* indices, int size,
 int llama2_sample(llama2_half* logits, int* indices, int size, float temperature, float top_p,
                   float coin, int* result, int pos);
 
+/* ------------------------------------------- steps of several requests at once
+ * The reference and the decoder below serve one sequence with a contiguous
+ * cache; there is no counterpart for what follows.  Several requests keep
+ * their cache rows in blocks of a shared pool and may start behind one prefix whose
+ * rows they share (a system prompt, or the prompt whose continuations are
+ * sampled in parallel).  A step is llama2_batch_tables once, then for every
+ * layer llama2_batch_qk_norm_rope and llama2_batch_attention.  All three are
+ * asynchronous on the library's stream and may be captured; everything that
+ * changes from step to step is read on the device, so that one captured
+ * step serves as long as n_requests, n_tokens and max_length stay large enough. */
+
+/* Keys and values of one layer: row r of block b, head h, starts at
+ * b * block_stride + (r * n_kv_heads + h) * head_size halfs.  A contiguous
+ * cache is one whose blocks follow each other in order. */
+typedef struct llama2_paged_cache {
+    llama2_half* key;   /* 16-byte aligned */
+    llama2_half* value; /* 16-byte aligned */
+    long long block_stride; /* halfs between blocks, a multiple of 8; 0: block_size * n_kv_heads * head_size */
+    int n_blocks;
+    int block_size; /* rows per block: a power of two, 8 .. 1024 */
+    int n_kv_heads;
+    int head_size; /* 64 or 128 */
+} llama2_paged_cache;
+
+/* The requests of a step.  Arrays are device memory.  n_tokens is the number of
+ * rows that the step's buffers have: rows behind the requests' own tokens (a
+ * batch padded to a captured size) have position and slot -1, and every
+ * operator leaves the rows of such tokens in its output as they were. */
+typedef struct llama2_batch {
+    int* block_tables;       /* [n_requests][table_stride]: the blocks of a request's own rows, in order */
+    int* lengths;            /* [n_requests]: own rows of a request, the new tokens included */
+    int* query_starts;       /* [n_requests + 1]: first token of every request, then the number of tokens */
+    int* positions;          /* [n_tokens]: prefix_length + own row of the token, or -1 */
+    int* slots;              /* [n_tokens]: block * block_size + row in the block, or -1 */
+    const int* prefix_table; /* [ceil(prefix_length / block_size)]: the blocks of the shared rows; null if none */
+    int n_requests;
+    int n_tokens;
+    int table_stride;
+    int prefix_length; /* rows that all requests share, in front of their own */
+    int max_length;    /* no request has more own rows than this (read by llama2_batch_attention) */
+} llama2_batch;
+
+/* Block tables and slots of a step, from the lengths.  Request b has cached[b] own
+ * rows and brings counts[b] tokens (none is allowed).  It gets the blocks that its new rows
+ * need from free_blocks[taken ..), in the order of the requests; batch->block_tables is
+ * extended in place, lengths, query_starts, positions and slots are written, and
+ * new_taken[0] is the number of free blocks taken so far.  lengths may be
+ * `cached` and new_taken may be `taken`; other arrays must not overlap.
+ * A request is refused -- its tokens get position and slot -1, its table and
+ * length stay as they are, it takes no block -- if the free blocks left do not suffice for
+ * it and all in front of it, if its rows would not fit into table_stride blocks, if its tokens
+ * reach beyond n_tokens, or if its count or length is negative.  A request that needs no
+ * block is not refused for want of blocks.
+ * Block ids are copied, not looked at; free_blocks and the tables must not hold an id twice.
+ * prefix_table and max_length are not read. */
+int llama2_batch_tables(const llama2_batch* batch, const int* cached, const int* counts,
+                        const int* free_blocks, int n_free, const int* taken, int* new_taken,
+                        int block_size);
+
+/* For every token with a position: q_output = rotated (normed) queries, and keys
+ * and values to the token's slot of the cache, the keys rotated (normed).  Head x
+ * of `head_size` elements: y = x / sqrt(mean(x^2) + eps) * gamma if gamma (q_gamma
+ * for queries, k_gamma for keys; head_size halfs, null: no norm), then pairs (i, i +
+ * head_size/2) rotated by position * theta^(-2 i / head_size) as llama2_rope does, one rounding at the
+ * end.  The angle is exact to 2^-32 of a turn at every position (llama2_rope's,
+ * like the reference's, loses bits as positions grow: the two differ by roundings).
+ * Rows of q, k, v and q_output are q_stride, kv_stride and q_output_stride halfs
+ * apart (multiples of 8, pointers 16-byte aligned), so that they may be parts of one buffer.
+ * q_output may be q with the same stride; it must not overlap otherwise.  No two tokens may
+ * have the same slot.  A token whose slot is not one of the cache's is not stored.
+ * Reads positions and slots of the batch.  1 <= theta. */
+int llama2_batch_qk_norm_rope(llama2_half* q_output, const llama2_half* q, const llama2_half* k,
+                              const llama2_half* v, const llama2_half* q_gamma,
+                              const llama2_half* k_gamma, const llama2_batch* batch,
+                              const llama2_paged_cache* cache, int n_heads, int q_output_stride,
+                              int q_stride, int kv_stride, float eps, float theta);
+
+/* Causal attention of all tokens: the token at position p of request b attends the
+ * prefix_length rows of the prefix table and the own rows 0 .. p - prefix_length
+ * of the request (row r: block_tables[b][r / block_size]); query head h
+ * uses key/value head h / (n_heads / n_kv_heads).  Scores and softmax stay in fp32,
+ * probabilities are rounded to fp16 relative to the largest one so far
+ * (llama2_multi_head_attention rounds scores to fp16 instead, as the reference
+ * does).  Rows of a block id outside the cache are not attended; a token left
+ * without rows gives zeros.  Rows behind a token's own, and the rest of the last block,
+ * have no influence whatever they hold.  The shared rows are read once for all requests.
+ * `output` must not overlap the other buffers.  Reads query_starts, positions,
+ * block_tables and prefix_table of the batch.
+ * Scratch: as llama2_multi_head_attention (call once before capturing). */
+int llama2_batch_attention(llama2_half* output, const llama2_half* query, const llama2_batch* batch,
+                           const llama2_paged_cache* cache, int n_heads, int output_stride,
+                           int query_stride, float scale);
+
 /* ------------------------------------------------------- converter repack
  * The tensor transformations of ModelConverter.RepackQWeightByName
  * (src/ModelConverter.cs:196-275) on device buffers: what turns an AWQ

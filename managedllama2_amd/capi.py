@@ -67,6 +67,19 @@ class RunState(C.Structure):
                 ("key_cache", vp), ("value_cache", vp), ("tokens", vp), ("indices", vp)]
 
 
+class PagedCache(C.Structure):
+    """llama2_paged_cache: keys and values of one layer in blocks."""
+    _fields_ = [("key", vp), ("value", vp), ("block_stride", C.c_longlong), ("n_blocks", i), ("block_size", i),
+                ("n_kv_heads", i), ("head_size", i)]
+
+
+class Batch(C.Structure):
+    """llama2_batch: the requests of a step."""
+    _fields_ = [("block_tables", vp), ("lengths", vp), ("query_starts", vp), ("positions", vp), ("slots", vp),
+                ("prefix_table", vp), ("n_requests", i), ("n_tokens", i), ("table_stride", i), ("prefix_length", i),
+                ("max_length", i)]
+
+
 _SIGNATURES = {
     "llama2_init": [i],
     "llama2_shutdown": [],
@@ -106,6 +119,9 @@ _SIGNATURES = {
     "llama2_cumulative_sum": [vp, i],
     "llama2_sample_top_p": [vp, vp, i, f, vp, i],
     "llama2_sample": [vp, vp, i, f, f, f, vp, i],
+    "llama2_batch_tables": [C.POINTER(Batch), vp, vp, vp, i, vp, vp, i],
+    "llama2_batch_qk_norm_rope": [vp, vp, vp, vp, vp, vp, C.POINTER(Batch), C.POINTER(PagedCache), i, i, i, i, f, f],
+    "llama2_batch_attention": [vp, vp, C.POINTER(Batch), C.POINTER(PagedCache), i, i, i, f],
     "llama2_repack_qdata": [vp, vp, i, i],
     "llama2_repack_scales": [vp, vp, i, i],
     "llama2_compact_scales_v1": [vp, vp, i, i],

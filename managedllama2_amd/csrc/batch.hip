@@ -1,0 +1,314 @@
+// The operators in front of the attention of a step of several requests: block tables and slots from the requests'
+// lengths, and the rotation of queries and keys (normed, where the model does that) with the store into the paged cache.
+#include "common.hpp"
+
+#include <cmath>
+
+namespace l2 {
+
+// ---------------------------------------------------------------- block tables
+struct TablesArgs {
+    int* block_tables;
+    int* lengths;
+    int* query_starts;
+    int* positions;
+    int* slots;
+    const int* cached;
+    const int* counts;
+    const int* free_blocks;
+    const int* taken;
+    int* new_taken;
+    int n_requests, n_tokens, table_stride, prefix_length, n_free, shift;
+};
+
+constexpr int kTablesBlock = 1024;
+
+// Inclusive prefix sum over the workgroup, each sum cut off at `most` (which keeps it associative for terms >= 0).
+__device__ __forceinline__ int block_scan(int v, int most, int* lds /* 16 */)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(v, d, 64);
+        v = lane >= d ? min(v + o, most) : v;
+    }
+    if (lane == 63)
+        lds[wave] = v;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < wave; ++w)
+        before = min(before + lds[w], most);
+    __syncthreads();
+    return min(v + before, most);
+}
+
+// One workgroup: a block of 1024 requests at a time, lane by lane, two prefix sums (tokens, blocks); then their tokens,
+// each of which finds its request in the sums.  A new block holds at least one new token, and the one in its
+// first row writes the table entry.
+__global__ __launch_bounds__(kTablesBlock) void batch_tables_kernel(TablesArgs a)
+{
+    __shared__ int sums[16];
+    __shared__ int begin[kTablesBlock], rows[kTablesBlock], from[kTablesBlock]; // from: first free block, -1: refused
+    __shared__ int most_taken;
+    const int size = 1 << a.shift, tid = threadIdx.x;
+    const int limit = a.table_stride > (0x7FFFFFFF >> a.shift) ? 0x7FFFFFFF : a.table_stride << a.shift;
+    const int taken = a.taken[0];
+    const int left = taken >= 0 && taken <= a.n_free ? a.n_free - taken : 0;
+    if (tid == 0)
+        most_taken = 0;
+    int tokens_before = 0, need_before = 0; // both cut off one above what can be granted
+    for (int first = 0; first < a.n_requests; first += kTablesBlock) {
+        const int b = first + tid, in_block = min(a.n_requests - first, kTablesBlock);
+        const int c = b < a.n_requests ? a.cached[b] : 0, n = b < a.n_requests ? a.counts[b] : 0;
+        const int tokens = min(max(n, 0), a.n_tokens + 1);
+        const int end = min(block_scan(tokens, a.n_tokens + 1, sums) + tokens_before, a.n_tokens + 1);
+        const bool fits = b < a.n_requests && c >= 0 && n >= 0 && c <= limit && n <= limit - c && end <= a.n_tokens;
+        const int have = fits ? (c >> a.shift) + ((c & (size - 1)) != 0) : 0;
+        const int total = fits ? ((c + n) >> a.shift) + (((c + n) & (size - 1)) != 0) : 0;
+        const int need = total - have;
+        const int upto = min(block_scan(min(need, left + 1), left + 1, sums) + need_before, left + 1);
+        const bool admitted = fits && (need == 0 || upto <= left);
+        begin[tid] = end;
+        rows[tid] = c;
+        from[tid] = admitted ? taken + upto - need : -1;
+        if (admitted && need > 0)
+            atomicMax(&most_taken, upto);
+        if (b < a.n_requests) {
+            a.query_starts[b + 1] = min(end, a.n_tokens);
+            a.lengths[b] = admitted ? c + n : c;
+        }
+        if (b == 0)
+            a.query_starts[0] = 0;
+        __syncthreads();
+        const int last = min(begin[kTablesBlock - 1], a.n_tokens);
+        for (int t = min(tokens_before, a.n_tokens) + tid; t < last; t += kTablesBlock) {
+            int lo = 0, hi = in_block - 1; // the first request whose tokens end behind t
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (begin[mid] > t)
+                    hi = mid;
+                else
+                    lo = mid + 1;
+            }
+            const int start_of = lo ? begin[lo - 1] : tokens_before;
+            const int cb = rows[lo], f = from[lo];
+            int position = -1, slot = -1;
+            if (f >= 0) {
+                const int row = cb + (t - start_of), page = row >> a.shift;
+                const int had = (cb >> a.shift) + ((cb & (size - 1)) != 0);
+                int* entry = a.block_tables + static_cast<size_t>(first + lo) * a.table_stride + page;
+                const int block = page >= had ? a.free_blocks[f + page - had] : *entry;
+                if ((row & (size - 1)) == 0)
+                    *entry = block;
+                position = a.prefix_length + row;
+                slot = (block << a.shift) + (row & (size - 1));
+            }
+            a.positions[t] = position;
+            a.slots[t] = slot;
+        }
+        tokens_before = begin[kTablesBlock - 1];
+        if (tid == kTablesBlock - 1)
+            sums[0] = upto;
+        __syncthreads();
+        need_before = sums[0];
+        __syncthreads();
+    }
+    for (int t = min(tokens_before, a.n_tokens) + tid; t < a.n_tokens; t += kTablesBlock) {
+        a.positions[t] = -1;
+        a.slots[t] = -1;
+    }
+    if (tid == 0)
+        a.new_taken[0] = taken + most_taken;
+}
+
+// ---------------------------------------------------------------- norm, rotation, store
+struct RopeArgs {
+    uint16_t* q_output;
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    const uint16_t* q_gamma;
+    const uint16_t* k_gamma;
+    const int* positions;
+    const int* slots;
+    uint16_t* key;
+    uint16_t* value;
+    long long block_stride;
+    long long n_slots;
+    int n_tokens, n_heads, n_kv_heads, head_size, q_output_stride, q_stride, kv_stride, shift;
+    float eps;
+    unsigned long long turns[64]; // theta^(-2 i / head_size) / 2 pi in units of 2^-64
+};
+
+// One wavefront per token and head, one lane per pair.
+__global__ __launch_bounds__(64) void batch_rope_kernel(RopeArgs a)
+{
+    const int t = blockIdx.x, u = blockIdx.y, i = threadIdx.x, half = a.head_size / 2;
+    const int position = a.positions[t];
+    if (position < 0 || i >= half)
+        return;
+    const int slot = a.slots[t];
+    const bool is_q = u < a.n_heads, is_k = !is_q && u < a.n_heads + a.n_kv_heads;
+    const int h = is_q ? u : is_k ? u - a.n_heads : u - a.n_heads - a.n_kv_heads;
+    const uint16_t* x = (is_q ? a.q + static_cast<size_t>(t) * a.q_stride
+                              : (is_k ? a.k : a.v) + static_cast<size_t>(t) * a.kv_stride) + h * a.head_size;
+    uint16_t* out;
+    if (is_q)
+        out = a.q_output + static_cast<size_t>(t) * a.q_output_stride + h * a.head_size;
+    else {
+        if (slot < 0 || slot >= a.n_slots)
+            return;
+        out = (is_k ? a.key : a.value) + (slot >> a.shift) * a.block_stride +
+              (static_cast<size_t>(slot & ((1 << a.shift) - 1)) * a.n_kv_heads + h) * a.head_size;
+    }
+    if (!is_q && !is_k) {
+        out[i] = x[i];
+        out[i + half] = x[i + half];
+        return;
+    }
+    float x0 = half_bits_to_float(x[i]), x1 = half_bits_to_float(x[i + half]);
+    const uint16_t* gamma = is_q ? a.q_gamma : a.k_gamma;
+    if (gamma) {
+        float ss = x0 * x0 + x1 * x1;
+        for (int d = half / 2; d; d >>= 1)
+            ss += __shfl_xor(ss, d, 64);
+        const float r = 1.0f / sqrtf(ss / static_cast<float>(a.head_size) + a.eps);
+        x0 = r * half_bits_to_float(gamma[i]) * x0;
+        x1 = r * half_bits_to_float(gamma[i + half]) * x1;
+    }
+    const int turn = static_cast<int>((static_cast<unsigned long long>(position) * a.turns[i]) >> 32);
+    float s, c;
+    sincospif(static_cast<float>(turn) * 0x1p-31f, &s, &c);
+    rope_rotate(out[i], out[i + half], x0, x1, c, s);
+}
+
+// ---------------------------------------------------------------- host side
+int check_paged_cache(const char* fn, const llama2_paged_cache* c, int n_heads)
+{
+    L2_CHECK(c && c->key && c->value, "%s: null pointer", fn);
+    L2_CHECK(aligned(c->key, 16) && aligned(c->value, 16), "%s: cache pointers must be 16-byte aligned", fn);
+    if (c->head_size != 64 && c->head_size != 128)
+        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: head_size=%d must be 64 or 128", fn, c->head_size);
+    L2_CHECK(c->block_size >= 8 && c->block_size <= 1024 && (c->block_size & (c->block_size - 1)) == 0,
+             "%s: block_size=%d must be a power of two from 8 to 1024", fn, c->block_size);
+    L2_CHECK(c->n_kv_heads > 0 && n_heads > 0 && n_heads % c->n_kv_heads == 0,
+             "%s: n_heads=%d must be a positive multiple of n_kv_heads=%d", fn, n_heads, c->n_kv_heads);
+    if (n_heads > kMaxAttnHeads)
+        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: n_heads=%d exceeds %d", fn, n_heads, kMaxAttnHeads);
+    const long long block = static_cast<long long>(c->block_size) * c->n_kv_heads * c->head_size;
+    L2_CHECK(c->block_stride == 0 || (c->block_stride >= block && c->block_stride % 8 == 0),
+             "%s: block_stride=%lld must be 0 or a multiple of 8 of at least %lld halfs", fn, c->block_stride, block);
+    L2_CHECK(c->n_blocks > 0 && c->n_blocks <= 0x7FFFFFFF / c->block_size,
+             "%s: n_blocks=%d must be positive, and n_blocks * block_size below 2^31", fn, c->n_blocks);
+    return LLAMA2_OK;
+}
+
+int check_batch(const char* fn, const llama2_batch* b)
+{
+    L2_CHECK(b, "%s: null batch", fn);
+    L2_CHECK(b->n_requests > 0 && b->n_requests <= kMaxBatchTokens && b->n_tokens > 0 && b->n_tokens <= kMaxBatchTokens,
+             "%s: n_requests=%d and n_tokens=%d must be 1 .. %d", fn, b->n_requests, b->n_tokens, kMaxBatchTokens);
+    L2_CHECK(b->prefix_length >= 0, "%s: prefix_length=%d is negative", fn, b->prefix_length);
+    return LLAMA2_OK;
+}
+
+static int log2_of(int power)
+{
+    int s = 0;
+    while ((1 << s) < power)
+        ++s;
+    return s;
+}
+
+} // namespace l2
+
+using namespace l2;
+
+extern "C" {
+
+int llama2_batch_tables(const llama2_batch* batch, const int* cached, const int* counts, const int* free_blocks, int n_free,
+                        const int* taken, int* new_taken, int block_size)
+{
+    L2_REQUIRE_INIT();
+    if (int rc = check_batch("llama2_batch_tables", batch))
+        return rc;
+    const llama2_batch& b = *batch;
+    L2_CHECK(b.block_tables && b.lengths && b.query_starts && b.positions && b.slots && cached && counts && taken && new_taken,
+             "llama2_batch_tables: null pointer");
+    L2_CHECK(n_free >= 0 && (free_blocks || n_free == 0), "llama2_batch_tables: n_free=%d free_blocks=%p", n_free,
+             static_cast<const void*>(free_blocks));
+    L2_CHECK(block_size >= 8 && block_size <= 1024 && (block_size & (block_size - 1)) == 0,
+             "llama2_batch_tables: block_size=%d must be a power of two from 8 to 1024", block_size);
+    L2_CHECK(b.table_stride > 0, "llama2_batch_tables: table_stride=%d must be positive", b.table_stride);
+    L2_CHECK(b.table_stride <= (0x7FFFFFFF - b.prefix_length) / block_size,
+             "llama2_batch_tables: positions of prefix_length=%d and table_stride=%d blocks of %d rows exceed 2^31", b.prefix_length,
+             b.table_stride, block_size);
+    TablesArgs a = {b.block_tables, b.lengths, b.query_starts, b.positions, b.slots, cached, counts, free_blocks, taken,
+                    new_taken, b.n_requests, b.n_tokens, b.table_stride, b.prefix_length, n_free, log2_of(block_size)};
+    hipLaunchKernelGGL(batch_tables_kernel, dim3(1), dim3(kTablesBlock), 0, ctx().stream, a);
+    L2_LAUNCH_CHECK("llama2_batch_tables");
+    return LLAMA2_OK;
+}
+
+int llama2_batch_qk_norm_rope(llama2_half* q_output, const llama2_half* q, const llama2_half* k, const llama2_half* v,
+                              const llama2_half* q_gamma, const llama2_half* k_gamma, const llama2_batch* batch,
+                              const llama2_paged_cache* cache, int n_heads, int q_output_stride, int q_stride, int kv_stride,
+                              float eps, float theta)
+{
+    const char* fn = "llama2_batch_qk_norm_rope";
+    L2_REQUIRE_INIT();
+    if (int rc = check_batch(fn, batch))
+        return rc;
+    if (int rc = check_paged_cache(fn, cache, n_heads))
+        return rc;
+    L2_CHECK(q_output && q && k && v && batch->positions && batch->slots, "%s: null pointer", fn);
+    L2_CHECK(aligned(q_output, 16) && aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(q_gamma, 16) &&
+                 aligned(k_gamma, 16), "%s: pointers must be 16-byte aligned", fn);
+    const int d = cache->head_size, q_row = n_heads * d, kv_row = cache->n_kv_heads * d;
+    L2_CHECK(q_stride >= q_row && q_output_stride >= q_row && kv_stride >= kv_row && q_stride % 8 == 0 && q_output_stride % 8 == 0 &&
+                 kv_stride % 8 == 0, "%s: strides %d, %d, %d must be multiples of 8 and hold a row of %d, %d, %d", fn, q_output_stride,
+             q_stride, kv_stride, q_row, q_row, kv_row);
+    L2_CHECK(theta >= 1.0f && theta <= 3.0e38f, "%s: theta=%g must be at least 1", fn, static_cast<double>(theta));
+    L2_CHECK(eps >= 0.0f, "%s: eps=%g is negative", fn, static_cast<double>(eps));
+    auto bytes = [&](int stride, int row) { return (static_cast<size_t>(batch->n_tokens - 1) * stride + row) * 2; };
+    const size_t out_bytes = bytes(q_output_stride, q_row);
+    L2_CHECK((q_output == q && q_output_stride == q_stride) || !overlap(q_output, out_bytes, q, bytes(q_stride, q_row)),
+             "%s: q_output overlaps q without being it", fn);
+    L2_CHECK((q_output == q && q_output_stride == q_stride) ||
+                 (!overlap(q_output, out_bytes, k, bytes(kv_stride, kv_row)) && !overlap(q_output, out_bytes, v, bytes(kv_stride, kv_row))),
+             "%s: q_output overlaps k or v", fn);
+    const long long block = static_cast<long long>(cache->block_size) * kv_row;
+    RopeArgs a = {};
+    a.q_output = q_output;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_gamma = q_gamma;
+    a.k_gamma = k_gamma;
+    a.positions = batch->positions;
+    a.slots = batch->slots;
+    a.key = cache->key;
+    a.value = cache->value;
+    a.block_stride = cache->block_stride ? cache->block_stride : block;
+    a.n_slots = static_cast<long long>(cache->n_blocks) * cache->block_size;
+    a.n_tokens = batch->n_tokens;
+    a.n_heads = n_heads;
+    a.n_kv_heads = cache->n_kv_heads;
+    a.head_size = d;
+    a.q_output_stride = q_output_stride;
+    a.q_stride = q_stride;
+    a.kv_stride = kv_stride;
+    a.shift = log2_of(cache->block_size);
+    a.eps = eps;
+    // A pair's turn per position, in 64 bits of fixed point: times a position, the bits above are whole turns and
+    // drop out by themselves.  2^31 positions times the error of 2^-58 relative leave 2^-29 of a turn.
+    const long double step = powl(static_cast<long double>(theta), -2.0L / d);
+    long double turn = 1.0L / (2.0L * 3.14159265358979323846264338327950288L) * 0x1p64L;
+    for (int i = 0; i < d / 2; ++i, turn *= step)
+        a.turns[i] = static_cast<unsigned long long>(turn);
+    hipLaunchKernelGGL(batch_rope_kernel, dim3(a.n_tokens, n_heads + 2 * a.n_kv_heads), dim3(64), 0, ctx().stream, a);
+    L2_LAUNCH_CHECK(fn);
+    return LLAMA2_OK;
+}
+
+} // extern "C"
