@@ -1,7 +1,29 @@
 // Attention of a step of several requests over a paged cache, behind a prefix that they share.
+//
+// out = sum_r softmax_r(scale q.k_r) v_r over the shared rows and the request's own, by the running maximum and sum.  The
+// queries of one key/value head (all of a group, all tokens that see the same rows) are the columns of
+//   S^T = K Q^T,   O^T = V^T P^T
+// on the matrix cores: with rows of the cache along the first operand, a lane ends up with the scores of ONE query, and
+// its probabilities are already the second operand of the second product.  A workgroup takes one item:
+//   shared   up to 128 columns out of all tokens (of any request) x a piece of the prefix: every shared row is read
+//            once per 128 columns instead of once per request;
+//   own      up to 128 columns of one request x a piece of its own rows (behind the prefix where a request has so many
+//            columns of its own that sharing would not save any reading).
+// Pieces leave fp32 sums, maximum and denominator; batch_attn_merge_kernel joins them in order.
 #include "common.hpp"
 
 namespace l2 {
+
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef float f16v_t __attribute__((ext_vector_type(16)));
+
+constexpr int kTileRows = 128; // columns (token, head of the group) per workgroup
+constexpr int kFewRows = 16;   // at most this many: the wavefronts split the cache rows instead of the columns
+constexpr int kPass = 64;      // cache rows per pass of many_rows; pieces are multiples of it
+// Probabilities enter the matrix cores as fp16 times 2^14: the largest is 16384, and one of 2^-38 is still a number.  Their
+// sum carries the same factor, so that it drops out of the quotient.
+constexpr float kProbShift = 14.0f;
 
 struct BatchAttnArgs {
     uint16_t* out;
@@ -12,64 +34,735 @@ struct BatchAttnArgs {
     const int* block_tables;
     const int* query_starts;
     const int* positions;
+    float* parts; // [slot][token][head][D] sums, then (maximum, denominator) of each; null: one piece, straight to `out`
+    float2* stats;
     long long block_stride;
     int n_requests, n_tokens, table_stride, prefix_length, max_rows;
     int n_blocks, shift, n_kv_heads, group, out_stride, q_stride;
-    float scale;
+    float scale; // times log2(e)
+    // items: [shared_splits x n_kv_heads][shared_tiles], then [own_splits][own_tiles][n_kv_heads]
+    int shared_tiles, shared_splits, shared_piece;
+    int own_tiles, own_piece, own_prefix; // own_prefix: prefix rows in front of a request's own, a multiple of kPass, or 0
 };
 
-// One wavefront per token and head: 64 / (D / 8) rows at a time, D / 8 lanes each.
-template <int D>
-__global__ __launch_bounds__(64) void batch_attn_simple_kernel(BatchAttnArgs a)
+// What a workgroup computes; the same in all its lanes.
+struct Item {
+    int token, row0, rows, kv_head; // column c: query head kv_head * group + (row0 + c) % group of token `token` + (row0 + c) / group
+    int tokens;                 // that the columns belong to
+    int p0, p1;                 // shared rows
+    int r0, r1;                 // own rows
+    const int* table;           // of the own rows
+    int slot;
+};
+
+__device__ __forceinline__ f4_t mfma16(h8_t x, h8_t y, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
+__device__ __forceinline__ f16v_t mfma32(h8_t x, h8_t y, f16v_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0); }
+
+__device__ __forceinline__ float max_xor16(float v)
 {
-    constexpr int L = D / 8;
-    const int t = blockIdx.x, h = blockIdx.y, kvh = h / a.group;
-    const int lane = threadIdx.x, c = lane % L, sub = lane / L;
-    const int position = a.positions[t];
-    if (position < 0)
-        return;
-    int b = 0;
-    while (b + 1 < a.n_requests && a.query_starts[b + 1] <= t)
-        ++b;
-    const int own = min(max(position - a.prefix_length + 1, 0), a.max_rows);
-    float q[8], o[8] = {};
-    for (int i = 0; i < 8; ++i)
-        q[i] = half_bits_to_float(a.q[static_cast<size_t>(t) * a.q_stride + h * D + c * 8 + i]);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_xor32(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ int row16_min(int v)
+{
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1)
+        v = min(v, __shfl_xor(v, x, 64));
+    return v;
+}
+
+// Own rows that the token attends.
+__device__ __forceinline__ int own_rows_of(const BatchAttnArgs& a, int token)
+{
+    const int p = a.positions[token];
+    return p < a.prefix_length ? 0 : min(p - a.prefix_length + 1, a.max_rows);
+}
+
+// exp2(v - most) times 2^14; without any score above -infinity everything is 0, not NaN.
+__device__ __forceinline__ float prob_base(float most) { return most == -INFINITY ? 0.0f : most - kProbShift; }
+__device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float weight_of(float m, float most) { return m == -INFINITY ? 0.0f : exp2_of(m - most); }
+
+// Any element infinite or NaN?  (bits 15 and 31 of the sum: all exponent bits set)
+__device__ __forceinline__ uint32_t not_finite(uint32_t v) { return ((v & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
+
+// Elements of a head (D of them) in row `row` of a table; 64-bit offsets: a cache may be larger than 4 GB.
+template <int D>
+__device__ __forceinline__ const uint16_t* row_address(const BatchAttnArgs& a, const uint16_t* cache, int block, int row, int kv_head)
+{
+    return cache + block * a.block_stride + ((row & ((1 << a.shift) - 1)) * a.n_kv_heads + kv_head) * static_cast<long long>(D);
+}
+
+__device__ __forceinline__ bool in_cache(const BatchAttnArgs& a, int block)
+{
+    return static_cast<unsigned>(block) < static_cast<unsigned>(a.n_blocks);
+}
+
+// ---------------------------------------------------------------- few columns
+// Up to 16 columns: bound by reading the cache.  Each of the 4 wavefronts takes every fourth tile of 32 rows, straight from
+// memory into the operands' registers.  Lane (g, c), g = lane / 16: keys of row 16 t + c, elements 32 j + 8 g .. + 7
+// (64 consecutive bytes of a row per load and row); values of the rows 16 t + 4 g .. + 3, whose scores the same lane holds, 1/16 of a
+// row each (4 whole rows per load), turned by byte permutations into columns: operand i holds elements c * D/16 + i.
+template <int D>
+__device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
+{
+    constexpr int KS = D / 32, VE = D / 16, VW = VE / 2; // k steps; elements and words of a value row per lane
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, c = lane & 15;
+    const int r = min(c, it.rows - 1);
+    const int token = it.token + (it.row0 + r) / a.group, head = it.kv_head * a.group + (it.row0 + r) % a.group;
+    const int limit = own_rows_of(a, token);
+    const int least = it.tokens > 1 ? row16_min(limit) : limit; // of all columns
+    h8_t qf[KS];
+#pragma unroll
+    for (int j = 0; j < KS; ++j)
+        qf[j] = *reinterpret_cast<const h8_t*>(a.q + static_cast<size_t>(token) * a.q_stride + head * D + j * 32 + g * 8);
+
+    f4_t o[VE];
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+        o[i] = f4_t{};
     float m = -INFINITY, sum = 0.0f;
-    for (int r = sub; r < a.prefix_length + own; r += 64 / L) {
-        const bool shared = r < a.prefix_length;
-        const int row = shared ? r : r - a.prefix_length;
-        const int block = shared ? a.prefix_table[row >> a.shift]
-                                 : a.block_tables[static_cast<size_t>(b) * a.table_stride + (row >> a.shift)];
-        if (static_cast<unsigned>(block) >= static_cast<unsigned>(a.n_blocks))
+
+    for (int seg = 0; seg < 2; ++seg) {
+        const int* table = seg ? it.table : a.prefix_table;
+        const int begin = seg ? it.r0 : it.p0, end = seg ? it.r1 : it.p1;
+        const int seen = seg ? limit : end, all_see = seg ? least : end;
+        if (begin + wave * 32 >= end)
             continue;
-        const size_t at = block * a.block_stride +
-                          (static_cast<size_t>(row & ((1 << a.shift) - 1)) * a.n_kv_heads + kvh) * D + c * 8;
-        float s = 0.0f;
-        for (int i = 0; i < 8; ++i)
-            s += q[i] * half_bits_to_float(a.key[at + i]);
-        for (int x = L / 2; x; x >>= 1)
-            s += __shfl_xor(s, x, 64);
-        s *= a.scale;
-        const float nm = fmaxf(m, s), base = nm == -INFINITY ? 0.0f : nm;
-        const float alpha = expf(m - base), p = expf(s - base);
-        m = nm;
-        sum = sum * alpha + p;
-        for (int i = 0; i < 8; ++i)
-            o[i] = o[i] * alpha + p * half_bits_to_float(a.value[at + i]);
+        const int last4 = (end - 1) & ~3;
+        auto block_of = [&](int row) { return table[min(row, last4) >> a.shift]; };
+        int kid[2], vid[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            kid[t] = block_of(begin + wave * 32 + 16 * t + (c & ~3));
+            vid[t] = block_of(begin + wave * 32 + 16 * t + 4 * g);
+        }
+        for (int tb = begin + wave * 32; tb < end; tb += 128) {
+            h8_t kf[2][KS];
+            uint32_t vr[8][VW];
+            bool ok[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int row = min(tb + 16 * t + (c & ~3), last4) + (c & 3);
+                const uint16_t* p = row_address<D>(a, a.key, in_cache(a, kid[t]) ? kid[t] : 0, row, it.kv_head) + g * 8;
+#pragma unroll
+                for (int j = 0; j < KS; ++j)
+                    kf[t][j] = *reinterpret_cast<const h8_t*>(p + j * 32);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                ok[t] = in_cache(a, vid[t]);
+                const int row = min(tb + 16 * t + 4 * g, last4);
+                const uint16_t* p = row_address<D>(a, a.value, ok[t] ? vid[t] : 0, row, it.kv_head) + c * VE;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t* w = reinterpret_cast<const uint32_t*>(p + static_cast<size_t>(i) * a.n_kv_heads * D);
+                    if constexpr (VW == 4) {
+                        const u32x4 x = *reinterpret_cast<const u32x4*>(w);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            vr[4 * t + i][k] = x[k];
+                    } else {
+                        const u32x2 x = *reinterpret_cast<const u32x2*>(w);
+                        vr[4 * t + i][0] = x[0];
+                        vr[4 * t + i][1] = x[1];
+                    }
+                }
+            }
+            if (tb + 128 < end) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    kid[t] = block_of(tb + 128 + 16 * t + (c & ~3));
+                    vid[t] = block_of(tb + 128 + 16 * t + 4 * g);
+                }
+            }
+            f4_t s[2] = {};
+#pragma unroll
+            for (int j = 0; j < KS; ++j)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    s[t] = mfma16(kf[t][j], qf[j], s[t]);
+            const bool whole = tb + 32 <= all_see && !__any(!ok[0] || !ok[1]);
+            float most = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float v = s[t][i] * a.scale;
+                    s[t][i] = whole || (tb + 16 * t + 4 * g + i < seen && ok[t]) ? v : -INFINITY;
+                    most = fmaxf(most, s[t][i]);
+                }
+            most = fmaxf(m, max_xor32(max_xor16(most)));
+            if (__any(most > m)) {
+                const float alpha = weight_of(m, most);
+                sum *= alpha;
+#pragma unroll
+                for (int i = 0; i < VE; ++i)
+                    o[i] *= alpha;
+                m = most;
+            }
+            const float base = prob_base(m);
+            h8_t p;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = exp2_of(s[t][i] - base);
+                    sum += e;
+                    p[4 * t + i] = static_cast<_Float16>(e);
+                }
+            bool careful = false;
+            if (!whole) { // what lies behind the last row, or in a block that is none, must not reach a sum through a 0
+                uint32_t bad = 0;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool keep = tb + 16 * t + 4 * g + i < end && ok[t];
+#pragma unroll
+                        for (int k = 0; k < VW; ++k) {
+                            vr[4 * t + i][k] = keep ? vr[4 * t + i][k] : 0u;
+                            bad |= not_finite(vr[4 * t + i][k]);
+                        }
+                    }
+                careful = __any(bad != 0);
+            }
+            if (!careful) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    u32x4 w;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        w[k] = __builtin_amdgcn_perm(vr[2 * k + 1][i >> 1], vr[2 * k][i >> 1], (i & 1) ? 0x07060302u : 0x05040100u);
+                    o[i] = mfma16(__builtin_bit_cast(h8_t, w), p, o[i]);
+                }
+            } else { // row by row, each kept only by the columns that attend it
+                for (int u = 0; u < 32; ++u) {
+                    const bool keep = tb + u < seen;
+                    const int e = (u >> 4) * 4 + (u & 3); // its element in the lanes of group (u / 4) % 4
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) {
+                        u32x4 w;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            w[k] = __builtin_amdgcn_perm(vr[2 * k + 1][i >> 1], vr[2 * k][i >> 1], (i & 1) ? 0x07060302u : 0x05040100u);
+                            w[k] &= g == ((u >> 2) & 3) && k == (e >> 1) ? ((e & 1) ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
+                        }
+                        const f4_t x = mfma16(__builtin_bit_cast(h8_t, w), p, f4_t{});
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            o[i][k] = keep ? o[i][k] + x[k] : o[i][k];
+                    }
+                }
+            }
+        }
     }
-    for (int x = L; x < 64; x <<= 1) {
-        const float om = __shfl_xor(m, x, 64), nm = fmaxf(m, om), base = nm == -INFINITY ? 0.0f : nm;
-        const float wa = expf(m - base), wb = expf(om - base);
-        sum = sum * wa + __shfl_xor(sum, x, 64) * wb;
-        for (int i = 0; i < 8; ++i)
-            o[i] = o[i] * wa + __shfl_xor(o[i], x, 64) * wb;
-        m = nm;
+    sum = add_xor32(add_xor16(sum));
+
+    // The four wavefronts' sums through LDS, then each adds up a quarter of the elements.
+    f4_t* all = reinterpret_cast<f4_t*>(lds);
+    float2* stat = reinterpret_cast<float2*>(lds + 4 * VE * 64 * 16);
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+        all[(wave * VE + i) * 64 + lane] = o[i];
+    if (g == 0)
+        stat[wave * 16 + c] = float2{m, sum};
+    __syncthreads();
+    float most = -INFINITY, total = 0.0f, weight[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+        most = fmaxf(most, stat[w * 16 + c].x);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float2 st = stat[w * 16 + c];
+        weight[w] = weight_of(st.x, most);
+        total = fmaf(weight[w], st.y, total);
     }
-    if (sub == 0)
+    if (c >= it.rows || a.positions[token] < 0)
+        return;
+    const size_t row = static_cast<size_t>(token) * a.n_kv_heads * a.group + head;
+    const size_t part = (static_cast<size_t>(it.slot) * a.n_tokens * a.n_kv_heads * a.group + row);
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    constexpr int PER = VE / 4; // elements of this wavefront: wave * PER ..
+    float e[PER][4];
+#pragma unroll
+    for (int x = 0; x < PER; ++x) {
+        f4_t v = {};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const f4_t y = all[(w * VE + wave * PER + x) * 64 + lane];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                v[k] = fmaf(weight[w], y[k], v[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            e[x][k] = v[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int x = 0; x < PER; ++x) {
+            const int d = (g * 4 + k) * VE + wave * PER + x;
+            if (a.parts)
+                a.parts[part * D + d] = e[x][k];
+            else
+                a.out[static_cast<size_t>(token) * a.out_stride + head * D + d] = float_to_half_bits(total == 0.0f ? 0.0f : e[x][k] * inv);
+        }
+    if (a.parts && wave == 0 && g == 0)
+        a.stats[part] = float2{most, total};
+}
+
+// ---------------------------------------------------------------- many columns
+// 17 to 128 columns, 32 per wavefront: passes of 64 rows through LDS, read by all four.  Keys as rows; values transposed, a
+// row of 64 cache rows per output element, in the order in which a lane holds their probabilities (4 rows of one
+// half of the lanes, 4 of the other); 16-byte pieces are exchanged by element so that reads have no bank conflicts.
+constexpr int kValueStride = kPass * 2;
+
+template <int D>
+struct ManyLds {
+    static constexpr int kKeyStride = D * 2 + 16;
+    static constexpr int kKeys = kPass * kKeyStride, kValues = D * kValueStride, kTotal = kKeys + kValues + 64;
+};
+
+__device__ __forceinline__ int value_offset(int d, int piece) // piece: 16 bytes
+{
+    return d * kValueStride + ((piece ^ (((d >> 1) ^ (d >> 3)) & 7)) << 4);
+}
+
+template <int D>
+__device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
+{
+    using L = ManyLds<D>;
+    constexpr int QS = D / 16, DT = D / 32, CH = D / 8; // k steps, tiles of output elements, 16-byte pieces of a row
+    char* ks = lds;
+    char* vs = lds + L::kKeys;
+    int* flags = reinterpret_cast<int*>(lds + L::kKeys + L::kValues);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int hl = lane >> 5, l31 = lane & 31;
+    const int r = wave * 32 + l31, rq = min(r, it.rows - 1);
+    const bool idle = wave * 32 >= it.rows;
+    const int token = it.token + (it.row0 + rq) / a.group, head = it.kv_head * a.group + (it.row0 + rq) % a.group;
+    const int limit = own_rows_of(a, token);
+    int most_rows = limit, least = -limit;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        most_rows = max(most_rows, __shfl_xor(most_rows, x, 64));
+        least = max(least, __shfl_xor(least, x, 64));
+    }
+    least = -least;
+
+    // Threads: 16 groups of 4 rows x D / 8 pieces; of heads of 64 one half of the threads takes keys, the other values.
+    const int unit = threadIdx.x % (16 * CH), piece = unit % CH, group4 = unit / CH;
+    const bool takes_k = D == 128 || threadIdx.x < 16 * CH, takes_v = D == 128 || !takes_k;
+
+    h8_t qf[QS];
+#pragma unroll
+    for (int j = 0; j < QS; ++j)
+        qf[j] = *reinterpret_cast<const h8_t*>(a.q + static_cast<size_t>(token) * a.q_stride + head * D + j * 16 + hl * 8);
+    f16v_t o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+        o[d] = f16v_t{};
+    float m = -INFINITY, sum = 0.0f;
+
+    for (int seg = 0; seg < 2; ++seg) {
+        const int* table = seg ? it.table : a.prefix_table;
+        const int begin = seg ? it.r0 : it.p0, end = seg ? it.r1 : it.p1;
+        if (begin >= end)
+            continue;
+        const int seen = seg ? limit : end, all_see = seg ? least : end, any_sees = seg ? most_rows : end;
+        const int last4 = (end - 1) & ~3;
+        auto block_of = [&](int tb) { return table[min(tb + 4 * group4, last4) >> a.shift]; };
+        u32x4 kr[4], vr[4];
+        bool bad_block = false;
+        auto request = [&](int tb, int block) {
+            const bool ok = in_cache(a, block);
+            const int row = min(tb + 4 * group4, last4);
+            const uint16_t* k = row_address<D>(a, a.key, ok ? block : 0, row, it.kv_head) + piece * 8;
+            const uint16_t* v = row_address<D>(a, a.value, ok ? block : 0, row, it.kv_head) + piece * 8;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (takes_k)
+                    kr[i] = *reinterpret_cast<const u32x4*>(k + static_cast<size_t>(i) * a.n_kv_heads * D);
+                if (takes_v)
+                    vr[i] = *reinterpret_cast<const u32x4*>(v + static_cast<size_t>(i) * a.n_kv_heads * D);
+            }
+            bad_block = !ok;
+        };
+        int next = block_of(begin);
+        request(begin, next);
+        next = block_of(begin + kPass);
+        for (int tb = begin; tb < end; tb += kPass) {
+            const bool none = __any(bad_block);
+            uint32_t bad = 0;
+            if (tb + kPass > end || none) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool keep = tb + 4 * group4 + i < end && !bad_block;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        vr[i][k] = keep ? vr[i][k] : 0u;
+                }
+            }
+            if (takes_v) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        bad |= not_finite(vr[i][k]);
+            }
+            const bool any_bad = __any(bad != 0);
+            __syncthreads(); // the previous pass has been read
+            if (takes_k) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<u32x4*>(ks + (4 * group4 + i) * L::kKeyStride + piece * 16) = kr[i];
+            }
+            if (takes_v) {
+                const int to = (group4 >> 2) * 2 + (group4 & 1), at = ((group4 >> 1) & 1) * 8;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const u32x2 even = {__builtin_amdgcn_perm(vr[1][k], vr[0][k], 0x05040100u),
+                                        __builtin_amdgcn_perm(vr[3][k], vr[2][k], 0x05040100u)};
+                    const u32x2 odd = {__builtin_amdgcn_perm(vr[1][k], vr[0][k], 0x07060302u),
+                                       __builtin_amdgcn_perm(vr[3][k], vr[2][k], 0x07060302u)};
+                    *reinterpret_cast<u32x2*>(vs + value_offset(piece * 8 + 2 * k, to) + at) = even;
+                    *reinterpret_cast<u32x2*>(vs + value_offset(piece * 8 + 2 * k + 1, to) + at) = odd;
+                }
+            }
+            // flags: 0 .. 3 not-finite values seen by a wavefront, 4 .. 7 blocks that are none (a bit per group of 4 rows)
+            if (lane == 0)
+                flags[wave] = any_bad;
+            if (none) {
+                const unsigned long long b = __ballot(bad_block && (takes_v));
+                if (lane == 0) {
+                    int bits = 0;
+                    for (int x = 0; x < 64; x += CH)
+                        bits |= static_cast<int>((b >> x) & 1) << ((threadIdx.x + x) % (16 * CH) / CH);
+                    flags[4 + wave] = bits;
+                }
+            } else if (lane == 0) {
+                flags[4 + wave] = 0;
+            }
+            __syncthreads();
+            if (tb + kPass < end) {
+                request(tb + kPass, next);
+                next = block_of(tb + 2 * kPass);
+            }
+            if (idle || tb >= any_sees)
+                continue;
+            const int no_block = flags[4] | flags[5] | flags[6] | flags[7];
+            const bool whole = tb + kPass <= all_see && no_block == 0;
+            const bool careful = tb + kPass > all_see && (flags[0] | flags[1] | flags[2] | flags[3]);
+
+            f16v_t s[2] = {};
+#pragma unroll
+            for (int j = 0; j < QS; ++j)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const h8_t kf = *reinterpret_cast<const h8_t*>(ks + (t * 32 + l31) * L::kKeyStride + j * 32 + hl * 16);
+                    s[t] = mfma32(kf, qf[j], s[t]);
+                }
+            float most = -INFINITY;
+            if (whole) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        s[t][i] *= a.scale;
+                        most = fmaxf(most, s[t][i]);
+                    }
+            } else {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int row = t * 32 + 8 * (i >> 2) + 4 * hl + (i & 3);
+                        const bool keep = tb + row < seen && !((no_block >> (row >> 2)) & 1);
+                        s[t][i] = keep ? s[t][i] * a.scale : -INFINITY;
+                        most = fmaxf(most, s[t][i]);
+                    }
+            }
+            most = fmaxf(m, max_xor32(most));
+            if (__any(most > m)) {
+                const float alpha = weight_of(m, most);
+                sum *= alpha;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    o[d] *= alpha;
+                m = most;
+            }
+            const float base = prob_base(m);
+            h8_t p[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float e = exp2_of(s[u >> 1][8 * (u & 1) + i] - base);
+                    sum += e;
+                    p[u][i] = static_cast<_Float16>(e);
+                }
+            if (!careful) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        o[d] = mfma32(*reinterpret_cast<const h8_t*>(vs + value_offset(d * 32 + l31, u * 2 + hl)), p[u], o[d]);
+            } else { // row by row, each kept only by the columns that attend it
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    for (int x = 0; x < 16; ++x) {
+                        const bool keep = tb + u * 16 + (x & 1) * 8 + (x >> 3) * 4 + ((x >> 1) & 3) < seen;
+                        const int e = (x & 1) * 4 + ((x >> 1) & 3); // its element in the lanes of half x / 8
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) {
+                            u32x4 w = *reinterpret_cast<const u32x4*>(vs + value_offset(d * 32 + l31, u * 2 + hl));
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                w[k] &= hl == (x >> 3) && k == (e >> 1) ? ((e & 1) ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
+                            const f16v_t y = mfma32(__builtin_bit_cast(h8_t, w), p[u], f16v_t{});
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                o[d][i] = keep ? o[d][i] + y[i] : o[d][i];
+                        }
+                    }
+            }
+        }
+    }
+    sum += __shfl_xor(sum, 32, 64);
+    if (r >= it.rows || a.positions[token] < 0)
+        return;
+    if (a.parts) {
+        const size_t row = static_cast<size_t>(token) * a.n_kv_heads * a.group + head;
+        const size_t part = static_cast<size_t>(it.slot) * a.n_tokens * a.n_kv_heads * a.group + row;
+        float* out = a.parts + part * D + 4 * hl;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<float4*>(out + d * 32 + 8 * k) = float4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+        if (hl == 0)
+            a.stats[part] = float2{m, sum};
+        return;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint16_t* out = a.out + static_cast<size_t>(token) * a.out_stride + head * D + 4 * hl;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            u32x2 w;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                w[x] = static_cast<uint32_t>(float_to_half_bits(o[d][4 * k + 2 * x] * inv)) |
+                       static_cast<uint32_t>(float_to_half_bits(o[d][4 * k + 2 * x + 1] * inv)) << 16;
+            *reinterpret_cast<u32x2*>(out + d * 32 + 8 * k) = w;
+        }
+}
+
+// The first of a request's tiles of columns: room for every request to end with a tile that is not full.
+__device__ __forceinline__ int first_tile(const BatchAttnArgs& a, int request)
+{
+    return min(max(a.query_starts[request], 0), a.n_tokens) * a.group / kTileRows + request;
+}
+
+template <int D>
+constexpr int kAttnLds = ManyLds<D>::kTotal > 4 * (D / 16) * 1024 + 512 ? ManyLds<D>::kTotal : 4 * (D / 16) * 1024 + 512;
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void batch_attn_kernel(BatchAttnArgs a)
+{
+    __shared__ __align__(16) char lds[kAttnLds<D>];
+    Item it = {};
+    int index = blockIdx.x;
+    const int shared_items = a.shared_tiles * a.shared_splits * a.n_kv_heads;
+    if (index < shared_items) {
+        const int tile = index % a.shared_tiles, rest = index / a.shared_tiles;
+        it.kv_head = rest % a.n_kv_heads;
+        it.slot = rest / a.n_kv_heads;
+        it.p0 = it.slot * a.shared_piece;
+        it.p1 = min(it.p0 + a.shared_piece, a.prefix_length);
+        it.row0 = tile * kTileRows;
+        it.rows = min(a.n_tokens * a.group - it.row0, kTileRows);
+        it.tokens = 1; // all see the same rows
+    } else {
+        index -= shared_items;
+        it.kv_head = index % a.n_kv_heads;
+        index /= a.n_kv_heads;
+        const int tile = index % a.own_tiles, split = index / a.own_tiles;
+        const int lane = threadIdx.x & 63;
+        int request = 0; // the last one whose first tile is not behind `tile`
+        for (int first = 1; first < a.n_requests; first += 64)
+            request += __popcll(__ballot(first + lane < a.n_requests && first_tile(a, first + lane) <= tile));
+        request = __builtin_amdgcn_readfirstlane(request);
+        const int start = min(max(a.query_starts[request], 0), a.n_tokens), stop = min(a.query_starts[request + 1], a.n_tokens);
+        it.row0 = (tile - first_tile(a, request)) * kTileRows;
+        it.rows = min((stop - start) * a.group - it.row0, kTileRows);
+        if (it.rows <= 0)
+            return;
+        it.token = start;
+        const int t0 = start + it.row0 / a.group, t1 = start + (it.row0 + it.rows - 1) / a.group;
+        it.tokens = t1 - t0 + 1;
+        int most = own_rows_of(a, t1);
+        if (it.tokens > 1) {
+            for (int t = t0 + lane; t <= t1; t += 64)
+                most = max(most, own_rows_of(a, t));
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1)
+                most = max(most, __shfl_xor(most, x, 64));
+            most = __builtin_amdgcn_readfirstlane(most);
+        }
+        const int from = split * a.own_piece, to = from + a.own_piece; // of the shared rows in front and its own
+        if (a.own_prefix) {
+            it.p0 = min(from, a.prefix_length);
+            it.p1 = min(to, a.prefix_length);
+        }
+        it.r0 = max(from - a.own_prefix, 0);
+        it.r1 = min(max(to - a.own_prefix, 0), most);
+        it.slot = a.shared_splits + split;
+        it.table = a.block_tables + static_cast<size_t>(request) * a.table_stride;
+        if (it.p0 >= it.p1 && it.r0 >= it.r1 && a.parts)
+            return;
+    }
+    if (it.rows <= kFewRows)
+        few_rows<D>(a, it, lds);
+    else
+        many_rows<D>(a, it, lds);
+}
+
+// Joins the pieces of a token's head, in order: LANES lanes per row, D / 8 of them side by side (8 elements each), the
+// others with every LANES * 8 / D-th piece.
+template <int D, int LANES>
+__global__ __launch_bounds__(256) void batch_attn_merge_kernel(BatchAttnArgs a)
+{
+    constexpr int SIDE = D / 8, DEEP = LANES / SIDE;
+    __shared__ float lds[LANES > 64 ? DEEP * SIDE * 8 : 1];
+    __shared__ float2 stat[LANES > 64 ? DEEP : 1];
+    const int rows = a.n_tokens * a.n_kv_heads * a.group; // < 2^31: checked on the host
+    const int row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES, x = lane % SIDE, deep = lane / SIDE;
+    const int token = min(row, rows - 1) / (a.n_kv_heads * a.group), head = row % (a.n_kv_heads * a.group);
+    if (row >= rows || a.positions[token] < 0)
+        return; // a whole wavefront at least, the whole workgroup where it has barriers
+    const int own = own_rows_of(a, token);
+    const int slots = a.shared_splits + (a.own_prefix + own + a.own_piece - 1) / a.own_piece;
+    float m = -INFINITY, sum = 0.0f, o[8] = {};
+    for (int s = deep; s < slots; s += DEEP) {
+        const size_t part = static_cast<size_t>(s) * rows + row;
+        const float2 st = a.stats[part];
+        const float4* p = reinterpret_cast<const float4*>(a.parts + part * D + x * 8);
+        const float4 v0 = p[0], v1 = p[1];
+        const float most = fmaxf(m, st.x), wa = weight_of(m, most), wb = weight_of(st.x, most);
+        m = most;
+        sum = fmaf(wb, st.y, sum * wa);
+        const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
         for (int i = 0; i < 8; ++i)
-            a.out[static_cast<size_t>(t) * a.out_stride + h * D + c * 8 + i] =
-                float_to_half_bits(sum == 0.0f ? 0.0f : o[i] / sum);
+            o[i] = fmaf(wb, v[i], o[i] * wa);
+    }
+    if constexpr (LANES == 64) {
+#pragma unroll
+        for (int d = SIDE; d < 64; d <<= 1) {
+            const float om = __shfl_xor(m, d, 64), most = fmaxf(m, om), wa = weight_of(m, most), wb = weight_of(om, most);
+            const bool lower = (lane & d) == 0; // the same order of the two terms on both sides
+            const float os = __shfl_xor(sum, d, 64);
+            sum = lower ? fmaf(wb, os, sum * wa) : fmaf(wa, sum, os * wb);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float ov = __shfl_xor(o[i], d, 64);
+                o[i] = lower ? fmaf(wb, ov, o[i] * wa) : fmaf(wa, o[i], ov * wb);
+            }
+            m = most;
+        }
+    } else {
+        if (x == 0)
+            stat[deep] = float2{m, sum};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            lds[(i * DEEP + deep) * SIDE + x] = o[i];
+        __syncthreads();
+        if (deep > 0)
+            return;
+        for (int d = 0; d < DEEP; ++d)
+            m = fmaxf(m, stat[d].x);
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            o[i] = 0.0f;
+        for (int d = 0; d < DEEP; ++d) {
+            const float w = weight_of(stat[d].x, m);
+            sum = fmaf(w, stat[d].y, sum);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                o[i] = fmaf(w, lds[(i * DEEP + d) * SIDE + x], o[i]);
+        }
+    }
+    if (deep > 0)
+        return;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        w[k] = static_cast<uint32_t>(float_to_half_bits(o[2 * k] * inv)) | static_cast<uint32_t>(float_to_half_bits(o[2 * k + 1] * inv)) << 16;
+    *reinterpret_cast<u32x4*>(a.out + static_cast<size_t>(token) * a.out_stride + head * D + x * 8) = w;
+}
+
+struct BatchAttnPlan {
+    int shared_tiles = 0, shared_splits = 0, shared_piece = kPass;
+    int own_tiles = 0, own_splits = 1, own_piece = kPass, own_prefix = 0;
+};
+
+static int round_up(int v, int to) { return ceil_div(v, to) * to; }
+
+// Pieces of rows: enough items for every compute unit to hold several, pieces not so long that one long request is
+// still at work when the others are done, not so short that joining them costs more than reading them.
+static BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int group, int max_rows)
+{
+    BatchAttnPlan p;
+    const int cus = ctx().num_cus > 0 ? ctx().num_cus : 256;
+    const long long columns = static_cast<long long>(b.n_tokens) * group;
+    p.own_tiles = static_cast<int>(columns / kTileRows) + b.n_requests;
+    const bool shared = b.prefix_length > 0 && columns < 64LL * b.n_requests && b.n_requests > 1;
+    p.own_prefix = shared ? 0 : round_up(b.prefix_length, kPass);
+    const int own_rows = p.own_prefix + max_rows;
+    const long long items = static_cast<long long>(p.own_tiles) * n_kv_heads;
+    auto pieces = [&](long long have, int rows, int longest) {
+        long long n = (8LL * cus + have - 1) / have;
+        const long long most = ceil_div(rows, 256), least = ceil_div(rows, longest);
+        n = n < most ? n : most;
+        n = n > least ? n : least;
+        return static_cast<int>(n < 256 ? n : 256);
+    };
+    p.own_piece = round_up(ceil_div(own_rows, pieces(items, own_rows, 1024)), kPass);
+    p.own_splits = ceil_div(own_rows, p.own_piece);
+    if (shared) {
+        p.shared_tiles = static_cast<int>((columns + kTileRows - 1) / kTileRows);
+        p.shared_piece = round_up(ceil_div(b.prefix_length, pieces(static_cast<long long>(p.shared_tiles) * n_kv_heads * 4,
+                                                                     b.prefix_length, 1024)), kPass);
+        p.shared_splits = ceil_div(b.prefix_length, p.shared_piece);
+    }
+    return p;
+}
+
+template <int D>
+static void batch_attn_launch(const BatchAttnArgs& a, int items, int slots)
+{
+    hipLaunchKernelGGL(batch_attn_kernel<D>, dim3(items), dim3(256), 0, ctx().stream, a);
+    if (!a.parts)
+        return;
+    const int rows = a.n_tokens * a.n_kv_heads * a.group;
+    if (slots <= 16)
+        hipLaunchKernelGGL((batch_attn_merge_kernel<D, 64>), dim3(ceil_div(rows, 4)), dim3(256), 0, ctx().stream, a);
+    else
+        hipLaunchKernelGGL((batch_attn_merge_kernel<D, 256>), dim3(rows), dim3(256), 0, ctx().stream, a);
 }
 
 } // namespace l2
@@ -123,12 +816,31 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
     a.group = n_heads / cache->n_kv_heads;
     a.out_stride = output_stride;
     a.q_stride = query_stride;
-    a.scale = scale;
-    const dim3 grid(b.n_tokens, n_heads);
+    a.scale = scale * 1.44269504088896340736f; // powers of two below
+    const BatchAttnPlan p = batch_attn_plan(b, a.n_kv_heads, a.group, a.max_rows);
+    a.shared_tiles = p.shared_tiles;
+    a.shared_splits = p.shared_splits;
+    a.shared_piece = p.shared_piece;
+    a.own_tiles = p.own_tiles;
+    a.own_piece = p.own_piece;
+    a.own_prefix = p.own_prefix;
+    const int slots = p.shared_splits + p.own_splits;
+    const long long rows = static_cast<long long>(b.n_tokens) * n_heads;
+    const long long items = static_cast<long long>(a.n_kv_heads) *
+                            (static_cast<long long>(p.shared_tiles) * p.shared_splits + static_cast<long long>(p.own_tiles) * p.own_splits);
+    if (rows > 0x7FFFFFFF / 4 || items > 0x7FFFFFFF)
+        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: %d tokens of %d heads in %d pieces are too many", fn, b.n_tokens, n_heads, slots);
+    if (slots > 1) {
+        const size_t part = static_cast<size_t>(slots) * rows;
+        if (int rc = ensure_attn_partials(part * (cache->head_size + 2) * sizeof(float)))
+            return rc;
+        a.parts = ctx().attn_partials;
+        a.stats = reinterpret_cast<float2*>(a.parts + part * cache->head_size);
+    }
     if (cache->head_size == 128)
-        hipLaunchKernelGGL(batch_attn_simple_kernel<128>, grid, dim3(64), 0, ctx().stream, a);
+        batch_attn_launch<128>(a, static_cast<int>(items), slots);
     else
-        hipLaunchKernelGGL(batch_attn_simple_kernel<64>, grid, dim3(64), 0, ctx().stream, a);
+        batch_attn_launch<64>(a, static_cast<int>(items), slots);
     L2_LAUNCH_CHECK(fn);
     return LLAMA2_OK;
 }
