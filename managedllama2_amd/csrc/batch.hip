@@ -3,6 +3,7 @@
 #include "common.hpp"
 
 #include <cmath>
+#include <cstring>
 
 namespace l2 {
 
@@ -135,51 +136,129 @@ struct RopeArgs {
     uint16_t* value;
     long long block_stride;
     long long n_slots;
-    int n_tokens, n_heads, n_kv_heads, head_size, q_output_stride, q_stride, kv_stride, shift;
+    int n_heads, n_kv_heads, per, q_output_stride, q_stride, kv_stride, shift; // per: heads per workgroup
     float eps;
     unsigned long long turns[64]; // theta^(-2 i / head_size) / 2 pi in units of 2^-64
 };
 
-// One wavefront per token and head, one lane per pair.
-__global__ __launch_bounds__(64) void batch_rope_kernel(RopeArgs a)
+// The value of the lane that holds the other half's elements of the same pairs.
+template <int D>
+__device__ __forceinline__ float other_half(float v)
 {
-    const int t = blockIdx.x, u = blockIdx.y, i = threadIdx.x, half = a.head_size / 2;
-    const int position = a.positions[t];
-    if (position < 0 || i >= half)
-        return;
-    const int slot = a.slots[t];
-    const bool is_q = u < a.n_heads, is_k = !is_q && u < a.n_heads + a.n_kv_heads;
-    const int h = is_q ? u : is_k ? u - a.n_heads : u - a.n_heads - a.n_kv_heads;
-    const uint16_t* x = (is_q ? a.q + static_cast<size_t>(t) * a.q_stride
-                              : (is_k ? a.k : a.v) + static_cast<size_t>(t) * a.kv_stride) + h * a.head_size;
-    uint16_t* out;
-    if (is_q)
-        out = a.q_output + static_cast<size_t>(t) * a.q_output_stride + h * a.head_size;
-    else {
-        if (slot < 0 || slot >= a.n_slots)
-            return;
-        out = (is_k ? a.key : a.value) + (slot >> a.shift) * a.block_stride +
-              (static_cast<size_t>(slot & ((1 << a.shift) - 1)) * a.n_kv_heads + h) * a.head_size;
+    if constexpr (D == 128)
+        return dpp_f32<DPP_ROW_ROR8>(v);
+    else
+        return dpp_f32<DPP_QUAD_XOR3>(dpp_f32<DPP_ROW_HALF_MIRROR>(v)); // lane ^ 7, then ^ 3
+}
+
+template <int D>
+__device__ __forceinline__ float head_sum(float v)
+{
+    v += dpp_f32<DPP_QUAD_XOR1>(v);
+    v += dpp_f32<DPP_QUAD_XOR2>(v);
+    v += dpp_f32<DPP_ROW_HALF_MIRROR>(v);
+    if constexpr (D == 128)
+        v += dpp_f32<DPP_ROW_MIRROR>(v);
+    return v;
+}
+
+// A workgroup takes `per` heads of one token (of its queries, keys and values side by side), D / 8 lanes per head with 16
+// bytes each; norms and the exchange of halves are row operations.  Sine and cosine of a token's angles are
+// computed once per workgroup, one pair per thread, while the heads are on their way: kRopeDeep loads per lane at a time.
+constexpr int kRopeDeep = 4;
+
+template <int D>
+__global__ __launch_bounds__(256) void batch_rope_kernel(RopeArgs a)
+{
+    constexpr int L = D / 8, HEADS = 256 / L; // lanes per head, heads side by side
+    __shared__ __align__(16) float cosines[D / 2];
+    __shared__ __align__(16) float sines[D / 2];
+    const int t = blockIdx.x, tid = threadIdx.x, c = tid % L;
+    const int position = a.positions[t], slot = a.slots[t];
+    const int units = a.n_heads + 2 * a.n_kv_heads, first = blockIdx.y * a.per + tid / L, end = min(units, (static_cast<int>(blockIdx.y) + 1) * a.per);
+    const bool stores = slot >= 0 && slot < a.n_slots;
+    const long long to = stores ? (slot >> a.shift) * a.block_stride +
+                                      static_cast<long long>(slot & ((1 << a.shift) - 1)) * a.n_kv_heads * D : 0;
+    u32x4 x[kRopeDeep];
+    auto load = [&](int u0) {
+#pragma unroll
+        for (int i = 0; i < kRopeDeep; ++i) {
+            const int u = u0 + i * HEADS;
+            if (u < end) {
+                const uint16_t* p = u < a.n_heads ? a.q + static_cast<size_t>(t) * a.q_stride + u * D
+                                    : u < a.n_heads + a.n_kv_heads
+                                        ? a.k + static_cast<size_t>(t) * a.kv_stride + (u - a.n_heads) * D
+                                        : a.v + static_cast<size_t>(t) * a.kv_stride + (u - a.n_heads - a.n_kv_heads) * D;
+                x[i] = *reinterpret_cast<const u32x4*>(p + c * 8);
+            }
+        }
+    };
+    load(first);
+    u32x4 gq = {}, gk = {};
+    if (a.q_gamma)
+        gq = *reinterpret_cast<const u32x4*>(a.q_gamma + c * 8);
+    if (a.k_gamma)
+        gk = *reinterpret_cast<const u32x4*>(a.k_gamma + c * 8);
+    if (position < 0)
+        return; // the whole workgroup
+    if (tid < D / 2) {
+        const int turn = static_cast<int>((static_cast<unsigned long long>(position) * a.turns[tid]) >> 32);
+        float s, cs;
+        sincospif(static_cast<float>(turn) * 0x1p-31f, &s, &cs);
+        cosines[tid] = cs;
+        sines[tid] = s;
     }
-    if (!is_q && !is_k) {
-        out[i] = x[i];
-        out[i + half] = x[i + half];
-        return;
+    __syncthreads();
+    float cs[8], sn[8]; // of this lane's pairs; the first half subtracts
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        cs[k] = cosines[c % (L / 2) * 8 + k];
+        sn[k] = c < L / 2 ? -sines[c % (L / 2) * 8 + k] : sines[c % (L / 2) * 8 + k];
     }
-    float x0 = half_bits_to_float(x[i]), x1 = half_bits_to_float(x[i + half]);
-    const uint16_t* gamma = is_q ? a.q_gamma : a.k_gamma;
-    if (gamma) {
-        float ss = x0 * x0 + x1 * x1;
-        for (int d = half / 2; d; d >>= 1)
-            ss += __shfl_xor(ss, d, 64);
-        const float r = 1.0f / sqrtf(ss / static_cast<float>(a.head_size) + a.eps);
-        x0 = r * half_bits_to_float(gamma[i]) * x0;
-        x1 = r * half_bits_to_float(gamma[i + half]) * x1;
+    for (int u0 = first; u0 - tid / L < end; u0 += kRopeDeep * HEADS) {
+        if (u0 != first)
+            load(u0);
+#pragma unroll
+        for (int i = 0; i < kRopeDeep; ++i) {
+            const int u = u0 + i * HEADS;
+            const bool is_q = u < a.n_heads, is_v = u >= a.n_heads + a.n_kv_heads;
+            u32x4 w = x[i];
+            if (!is_v) {
+                float f[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    f[2 * k] = static_cast<float>(as_h2(w[k])[0]);
+                    f[2 * k + 1] = static_cast<float>(as_h2(w[k])[1]);
+                }
+                if (is_q ? a.q_gamma != nullptr : a.k_gamma != nullptr) {
+                    float ss = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        ss = __builtin_fmaf(f[k], f[k], ss);
+                    const float r = 1.0f / sqrtf(head_sum<D>(ss) / static_cast<float>(D) + a.eps);
+                    const u32x4 g = is_q ? gq : gk;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        f[2 * k] *= r * static_cast<float>(as_h2(g[k])[0]);
+                        f[2 * k + 1] *= r * static_cast<float>(as_h2(g[k])[1]);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float y0 = __builtin_fmaf(f[2 * k], cs[2 * k], other_half<D>(f[2 * k]) * sn[2 * k]);
+                    const float y1 = __builtin_fmaf(f[2 * k + 1], cs[2 * k + 1], other_half<D>(f[2 * k + 1]) * sn[2 * k + 1]);
+                    w[k] = static_cast<uint32_t>(float_to_half_bits(y0)) | static_cast<uint32_t>(float_to_half_bits(y1)) << 16;
+                }
+            }
+            if (u < end) {
+                if (is_q)
+                    *reinterpret_cast<u32x4*>(a.q_output + static_cast<size_t>(t) * a.q_output_stride + u * D + c * 8) = w;
+                else if (stores)
+                    *reinterpret_cast<u32x4*>((is_v ? a.value + (u - a.n_heads - a.n_kv_heads) * D : a.key + (u - a.n_heads) * D) +
+                                              to + c * 8) = w;
+            }
+        }
     }
-    const int turn = static_cast<int>((static_cast<unsigned long long>(position) * a.turns[i]) >> 32);
-    float s, c;
-    sincospif(static_cast<float>(turn) * 0x1p-31f, &s, &c);
-    rope_rotate(out[i], out[i + half], x0, x1, c, s);
 }
 
 // ---------------------------------------------------------------- host side
@@ -218,6 +297,25 @@ static int log2_of(int power)
     while ((1 << s) < power)
         ++s;
     return s;
+}
+
+// A pair's turns per position, in 64 bits of fixed point: times a position, the bits above are whole turns and drop out
+// by themselves; 2^31 positions times the error of 2^-58 relative leave 2^-29 of a turn.  A model has one theta, so the
+// last table is kept (1.5 us to make); the caller holds the library's lock.
+static const unsigned long long* turns_of(float theta, int head_size)
+{
+    static unsigned long long turns[64];
+    static float of_theta = 0.0f;
+    static int of_size = 0;
+    if (theta != of_theta || head_size != of_size) {
+        const long double step = powl(static_cast<long double>(theta), -2.0L / head_size);
+        long double turn = 1.0L / (2.0L * 3.14159265358979323846264338327950288L) * 0x1p64L;
+        for (int i = 0; i < head_size / 2; ++i, turn *= step)
+            turns[i] = static_cast<unsigned long long>(turn);
+        of_theta = theta;
+        of_size = head_size;
+    }
+    return turns;
 }
 
 } // namespace l2
@@ -291,22 +389,24 @@ int llama2_batch_qk_norm_rope(llama2_half* q_output, const llama2_half* q, const
     a.value = cache->value;
     a.block_stride = cache->block_stride ? cache->block_stride : block;
     a.n_slots = static_cast<long long>(cache->n_blocks) * cache->block_size;
-    a.n_tokens = batch->n_tokens;
     a.n_heads = n_heads;
     a.n_kv_heads = cache->n_kv_heads;
-    a.head_size = d;
     a.q_output_stride = q_output_stride;
     a.q_stride = q_stride;
     a.kv_stride = kv_stride;
     a.shift = log2_of(cache->block_size);
     a.eps = eps;
-    // A pair's turn per position, in 64 bits of fixed point: times a position, the bits above are whole turns and
-    // drop out by themselves.  2^31 positions times the error of 2^-58 relative leave 2^-29 of a turn.
-    const long double step = powl(static_cast<long double>(theta), -2.0L / d);
-    long double turn = 1.0L / (2.0L * 3.14159265358979323846264338327950288L) * 0x1p64L;
-    for (int i = 0; i < d / 2; ++i, turn *= step)
-        a.turns[i] = static_cast<unsigned long long>(turn);
-    hipLaunchKernelGGL(batch_rope_kernel, dim3(a.n_tokens, n_heads + 2 * a.n_kv_heads), dim3(64), 0, ctx().stream, a);
+    memcpy(a.turns, turns_of(theta, d), sizeof(a.turns));
+    // Few tokens: as few heads per workgroup as are side by side, which is quickest; many: a workgroup computes the
+    // angles of a token once for all its heads.
+    const int units = n_heads + 2 * a.n_kv_heads, side = 256 / (d / 8);
+    const int parts = ceil_div(units, side), want = ceil_div(4 * ctx().num_cus, batch->n_tokens);
+    a.per = ceil_div(parts, parts < want ? parts : want) * side;
+    const dim3 grid(batch->n_tokens, ceil_div(units, a.per));
+    if (d == 128)
+        hipLaunchKernelGGL(batch_rope_kernel<128>, grid, dim3(256), 0, ctx().stream, a);
+    else
+        hipLaunchKernelGGL(batch_rope_kernel<64>, grid, dim3(256), 0, ctx().stream, a);
     L2_LAUNCH_CHECK(fn);
     return LLAMA2_OK;
 }

@@ -18,11 +18,12 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 typedef float f16v_t __attribute__((ext_vector_type(16)));
 
-constexpr int kTileRows = 128; // columns (token, head of the group) per workgroup
+constexpr int kManyRows = 128; // columns (token, head of the group) per workgroup
 constexpr int kFewRows = 16;   // at most this many: the wavefronts split the cache rows instead of the columns
 constexpr int kPass = 64;      // cache rows per pass of many_rows; pieces are multiples of it
 // Probabilities enter the matrix cores as fp16 times 2^14: the largest is 16384, and one of 2^-38 is still a number.  Their
 // sum carries the same factor, so that it drops out of the quotient.
+constexpr int kMaxPieces = 256; // of a request's rows, and of the prefix
 constexpr float kProbShift = 14.0f;
 
 struct BatchAttnArgs {
@@ -42,7 +43,7 @@ struct BatchAttnArgs {
     float scale; // times log2(e)
     // items: [shared_splits x n_kv_heads][shared_tiles], then [own_splits][own_tiles][n_kv_heads]
     int shared_tiles, shared_splits, shared_piece;
-    int own_tiles, own_piece, own_prefix; // own_prefix: prefix rows in front of a request's own, a multiple of kPass, or 0
+    int own_items, own_tiles, own_piece, own_prefix; // own_prefix: prefix rows in front of a request's own, a multiple of kPass, or 0
 };
 
 // What a workgroup computes; the same in all its lanes.
@@ -77,10 +78,9 @@ __device__ __forceinline__ int row16_min(int v)
     return v;
 }
 
-// Own rows that the token attends.
-__device__ __forceinline__ int own_rows_of(const BatchAttnArgs& a, int token)
+// Own rows that a token at position p attends.
+__device__ __forceinline__ int own_rows_of(const BatchAttnArgs& a, int p)
 {
-    const int p = a.positions[token];
     return p < a.prefix_length ? 0 : min(p - a.prefix_length + 1, a.max_rows);
 }
 
@@ -117,7 +117,8 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
     const int g = lane >> 4, c = lane & 15;
     const int r = min(c, it.rows - 1);
     const int token = it.token + (it.row0 + r) / a.group, head = it.kv_head * a.group + (it.row0 + r) % a.group;
-    const int limit = own_rows_of(a, token);
+    const int position = a.positions[token];
+    const int limit = own_rows_of(a, position);
     const int least = it.tokens > 1 ? row16_min(limit) : limit; // of all columns
     h8_t qf[KS];
 #pragma unroll
@@ -285,7 +286,7 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
         weight[w] = weight_of(st.x, most);
         total = fmaf(weight[w], st.y, total);
     }
-    if (c >= it.rows || a.positions[token] < 0)
+    if (c >= it.rows || position < 0)
         return;
     const size_t row = static_cast<size_t>(token) * a.n_kv_heads * a.group + head;
     const size_t part = (static_cast<size_t>(it.slot) * a.n_tokens * a.n_kv_heads * a.group + row);
@@ -350,7 +351,8 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
     const int r = wave * 32 + l31, rq = min(r, it.rows - 1);
     const bool idle = wave * 32 >= it.rows;
     const int token = it.token + (it.row0 + rq) / a.group, head = it.kv_head * a.group + (it.row0 + rq) % a.group;
-    const int limit = own_rows_of(a, token);
+    const int position = a.positions[token];
+    const int limit = own_rows_of(a, position);
     int most_rows = limit, least = -limit;
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) {
@@ -538,7 +540,7 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
         }
     }
     sum += __shfl_xor(sum, 32, 64);
-    if (r >= it.rows || a.positions[token] < 0)
+    if (r >= it.rows || position < 0)
         return;
     if (a.parts) {
         const size_t row = static_cast<size_t>(token) * a.n_kv_heads * a.group + head;
@@ -569,21 +571,42 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
 }
 
 // The first of a request's tiles of columns: room for every request to end with a tile that is not full.
-__device__ __forceinline__ int first_tile(const BatchAttnArgs& a, int request)
+template <int TILE>
+__device__ __forceinline__ int first_tile(const BatchAttnArgs& a, int start, int request)
 {
-    return min(max(a.query_starts[request], 0), a.n_tokens) * a.group / kTileRows + request;
+    return start * a.group / TILE + request;
+}
+
+// One value for the whole wavefront, through the scalar cache: it does not queue behind the cache rows that the vector
+// memory path is busy with.
+__device__ __forceinline__ int uniform_load(const int* p, int i)
+{
+    typedef const int __attribute__((address_space(4))) * Scalar;
+    return ((Scalar)p)[__builtin_amdgcn_readfirstlane(i)];
+}
+
+__device__ __forceinline__ int request_start(const BatchAttnArgs& a, int request)
+{
+    return min(max(uniform_load(a.query_starts, request), 0), a.n_tokens);
 }
 
 template <int D>
-constexpr int kAttnLds = ManyLds<D>::kTotal > 4 * (D / 16) * 1024 + 512 ? ManyLds<D>::kTotal : 4 * (D / 16) * 1024 + 512;
-
+constexpr int kFewLds = 4 * (D / 16) * 1024 + 512;
 template <int D>
-__global__ __launch_bounds__(256, 2) void batch_attn_kernel(BatchAttnArgs a)
+constexpr int kAttnLds = ManyLds<D>::kTotal > kFewLds<D> ? ManyLds<D>::kTotal : kFewLds<D>;
+
+template <int D, bool MANY>
+__global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttnArgs a)
 {
-    __shared__ __align__(16) char lds[kAttnLds<D>];
+    constexpr int kTileRows = MANY ? kManyRows : kFewRows;
+    __shared__ __align__(16) char lds[MANY ? kAttnLds<D> : kFewLds<D>];
     Item it = {};
-    int index = blockIdx.x;
     const int shared_items = a.shared_tiles * a.shared_splits * a.n_kv_heads;
+    // Wide tiles of shared rows first, they take longest; narrow ones last, to fill up what long requests leave idle (64
+    // conversations 133 -> 125 us).
+    int index = blockIdx.x;
+    if (!MANY)
+        index = index < a.own_items ? index + shared_items : index - a.own_items;
     if (index < shared_items) {
         const int tile = index % a.shared_tiles, rest = index / a.shared_tiles;
         it.kv_head = rest % a.n_kv_heads;
@@ -595,26 +618,37 @@ __global__ __launch_bounds__(256, 2) void batch_attn_kernel(BatchAttnArgs a)
         it.tokens = 1; // all see the same rows
     } else {
         index -= shared_items;
-        it.kv_head = index % a.n_kv_heads;
-        index /= a.n_kv_heads;
-        const int tile = index % a.own_tiles, split = index / a.own_tiles;
-        const int lane = threadIdx.x & 63;
-        int request = 0; // the last one whose first tile is not behind `tile`
-        for (int first = 1; first < a.n_requests; first += 64)
-            request += __popcll(__ballot(first + lane < a.n_requests && first_tile(a, first + lane) <= tile));
-        request = __builtin_amdgcn_readfirstlane(request);
-        const int start = min(max(a.query_starts[request], 0), a.n_tokens), stop = min(a.query_starts[request + 1], a.n_tokens);
-        it.row0 = (tile - first_tile(a, request)) * kTileRows;
+        const int of_heads = index / a.n_kv_heads;
+        const int tile = of_heads % a.own_tiles, split = of_heads / a.own_tiles;
+        // The workgroups of an XCD (every eighth) take all heads in turn: the rows of one head alone lie in few of its L2's
+        // channels.
+        it.kv_head = (index + of_heads) % a.n_kv_heads;
+        // The request: the one it would be if all brought one token, else by counting, 64 at a time.
+        int request = min(((tile + 1) * kTileRows - 1) / (kTileRows + a.group), a.n_requests - 1);
+        int start = request_start(a, request), stop = request_start(a, request + 1);
+        if (first_tile<kTileRows>(a, start, request) > tile || first_tile<kTileRows>(a, stop, request + 1) <= tile) {
+            const int lane = threadIdx.x & 63;
+            request = 0; // the last one whose first tile is not behind `tile`
+            for (int first = 1; first < a.n_requests; first += 64) {
+                const int b = min(first + lane, a.n_requests);
+                request += __popcll(__ballot(b < a.n_requests &&
+                                             first_tile<kTileRows>(a, min(max(a.query_starts[b], 0), a.n_tokens), b) <= tile));
+            }
+            request = __builtin_amdgcn_readfirstlane(request);
+            start = request_start(a, request);
+            stop = request_start(a, request + 1);
+        }
+        it.row0 = (tile - first_tile<kTileRows>(a, start, request)) * kTileRows;
         it.rows = min((stop - start) * a.group - it.row0, kTileRows);
-        if (it.rows <= 0)
+        if (it.rows <= 0 || it.row0 < 0)
             return;
         it.token = start;
         const int t0 = start + it.row0 / a.group, t1 = start + (it.row0 + it.rows - 1) / a.group;
         it.tokens = t1 - t0 + 1;
-        int most = own_rows_of(a, t1);
+        int most = own_rows_of(a, uniform_load(a.positions, t1));
         if (it.tokens > 1) {
-            for (int t = t0 + lane; t <= t1; t += 64)
-                most = max(most, own_rows_of(a, t));
+            for (int t = t0 + static_cast<int>(threadIdx.x & 63); t <= t1; t += 64)
+                most = max(most, own_rows_of(a, a.positions[t]));
 #pragma unroll
             for (int x = 1; x < 64; x <<= 1)
                 most = max(most, __shfl_xor(most, x, 64));
@@ -632,10 +666,13 @@ __global__ __launch_bounds__(256, 2) void batch_attn_kernel(BatchAttnArgs a)
         if (it.p0 >= it.p1 && it.r0 >= it.r1 && a.parts)
             return;
     }
-    if (it.rows <= kFewRows)
-        few_rows<D>(a, it, lds);
-    else
-        many_rows<D>(a, it, lds);
+    if constexpr (MANY) {
+        if (it.rows > kFewRows) {
+            many_rows<D>(a, it, lds);
+            return;
+        }
+    }
+    few_rows<D>(a, it, lds);
 }
 
 // Joins the pieces of a token's head, in order: LANES lanes per row, D / 8 of them side by side (8 elements each), the
@@ -652,7 +689,7 @@ __global__ __launch_bounds__(256) void batch_attn_merge_kernel(BatchAttnArgs a)
     const int token = min(row, rows - 1) / (a.n_kv_heads * a.group), head = row % (a.n_kv_heads * a.group);
     if (row >= rows || a.positions[token] < 0)
         return; // a whole wavefront at least, the whole workgroup where it has barriers
-    const int own = own_rows_of(a, token);
+    const int own = own_rows_of(a, a.positions[token]);
     const int slots = a.shared_splits + (a.own_prefix + own + a.own_piece - 1) / a.own_piece;
     float m = -INFINITY, sum = 0.0f, o[8] = {};
     for (int s = deep; s < slots; s += DEEP) {
@@ -716,46 +753,61 @@ __global__ __launch_bounds__(256) void batch_attn_merge_kernel(BatchAttnArgs a)
 }
 
 struct BatchAttnPlan {
+    bool many = false;
     int shared_tiles = 0, shared_splits = 0, shared_piece = kPass;
     int own_tiles = 0, own_splits = 1, own_piece = kPass, own_prefix = 0;
 };
 
 static int round_up(int v, int to) { return ceil_div(v, to) * to; }
 
-// Pieces of rows: enough items for every compute unit to hold several, pieces not so long that one long request is
-// still at work when the others are done, not so short that joining them costs more than reading them.
+// Pieces of `rows` cache rows, for `items` of them in each piece: enough that every compute unit has 4 workgroups, but
+// not shorter than 256 rows, where joining costs more than it gives, nor longer than `longest`.
+static int batch_attn_piece(long long items, int rows, int longest, int cus)
+{
+    const long long want = (4LL * cus + items - 1) / items, most = ceil_div(rows, 256), least = ceil_div(rows, longest);
+    long long n = want < most ? want : most;
+    n = n > least ? n : least;
+    n = n < kMaxPieces ? n : kMaxPieces;
+    return round_up(ceil_div(rows, static_cast<int>(n)), kPass);
+}
+
+// Sharing pays while a request has fewer than 64 columns of its own: more fill a workgroup's columns anyway, and the
+// prefix becomes the front of every request's rows.  Rows without limit for such columns (one piece unless
+// there are few items: whole prompts are bound by the matrix cores, and their sums would weigh more than the cache);
+// pieces of 1024 rows for few columns, so that a long request ends with the others (64 conversations: 512 rows 133 us, 1024
+// 133, 4096 170; four documents of up to 131000 rows: 215, 203, 218).
 static BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int group, int max_rows)
 {
     BatchAttnPlan p;
     const int cus = ctx().num_cus > 0 ? ctx().num_cus : 256;
     const long long columns = static_cast<long long>(b.n_tokens) * group;
-    p.own_tiles = static_cast<int>(columns / kTileRows) + b.n_requests;
-    const bool shared = b.prefix_length > 0 && columns < 64LL * b.n_requests && b.n_requests > 1;
+    const bool fill = columns >= 64LL * b.n_requests;
+    const bool shared = b.prefix_length > 0 && !fill && b.n_requests > 1;
+    // Up to 128 shared columns are cheaper as tiles of 16 that read the prefix out of the L2 again: the kernel without
+    // the wide tiles has 3 wavefronts per SIMD instead of 2 (72 columns: 133 us, 140).
+    p.many = columns > static_cast<long long>(kFewRows) * b.n_requests || (shared && columns > 128);
+    const int tile = p.many ? kManyRows : kFewRows;
+    p.own_tiles = static_cast<int>(columns / tile) + b.n_requests;
     p.own_prefix = shared ? 0 : round_up(b.prefix_length, kPass);
     const int own_rows = p.own_prefix + max_rows;
-    const long long items = static_cast<long long>(p.own_tiles) * n_kv_heads;
-    auto pieces = [&](long long have, int rows, int longest) {
-        long long n = (8LL * cus + have - 1) / have;
-        const long long most = ceil_div(rows, 256), least = ceil_div(rows, longest);
-        n = n < most ? n : most;
-        n = n > least ? n : least;
-        return static_cast<int>(n < 256 ? n : 256);
-    };
-    p.own_piece = round_up(ceil_div(own_rows, pieces(items, own_rows, 1024)), kPass);
+    p.own_piece = batch_attn_piece(static_cast<long long>(p.own_tiles) * n_kv_heads, own_rows, fill ? own_rows : 1024, cus);
     p.own_splits = ceil_div(own_rows, p.own_piece);
     if (shared) {
-        p.shared_tiles = static_cast<int>((columns + kTileRows - 1) / kTileRows);
-        p.shared_piece = round_up(ceil_div(b.prefix_length, pieces(static_cast<long long>(p.shared_tiles) * n_kv_heads * 4,
-                                                                     b.prefix_length, 1024)), kPass);
+        p.shared_tiles = static_cast<int>((columns + tile - 1) / tile);
+        // a quarter of the workgroups: a shared piece has more columns than an own one
+        p.shared_piece = batch_attn_piece(4LL * p.shared_tiles * n_kv_heads, b.prefix_length, 1024, cus);
         p.shared_splits = ceil_div(b.prefix_length, p.shared_piece);
     }
     return p;
 }
 
 template <int D>
-static void batch_attn_launch(const BatchAttnArgs& a, int items, int slots)
+static void batch_attn_launch(const BatchAttnArgs& a, bool many, int items, int slots)
 {
-    hipLaunchKernelGGL(batch_attn_kernel<D>, dim3(items), dim3(256), 0, ctx().stream, a);
+    if (many)
+        hipLaunchKernelGGL((batch_attn_kernel<D, true>), dim3(items), dim3(256), 0, ctx().stream, a);
+    else
+        hipLaunchKernelGGL((batch_attn_kernel<D, false>), dim3(items), dim3(256), 0, ctx().stream, a);
     if (!a.parts)
         return;
     const int rows = a.n_tokens * a.n_kv_heads * a.group;
@@ -821,6 +873,7 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
     a.shared_tiles = p.shared_tiles;
     a.shared_splits = p.shared_splits;
     a.shared_piece = p.shared_piece;
+    a.own_items = p.own_tiles * p.own_splits * a.n_kv_heads;
     a.own_tiles = p.own_tiles;
     a.own_piece = p.own_piece;
     a.own_prefix = p.own_prefix;
@@ -838,9 +891,9 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
         a.stats = reinterpret_cast<float2*>(a.parts + part * cache->head_size);
     }
     if (cache->head_size == 128)
-        batch_attn_launch<128>(a, static_cast<int>(items), slots);
+        batch_attn_launch<128>(a, p.many, static_cast<int>(items), slots);
     else
-        batch_attn_launch<64>(a, static_cast<int>(items), slots);
+        batch_attn_launch<64>(a, p.many, static_cast<int>(items), slots);
     L2_LAUNCH_CHECK(fn);
     return LLAMA2_OK;
 }
