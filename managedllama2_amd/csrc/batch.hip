@@ -1,6 +1,7 @@
 // The operators in front of the attention of a step of several requests: block tables and slots from the requests'
 // lengths, and the rotation of queries and keys (normed, where the model does that) with the store into the paged cache.
 #include "common.hpp"
+#include "batch_plan.hpp"
 
 #include <cmath>
 #include <cstring>
@@ -71,7 +72,7 @@ __global__ __launch_bounds__(kTablesBlock) void batch_tables_kernel(TablesArgs a
         const bool admitted = fits && (need == 0 || upto <= left);
         begin[tid] = end;
         rows[tid] = c;
-        from[tid] = admitted ? taken + upto - need : -1;
+        from[tid] = !admitted ? -1 : need > 0 ? taken + upto - need : 0;
         if (admitted && need > 0)
             atomicMax(&most_taken, upto);
         if (b < a.n_requests) {
@@ -262,43 +263,6 @@ __global__ __launch_bounds__(256) void batch_rope_kernel(RopeArgs a)
 }
 
 // ---------------------------------------------------------------- host side
-int check_paged_cache(const char* fn, const llama2_paged_cache* c, int n_heads)
-{
-    L2_CHECK(c && c->key && c->value, "%s: null pointer", fn);
-    L2_CHECK(aligned(c->key, 16) && aligned(c->value, 16), "%s: cache pointers must be 16-byte aligned", fn);
-    if (c->head_size != 64 && c->head_size != 128)
-        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: head_size=%d must be 64 or 128", fn, c->head_size);
-    L2_CHECK(c->block_size >= 8 && c->block_size <= 1024 && (c->block_size & (c->block_size - 1)) == 0,
-             "%s: block_size=%d must be a power of two from 8 to 1024", fn, c->block_size);
-    L2_CHECK(c->n_kv_heads > 0 && n_heads > 0 && n_heads % c->n_kv_heads == 0,
-             "%s: n_heads=%d must be a positive multiple of n_kv_heads=%d", fn, n_heads, c->n_kv_heads);
-    if (n_heads > kMaxAttnHeads)
-        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: n_heads=%d exceeds %d", fn, n_heads, kMaxAttnHeads);
-    const long long block = static_cast<long long>(c->block_size) * c->n_kv_heads * c->head_size;
-    L2_CHECK(c->block_stride == 0 || (c->block_stride >= block && c->block_stride % 8 == 0),
-             "%s: block_stride=%lld must be 0 or a multiple of 8 of at least %lld halfs", fn, c->block_stride, block);
-    L2_CHECK(c->n_blocks > 0 && c->n_blocks <= 0x7FFFFFFF / c->block_size,
-             "%s: n_blocks=%d must be positive, and n_blocks * block_size below 2^31", fn, c->n_blocks);
-    return LLAMA2_OK;
-}
-
-int check_batch(const char* fn, const llama2_batch* b)
-{
-    L2_CHECK(b, "%s: null batch", fn);
-    L2_CHECK(b->n_requests > 0 && b->n_requests <= kMaxBatchTokens && b->n_tokens > 0 && b->n_tokens <= kMaxBatchTokens,
-             "%s: n_requests=%d and n_tokens=%d must be 1 .. %d", fn, b->n_requests, b->n_tokens, kMaxBatchTokens);
-    L2_CHECK(b->prefix_length >= 0, "%s: prefix_length=%d is negative", fn, b->prefix_length);
-    return LLAMA2_OK;
-}
-
-static int log2_of(int power)
-{
-    int s = 0;
-    while ((1 << s) < power)
-        ++s;
-    return s;
-}
-
 // A pair's turns per position, in 64 bits of fixed point: times a position, the bits above are whole turns and drop out
 // by themselves; 2^31 positions times the error of 2^-58 relative leave 2^-29 of a turn.  A model has one theta, so the
 // last table is kept (1.5 us to make); the caller holds the library's lock.
@@ -328,19 +292,9 @@ int llama2_batch_tables(const llama2_batch* batch, const int* cached, const int*
                         const int* taken, int* new_taken, int block_size)
 {
     L2_REQUIRE_INIT();
-    if (int rc = check_batch("llama2_batch_tables", batch))
+    if (int rc = check_batch_tables(batch, cached, counts, free_blocks, n_free, taken, new_taken, block_size))
         return rc;
     const llama2_batch& b = *batch;
-    L2_CHECK(b.block_tables && b.lengths && b.query_starts && b.positions && b.slots && cached && counts && taken && new_taken,
-             "llama2_batch_tables: null pointer");
-    L2_CHECK(n_free >= 0 && (free_blocks || n_free == 0), "llama2_batch_tables: n_free=%d free_blocks=%p", n_free,
-             static_cast<const void*>(free_blocks));
-    L2_CHECK(block_size >= 8 && block_size <= 1024 && (block_size & (block_size - 1)) == 0,
-             "llama2_batch_tables: block_size=%d must be a power of two from 8 to 1024", block_size);
-    L2_CHECK(b.table_stride > 0, "llama2_batch_tables: table_stride=%d must be positive", b.table_stride);
-    L2_CHECK(b.table_stride <= (0x7FFFFFFF - b.prefix_length) / block_size,
-             "llama2_batch_tables: positions of prefix_length=%d and table_stride=%d blocks of %d rows exceed 2^31", b.prefix_length,
-             b.table_stride, block_size);
     TablesArgs a = {b.block_tables, b.lengths, b.query_starts, b.positions, b.slots, cached, counts, free_blocks, taken,
                     new_taken, b.n_requests, b.n_tokens, b.table_stride, b.prefix_length, n_free, log2_of(block_size)};
     hipLaunchKernelGGL(batch_tables_kernel, dim3(1), dim3(kTablesBlock), 0, ctx().stream, a);
@@ -355,27 +309,10 @@ int llama2_batch_qk_norm_rope(llama2_half* q_output, const llama2_half* q, const
 {
     const char* fn = "llama2_batch_qk_norm_rope";
     L2_REQUIRE_INIT();
-    if (int rc = check_batch(fn, batch))
+    if (int rc = check_batch_rope(q_output, q, k, v, q_gamma, k_gamma, batch, cache, n_heads, q_output_stride, q_stride, kv_stride, eps,
+                                  theta))
         return rc;
-    if (int rc = check_paged_cache(fn, cache, n_heads))
-        return rc;
-    L2_CHECK(q_output && q && k && v && batch->positions && batch->slots, "%s: null pointer", fn);
-    L2_CHECK(aligned(q_output, 16) && aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(q_gamma, 16) &&
-                 aligned(k_gamma, 16), "%s: pointers must be 16-byte aligned", fn);
-    const int d = cache->head_size, q_row = n_heads * d, kv_row = cache->n_kv_heads * d;
-    L2_CHECK(q_stride >= q_row && q_output_stride >= q_row && kv_stride >= kv_row && q_stride % 8 == 0 && q_output_stride % 8 == 0 &&
-                 kv_stride % 8 == 0, "%s: strides %d, %d, %d must be multiples of 8 and hold a row of %d, %d, %d", fn, q_output_stride,
-             q_stride, kv_stride, q_row, q_row, kv_row);
-    L2_CHECK(theta >= 1.0f && theta <= 3.0e38f, "%s: theta=%g must be at least 1", fn, static_cast<double>(theta));
-    L2_CHECK(eps >= 0.0f, "%s: eps=%g is negative", fn, static_cast<double>(eps));
-    auto bytes = [&](int stride, int row) { return (static_cast<size_t>(batch->n_tokens - 1) * stride + row) * 2; };
-    const size_t out_bytes = bytes(q_output_stride, q_row);
-    L2_CHECK((q_output == q && q_output_stride == q_stride) || !overlap(q_output, out_bytes, q, bytes(q_stride, q_row)),
-             "%s: q_output overlaps q without being it", fn);
-    L2_CHECK((q_output == q && q_output_stride == q_stride) ||
-                 (!overlap(q_output, out_bytes, k, bytes(kv_stride, kv_row)) && !overlap(q_output, out_bytes, v, bytes(kv_stride, kv_row))),
-             "%s: q_output overlaps k or v", fn);
-    const long long block = static_cast<long long>(cache->block_size) * kv_row;
+    const int d = cache->head_size;
     RopeArgs a = {};
     a.q_output = q_output;
     a.q = q;
@@ -387,7 +324,7 @@ int llama2_batch_qk_norm_rope(llama2_half* q_output, const llama2_half* q, const
     a.slots = batch->slots;
     a.key = cache->key;
     a.value = cache->value;
-    a.block_stride = cache->block_stride ? cache->block_stride : block;
+    a.block_stride = block_halfs(*cache);
     a.n_slots = static_cast<long long>(cache->n_blocks) * cache->block_size;
     a.n_heads = n_heads;
     a.n_kv_heads = cache->n_kv_heads;

@@ -11,6 +11,7 @@
 //            columns of its own that sharing would not save any reading).
 // Pieces leave fp32 sums, maximum and denominator; batch_attn_merge_kernel joins them in order.
 #include "common.hpp"
+#include "batch_plan.hpp"
 
 namespace l2 {
 
@@ -18,12 +19,8 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 typedef float f16v_t __attribute__((ext_vector_type(16)));
 
-constexpr int kManyRows = 128; // columns (token, head of the group) per workgroup
-constexpr int kFewRows = 16;   // at most this many: the wavefronts split the cache rows instead of the columns
-constexpr int kPass = 64;      // cache rows per pass of many_rows; pieces are multiples of it
 // Probabilities enter the matrix cores as fp16 times 2^14: the largest is 16384, and one of 2^-38 is still a number.  Their
 // sum carries the same factor, so that it drops out of the quotient.
-constexpr int kMaxPieces = 256; // of a request's rows, and of the prefix
 constexpr float kProbShift = 14.0f;
 
 struct BatchAttnArgs {
@@ -752,55 +749,6 @@ __global__ __launch_bounds__(256) void batch_attn_merge_kernel(BatchAttnArgs a)
     *reinterpret_cast<u32x4*>(a.out + static_cast<size_t>(token) * a.out_stride + head * D + x * 8) = w;
 }
 
-struct BatchAttnPlan {
-    bool many = false;
-    int shared_tiles = 0, shared_splits = 0, shared_piece = kPass;
-    int own_tiles = 0, own_splits = 1, own_piece = kPass, own_prefix = 0;
-};
-
-static int round_up(int v, int to) { return ceil_div(v, to) * to; }
-
-// Pieces of `rows` cache rows, for `items` of them in each piece: enough that every compute unit has 4 workgroups, but
-// not shorter than 256 rows, where joining costs more than it gives, nor longer than `longest`.
-static int batch_attn_piece(long long items, int rows, int longest, int cus)
-{
-    const long long want = (4LL * cus + items - 1) / items, most = ceil_div(rows, 256), least = ceil_div(rows, longest);
-    long long n = want < most ? want : most;
-    n = n > least ? n : least;
-    n = n < kMaxPieces ? n : kMaxPieces;
-    return round_up(ceil_div(rows, static_cast<int>(n)), kPass);
-}
-
-// Sharing pays while a request has fewer than 64 columns of its own: more fill a workgroup's columns anyway, and the
-// prefix becomes the front of every request's rows.  Rows without limit for such columns (one piece unless
-// there are few items: whole prompts are bound by the matrix cores, and their sums would weigh more than the cache);
-// pieces of 1024 rows for few columns, so that a long request ends with the others (64 conversations: 512 rows 133 us, 1024
-// 133, 4096 170; four documents of up to 131000 rows: 215, 203, 218).
-static BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int group, int max_rows)
-{
-    BatchAttnPlan p;
-    const int cus = ctx().num_cus > 0 ? ctx().num_cus : 256;
-    const long long columns = static_cast<long long>(b.n_tokens) * group;
-    const bool fill = columns >= 64LL * b.n_requests;
-    const bool shared = b.prefix_length > 0 && !fill && b.n_requests > 1;
-    // Up to 128 shared columns are cheaper as tiles of 16 that read the prefix out of the L2 again: the kernel without
-    // the wide tiles has 3 wavefronts per SIMD instead of 2 (72 columns: 133 us, 140).
-    p.many = columns > static_cast<long long>(kFewRows) * b.n_requests || (shared && columns > 128);
-    const int tile = p.many ? kManyRows : kFewRows;
-    p.own_tiles = static_cast<int>(columns / tile) + b.n_requests;
-    p.own_prefix = shared ? 0 : round_up(b.prefix_length, kPass);
-    const int own_rows = p.own_prefix + max_rows;
-    p.own_piece = batch_attn_piece(static_cast<long long>(p.own_tiles) * n_kv_heads, own_rows, fill ? own_rows : 1024, cus);
-    p.own_splits = ceil_div(own_rows, p.own_piece);
-    if (shared) {
-        p.shared_tiles = static_cast<int>((columns + tile - 1) / tile);
-        // a quarter of the workgroups: a shared piece has more columns than an own one
-        p.shared_piece = batch_attn_piece(4LL * p.shared_tiles * n_kv_heads, b.prefix_length, 1024, cus);
-        p.shared_splits = ceil_div(b.prefix_length, p.shared_piece);
-    }
-    return p;
-}
-
 template <int D>
 static void batch_attn_launch(const BatchAttnArgs& a, bool many, int items, int slots)
 {
@@ -828,23 +776,15 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
 {
     const char* fn = "llama2_batch_attention";
     L2_REQUIRE_INIT();
-    if (int rc = check_batch(fn, batch))
-        return rc;
-    if (int rc = check_paged_cache(fn, cache, n_heads))
+    if (int rc = check_batch_attention(output, query, batch, cache, n_heads, output_stride, query_stride, scale))
         return rc;
     const llama2_batch& b = *batch;
-    L2_CHECK(output && query && b.block_tables && b.query_starts && b.positions && (b.prefix_table || b.prefix_length == 0),
-             "%s: null pointer", fn);
-    L2_CHECK(aligned(output, 16) && aligned(query, 16), "%s: pointers must be 16-byte aligned", fn);
-    const int row = n_heads * cache->head_size;
-    L2_CHECK(output_stride >= row && query_stride >= row && output_stride % 8 == 0 && query_stride % 8 == 0,
-             "%s: strides %d, %d must be multiples of 8 and hold a row of %d", fn, output_stride, query_stride, row);
-    L2_CHECK(!overlap(output, (static_cast<size_t>(b.n_tokens - 1) * output_stride + row) * 2, query,
-                      (static_cast<size_t>(b.n_tokens - 1) * query_stride + row) * 2), "%s: output overlaps query", fn);
-    L2_CHECK(b.table_stride > 0 && b.max_length > 0 && b.max_length <= (0x7FFFFFFF - 4096 - b.prefix_length),
-             "%s: table_stride=%d and max_length=%d must be positive, and below 2^31 rows with the prefix", fn, b.table_stride,
-             b.max_length);
     const long long table_rows = static_cast<long long>(b.table_stride) * cache->block_size;
+    const int max_rows = table_rows < b.max_length ? static_cast<int>(table_rows) : b.max_length, group = n_heads / cache->n_kv_heads;
+    const BatchAttnPlan p = batch_attn_plan(b, cache->n_kv_heads, group, max_rows, ctx().num_cus > 0 ? ctx().num_cus : 256);
+    const long long rows = static_cast<long long>(b.n_tokens) * n_heads, items = p.items(cache->n_kv_heads);
+    if (rows > 0x7FFFFFFF / 4 || items > 0x7FFFFFFF)
+        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: %d tokens of %d heads in %d pieces are too many", fn, b.n_tokens, n_heads, p.slots());
     BatchAttnArgs a = {};
     a.out = output;
     a.q = query;
@@ -854,46 +794,37 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
     a.block_tables = b.block_tables;
     a.query_starts = b.query_starts;
     a.positions = b.positions;
-    a.block_stride = cache->block_stride ? cache->block_stride
-                                         : static_cast<long long>(cache->block_size) * cache->n_kv_heads * cache->head_size;
+    a.block_stride = block_halfs(*cache);
     a.n_requests = b.n_requests;
     a.n_tokens = b.n_tokens;
     a.table_stride = b.table_stride;
     a.prefix_length = b.prefix_length;
-    a.max_rows = table_rows < b.max_length ? static_cast<int>(table_rows) : b.max_length;
+    a.max_rows = max_rows;
     a.n_blocks = cache->n_blocks;
-    for (a.shift = 3; (1 << a.shift) < cache->block_size; ++a.shift) {
-    }
+    a.shift = log2_of(cache->block_size);
     a.n_kv_heads = cache->n_kv_heads;
-    a.group = n_heads / cache->n_kv_heads;
+    a.group = group;
     a.out_stride = output_stride;
     a.q_stride = query_stride;
     a.scale = scale * 1.44269504088896340736f; // powers of two below
-    const BatchAttnPlan p = batch_attn_plan(b, a.n_kv_heads, a.group, a.max_rows);
     a.shared_tiles = p.shared_tiles;
     a.shared_splits = p.shared_splits;
     a.shared_piece = p.shared_piece;
-    a.own_items = p.own_tiles * p.own_splits * a.n_kv_heads;
+    a.own_items = static_cast<int>(items) - p.shared_tiles * p.shared_splits * a.n_kv_heads;
     a.own_tiles = p.own_tiles;
     a.own_piece = p.own_piece;
     a.own_prefix = p.own_prefix;
-    const int slots = p.shared_splits + p.own_splits;
-    const long long rows = static_cast<long long>(b.n_tokens) * n_heads;
-    const long long items = static_cast<long long>(a.n_kv_heads) *
-                            (static_cast<long long>(p.shared_tiles) * p.shared_splits + static_cast<long long>(p.own_tiles) * p.own_splits);
-    if (rows > 0x7FFFFFFF / 4 || items > 0x7FFFFFFF)
-        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: %d tokens of %d heads in %d pieces are too many", fn, b.n_tokens, n_heads, slots);
-    if (slots > 1) {
-        const size_t part = static_cast<size_t>(slots) * rows;
+    if (p.slots() > 1) {
+        const size_t part = static_cast<size_t>(p.slots()) * rows;
         if (int rc = ensure_attn_partials(part * (cache->head_size + 2) * sizeof(float)))
             return rc;
         a.parts = ctx().attn_partials;
         a.stats = reinterpret_cast<float2*>(a.parts + part * cache->head_size);
     }
     if (cache->head_size == 128)
-        batch_attn_launch<128>(a, p.many, static_cast<int>(items), slots);
+        batch_attn_launch<128>(a, p.many, static_cast<int>(items), p.slots());
     else
-        batch_attn_launch<64>(a, p.many, static_cast<int>(items), slots);
+        batch_attn_launch<64>(a, p.many, static_cast<int>(items), p.slots());
     L2_LAUNCH_CHECK(fn);
     return LLAMA2_OK;
 }

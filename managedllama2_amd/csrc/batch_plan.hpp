@@ -1,0 +1,230 @@
+// Host side of the operators of a step of several requests, without a GPU call in it: what arguments are refused, and how
+// the attention is cut into workgroups.  Uses L2_CHECK, fail, aligned, overlap and ceil_div of whoever includes it.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+
+#include "../../include/llama2_hip.h"
+
+namespace l2 {
+
+constexpr int kMaxBatchTokens = 1 << 20; // tokens and requests of a step
+constexpr int kMaxBatchHeads = 1024;
+
+constexpr int kManyRows = 128; // columns (token, head of the group) of a workgroup's widest tile
+constexpr int kFewRows = 16;   // at most this many: the wavefronts split the cache rows instead of the columns
+constexpr int kPass = 64;      // cache rows per pass of wide tiles; pieces are multiples of it
+constexpr int kMaxPieces = 256; // of a request's rows, and of the prefix
+
+inline int round_up(int v, int to) { return ceil_div(v, to) * to; }
+
+inline int log2_of(int power)
+{
+    int s = 0;
+    while ((1 << s) < power)
+        ++s;
+    return s;
+}
+
+// ---------------------------------------------------------------- refusals
+inline int check_block_size(const char* fn, int block_size)
+{
+    L2_CHECK(block_size >= 8 && block_size <= 1024 && (block_size & (block_size - 1)) == 0,
+             "%s: block_size=%d must be a power of two from 8 to 1024", fn, block_size);
+    return LLAMA2_OK;
+}
+
+inline int check_batch(const char* fn, const llama2_batch* b)
+{
+    L2_CHECK(b, "%s: null batch", fn);
+    L2_CHECK(b->n_requests > 0 && b->n_requests <= kMaxBatchTokens && b->n_tokens > 0 && b->n_tokens <= kMaxBatchTokens,
+             "%s: n_requests=%d and n_tokens=%d must be 1 .. %d", fn, b->n_requests, b->n_tokens, kMaxBatchTokens);
+    L2_CHECK(b->prefix_length >= 0, "%s: prefix_length=%d is negative", fn, b->prefix_length);
+    L2_CHECK(aligned(b->block_tables, 4) && aligned(b->lengths, 4) && aligned(b->query_starts, 4) && aligned(b->positions, 4) &&
+                 aligned(b->slots, 4) && aligned(b->prefix_table, 4), "%s: misaligned array in the batch", fn);
+    return LLAMA2_OK;
+}
+
+inline long long block_halfs(const llama2_paged_cache& c)
+{
+    return c.block_stride ? c.block_stride : static_cast<long long>(c.block_size) * c.n_kv_heads * c.head_size;
+}
+
+inline size_t cache_bytes(const llama2_paged_cache& c) // of keys, or of values
+{
+    return (static_cast<size_t>(c.n_blocks - 1) * block_halfs(c) + static_cast<size_t>(c.block_size) * c.n_kv_heads * c.head_size) * 2;
+}
+
+inline int check_paged_cache(const char* fn, const llama2_paged_cache* c, int n_heads)
+{
+    L2_CHECK(c && c->key && c->value, "%s: null cache", fn);
+    L2_CHECK(aligned(c->key, 16) && aligned(c->value, 16), "%s: cache pointers must be 16-byte aligned", fn);
+    if (c->head_size != 64 && c->head_size != 128)
+        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: head_size=%d must be 64 or 128", fn, c->head_size);
+    if (int rc = check_block_size(fn, c->block_size))
+        return rc;
+    L2_CHECK(c->n_kv_heads > 0 && n_heads > 0 && n_heads % c->n_kv_heads == 0,
+             "%s: n_heads=%d must be a positive multiple of n_kv_heads=%d", fn, n_heads, c->n_kv_heads);
+    if (n_heads > kMaxBatchHeads)
+        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: n_heads=%d exceeds %d", fn, n_heads, kMaxBatchHeads);
+    const long long block = static_cast<long long>(c->block_size) * c->n_kv_heads * c->head_size;
+    L2_CHECK(c->n_blocks > 0 && c->n_blocks <= 0x7FFFFFFF / c->block_size,
+             "%s: n_blocks=%d must be positive, and n_blocks * block_size below 2^31", fn, c->n_blocks);
+    L2_CHECK(c->block_stride == 0 || (c->block_stride >= block && c->block_stride % 8 == 0 && c->block_stride <= (1LL << 45) / c->n_blocks),
+             "%s: block_stride=%lld must be 0 or a multiple of 8 of at least %lld halfs", fn, c->block_stride, block);
+    return LLAMA2_OK;
+}
+
+inline size_t rows_bytes(int rows, int stride, int width) { return (static_cast<size_t>(rows - 1) * stride + width) * 2; }
+
+inline int check_batch_tables(const llama2_batch* batch, const int* cached, const int* counts, const int* free_blocks, int n_free,
+                              const int* taken, const int* new_taken, int block_size)
+{
+    const char* fn = "llama2_batch_tables";
+    if (int rc = check_batch(fn, batch))
+        return rc;
+    const llama2_batch& b = *batch;
+    L2_CHECK(b.block_tables && b.lengths && b.query_starts && b.positions && b.slots && cached && counts && taken && new_taken,
+             "%s: null pointer", fn);
+    L2_CHECK(aligned(cached, 4) && aligned(counts, 4) && aligned(free_blocks, 4) && aligned(taken, 4) && aligned(new_taken, 4),
+             "%s: misaligned pointer", fn);
+    L2_CHECK(n_free >= 0 && n_free < 0x7FFFFFFF && (free_blocks || n_free == 0), "%s: n_free=%d free_blocks=%p", fn, n_free,
+             static_cast<const void*>(free_blocks));
+    if (int rc = check_block_size(fn, block_size))
+        return rc;
+    L2_CHECK(b.table_stride > 0 && b.table_stride <= (0x7FFFFFFF - b.prefix_length) / block_size,
+             "%s: table_stride=%d must be positive, and prefix_length=%d + table_stride * block_size below 2^31", fn, b.table_stride,
+             b.prefix_length);
+    const size_t requests = static_cast<size_t>(b.n_requests) * 4, tokens = static_cast<size_t>(b.n_tokens) * 4;
+    const struct {
+        const void* p;
+        size_t bytes;
+    } written[] = {{b.block_tables, requests * b.table_stride}, {b.lengths, requests}, {b.query_starts, requests + 4},
+                   {b.positions, tokens}, {b.slots, tokens}, {new_taken, 4}},
+      read[] = {{cached, requests}, {counts, requests}, {free_blocks, static_cast<size_t>(n_free) * 4}, {taken, 4}};
+    for (int i = 0; i < 6; ++i) {
+        for (int j = 0; j < i; ++j)
+            L2_CHECK(!overlap(written[i].p, written[i].bytes, written[j].p, written[j].bytes), "%s: output arrays overlap", fn);
+        for (int j = 0; j < 4; ++j) {
+            const bool in_place = written[i].p == read[j].p && ((i == 1 && j == 0) || (i == 5 && j == 3));
+            L2_CHECK(in_place || !overlap(written[i].p, written[i].bytes, read[j].p, read[j].bytes),
+                     "%s: an output overlaps an input (lengths may be cached, and new_taken taken)", fn);
+        }
+    }
+    return LLAMA2_OK;
+}
+
+inline int check_batch_rope(const llama2_half* q_output, const llama2_half* q, const llama2_half* k, const llama2_half* v,
+                            const llama2_half* q_gamma, const llama2_half* k_gamma, const llama2_batch* batch,
+                            const llama2_paged_cache* cache, int n_heads, int q_output_stride, int q_stride, int kv_stride, float eps,
+                            float theta)
+{
+    const char* fn = "llama2_batch_qk_norm_rope";
+    if (int rc = check_batch(fn, batch))
+        return rc;
+    if (int rc = check_paged_cache(fn, cache, n_heads))
+        return rc;
+    L2_CHECK(q_output && q && k && v && batch->positions && batch->slots, "%s: null pointer", fn);
+    L2_CHECK(aligned(q_output, 16) && aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(q_gamma, 16) &&
+                 aligned(k_gamma, 16), "%s: pointers must be 16-byte aligned", fn);
+    const int q_row = n_heads * cache->head_size, kv_row = cache->n_kv_heads * cache->head_size, t = batch->n_tokens;
+    L2_CHECK(q_stride >= q_row && q_output_stride >= q_row && kv_stride >= kv_row && q_stride % 8 == 0 && q_output_stride % 8 == 0 &&
+                 kv_stride % 8 == 0, "%s: strides %d, %d, %d must be multiples of 8 and hold a row of %d, %d, %d", fn, q_output_stride,
+             q_stride, kv_stride, q_row, q_row, kv_row);
+    L2_CHECK(theta >= 1.0f && theta <= 3.0e38f, "%s: theta=%g must be at least 1", fn, static_cast<double>(theta));
+    L2_CHECK(eps >= 0.0f && eps <= 3.0e38f, "%s: eps=%g must not be negative", fn, static_cast<double>(eps));
+    const size_t out_bytes = rows_bytes(t, q_output_stride, q_row), kv_bytes = rows_bytes(t, kv_stride, kv_row);
+    const bool in_place = q_output == q && q_output_stride == q_stride;
+    L2_CHECK(in_place || !overlap(q_output, out_bytes, q, rows_bytes(t, q_stride, q_row)), "%s: q_output overlaps q without being it", fn);
+    // in place, the rows of k and v may lie between those of q
+    L2_CHECK(in_place || (!overlap(q_output, out_bytes, k, kv_bytes) && !overlap(q_output, out_bytes, v, kv_bytes)),
+             "%s: q_output overlaps k or v", fn);
+    const void* written[] = {cache->key, cache->value};
+    for (const void* c : written)
+        L2_CHECK(!overlap(c, cache_bytes(*cache), q, rows_bytes(t, q_stride, q_row)) && !overlap(c, cache_bytes(*cache), k, kv_bytes) &&
+                     !overlap(c, cache_bytes(*cache), v, kv_bytes) && !overlap(c, cache_bytes(*cache), q_output, out_bytes),
+                 "%s: the cache overlaps q, k, v or q_output", fn);
+    return LLAMA2_OK;
+}
+
+inline int check_batch_attention(const llama2_half* output, const llama2_half* query, const llama2_batch* batch,
+                                 const llama2_paged_cache* cache, int n_heads, int output_stride, int query_stride, float scale)
+{
+    const char* fn = "llama2_batch_attention";
+    if (int rc = check_batch(fn, batch))
+        return rc;
+    if (int rc = check_paged_cache(fn, cache, n_heads))
+        return rc;
+    const llama2_batch& b = *batch;
+    L2_CHECK(output && query && b.block_tables && b.query_starts && b.positions && (b.prefix_table || b.prefix_length == 0),
+             "%s: null pointer", fn);
+    L2_CHECK(aligned(output, 16) && aligned(query, 16), "%s: pointers must be 16-byte aligned", fn);
+    const int row = n_heads * cache->head_size;
+    L2_CHECK(output_stride >= row && query_stride >= row && output_stride % 8 == 0 && query_stride % 8 == 0,
+             "%s: strides %d, %d must be multiples of 8 and hold a row of %d", fn, output_stride, query_stride, row);
+    L2_CHECK(scale >= -3.0e37f && scale <= 3.0e37f, "%s: scale=%g is not a finite number", fn, static_cast<double>(scale));
+    const size_t out_bytes = rows_bytes(b.n_tokens, output_stride, row);
+    L2_CHECK(!overlap(output, out_bytes, query, rows_bytes(b.n_tokens, query_stride, row)) &&
+                 !overlap(output, out_bytes, cache->key, cache_bytes(*cache)) && !overlap(output, out_bytes, cache->value, cache_bytes(*cache)),
+             "%s: output overlaps query or the cache", fn);
+    L2_CHECK(b.table_stride > 0 && b.max_length > 0 && b.max_length <= 0x7FFFFFFF - 4096 - b.prefix_length,
+             "%s: table_stride=%d and max_length=%d must be positive, and max_length with prefix_length=%d below 2^31", fn,
+             b.table_stride, b.max_length, b.prefix_length);
+    return LLAMA2_OK;
+}
+
+// ---------------------------------------------------------------- how the attention is cut
+struct BatchAttnPlan {
+    bool many = false; // the kernel with wide tiles
+    int shared_tiles = 0, shared_splits = 0, shared_piece = kPass;
+    int own_tiles = 0, own_splits = 1, own_piece = kPass;
+    int own_prefix = 0; // prefix rows in front of a request's own, a multiple of kPass; 0: none, or shared
+    int slots() const { return shared_splits + own_splits; }
+    long long items(int n_kv_heads) const
+    {
+        return (static_cast<long long>(shared_tiles) * shared_splits + static_cast<long long>(own_tiles) * own_splits) * n_kv_heads;
+    }
+};
+
+// Pieces of `rows` cache rows, for `items` of them in each piece: enough that every compute unit has 4 workgroups, but
+// not shorter than 256 rows, where joining costs more than it gives, nor longer than `longest`.
+inline int batch_attn_piece(long long items, int rows, int longest, int cus)
+{
+    const long long want = (4LL * cus + items - 1) / items, most = ceil_div(rows, 256), least = ceil_div(rows, longest);
+    long long n = want < most ? want : most;
+    n = n > least ? n : least;
+    n = n < kMaxPieces ? n : kMaxPieces;
+    return round_up(ceil_div(rows, static_cast<int>(n)), kPass);
+}
+
+// Sharing pays while a request has fewer than 64 columns of its own: more fill a workgroup's columns anyway, and the
+// prefix becomes the front of every request's rows.  Rows without limit for such columns (one piece unless
+// there are few items: whole prompts are bound by the matrix cores, and their sums would weigh more than the cache);
+// pieces of 1024 rows for few columns, so that a long request ends with the others (64 conversations: 512 rows 133 us, 1024
+// 133, 4096 170; four documents of up to 131000 rows: 215, 203, 218).
+inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int group, int max_rows, int cus)
+{
+    BatchAttnPlan p;
+    const long long columns = static_cast<long long>(b.n_tokens) * group;
+    const bool fill = columns >= 64LL * b.n_requests;
+    const bool shared = b.prefix_length > 0 && !fill && b.n_requests > 1;
+    // Up to 128 shared columns are cheaper as tiles of 16 that read the prefix out of the L2 again: the kernel without
+    // the wide tiles has 3 wavefronts per SIMD instead of 2 (72 columns: 133 us, 140).
+    p.many = columns > static_cast<long long>(kFewRows) * b.n_requests || (shared && columns > 128);
+    const int tile = p.many ? kManyRows : kFewRows;
+    p.own_tiles = static_cast<int>(columns / tile) + b.n_requests;
+    p.own_prefix = shared ? 0 : round_up(b.prefix_length, kPass);
+    const int own_rows = p.own_prefix + max_rows;
+    p.own_piece = batch_attn_piece(static_cast<long long>(p.own_tiles) * n_kv_heads, own_rows, fill ? own_rows : 1024, cus);
+    p.own_splits = ceil_div(own_rows, p.own_piece);
+    if (shared) {
+        p.shared_tiles = static_cast<int>((columns + tile - 1) / tile);
+        // a quarter of the workgroups: a shared piece has more columns than an own one
+        p.shared_piece = batch_attn_piece(4LL * p.shared_tiles * n_kv_heads, b.prefix_length, 1024, cus);
+        p.shared_splits = ceil_div(b.prefix_length, p.shared_piece);
+    }
+    return p;
+}
+
+} // namespace l2

@@ -59,11 +59,6 @@ int resolve_vec_mat_static_scratch(int device);
 int sample_launch(const char* fn, SamplerScratch* scratch, uint16_t* logits, int* indices, int size, float temperature,
                   float top_p, float coin, int* result, int pos, bool token_only, const HostStep* host = nullptr);
 
-// Arguments that the operators of a step of several requests share (batch.hip).
-constexpr int kMaxBatchTokens = 1 << 20;
-int check_paged_cache(const char* fn, const llama2_paged_cache* cache, int n_heads);
-int check_batch(const char* fn, const llama2_batch* batch);
-
 // HIP's current device is a per-thread setting: a host thread other than the one that called
 // llama2_init (a thread-pool worker of the managed host, say) is bound to the library's device on
 // its first call.
