@@ -19,9 +19,12 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 typedef float f16v_t __attribute__((ext_vector_type(16)));
 
-// Probabilities enter the matrix cores as fp16 times 2^14: the largest is 16384, and one of 2^-38 is still a number.  Their
-// sum carries the same factor, so that it drops out of the quotient.
-constexpr float kProbShift = 14.0f;
+// Probabilities enter the matrix cores as fp16, relative to a reference m that follows the running maximum only when that is
+// more than 2^8 above it (rescaling the sums is a fifth of a wide pass's vector work, and one of 32 columns has a new
+// maximum in nearly every pass): 2^6 exp2(score - m) is at most 2^14, and one of 2^-30 is still a number.  The sum carries
+// the same factors, so that they drop out of the quotient.
+constexpr float kProbShift = 6.0f;
+constexpr float kSlack = 8.0f;
 
 struct BatchAttnArgs {
     uint16_t* out;
@@ -37,7 +40,8 @@ struct BatchAttnArgs {
     long long block_stride;
     int n_requests, n_tokens, table_stride, prefix_length, max_rows;
     int n_blocks, shift, n_kv_heads, group, out_stride, q_stride;
-    float scale; // times log2(e)
+    float scale; // its absolute value times log2(e), positive
+    uint32_t q_sign; // what turns the queries over where the scale is negative
     // items: [shared_splits x n_kv_heads][shared_tiles], then [own_splits][own_tiles][n_kv_heads]
     int shared_tiles, shared_splits, shared_piece;
     int own_items, own_tiles, own_piece, own_prefix; // own_prefix: prefix rows in front of a request's own, a multiple of kPass, or 0
@@ -81,7 +85,7 @@ __device__ __forceinline__ int own_rows_of(const BatchAttnArgs& a, int p)
     return p < a.prefix_length ? 0 : min(p - a.prefix_length + 1, a.max_rows);
 }
 
-// exp2(v - most) times 2^14; without any score above -infinity everything is 0, not NaN.
+// exp2(v - base) is the probability times 2^6; without any score above -infinity everything is 0, not NaN.
 __device__ __forceinline__ float prob_base(float most) { return most == -INFINITY ? 0.0f : most - kProbShift; }
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ float weight_of(float m, float most) { return m == -INFINITY ? 0.0f : exp2_of(m - most); }
@@ -99,6 +103,15 @@ __device__ __forceinline__ const uint16_t* row_address(const BatchAttnArgs& a, c
 __device__ __forceinline__ bool in_cache(const BatchAttnArgs& a, int block)
 {
     return static_cast<unsigned>(block) < static_cast<unsigned>(a.n_blocks);
+}
+
+__device__ __forceinline__ h8_t load_query(const BatchAttnArgs& a, int token, int at)
+{
+    u32x4 v = *reinterpret_cast<const u32x4*>(a.q + static_cast<size_t>(token) * a.q_stride + at);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        v[k] ^= a.q_sign;
+    return __builtin_bit_cast(h8_t, v);
 }
 
 // ---------------------------------------------------------------- few columns
@@ -120,7 +133,7 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
     h8_t qf[KS];
 #pragma unroll
     for (int j = 0; j < KS; ++j)
-        qf[j] = *reinterpret_cast<const h8_t*>(a.q + static_cast<size_t>(token) * a.q_stride + head * D + j * 32 + g * 8);
+        qf[j] = load_query(a, token, head * D + j * 32 + g * 8);
 
     f4_t o[VE];
 #pragma unroll
@@ -197,8 +210,9 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
                     s[t][i] = whole || (tb + 16 * t + 4 * g + i < seen && ok[t]) ? v : -INFINITY;
                     most = fmaxf(most, s[t][i]);
                 }
-            most = fmaxf(m, max_xor32(max_xor16(most)));
-            if (__any(most > m)) {
+            most = max_xor32(max_xor16(most));
+            if (__any(most > m + kSlack)) {
+                most = fmaxf(m, most);
                 const float alpha = weight_of(m, most);
                 sum *= alpha;
 #pragma unroll
@@ -319,30 +333,48 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
 }
 
 // ---------------------------------------------------------------- many columns
-// 17 to 128 columns, 32 per wavefront: passes of 64 rows through LDS, read by all four.  Keys as rows; values transposed, a
-// row of 64 cache rows per output element, in the order in which a lane holds their probabilities (4 rows of one
-// half of the lanes, 4 of the other); 16-byte pieces are exchanged by element so that reads have no bank conflicts.
-constexpr int kValueStride = kPass * 2;
-
+// 17 to 128 columns, 32 per wavefront: passes of 64 rows through LDS, read by all four.  The rows of the next pass go
+// straight from memory into the other of two LDS buffers while this one is computed, so a pass has one barrier and no
+// register holds rows in flight.  Rows lie in LDS as in the cache, their 16-byte pieces exchanged by row so that reads have
+// no bank conflicts; values come out transposed (ds_read_b64_tr_b16: 4 rows of 16 elements per 16 lanes, a column each), in
+// the order in which a lane holds their probabilities (4 rows of one half of the lanes, 4 of the other).
 template <int D>
 struct ManyLds {
-    static constexpr int kKeyStride = D * 2 + 16;
-    static constexpr int kKeys = kPass * kKeyStride, kValues = D * kValueStride, kTotal = kKeys + kValues + 64;
+    static constexpr int kRow = D * 2, kPieces = D / 8;      // bytes and 16-byte pieces of a row
+    static constexpr int kTensor = kPass * kRow;             // keys, or values, of a pass
+    static constexpr int kBuffer = 2 * kTensor, kFlags = 2 * kBuffer, kTotal = kFlags + 32;
+    // A wavefront reads keys of 16 rows at the same piece at a time, values of 8 rows at 2 x 2 neighbouring pieces.
+    static __device__ __forceinline__ int key_piece(int row, int piece) { return piece ^ (D == 128 ? row & 15 : (row >> 1) & 7); }
+    static __device__ __forceinline__ int value_piece(int row, int piece) { return piece ^ (D == 128 ? (row & 7) * 2 : ((row >> 1) & 3) * 2); }
 };
 
-__device__ __forceinline__ int value_offset(int d, int piece) // piece: 16 bytes
+// 64 lanes x 16 bytes from base + offset (per lane) straight into LDS at `lds` + 16 lane.  Inline assembly because the
+// compiler would wait for it in front of the next read of any LDS; whoever reads the data waits for vmcnt.
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t lds)
 {
-    return d * kValueStride + ((piece ^ (((d >> 1) ^ (d >> 3)) & 7)) << 4);
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "{m0}"(lds), "v"(offset), "s"(base) : "memory");
+}
+
+// One value for the whole wavefront, through the scalar cache: it does not queue behind the cache rows that the vector
+// memory path is busy with.
+__device__ __forceinline__ int uniform_load(const int* p, int i)
+{
+    typedef const int __attribute__((address_space(4))) * Scalar;
+    return ((Scalar)p)[__builtin_amdgcn_readfirstlane(i)];
+}
+
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ h4_t read_transposed(const char* p)
+{
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(h4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p)));
 }
 
 template <int D>
 __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
 {
     using L = ManyLds<D>;
-    constexpr int QS = D / 16, DT = D / 32, CH = D / 8; // k steps, tiles of output elements, 16-byte pieces of a row
-    char* ks = lds;
-    char* vs = lds + L::kKeys;
-    int* flags = reinterpret_cast<int*>(lds + L::kKeys + L::kValues);
+    constexpr int QS = D / 16, DT = D / 32; // k steps, tiles of output elements
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hl = lane >> 5, l31 = lane & 31;
     const int r = wave * 32 + l31, rq = min(r, it.rows - 1);
@@ -356,21 +388,28 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
         most_rows = max(most_rows, __shfl_xor(most_rows, x, 64));
         least = max(least, __shfl_xor(least, x, 64));
     }
-    least = -least;
-
-    // Threads: 16 groups of 4 rows x D / 8 pieces; of heads of 64 one half of the threads takes keys, the other values.
-    const int unit = threadIdx.x % (16 * CH), piece = unit % CH, group4 = unit / CH;
-    const bool takes_k = D == 128 || threadIdx.x < 16 * CH, takes_v = D == 128 || !takes_k;
+    most_rows = __builtin_amdgcn_readfirstlane(most_rows);
+    least = -__builtin_amdgcn_readfirstlane(least);
 
     h8_t qf[QS];
 #pragma unroll
     for (int j = 0; j < QS; ++j)
-        qf[j] = *reinterpret_cast<const h8_t*>(a.q + static_cast<size_t>(token) * a.q_stride + head * D + j * 16 + hl * 8);
+        qf[j] = load_query(a, token, head * D + j * 16 + hl * 8);
     f16v_t o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
         o[d] = f16v_t{};
-    float m = -INFINITY, sum = 0.0f;
+    float m = -INFINITY, sum = 0.0f; // m: the exponents' reference, at most kSlack below the largest score
+
+    // A wavefront loads rows 16 wave .. + 15 of a pass, 8 at a time: those lie in one block.
+    constexpr int AT_ONCE = 1024 / L::kRow, LOADS = 8 / AT_ONCE; // rows per load, loads per 8 rows
+    const uint32_t row_bytes = static_cast<uint32_t>(a.n_kv_heads) * D * 2;
+    const int in_load = lane / L::kPieces, piece = lane % L::kPieces;
+    int* const flags = reinterpret_cast<int*>(lds + L::kFlags); // [buffer][wavefront]: which of its blocks are none
+    const uint32_t lds_base = __builtin_amdgcn_readfirstlane(
+        static_cast<int>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds)));
+    // address of the values that a lane reads transposed: row (lane / 16 / 2) * 4 + lane % 16 / 4 of 8, elements lane / 16 % 2 * 16 + lane % 4 * 4
+    const int tr_row = hl * 4 + ((lane & 15) >> 2), tr_piece = ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1), tr_byte = (lane & 1) * 8;
 
     for (int seg = 0; seg < 2; ++seg) {
         const int* table = seg ? it.table : a.prefix_table;
@@ -378,120 +417,93 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
         if (begin >= end)
             continue;
         const int seen = seg ? limit : end, all_see = seg ? least : end, any_sees = seg ? most_rows : end;
-        const int last4 = (end - 1) & ~3;
-        auto block_of = [&](int tb) { return table[min(tb + 4 * group4, last4) >> a.shift]; };
-        u32x4 kr[4], vr[4];
-        bool bad_block = false;
-        auto request = [&](int tb, int block) {
-            const bool ok = in_cache(a, block);
-            const int row = min(tb + 4 * group4, last4);
-            const uint16_t* k = row_address<D>(a, a.key, ok ? block : 0, row, it.kv_head) + piece * 8;
-            const uint16_t* v = row_address<D>(a, a.value, ok ? block : 0, row, it.kv_head) + piece * 8;
+        const int last8 = (end - 1) & ~7;
+        auto block_of = [&](int row) { return uniform_load(table, min(row, last8) >> a.shift); };
+        int block[2]; // of the pass that is requested next
+        auto look_up = [&](int tb) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (takes_k)
-                    kr[i] = *reinterpret_cast<const u32x4*>(k + static_cast<size_t>(i) * a.n_kv_heads * D);
-                if (takes_v)
-                    vr[i] = *reinterpret_cast<const u32x4*>(v + static_cast<size_t>(i) * a.n_kv_heads * D);
-            }
-            bad_block = !ok;
+            for (int h = 0; h < 2; ++h)
+                block[h] = block_of(tb + wave * 16 + h * 8);
         };
-        int next = block_of(begin);
-        request(begin, next);
-        next = block_of(begin + kPass);
-        for (int tb = begin; tb < end; tb += kPass) {
-            const bool none = __any(bad_block);
-            uint32_t bad = 0;
-            if (tb + kPass > end || none) {
+        auto request = [&](int tb, int buffer) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool keep = tb + 4 * group4 + i < end && !bad_block;
+            for (int h = 0; h < 2; ++h) {
+                const int first = wave * 16 + h * 8;
+                const long long at = (in_cache(a, block[h]) ? block[h] : 0) * a.block_stride +
+                                     ((min(tb + first, last8) & ((1 << a.shift) - 1)) * a.n_kv_heads + it.kv_head) * static_cast<long long>(D);
+                const uint32_t to = lds_base + buffer * L::kBuffer + first * L::kRow;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        vr[i][k] = keep ? vr[i][k] : 0u;
+                for (int x = 0; x < LOADS; ++x) {
+                    const int row = x * AT_ONCE + in_load; // of the 8; first is a multiple of 8, and of 16 for h = 0
+                    load_to_lds(a.key + at, row * row_bytes + L::key_piece(h * 8 + row, piece) * 16, to + x * 1024);
+                }
+#pragma unroll
+                for (int x = 0; x < LOADS; ++x) {
+                    const int row = x * AT_ONCE + in_load;
+                    load_to_lds(a.value + at, row * row_bytes + L::value_piece(h * 8 + row, piece) * 16, to + L::kTensor + x * 1024);
                 }
             }
-            if (takes_v) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        bad |= not_finite(vr[i][k]);
-            }
-            const bool any_bad = __any(bad != 0);
-            __syncthreads(); // the previous pass has been read
-            if (takes_k) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<u32x4*>(ks + (4 * group4 + i) * L::kKeyStride + piece * 16) = kr[i];
-            }
-            if (takes_v) {
-                const int to = (group4 >> 2) * 2 + (group4 & 1), at = ((group4 >> 1) & 1) * 8;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const u32x2 even = {__builtin_amdgcn_perm(vr[1][k], vr[0][k], 0x05040100u),
-                                        __builtin_amdgcn_perm(vr[3][k], vr[2][k], 0x05040100u)};
-                    const u32x2 odd = {__builtin_amdgcn_perm(vr[1][k], vr[0][k], 0x07060302u),
-                                       __builtin_amdgcn_perm(vr[3][k], vr[2][k], 0x07060302u)};
-                    *reinterpret_cast<u32x2*>(vs + value_offset(piece * 8 + 2 * k, to) + at) = even;
-                    *reinterpret_cast<u32x2*>(vs + value_offset(piece * 8 + 2 * k + 1, to) + at) = odd;
+        };
+        __syncthreads(); // the last pass of the shared rows has been read
+        look_up(begin);
+        int no_block = (!in_cache(a, block[0]) ? 1 : 0) | (!in_cache(a, block[1]) ? 2 : 0); // of the pass that is on its way
+        request(begin, 0);
+        look_up(begin + kPass);
+        int buffer = 0;
+        for (int tb = begin; tb < end; tb += kPass, buffer ^= 1) {
+            char* const ks = lds + buffer * L::kBuffer;
+            char* const vs = ks + L::kTensor;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // this wavefront's share of the pass lies in LDS
+            if (no_block || tb + wave * 16 + 16 > end) {
+                // What lies behind the last row, or in a block that is none, must not reach a sum through a probability of 0.
+                for (int x = lane; x < 16 * L::kPieces; x += 64) {
+                    const int row = x / L::kPieces;
+                    if (tb + wave * 16 + row >= end || ((no_block >> (row >> 3)) & 1))
+                        *reinterpret_cast<u32x4*>(vs + (wave * 16 + row) * L::kRow + x % L::kPieces * 16) = u32x4{};
                 }
             }
-            // flags: 0 .. 3 not-finite values seen by a wavefront, 4 .. 7 blocks that are none (a bit per group of 4 rows)
             if (lane == 0)
-                flags[wave] = any_bad;
-            if (none) {
-                const unsigned long long b = __ballot(bad_block && (takes_v));
-                if (lane == 0) {
-                    int bits = 0;
-                    for (int x = 0; x < 64; x += CH)
-                        bits |= static_cast<int>((b >> x) & 1) << ((threadIdx.x + x) % (16 * CH) / CH);
-                    flags[4 + wave] = bits;
-                }
-            } else if (lane == 0) {
-                flags[4 + wave] = 0;
-            }
-            __syncthreads();
+                flags[buffer * 4 + wave] = no_block;
+            __syncthreads(); // everybody's share does, and the other buffer has been read
             if (tb + kPass < end) {
-                request(tb + kPass, next);
-                next = block_of(tb + 2 * kPass);
+                no_block = (!in_cache(a, block[0]) ? 1 : 0) | (!in_cache(a, block[1]) ? 2 : 0);
+                request(tb + kPass, buffer ^ 1);
+                look_up(tb + 2 * kPass);
             }
             if (idle || tb >= any_sees)
                 continue;
-            const int no_block = flags[4] | flags[5] | flags[6] | flags[7];
-            const bool whole = tb + kPass <= all_see && no_block == 0;
-            const bool careful = tb + kPass > all_see && (flags[0] | flags[1] | flags[2] | flags[3]);
+            int no_rows = 0; // a bit per 8 rows
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                no_rows |= flags[buffer * 4 + w] << (2 * w);
+            no_rows = __builtin_amdgcn_readfirstlane(no_rows);
 
             f16v_t s[2] = {};
 #pragma unroll
             for (int j = 0; j < QS; ++j)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const h8_t kf = *reinterpret_cast<const h8_t*>(ks + (t * 32 + l31) * L::kKeyStride + j * 32 + hl * 16);
-                    s[t] = mfma32(kf, qf[j], s[t]);
+                    const int row = t * 32 + l31;
+                    s[t] = mfma32(*reinterpret_cast<const h8_t*>(ks + row * L::kRow + L::key_piece(row, j * 2 + hl) * 16), qf[j], s[t]);
                 }
-            float most = -INFINITY;
-            if (whole) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        s[t][i] *= a.scale;
-                        most = fmaxf(most, s[t][i]);
-                    }
-            } else {
+            if (tb + kPass > all_see || no_rows) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int row = t * 32 + 8 * (i >> 2) + 4 * hl + (i & 3);
-                        const bool keep = tb + row < seen && !((no_block >> (row >> 2)) & 1);
-                        s[t][i] = keep ? s[t][i] * a.scale : -INFINITY;
-                        most = fmaxf(most, s[t][i]);
+                        s[t][i] = tb + row < seen && !((no_rows >> (row >> 3)) & 1) ? s[t][i] : -INFINITY;
                     }
             }
-            most = fmaxf(m, max_xor32(most));
-            if (__any(most > m)) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    most = fmaxf(most, s[t][i]);
+            most = max_xor32(most) * a.scale;
+            if (__any(most > m + kSlack)) {
+                most = fmaxf(m, most);
                 const float alpha = weight_of(m, most);
                 sum *= alpha;
 #pragma unroll
@@ -504,17 +516,44 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float e = exp2_of(s[u >> 1][8 * (u & 1) + i] - base);
-                    sum += e;
-                    p[u][i] = static_cast<_Float16>(e);
+                for (int i = 0; i < 8; i += 2) {
+                    h2_t e;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        e[x] = static_cast<_Float16>(exp2_of(__builtin_fmaf(s[u >> 1][8 * (u & 1) + i + x], a.scale, -base)));
+                    p[u][i] = e[0];
+                    p[u][i + 1] = e[1];
+                    sum = dot2(as_u32(e), 0x3C003C00u, sum); // of the rounded ones, in fp32
                 }
+            bool careful = false; // an infinite or NaN value that some columns attend and others do not
+            if (tb + kPass > all_see) {
+                uint32_t bad = 0;
+                for (int x = lane; x < kPass * L::kPieces; x += 64) {
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(vs + x * 16);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        bad |= not_finite(v[k]);
+                }
+                careful = __any(bad != 0);
+            }
+            auto values = [&](int d, int u) { // elements 32 d + lane % 32 of rows 16 u + 8 (j / 4) + 4 hl + j % 4
+                h8_t v;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int row = u * 16 + half * 8 + tr_row;
+                    const h4_t x = read_transposed(vs + row * L::kRow + L::value_piece(row, d * 4 + tr_piece) * 16 + tr_byte);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        v[half * 4 + k] = x[k];
+                }
+                return v;
+            };
             if (!careful) {
 #pragma unroll
-                for (int d = 0; d < DT; ++d)
+                for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        o[d] = mfma32(*reinterpret_cast<const h8_t*>(vs + value_offset(d * 32 + l31, u * 2 + hl)), p[u], o[d]);
+                    for (int d = 0; d < DT; ++d)
+                        o[d] = mfma32(values(d, u), p[u], o[d]);
             } else { // row by row, each kept only by the columns that attend it
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
@@ -523,7 +562,7 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
                         const int e = (x & 1) * 4 + ((x >> 1) & 3); // its element in the lanes of half x / 8
 #pragma unroll
                         for (int d = 0; d < DT; ++d) {
-                            u32x4 w = *reinterpret_cast<const u32x4*>(vs + value_offset(d * 32 + l31, u * 2 + hl));
+                            u32x4 w = __builtin_bit_cast(u32x4, values(d, u));
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
                                 w[k] &= hl == (x >> 3) && k == (e >> 1) ? ((e & 1) ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
@@ -572,14 +611,6 @@ template <int TILE>
 __device__ __forceinline__ int first_tile(const BatchAttnArgs& a, int start, int request)
 {
     return start * a.group / TILE + request;
-}
-
-// One value for the whole wavefront, through the scalar cache: it does not queue behind the cache rows that the vector
-// memory path is busy with.
-__device__ __forceinline__ int uniform_load(const int* p, int i)
-{
-    typedef const int __attribute__((address_space(4))) * Scalar;
-    return ((Scalar)p)[__builtin_amdgcn_readfirstlane(i)];
 }
 
 __device__ __forceinline__ int request_start(const BatchAttnArgs& a, int request)
@@ -806,7 +837,9 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
     a.group = group;
     a.out_stride = output_stride;
     a.q_stride = query_stride;
-    a.scale = scale * 1.44269504088896340736f; // powers of two below
+    // powers of two from here on; never 0, which would make NaN of a score that is masked with -infinity
+    a.scale = fmaxf(fabsf(scale) * 1.44269504088896340736f, 1.17549435e-38f);
+    a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
     a.shared_tiles = p.shared_tiles;
     a.shared_splits = p.shared_splits;
     a.shared_piece = p.shared_piece;
