@@ -42,8 +42,8 @@ struct BatchAttnArgs {
     int n_blocks, shift, n_kv_heads, group, out_stride, q_stride;
     float scale; // its absolute value times log2(e), positive
     uint32_t q_sign; // what turns the queries over where the scale is negative
-    // items: [shared_splits x n_kv_heads][shared_tiles], then [own_splits][own_tiles][n_kv_heads]
-    int shared_tiles, shared_splits, shared_piece;
+    // items: [shared_splits x n_kv_heads, by eights][shared_tiles][of the eight], and [own_splits][own_tiles][n_kv_heads]
+    int shared_items, shared_tiles, shared_splits, shared_piece;
     int own_items, own_tiles, own_piece, own_prefix; // own_prefix: prefix rows in front of a request's own, a multiple of kPass, or 0
 };
 
@@ -51,6 +51,7 @@ struct BatchAttnArgs {
 struct Item {
     int token, row0, rows, kv_head; // column c: query head kv_head * group + (row0 + c) % group of token `token` + (row0 + c) / group
     int tokens;                 // that the columns belong to
+    int least;                  // own rows that all columns attend
     int p0, p1;                 // shared rows
     int r0, r1;                 // own rows
     const int* table;           // of the own rows
@@ -71,12 +72,12 @@ __device__ __forceinline__ float max_xor32(float v)
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-__device__ __forceinline__ int row16_min(int v)
+// One value for the whole wavefront, through the scalar cache: it does not queue behind the cache rows that the vector
+// memory path is busy with.
+__device__ __forceinline__ int uniform_load(const int* p, int i)
 {
-#pragma unroll
-    for (int x = 1; x < 16; x <<= 1)
-        v = min(v, __shfl_xor(v, x, 64));
-    return v;
+    typedef const int __attribute__((address_space(4))) * Scalar;
+    return ((Scalar)p)[__builtin_amdgcn_readfirstlane(i)];
 }
 
 // Own rows that a token at position p attends.
@@ -98,6 +99,12 @@ template <int D>
 __device__ __forceinline__ const uint16_t* row_address(const BatchAttnArgs& a, const uint16_t* cache, int block, int row, int kv_head)
 {
     return cache + block * a.block_stride + ((row & ((1 << a.shift) - 1)) * a.n_kv_heads + kv_head) * static_cast<long long>(D);
+}
+
+// What an infinite or NaN value adds to a sum that it is a part of.
+__device__ __forceinline__ float special_part(uint16_t h)
+{
+    return (h & 0x7C00u) == 0x7C00u ? half_bits_to_float(h) : 0.0f;
 }
 
 __device__ __forceinline__ bool in_cache(const BatchAttnArgs& a, int block)
@@ -129,7 +136,7 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
     const int token = it.token + (it.row0 + r) / a.group, head = it.kv_head * a.group + (it.row0 + r) % a.group;
     const int position = a.positions[token];
     const int limit = own_rows_of(a, position);
-    const int least = it.tokens > 1 ? row16_min(limit) : limit; // of all columns
+    const int least = it.least;
     h8_t qf[KS];
 #pragma unroll
     for (int j = 0; j < KS; ++j)
@@ -230,8 +237,10 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
                     sum += e;
                     p[4 * t + i] = static_cast<_Float16>(e);
                 }
-            bool careful = false;
-            if (!whole) { // what lies behind the last row, or in a block that is none, must not reach a sum through a 0
+            bool special = false;
+            if (!whole) {
+                // What lies behind the last row, or in a block that is none, and what is infinite or NaN in rows that some
+                // columns attend and others do not, must not reach a sum through a probability of 0.
                 uint32_t bad = 0;
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -240,40 +249,33 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
                         const bool keep = tb + 16 * t + 4 * g + i < end && ok[t];
 #pragma unroll
                         for (int k = 0; k < VW; ++k) {
-                            vr[4 * t + i][k] = keep ? vr[4 * t + i][k] : 0u;
-                            bad |= not_finite(vr[4 * t + i][k]);
+                            const uint32_t v = keep ? vr[4 * t + i][k] : 0u, b = not_finite(v);
+                            vr[4 * t + i][k] = v & ~((b >> 15) * 0xFFFFu);
+                            bad |= b;
                         }
                     }
-                careful = __any(bad != 0);
+                special = __any(bad != 0);
             }
-            if (!careful) {
 #pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    u32x4 w;
+            for (int i = 0; i < VE; ++i) {
+                u32x4 w;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        w[k] = __builtin_amdgcn_perm(vr[2 * k + 1][i >> 1], vr[2 * k][i >> 1], (i & 1) ? 0x07060302u : 0x05040100u);
-                    o[i] = mfma16(__builtin_bit_cast(h8_t, w), p, o[i]);
-                }
-            } else { // row by row, each kept only by the columns that attend it
-                for (int u = 0; u < 32; ++u) {
-                    const bool keep = tb + u < seen;
-                    const int e = (u >> 4) * 4 + (u & 3); // its element in the lanes of group (u / 4) % 4
+                for (int k = 0; k < 4; ++k)
+                    w[k] = __builtin_amdgcn_perm(vr[2 * k + 1][i >> 1], vr[2 * k][i >> 1], (i & 1) ? 0x07060302u : 0x05040100u);
+                o[i] = mfma16(__builtin_bit_cast(h8_t, w), p, o[i]);
+            }
+            if (special) // to the columns that attend them
+                for (int row = tb; row < min(tb + 32, end); ++row) {
+                    const int block = uniform_load(table, row >> a.shift);
+                    if (!in_cache(a, block))
+                        continue;
+                    const uint16_t* v = row_address<D>(a, a.value, block, row, it.kv_head);
 #pragma unroll
-                    for (int i = 0; i < VE; ++i) {
-                        u32x4 w;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            w[k] = __builtin_amdgcn_perm(vr[2 * k + 1][i >> 1], vr[2 * k][i >> 1], (i & 1) ? 0x07060302u : 0x05040100u);
-                            w[k] &= g == ((u >> 2) & 3) && k == (e >> 1) ? ((e & 1) ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
-                        }
-                        const f4_t x = mfma16(__builtin_bit_cast(h8_t, w), p, f4_t{});
+                    for (int i = 0; i < VE; ++i)
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            o[i][k] = keep ? o[i][k] + x[k] : o[i][k];
-                    }
+                            o[i][k] += row < seen ? special_part(v[(g * 4 + k) * VE + i]) : 0.0f;
                 }
-            }
         }
     }
     sum = add_xor32(add_xor16(sum));
@@ -355,14 +357,6 @@ __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, u
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "{m0}"(lds), "v"(offset), "s"(base) : "memory");
 }
 
-// One value for the whole wavefront, through the scalar cache: it does not queue behind the cache rows that the vector
-// memory path is busy with.
-__device__ __forceinline__ int uniform_load(const int* p, int i)
-{
-    typedef const int __attribute__((address_space(4))) * Scalar;
-    return ((Scalar)p)[__builtin_amdgcn_readfirstlane(i)];
-}
-
 typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ h4_t read_transposed(const char* p)
 {
@@ -405,7 +399,7 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
     constexpr int AT_ONCE = 1024 / L::kRow, LOADS = 8 / AT_ONCE; // rows per load, loads per 8 rows
     const uint32_t row_bytes = static_cast<uint32_t>(a.n_kv_heads) * D * 2;
     const int in_load = lane / L::kPieces, piece = lane % L::kPieces;
-    int* const flags = reinterpret_cast<int*>(lds + L::kFlags); // [buffer][wavefront]: which of its blocks are none
+    int* const flags = reinterpret_cast<int*>(lds + L::kFlags); // [buffer][wavefront]: bits 0, 1: which of its blocks are none, 2: not finite
     const uint32_t lds_base = __builtin_amdgcn_readfirstlane(
         static_cast<int>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds)));
     // address of the values that a lane reads transposed: row (lane / 16 / 2) * 4 + lane % 16 / 4 of 8, elements lane / 16 % 2 * 16 + lane % 4 * 4
@@ -417,6 +411,7 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
         if (begin >= end)
             continue;
         const int seen = seg ? limit : end, all_see = seg ? least : end, any_sees = seg ? most_rows : end;
+        const int wg_all_see = min(seg ? it.least : end, end);
         const int last8 = (end - 1) & ~7;
         auto block_of = [&](int row) { return uniform_load(table, min(row, last8) >> a.shift); };
         int block[2]; // of the pass that is requested next
@@ -454,16 +449,30 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
             char* const ks = lds + buffer * L::kBuffer;
             char* const vs = ks + L::kTensor;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // this wavefront's share of the pass lies in LDS
-            if (no_block || tb + wave * 16 + 16 > end) {
-                // What lies behind the last row, or in a block that is none, must not reach a sum through a probability of 0.
+            int found = 0;
+            if (no_block || tb + kPass > wg_all_see) {
+                // What lies behind the last row, or in a block that is none, and what is infinite or NaN in rows that some
+                // columns attend and others do not, must not reach a sum through a probability of 0.
                 for (int x = lane; x < 16 * L::kPieces; x += 64) {
                     const int row = x / L::kPieces;
+                    u32x4* at = reinterpret_cast<u32x4*>(vs + (wave * 16 + row) * L::kRow + x % L::kPieces * 16);
+                    u32x4 v = *at;
                     if (tb + wave * 16 + row >= end || ((no_block >> (row >> 3)) & 1))
-                        *reinterpret_cast<u32x4*>(vs + (wave * 16 + row) * L::kRow + x % L::kPieces * 16) = u32x4{};
+                        v = u32x4{};
+                    uint32_t bad = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t b = not_finite(v[k]);
+                        v[k] &= ~((b >> 15) * 0xFFFFu);
+                        bad |= b;
+                    }
+                    *at = v;
+                    found |= bad ? 4 : 0;
                 }
+                found = __any(found) ? 4 : 0;
             }
             if (lane == 0)
-                flags[buffer * 4 + wave] = no_block;
+                flags[buffer * 4 + wave] = no_block | found;
             __syncthreads(); // everybody's share does, and the other buffer has been read
             if (tb + kPass < end) {
                 no_block = (!in_cache(a, block[0]) ? 1 : 0) | (!in_cache(a, block[1]) ? 2 : 0);
@@ -472,11 +481,15 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
             }
             if (idle || tb >= any_sees)
                 continue;
-            int no_rows = 0; // a bit per 8 rows
+            int no_rows = 0, said = 0; // no_rows: a bit per 8 rows
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-                no_rows |= flags[buffer * 4 + w] << (2 * w);
+            for (int w = 0; w < 4; ++w) {
+                const int f = flags[buffer * 4 + w];
+                no_rows |= (f & 3) << (2 * w);
+                said |= f;
+            }
             no_rows = __builtin_amdgcn_readfirstlane(no_rows);
+            said = __builtin_amdgcn_readfirstlane(said);
 
             f16v_t s[2] = {};
 #pragma unroll
@@ -525,17 +538,6 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
                     p[u][i + 1] = e[1];
                     sum = dot2(as_u32(e), 0x3C003C00u, sum); // of the rounded ones, in fp32
                 }
-            bool careful = false; // an infinite or NaN value that some columns attend and others do not
-            if (tb + kPass > all_see) {
-                uint32_t bad = 0;
-                for (int x = lane; x < kPass * L::kPieces; x += 64) {
-                    const u32x4 v = *reinterpret_cast<const u32x4*>(vs + x * 16);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        bad |= not_finite(v[k]);
-                }
-                careful = __any(bad != 0);
-            }
             auto values = [&](int d, int u) { // elements 32 d + lane % 32 of rows 16 u + 8 (j / 4) + 4 hl + j % 4
                 h8_t v;
 #pragma unroll
@@ -548,31 +550,23 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
                 }
                 return v;
             };
-            if (!careful) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    o[d] = mfma32(values(d, u), p[u], o[d]);
+            if (said & 4) // values that are not finite, taken out above: to the columns that attend them
+                for (int row = tb; row < min(tb + kPass, end); ++row) {
+                    const int block_id = uniform_load(table, row >> a.shift);
+                    if (!in_cache(a, block_id))
+                        continue;
+                    const uint16_t* v = row_address<D>(a, a.value, block_id, row, it.kv_head) + 4 * hl;
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
-                        o[d] = mfma32(values(d, u), p[u], o[d]);
-            } else { // row by row, each kept only by the columns that attend it
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    for (int x = 0; x < 16; ++x) {
-                        const bool keep = tb + u * 16 + (x & 1) * 8 + (x >> 3) * 4 + ((x >> 1) & 3) < seen;
-                        const int e = (x & 1) * 4 + ((x >> 1) & 3); // its element in the lanes of half x / 8
-#pragma unroll
-                        for (int d = 0; d < DT; ++d) {
-                            u32x4 w = __builtin_bit_cast(u32x4, values(d, u));
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                w[k] &= hl == (x >> 3) && k == (e >> 1) ? ((e & 1) ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
-                            const f16v_t y = mfma32(__builtin_bit_cast(h8_t, w), p[u], f16v_t{});
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                o[d][i] = keep ? o[d][i] + y[i] : o[d][i];
-                        }
-                    }
-            }
+                        for (int x = 0; x < 16; ++x)
+                            o[d][x] += row < seen ? special_part(v[d * 32 + 8 * (x >> 2) + (x & 3)]) : 0.0f;
+                }
         }
     }
     sum += __shfl_xor(sum, 32, 64);
@@ -629,14 +623,17 @@ __global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttn
     constexpr int kTileRows = MANY ? kManyRows : kFewRows;
     __shared__ __align__(16) char lds[MANY ? kAttnLds<D> : kFewLds<D>];
     Item it = {};
-    const int shared_items = a.shared_tiles * a.shared_splits * a.n_kv_heads;
+    const int shared_items = a.shared_items;
     // Wide tiles of shared rows first, they take longest; narrow ones last, to fill up what long requests leave idle (64
     // conversations 133 -> 125 us).
     int index = blockIdx.x;
     if (!MANY)
         index = index < a.own_items ? index + shared_items : index - a.own_items;
     if (index < shared_items) {
-        const int tile = index % a.shared_tiles, rest = index / a.shared_tiles;
+        // The tiles of a piece to one XCD: they read the same rows.
+        const int eight = index / (8 * a.shared_tiles), tile = index % (8 * a.shared_tiles) / 8, rest = eight * 8 + index % 8;
+        if (rest >= a.shared_splits * a.n_kv_heads)
+            return;
         it.kv_head = rest % a.n_kv_heads;
         it.slot = rest / a.n_kv_heads;
         it.p0 = it.slot * a.shared_piece;
@@ -648,9 +645,10 @@ __global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttn
         index -= shared_items;
         const int of_heads = index / a.n_kv_heads;
         const int tile = of_heads % a.own_tiles, split = of_heads / a.own_tiles;
-        // The workgroups of an XCD (every eighth) take all heads in turn: the rows of one head alone lie in few of its L2's
-        // channels.
-        it.kv_head = (index + of_heads) % a.n_kv_heads;
+        // An XCD gets every eighth workgroup.  Wide tiles: a head's tiles all go to one, whose L2 then serves the rows to
+        // all of them.  Narrow ones read every row once: an XCD takes all heads in turn, because the rows of one head
+        // alone lie in few channels of its L2.
+        it.kv_head = (MANY ? index : index + of_heads) % a.n_kv_heads;
         // The request: the one it would be if all brought one token, else by counting, 64 at a time.
         int request = min(((tile + 1) * kTileRows - 1) / (kTileRows + a.group), a.n_requests - 1);
         int start = request_start(a, request), stop = request_start(a, request + 1);
@@ -674,13 +672,21 @@ __global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttn
         const int t0 = start + it.row0 / a.group, t1 = start + (it.row0 + it.rows - 1) / a.group;
         it.tokens = t1 - t0 + 1;
         int most = own_rows_of(a, uniform_load(a.positions, t1));
+        it.least = most;
         if (it.tokens > 1) {
-            for (int t = t0 + static_cast<int>(threadIdx.x & 63); t <= t1; t += 64)
-                most = max(most, own_rows_of(a, a.positions[t]));
+            int fewest = -most;
+            for (int t = t0 + static_cast<int>(threadIdx.x & 63); t <= t1; t += 64) {
+                const int own = own_rows_of(a, a.positions[t]);
+                most = max(most, own);
+                fewest = max(fewest, -own);
+            }
 #pragma unroll
-            for (int x = 1; x < 64; x <<= 1)
+            for (int x = 1; x < 64; x <<= 1) {
                 most = max(most, __shfl_xor(most, x, 64));
+                fewest = max(fewest, __shfl_xor(fewest, x, 64));
+            }
             most = __builtin_amdgcn_readfirstlane(most);
+            it.least = -__builtin_amdgcn_readfirstlane(fewest);
         }
         const int from = split * a.own_piece, to = from + a.own_piece; // of the shared rows in front and its own
         if (a.own_prefix) {
@@ -843,7 +849,8 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
     a.shared_tiles = p.shared_tiles;
     a.shared_splits = p.shared_splits;
     a.shared_piece = p.shared_piece;
-    a.own_items = static_cast<int>(items) - p.shared_tiles * p.shared_splits * a.n_kv_heads;
+    a.shared_items = static_cast<int>(p.shared_items(a.n_kv_heads));
+    a.own_items = static_cast<int>(items) - a.shared_items;
     a.own_tiles = p.own_tiles;
     a.own_piece = p.own_piece;
     a.own_prefix = p.own_prefix;

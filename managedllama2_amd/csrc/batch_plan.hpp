@@ -181,10 +181,9 @@ struct BatchAttnPlan {
     int own_tiles = 0, own_splits = 1, own_piece = kPass;
     int own_prefix = 0; // prefix rows in front of a request's own, a multiple of kPass; 0: none, or shared
     int slots() const { return shared_splits + own_splits; }
-    long long items(int n_kv_heads) const
-    {
-        return (static_cast<long long>(shared_tiles) * shared_splits + static_cast<long long>(own_tiles) * own_splits) * n_kv_heads;
-    }
+    // (piece, key/value head) pairs by eights, one for each XCD
+    long long shared_items(int n_kv_heads) const { return (static_cast<long long>(shared_splits) * n_kv_heads + 7) / 8 * 8 * shared_tiles; }
+    long long items(int n_kv_heads) const { return shared_items(n_kv_heads) + static_cast<long long>(own_tiles) * own_splits * n_kv_heads; }
 };
 
 // Pieces of `rows` cache rows, for `items` of them in each piece: enough that every compute unit has 4 workgroups, but
