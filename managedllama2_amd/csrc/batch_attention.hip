@@ -37,6 +37,8 @@ struct BatchAttnArgs {
     const int* positions;
     float* parts; // [slot][token][head][D] sums, then (maximum, denominator) of each; null: one piece, straight to `out`
     float2* stats;
+    unsigned* counters; // [token][key/value head], zero between launches: pieces are joined by whoever leaves the last one; or null
+    uint32_t parts_bytes;
     long long block_stride;
     int n_requests, n_tokens, table_stride, prefix_length, max_rows;
     int n_blocks, shift, n_kv_heads, group, out_stride, q_stride;
@@ -56,6 +58,7 @@ struct Item {
     int r0, r1;                 // own rows
     const int* table;           // of the own rows
     int slot;
+    int split;                  // which piece of the own rows, -1: of the shared ones
 };
 
 __device__ __forceinline__ f4_t mfma16(h8_t x, h8_t y, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
@@ -119,6 +122,65 @@ __device__ __forceinline__ h8_t load_query(const BatchAttnArgs& a, int token, in
     for (int k = 0; k < 4; ++k)
         v[k] ^= a.q_sign;
     return __builtin_bit_cast(h8_t, v);
+}
+
+// ---------------------------------------------------------------- joining pieces
+template <int D>
+__device__ __forceinline__ void store_joined(const BatchAttnArgs& a, int token, int head, int x, float sum, const float (&o)[8])
+{
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        w[k] = static_cast<uint32_t>(float_to_half_bits(o[2 * k] * inv)) | static_cast<uint32_t>(float_to_half_bits(o[2 * k + 1] * inv)) << 16;
+    *reinterpret_cast<u32x4*>(a.out + static_cast<size_t>(token) * a.out_stride + head * D + x * 8) = w;
+}
+
+// What the groups of D / 8 lanes of a wavefront have, as one.
+template <int D>
+__device__ __forceinline__ void join_lanes(const BatchAttnArgs& a, int token, int head, float m, float sum, float (&o)[8])
+{
+    constexpr int SIDE = D / 8;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = SIDE; d < 64; d <<= 1) {
+        const float om = __shfl_xor(m, d, 64), most = fmaxf(m, om), wa = weight_of(m, most), wb = weight_of(om, most);
+        const bool lower = (lane & d) == 0; // the same order of the two terms on both sides
+        const float os = __shfl_xor(sum, d, 64);
+        sum = lower ? fmaf(wb, os, sum * wa) : fmaf(wa, sum, os * wb);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float ov = __shfl_xor(o[i], d, 64);
+            o[i] = lower ? fmaf(wb, ov, o[i] * wa) : fmaf(wa, o[i], ov * wb);
+        }
+        m = most;
+    }
+    if (lane < SIDE)
+        store_joined<D>(a, token, head, lane, sum, o);
+}
+
+// One token's head by a wavefront: D / 8 lanes side by side (8 elements each), the others with every 512 / D-th piece.
+template <int D>
+__device__ void join_pieces(const BatchAttnArgs& a, int token, int head, __amdgpu_buffer_rsrc_t parts)
+{
+    constexpr int SIDE = D / 8, DEEP = 64 / SIDE;
+    const int lane = threadIdx.x & 63, x = lane % SIDE, deep = lane / SIDE;
+    const int heads = a.n_kv_heads * a.group, rows = a.n_tokens * heads;
+    const int slots = a.shared_splits + (a.own_prefix + own_rows_of(a, a.positions[token]) + a.own_piece - 1) / a.own_piece;
+    float m = -INFINITY, sum = 0.0f, o[8] = {};
+    for (int s = deep; s < slots; s += DEEP) {
+        const int part = s * rows + token * heads + head; // parts_bytes < 2^31
+        const float pm = load_agent(&a.stats[part].x), ps = load_agent(&a.stats[part].y);
+        const u32x4 v0 = __builtin_amdgcn_raw_buffer_load_b128(parts, (part * D + x * 8) * 4, 0, kAuxAgent);
+        const u32x4 v1 = __builtin_amdgcn_raw_buffer_load_b128(parts, (part * D + x * 8) * 4 + 16, 0, kAuxAgent);
+        const float most = fmaxf(m, pm), wa = weight_of(m, most), wb = weight_of(pm, most);
+        m = most;
+        sum = fmaf(wb, ps, sum * wa);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            o[i] = fmaf(wb, __uint_as_float(i < 4 ? v0[i] : v1[i - 4]), o[i] * wa);
+    }
+    join_lanes<D>(a, token, head, m, sum, o);
 }
 
 // ---------------------------------------------------------------- few columns
@@ -280,12 +342,16 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
     }
     sum = add_xor32(add_xor16(sum));
 
-    // The four wavefronts' sums through LDS, then each adds up a quarter of the elements.
+    // The four wavefronts' sums through LDS, then each adds up a quarter of the elements: those with k == wave, which are
+    // VE neighbours in each lane.
+    constexpr int QUADS = VE / 4;
     f4_t* all = reinterpret_cast<f4_t*>(lds);
     float2* stat = reinterpret_cast<float2*>(lds + 4 * VE * 64 * 16);
 #pragma unroll
-    for (int i = 0; i < VE; ++i)
-        all[(wave * VE + i) * 64 + lane] = o[i];
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int x = 0; x < QUADS; ++x)
+            all[((wave * 4 + k) * QUADS + x) * 64 + lane] = f4_t{o[4 * x][k], o[4 * x + 1][k], o[4 * x + 2][k], o[4 * x + 3][k]};
     if (g == 0)
         stat[wave * 16 + c] = float2{m, sum};
     __syncthreads();
@@ -299,39 +365,76 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
         weight[w] = weight_of(st.x, most);
         total = fmaf(weight[w], st.y, total);
     }
-    if (c >= it.rows || position < 0)
-        return;
-    const size_t row = static_cast<size_t>(token) * a.n_kv_heads * a.group + head;
-    const size_t part = (static_cast<size_t>(it.slot) * a.n_tokens * a.n_kv_heads * a.group + row);
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    constexpr int PER = VE / 4; // elements of this wavefront: wave * PER ..
-    float e[PER][4];
+    f4_t e[QUADS];
 #pragma unroll
-    for (int x = 0; x < PER; ++x) {
-        f4_t v = {};
+    for (int x = 0; x < QUADS; ++x) {
+        e[x] = f4_t{};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const f4_t y = all[(w * VE + wave * PER + x) * 64 + lane];
+            const f4_t y = all[((w * 4 + wave) * QUADS + x) * 64 + lane];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                v[k] = fmaf(weight[w], y[k], v[k]);
+                e[x][k] = fmaf(weight[w], y[k], e[x][k]);
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            e[x][k] = v[k];
     }
+    const bool live = c < it.rows && position >= 0;
+    const int rows = a.n_tokens * a.n_kv_heads * a.group, d = (g * 4 + wave) * VE; // rows < 2^29
+    const size_t part = static_cast<size_t>(it.slot) * rows + static_cast<size_t>(token) * a.n_kv_heads * a.group + head;
+    if (live && !a.parts) {
+        typedef _Float16 Halfs __attribute__((ext_vector_type(VE)));
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        Halfs h;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+        for (int x = 0; x < VE; ++x)
+            h[x] = __builtin_bit_cast(_Float16, float_to_half_bits(e[x / 4][x % 4] * inv));
+        *reinterpret_cast<Halfs*>(a.out + static_cast<size_t>(token) * a.out_stride + head * D + d) = h;
+    }
+    if (live && a.parts) {
 #pragma unroll
-        for (int x = 0; x < PER; ++x) {
-            const int d = (g * 4 + k) * VE + wave * PER + x;
-            if (a.parts)
-                a.parts[part * D + d] = e[x][k];
+        for (int x = 0; x < QUADS; ++x) {
+            float* to = a.parts + part * D + d + 4 * x;
+            if (a.counters) // written through, for the workgroup that joins the pieces in this launch
+                asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(to), "v"(e[x]) : "memory");
             else
-                a.out[static_cast<size_t>(token) * a.out_stride + head * D + d] = float_to_half_bits(total == 0.0f ? 0.0f : e[x][k] * inv);
+                *reinterpret_cast<f4_t*>(to) = e[x];
         }
-    if (a.parts && wave == 0 && g == 0)
-        a.stats[part] = float2{most, total};
+        if (wave == 0 && g == 0) {
+            store_agent(&a.stats[part].x, most);
+            store_agent(&a.stats[part].y, total);
+        }
+    }
+    if (!a.counters)
+        return;
+
+    // Tokens whose last piece this was (their columns lie in one tile each: the group divides 16).
+    wait_agent_stores();
+    __syncthreads();
+    unsigned* const done = reinterpret_cast<unsigned*>(lds);
+    if (wave == 0) {
+        bool last = false;
+        if (lane * a.group < it.rows) {
+            const int t = it.token + it.row0 / a.group + lane, p = a.positions[t];
+            const int pieces = (a.own_prefix + own_rows_of(a, p) + a.own_piece - 1) / a.own_piece;
+            if (p >= 0 && it.split < pieces) {
+                unsigned* const counter = a.counters + t * a.n_kv_heads + it.kv_head;
+                last = add_agent(counter, 1) + 1 == static_cast<unsigned>(a.shared_splits + pieces);
+                if (last)
+                    store_agent(counter, 0);
+            }
+        }
+        const unsigned mask = static_cast<unsigned>(__ballot(last));
+        if (lane == 0)
+            *done = mask;
+    }
+    __syncthreads();
+    unsigned left = __builtin_amdgcn_readfirstlane(*done);
+    const __amdgpu_buffer_rsrc_t parts = make_rsrc(a.parts, a.parts_bytes);
+    for (int k = 0; left; left &= left - 1)
+        for (int h = 0; h < a.group; ++h, ++k)
+            if ((k & 3) == wave) {
+                const int t = it.token + it.row0 / a.group + __builtin_ctz(left);
+                join_pieces<D>(a, t, it.kv_head * a.group + h, parts);
+            }
 }
 
 // ---------------------------------------------------------------- many columns
@@ -641,6 +744,7 @@ __global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttn
         it.row0 = tile * kTileRows;
         it.rows = min(a.n_tokens * a.group - it.row0, kTileRows);
         it.tokens = 1; // all see the same rows
+        it.split = -1;
     } else {
         index -= shared_items;
         const int of_heads = index / a.n_kv_heads;
@@ -696,6 +800,7 @@ __global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttn
         it.r0 = max(from - a.own_prefix, 0);
         it.r1 = min(max(to - a.own_prefix, 0), most);
         it.slot = a.shared_splits + split;
+        it.split = split;
         it.table = a.block_tables + static_cast<size_t>(request) * a.table_stride;
         if (it.p0 >= it.p1 && it.r0 >= it.r1 && a.parts)
             return;
@@ -709,22 +814,21 @@ __global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttn
     few_rows<D>(a, it, lds);
 }
 
-// Joins the pieces of a token's head, in order: LANES lanes per row, D / 8 of them side by side (8 elements each), the
-// others with every LANES * 8 / D-th piece.
+// Joins the pieces of a token's head, in order, where no workgroup of the attention does: LANES lanes per row, D / 8 of
+// them side by side (8 elements each), the others with every LANES * 8 / D-th piece.
 template <int D, int LANES>
 __global__ __launch_bounds__(256) void batch_attn_merge_kernel(BatchAttnArgs a)
 {
     constexpr int SIDE = D / 8, DEEP = LANES / SIDE;
     __shared__ float lds[LANES > 64 ? DEEP * SIDE * 8 : 1];
     __shared__ float2 stat[LANES > 64 ? DEEP : 1];
-    const int rows = a.n_tokens * a.n_kv_heads * a.group; // < 2^31: checked on the host
+    const int heads = a.n_kv_heads * a.group, rows = a.n_tokens * heads; // < 2^29: checked on the host
     const int row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     const int lane = threadIdx.x % LANES, x = lane % SIDE, deep = lane / SIDE;
-    const int token = min(row, rows - 1) / (a.n_kv_heads * a.group), head = row % (a.n_kv_heads * a.group);
+    const int token = min(row, rows - 1) / heads, head = row % heads;
     if (row >= rows || a.positions[token] < 0)
         return; // a whole wavefront at least, the whole workgroup where it has barriers
-    const int own = own_rows_of(a, a.positions[token]);
-    const int slots = a.shared_splits + (a.own_prefix + own + a.own_piece - 1) / a.own_piece;
+    const int slots = a.shared_splits + (a.own_prefix + own_rows_of(a, a.positions[token]) + a.own_piece - 1) / a.own_piece;
     float m = -INFINITY, sum = 0.0f, o[8] = {};
     for (int s = deep; s < slots; s += DEEP) {
         const size_t part = static_cast<size_t>(s) * rows + row;
@@ -740,19 +844,7 @@ __global__ __launch_bounds__(256) void batch_attn_merge_kernel(BatchAttnArgs a)
             o[i] = fmaf(wb, v[i], o[i] * wa);
     }
     if constexpr (LANES == 64) {
-#pragma unroll
-        for (int d = SIDE; d < 64; d <<= 1) {
-            const float om = __shfl_xor(m, d, 64), most = fmaxf(m, om), wa = weight_of(m, most), wb = weight_of(om, most);
-            const bool lower = (lane & d) == 0; // the same order of the two terms on both sides
-            const float os = __shfl_xor(sum, d, 64);
-            sum = lower ? fmaf(wb, os, sum * wa) : fmaf(wa, sum, os * wb);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float ov = __shfl_xor(o[i], d, 64);
-                o[i] = lower ? fmaf(wb, ov, o[i] * wa) : fmaf(wa, o[i], ov * wb);
-            }
-            m = most;
-        }
+        join_lanes<D>(a, token, head, m, sum, o);
     } else {
         if (x == 0)
             stat[deep] = float2{m, sum};
@@ -775,15 +867,8 @@ __global__ __launch_bounds__(256) void batch_attn_merge_kernel(BatchAttnArgs a)
             for (int i = 0; i < 8; ++i)
                 o[i] = fmaf(w, lds[(i * DEEP + d) * SIDE + x], o[i]);
         }
+        store_joined<D>(a, token, head, x, sum, o);
     }
-    if (deep > 0)
-        return;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    u32x4 w;
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-        w[k] = static_cast<uint32_t>(float_to_half_bits(o[2 * k] * inv)) | static_cast<uint32_t>(float_to_half_bits(o[2 * k + 1] * inv)) << 16;
-    *reinterpret_cast<u32x4*>(a.out + static_cast<size_t>(token) * a.out_stride + head * D + x * 8) = w;
 }
 
 template <int D>
@@ -793,7 +878,7 @@ static void batch_attn_launch(const BatchAttnArgs& a, bool many, int items, int 
         hipLaunchKernelGGL((batch_attn_kernel<D, true>), dim3(items), dim3(256), 0, ctx().stream, a);
     else
         hipLaunchKernelGGL((batch_attn_kernel<D, false>), dim3(items), dim3(256), 0, ctx().stream, a);
-    if (!a.parts)
+    if (!a.parts || a.counters)
         return;
     const int rows = a.n_tokens * a.n_kv_heads * a.group;
     if (slots <= 16)
@@ -860,6 +945,13 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
             return rc;
         a.parts = ctx().attn_partials;
         a.stats = reinterpret_cast<float2*>(a.parts + part * cache->head_size);
+        // Joined in the same launch: few pieces of few columns, which one wavefront per column has done sooner than another
+        // launch begins.
+        const size_t bytes = part * cache->head_size * sizeof(float);
+        if (!p.many && p.shared_splits == 0 && p.slots() <= 16 && kFewRows % group == 0 && rows / group <= kMaxBatchCounters && bytes < (1u << 31)) {
+            a.counters = ctx().batch_counters;
+            a.parts_bytes = static_cast<uint32_t>(bytes);
+        }
     }
     if (cache->head_size == 128)
         batch_attn_launch<128>(a, p.many, static_cast<int>(items), p.slots());

@@ -41,12 +41,15 @@ struct Context {
     int n_retired_partials = 0;
     // per-head arrival counters of llama2_multi_head_attention (zero between launches)
     unsigned* attn_counters = nullptr;
+    // arrival counters of llama2_batch_attention, per token and key/value head (zero between launches)
+    unsigned* batch_counters = nullptr;
     SamplerScratch* sampler = nullptr; // between the sampler modules' launches (sampler_kernels.hpp)
     // Pinned: where a kernel leaves the token that the call behind it returns (a copy of 4 bytes is a launch of 4.3 us)
     int* host_token = nullptr;
 };
 
 constexpr int kMaxAttnHeads = 1024;
+constexpr int kMaxBatchCounters = 1 << 16;
 
 Context& ctx();
 int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));

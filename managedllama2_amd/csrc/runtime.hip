@@ -106,6 +106,8 @@ int llama2_init(int device)
     L2_HIP(hipStreamCreateWithFlags(&c.stream, hipStreamNonBlocking));
     L2_HIP(hipMalloc(reinterpret_cast<void**>(&c.attn_counters), kMaxAttnHeads * sizeof(unsigned)));
     L2_HIP(hipMemset(c.attn_counters, 0, kMaxAttnHeads * sizeof(unsigned)));
+    L2_HIP(hipMalloc(reinterpret_cast<void**>(&c.batch_counters), kMaxBatchCounters * sizeof(unsigned)));
+    L2_HIP(hipMemset(c.batch_counters, 0, kMaxBatchCounters * sizeof(unsigned)));
     L2_HIP(hipMalloc(reinterpret_cast<void**>(&c.sampler), sizeof(SamplerScratch)));
     L2_HIP(hipHostMalloc(reinterpret_cast<void**>(&c.host_token), sizeof(int), hipHostMallocMapped | hipHostMallocCoherent));
     c.device = device;
@@ -139,6 +141,9 @@ int llama2_shutdown(void)
     if (c.attn_counters)
         L2_HIP(hipFree(c.attn_counters));
     c.attn_counters = nullptr;
+    if (c.batch_counters)
+        L2_HIP(hipFree(c.batch_counters));
+    c.batch_counters = nullptr;
     if (c.sampler)
         L2_HIP(hipFree(c.sampler));
     c.sampler = nullptr;
