@@ -4,7 +4,6 @@
 #include "batch_plan.hpp"
 
 #include <cmath>
-#include <cstring>
 
 namespace l2 {
 
@@ -20,6 +19,8 @@ struct TablesArgs {
     const int* free_blocks;
     const int* taken;
     int* new_taken;
+    unsigned* arrivals; // zero between launches
+    bool apart;         // lengths and new_taken are not what is read
     int n_requests, n_tokens, table_stride, prefix_length, n_free, shift;
 };
 
@@ -44,83 +45,109 @@ __device__ __forceinline__ int block_scan(int v, int most, int* lds /* 16 */)
     return min(v + before, most);
 }
 
-// One workgroup: a block of 1024 requests at a time, lane by lane, two prefix sums (tokens, blocks); then their tokens,
-// each of which finds its request in the sums.  A new block holds at least one new token, and the one in its
-// first row writes the table entry.
+// A block of 1024 requests at a time, lane by lane, two prefix sums (tokens, blocks); then their tokens, each of which
+// finds its request in the sums.  A new block holds at least one new token, and the one in its first row writes the
+// table entry.  Latency bounds it: lengths, sums, entries and stores follow each other.
+//
+// Workgroups of several compute the same sums and take every so many thousandth token each (14579 tokens: one workgroup 15.6
+// us, 15 workgroups 7.0).  Where lengths or the number of taken blocks are updated in place, the last workgroup to have
+// read them writes them.
 __global__ __launch_bounds__(kTablesBlock) void batch_tables_kernel(TablesArgs a)
 {
     __shared__ int sums[16];
     __shared__ int begin[kTablesBlock], rows[kTablesBlock], from[kTablesBlock]; // from: first free block, -1: refused
     __shared__ int most_taken;
+    __shared__ unsigned arrived;
     const int size = 1 << a.shift, tid = threadIdx.x;
     const int limit = a.table_stride > (0x7FFFFFFF >> a.shift) ? 0x7FFFFFFF : a.table_stride << a.shift;
     const int taken = a.taken[0];
     const int left = taken >= 0 && taken <= a.n_free ? a.n_free - taken : 0;
-    if (tid == 0)
-        most_taken = 0;
-    int tokens_before = 0, need_before = 0; // both cut off one above what can be granted
-    for (int first = 0; first < a.n_requests; first += kTablesBlock) {
-        const int b = first + tid, in_block = min(a.n_requests - first, kTablesBlock);
-        const int c = b < a.n_requests ? a.cached[b] : 0, n = b < a.n_requests ? a.counts[b] : 0;
-        const int tokens = min(max(n, 0), a.n_tokens + 1);
-        const int end = min(block_scan(tokens, a.n_tokens + 1, sums) + tokens_before, a.n_tokens + 1);
-        const bool fits = b < a.n_requests && c >= 0 && n >= 0 && c <= limit && n <= limit - c && end <= a.n_tokens;
-        const int have = fits ? (c >> a.shift) + ((c & (size - 1)) != 0) : 0;
-        const int total = fits ? ((c + n) >> a.shift) + (((c + n) & (size - 1)) != 0) : 0;
-        const int need = total - have;
-        const int upto = min(block_scan(min(need, left + 1), left + 1, sums) + need_before, left + 1);
-        const bool admitted = fits && (need == 0 || upto <= left);
-        begin[tid] = end;
-        rows[tid] = c;
-        from[tid] = !admitted ? -1 : need > 0 ? taken + upto - need : 0;
-        if (admitted && need > 0)
-            atomicMax(&most_taken, upto);
-        if (b < a.n_requests) {
-            a.query_starts[b + 1] = min(end, a.n_tokens);
-            a.lengths[b] = admitted ? c + n : c;
-        }
-        if (b == 0)
-            a.query_starts[0] = 0;
-        __syncthreads();
-        const int last = min(begin[kTablesBlock - 1], a.n_tokens);
-        for (int t = min(tokens_before, a.n_tokens) + tid; t < last; t += kTablesBlock) {
-            int lo = 0, hi = in_block - 1; // the first request whose tokens end behind t
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (begin[mid] > t)
-                    hi = mid;
-                else
-                    lo = mid + 1;
+    const int every = static_cast<int>(gridDim.x) * kTablesBlock;
+    int t = static_cast<int>(blockIdx.x) * kTablesBlock + tid; // this thread's next token
+    bool lengths = gridDim.x == 1 || (a.apart && blockIdx.x == 0), starts = blockIdx.x == 0;
+    for (;;) {
+        if (tid == 0)
+            most_taken = 0;
+        int tokens_before = 0, need_before = 0; // both cut off one above what can be granted
+        for (int first = 0; first < a.n_requests; first += kTablesBlock) {
+            const int b = first + tid, in_block = min(a.n_requests - first, kTablesBlock);
+            const int c = b < a.n_requests ? a.cached[b] : 0, n = b < a.n_requests ? a.counts[b] : 0;
+            const int tokens = min(max(n, 0), a.n_tokens + 1);
+            const int end = min(block_scan(tokens, a.n_tokens + 1, sums) + tokens_before, a.n_tokens + 1);
+            const bool fits = b < a.n_requests && c >= 0 && n >= 0 && c <= limit && n <= limit - c && end <= a.n_tokens;
+            const int have = fits ? (c >> a.shift) + ((c & (size - 1)) != 0) : 0;
+            const int total = fits ? ((c + n) >> a.shift) + (((c + n) & (size - 1)) != 0) : 0;
+            const int need = total - have;
+            const int upto = min(block_scan(min(need, left + 1), left + 1, sums) + need_before, left + 1);
+            const bool admitted = fits && (need == 0 || upto <= left);
+            begin[tid] = end;
+            rows[tid] = c;
+            from[tid] = !admitted ? -1 : need > 0 ? taken + upto - need : 0;
+            if (admitted && need > 0)
+                atomicMax(&most_taken, upto);
+            if (b < a.n_requests) {
+                if (starts)
+                    a.query_starts[b + 1] = min(end, a.n_tokens);
+                if (lengths)
+                    a.lengths[b] = admitted ? c + n : c;
             }
-            const int start_of = lo ? begin[lo - 1] : tokens_before;
-            const int cb = rows[lo], f = from[lo];
-            int position = -1, slot = -1;
-            if (f >= 0) {
-                const int row = cb + (t - start_of), page = row >> a.shift;
-                const int had = (cb >> a.shift) + ((cb & (size - 1)) != 0);
-                int* entry = a.block_tables + static_cast<size_t>(first + lo) * a.table_stride + page;
-                const int block = page >= had ? a.free_blocks[f + page - had] : *entry;
-                if ((row & (size - 1)) == 0)
-                    *entry = block;
-                position = a.prefix_length + row;
-                slot = (block << a.shift) + (row & (size - 1));
+            if (b == 0 && starts)
+                a.query_starts[0] = 0;
+            if (tid == kTablesBlock - 1)
+                sums[0] = upto;
+            __syncthreads();
+            need_before = sums[0];
+            const int last = min(begin[kTablesBlock - 1], a.n_tokens);
+            for (; t < last; t += every) {
+                int lo = 0, hi = in_block - 1; // the first request whose tokens end behind t
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if (begin[mid] > t)
+                        hi = mid;
+                    else
+                        lo = mid + 1;
+                }
+                const int start_of = lo ? begin[lo - 1] : tokens_before;
+                const int cb = rows[lo], f = from[lo];
+                int position = -1, slot = -1;
+                if (f >= 0) {
+                    const int row = cb + (t - start_of), page = row >> a.shift;
+                    const int had = (cb >> a.shift) + ((cb & (size - 1)) != 0);
+                    int* entry = a.block_tables + static_cast<size_t>(first + lo) * a.table_stride + page;
+                    const int block = page >= had ? a.free_blocks[f + page - had] : *entry;
+                    if ((row & (size - 1)) == 0)
+                        *entry = block;
+                    position = a.prefix_length + row;
+                    slot = (block << a.shift) + (row & (size - 1));
+                }
+                a.positions[t] = position;
+                a.slots[t] = slot;
             }
-            a.positions[t] = position;
-            a.slots[t] = slot;
+            tokens_before = begin[kTablesBlock - 1];
+            __syncthreads();
         }
-        tokens_before = begin[kTablesBlock - 1];
-        if (tid == kTablesBlock - 1)
-            sums[0] = upto;
+        for (; t < a.n_tokens; t += every) {
+            a.positions[t] = -1;
+            a.slots[t] = -1;
+        }
+        if (lengths) {
+            if (tid == 0)
+                a.new_taken[0] = taken + most_taken;
+            return;
+        }
+        if (a.apart)
+            return;
+        if (tid == 0)
+            arrived = add_agent(a.arrivals, 1);
         __syncthreads();
-        need_before = sums[0];
+        if (arrived + 1 != gridDim.x)
+            return;
+        if (tid == 0)
+            store_agent(a.arrivals, 0u);
+        lengths = true; // once more, for the lengths alone
+        starts = false;
         __syncthreads();
     }
-    for (int t = min(tokens_before, a.n_tokens) + tid; t < a.n_tokens; t += kTablesBlock) {
-        a.positions[t] = -1;
-        a.slots[t] = -1;
-    }
-    if (tid == 0)
-        a.new_taken[0] = taken + most_taken;
 }
 
 // ---------------------------------------------------------------- norm, rotation, store
@@ -139,8 +166,19 @@ struct RopeArgs {
     long long n_slots;
     int n_heads, n_kv_heads, per, q_output_stride, q_stride, kv_stride, shift; // per: heads per workgroup
     float eps;
-    unsigned long long turns[64]; // theta^(-2 i / head_size) / 2 pi in units of 2^-64
+    unsigned long long powers[6]; // theta^(-2 i / head_size) for i = 1, 2, 4 .. 32, in units of 2^-64
 };
+
+// Turns per position of pair i, theta^(-2 i / head_size) / 2 pi, in 64 bits of fixed point: times a position, the bits above are
+// whole turns and drop out by themselves.  2^31 positions times six products off by 2^-64 each leave 2^-30 of a turn.
+__device__ __forceinline__ unsigned long long turns_of(const unsigned long long (&powers)[6], int i)
+{
+    unsigned long long v = 0x28BE60DB9391054Bull; // 1 / 2 pi
+#pragma unroll
+    for (int k = 0; k < 6; ++k)
+        v = (i >> k) & 1 ? __umul64hi(v, powers[k]) : v;
+    return v;
+}
 
 // The value of the lane that holds the other half's elements of the same pairs.
 template <int D>
@@ -203,7 +241,7 @@ __global__ __launch_bounds__(256) void batch_rope_kernel(RopeArgs a)
     if (position < 0)
         return; // the whole workgroup
     if (tid < D / 2) {
-        const int turn = static_cast<int>((static_cast<unsigned long long>(position) * a.turns[tid]) >> 32);
+        const int turn = static_cast<int>((static_cast<unsigned long long>(position) * turns_of(a.powers, tid)) >> 32);
         float s, cs;
         sincospif(static_cast<float>(turn) * 0x1p-31f, &s, &cs);
         cosines[tid] = cs;
@@ -263,25 +301,6 @@ __global__ __launch_bounds__(256) void batch_rope_kernel(RopeArgs a)
 }
 
 // ---------------------------------------------------------------- host side
-// A pair's turns per position, in 64 bits of fixed point: times a position, the bits above are whole turns and drop out
-// by themselves; 2^31 positions times the error of 2^-58 relative leave 2^-29 of a turn.  A model has one theta, so the
-// last table is kept (1.5 us to make); the caller holds the library's lock.
-static const unsigned long long* turns_of(float theta, int head_size)
-{
-    static unsigned long long turns[64];
-    static float of_theta = 0.0f;
-    static int of_size = 0;
-    if (theta != of_theta || head_size != of_size) {
-        const long double step = powl(static_cast<long double>(theta), -2.0L / head_size);
-        long double turn = 1.0L / (2.0L * 3.14159265358979323846264338327950288L) * 0x1p64L;
-        for (int i = 0; i < head_size / 2; ++i, turn *= step)
-            turns[i] = static_cast<unsigned long long>(turn);
-        of_theta = theta;
-        of_size = head_size;
-    }
-    return turns;
-}
-
 } // namespace l2
 
 using namespace l2;
@@ -296,8 +315,9 @@ int llama2_batch_tables(const llama2_batch* batch, const int* cached, const int*
         return rc;
     const llama2_batch& b = *batch;
     TablesArgs a = {b.block_tables, b.lengths, b.query_starts, b.positions, b.slots, cached, counts, free_blocks, taken,
-                    new_taken, b.n_requests, b.n_tokens, b.table_stride, b.prefix_length, n_free, log2_of(block_size)};
-    hipLaunchKernelGGL(batch_tables_kernel, dim3(1), dim3(kTablesBlock), 0, ctx().stream, a);
+                    new_taken, ctx().batch_counters + kMaxBatchCounters, b.lengths != cached && new_taken != taken, b.n_requests, b.n_tokens, b.table_stride, b.prefix_length, n_free, log2_of(block_size)};
+    const int groups = ceil_div(b.n_tokens, kTablesBlock);
+    hipLaunchKernelGGL(batch_tables_kernel, dim3(groups < 64 ? groups : 64), dim3(kTablesBlock), 0, ctx().stream, a);
     L2_LAUNCH_CHECK("llama2_batch_tables");
     return LLAMA2_OK;
 }
@@ -333,7 +353,11 @@ int llama2_batch_qk_norm_rope(llama2_half* q_output, const llama2_half* q, const
     a.kv_stride = kv_stride;
     a.shift = log2_of(cache->block_size);
     a.eps = eps;
-    memcpy(a.turns, turns_of(theta, d), sizeof(a.turns));
+    long double power = powl(static_cast<long double>(theta), -2.0L / d);
+    for (unsigned long long& p : a.powers) { // of theta 1: the largest number below 1
+        p = power >= 1.0L ? ~0ull : static_cast<unsigned long long>(power * 0x1p64L);
+        power *= power;
+    }
     // Few tokens: as few heads per workgroup as are side by side, which is quickest; many: a workgroup computes the
     // angles of a token once for all its heads.
     const int units = n_heads + 2 * a.n_kv_heads, side = 256 / (d / 8);

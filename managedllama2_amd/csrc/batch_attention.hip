@@ -83,6 +83,20 @@ __device__ __forceinline__ int uniform_load(const int* p, int i)
     return ((Scalar)p)[__builtin_amdgcn_readfirstlane(i)];
 }
 
+// Largest of the wavefront's values, the same in all lanes; by row operations, shuffles are round trips through LDS.
+__device__ __forceinline__ int wave_max_int(int v)
+{
+#define L2_MAX_STEP(ctrl, rows) v = max(v, __builtin_amdgcn_update_dpp(v, v, ctrl, rows, 0xF, false))
+    L2_MAX_STEP(DPP_QUAD_XOR1, 0xF);
+    L2_MAX_STEP(DPP_QUAD_XOR2, 0xF);
+    L2_MAX_STEP(DPP_ROW_HALF_MIRROR, 0xF);
+    L2_MAX_STEP(DPP_ROW_MIRROR, 0xF);
+    L2_MAX_STEP(DPP_ROW_BCAST15, 0xA);
+    L2_MAX_STEP(DPP_ROW_BCAST31, 0xC);
+#undef L2_MAX_STEP
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
 // Own rows that a token at position p attends.
 __device__ __forceinline__ int own_rows_of(const BatchAttnArgs& a, int p)
 {
@@ -477,21 +491,13 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
     const int r = wave * 32 + l31, rq = min(r, it.rows - 1);
     const bool idle = wave * 32 >= it.rows;
     const int token = it.token + (it.row0 + rq) / a.group, head = it.kv_head * a.group + (it.row0 + rq) % a.group;
-    const int position = a.positions[token];
-    const int limit = own_rows_of(a, position);
-    int most_rows = limit, least = -limit;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-        most_rows = max(most_rows, __shfl_xor(most_rows, x, 64));
-        least = max(least, __shfl_xor(least, x, 64));
-    }
-    most_rows = __builtin_amdgcn_readfirstlane(most_rows);
-    least = -__builtin_amdgcn_readfirstlane(least);
-
     h8_t qf[QS];
 #pragma unroll
     for (int j = 0; j < QS; ++j)
         qf[j] = load_query(a, token, head * D + j * 16 + hl * 8);
+    const int position = a.positions[token];
+    const int limit = own_rows_of(a, position);
+    const int most_rows = wave_max_int(limit), least = -wave_max_int(-limit);
     f16v_t o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -758,15 +764,18 @@ __global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttn
         int start = request_start(a, request), stop = request_start(a, request + 1);
         if (first_tile<kTileRows>(a, start, request) > tile || first_tile<kTileRows>(a, stop, request + 1) <= tile) {
             const int lane = threadIdx.x & 63;
-            request = 0; // the last one whose first tile is not behind `tile`
-            for (int first = 1; first < a.n_requests; first += 64) {
-                const int b = min(first + lane, a.n_requests);
-                request += __popcll(__ballot(b < a.n_requests &&
-                                             first_tile<kTileRows>(a, min(max(a.query_starts[b], 0), a.n_tokens), b) <= tile));
+            for (int first = 0; first < a.n_requests; first += 64) { // the last one whose first tile is not behind `tile`
+                const int b = min(first + lane, a.n_requests - 1);
+                const int from = min(max(a.query_starts[b], 0), a.n_tokens), to = min(max(a.query_starts[b + 1], 0), a.n_tokens);
+                const int n = __popcll(__ballot(first + lane < a.n_requests && first_tile<kTileRows>(a, from, b) <= tile));
+                if (n > 0) {
+                    request = first + n - 1;
+                    start = __builtin_amdgcn_readlane(from, n - 1);
+                    stop = __builtin_amdgcn_readlane(to, n - 1);
+                }
+                if (n < 64)
+                    break;
             }
-            request = __builtin_amdgcn_readfirstlane(request);
-            start = request_start(a, request);
-            stop = request_start(a, request + 1);
         }
         it.row0 = (tile - first_tile<kTileRows>(a, start, request)) * kTileRows;
         it.rows = min((stop - start) * a.group - it.row0, kTileRows);
@@ -784,13 +793,8 @@ __global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttn
                 most = max(most, own);
                 fewest = max(fewest, -own);
             }
-#pragma unroll
-            for (int x = 1; x < 64; x <<= 1) {
-                most = max(most, __shfl_xor(most, x, 64));
-                fewest = max(fewest, __shfl_xor(fewest, x, 64));
-            }
-            most = __builtin_amdgcn_readfirstlane(most);
-            it.least = -__builtin_amdgcn_readfirstlane(fewest);
+            most = wave_max_int(most);
+            it.least = -wave_max_int(fewest);
         }
         const int from = split * a.own_piece, to = from + a.own_piece; // of the shared rows in front and its own
         if (a.own_prefix) {

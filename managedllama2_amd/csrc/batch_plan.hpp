@@ -186,42 +186,55 @@ struct BatchAttnPlan {
     long long items(int n_kv_heads) const { return shared_items(n_kv_heads) + static_cast<long long>(own_tiles) * own_splits * n_kv_heads; }
 };
 
-// Pieces of `rows` cache rows, for `items` of them in each piece: enough that every compute unit has 4 workgroups, but
-// not shorter than 128 rows (one round of the 4 wavefronts; 777 rows of 32 heads: 64 rows 11.5 us, 128 9.9, 256 11.0), nor longer than `longest`.
-inline int batch_attn_piece(long long items, int rows, int longest, int cus)
+// Pieces of `rows` cache rows, for `items` of them in each piece: `want` workgroups altogether, but pieces not shorter than
+// `shortest` nor longer than `longest`.
+inline int batch_attn_piece(long long items, int rows, int shortest, int longest, long long want)
 {
-    const long long want = (4LL * cus + items - 1) / items, most = ceil_div(rows, 128), least = ceil_div(rows, longest);
-    long long n = want < most ? want : most;
+    const long long enough = (want + items - 1) / items, most = ceil_div(rows, shortest), least = ceil_div(rows, longest);
+    long long n = enough < most ? enough : most;
     n = n > least ? n : least;
     n = n < kMaxPieces ? n : kMaxPieces;
     return round_up(ceil_div(rows, static_cast<int>(n)), kPass);
 }
 
-// Sharing pays while a request has fewer than 64 columns of its own: more fill a workgroup's columns anyway, and the
-// prefix becomes the front of every request's rows.  Rows without limit for such columns (one piece unless
-// there are few items: whole prompts are bound by the matrix cores, and their sums would weigh more than the cache);
-// pieces of 1024 rows for few columns, so that a long request ends with the others (64 conversations: 512 rows 133 us, 1024
-// 133, 4096 170; four documents of up to 131000 rows: 215, 203, 218).
+// Sharing pays while a request has fewer than 64 columns of its own (more fill a workgroup's columns anyway, and the
+// prefix becomes the front of every request's rows), and where the prefix, read once more for every other request, is
+// more than joining the pieces costs: about 2^15 rows of a head.
+//
+// Narrow tiles: pieces so that every compute unit has 4 workgroups, of 128 rows at least (one round of the 4 wavefronts;
+// 777 rows of 32 heads: 64 rows 11.5 us, 128 9.9, 256 11.0) and 1024 at most, so that a long request ends with the others
+// (64 conversations: 512 rows 133 us, 1024 133, 4096 170; four documents of up to 131000 rows: 215, 203, 218).
+// Wide tiles are bound by the matrix cores, and the sums of their pieces weigh more than the cache: 2 workgroups per
+// compute unit, of 512 rows at least.
 inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int group, int max_rows, int cus)
 {
     BatchAttnPlan p;
     const long long columns = static_cast<long long>(b.n_tokens) * group;
     const bool fill = columns >= 64LL * b.n_requests;
-    const bool shared = b.prefix_length > 0 && !fill && b.n_requests > 1;
-    // Up to 128 shared columns are cheaper as tiles of 16 that read the prefix out of the L2 again: the kernel without
-    // the wide tiles has 3 wavefronts per SIMD instead of 2 (72 columns: 133 us, 140).
-    p.many = columns > static_cast<long long>(kFewRows) * b.n_requests || (shared && columns > 128);
+    const bool shared = !fill && static_cast<long long>(b.n_requests - 1) * b.prefix_length * n_kv_heads >= 1 << 15;
+    // Up to 128 shared columns are cheaper as tiles of 16 that read the prefix out of the L2 again, if that is little next to
+    // the requests' own rows: the kernel without the wide tiles has 3 wavefronts per SIMD instead of 2 (72 columns, 1024
+    // shared rows, up to 4000 own ones: 121 us, 130; 75 columns, 2558 and 84: 54, 42).
+    const long long again = (columns + kFewRows - 1) / kFewRows - 1;
+    const bool wide = columns > 128 || again * b.prefix_length * 16 > static_cast<long long>(b.n_requests) * max_rows;
+    p.many = columns > static_cast<long long>(kFewRows) * b.n_requests || (shared && wide);
     const int tile = p.many ? kManyRows : kFewRows;
     p.own_tiles = static_cast<int>(columns / tile) + b.n_requests;
     p.own_prefix = shared ? 0 : round_up(b.prefix_length, kPass);
     const int own_rows = p.own_prefix + max_rows;
-    p.own_piece = batch_attn_piece(static_cast<long long>(p.own_tiles) * n_kv_heads, own_rows, fill ? own_rows : 1024, cus);
+    const long long items = static_cast<long long>(p.own_tiles) * n_kv_heads;
+    if (fill)
+        p.own_piece = batch_attn_piece(items, own_rows, 1024, own_rows, 2LL * cus);
+    else if (p.many && items >= cus)
+        p.own_piece = batch_attn_piece(items, own_rows, 512, 1024, 4LL * cus);
+    else
+        p.own_piece = batch_attn_piece(items, own_rows, 128, 1024, p.many ? cus : 4LL * cus);
     p.own_splits = ceil_div(own_rows, p.own_piece);
     if (shared) {
         p.shared_tiles = static_cast<int>((columns + tile - 1) / tile);
-        // an eighth of the workgroups: a shared piece has more columns than an own one (16 samples behind 2048 rows: a quarter
-        // 20.8 us, an eighth 19.4)
-        p.shared_piece = batch_attn_piece(8LL * p.shared_tiles * n_kv_heads, b.prefix_length, 1024, cus);
+        // half a workgroup per compute unit: a shared piece has more columns than an own one (16 samples behind 2048 rows: a
+        // whole one 20.8 us, half a one 19.4)
+        p.shared_piece = batch_attn_piece(static_cast<long long>(p.shared_tiles) * n_kv_heads, b.prefix_length, 128, 1024, cus / 2);
         p.shared_splits = ceil_div(b.prefix_length, p.shared_piece);
     }
     return p;

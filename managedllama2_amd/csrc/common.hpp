@@ -41,7 +41,8 @@ struct Context {
     int n_retired_partials = 0;
     // per-head arrival counters of llama2_multi_head_attention (zero between launches)
     unsigned* attn_counters = nullptr;
-    // arrival counters of llama2_batch_attention, per token and key/value head (zero between launches)
+    // arrival counters of llama2_batch_attention, per token and key/value head, and of llama2_batch_tables, the last one (zero
+    // between launches)
     unsigned* batch_counters = nullptr;
     SamplerScratch* sampler = nullptr; // between the sampler modules' launches (sampler_kernels.hpp)
     // Pinned: where a kernel leaves the token that the call behind it returns (a copy of 4 bytes is a launch of 4.3 us)

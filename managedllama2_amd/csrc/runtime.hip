@@ -106,8 +106,8 @@ int llama2_init(int device)
     L2_HIP(hipStreamCreateWithFlags(&c.stream, hipStreamNonBlocking));
     L2_HIP(hipMalloc(reinterpret_cast<void**>(&c.attn_counters), kMaxAttnHeads * sizeof(unsigned)));
     L2_HIP(hipMemset(c.attn_counters, 0, kMaxAttnHeads * sizeof(unsigned)));
-    L2_HIP(hipMalloc(reinterpret_cast<void**>(&c.batch_counters), kMaxBatchCounters * sizeof(unsigned)));
-    L2_HIP(hipMemset(c.batch_counters, 0, kMaxBatchCounters * sizeof(unsigned)));
+    L2_HIP(hipMalloc(reinterpret_cast<void**>(&c.batch_counters), (kMaxBatchCounters + 1) * sizeof(unsigned)));
+    L2_HIP(hipMemset(c.batch_counters, 0, (kMaxBatchCounters + 1) * sizeof(unsigned)));
     L2_HIP(hipMalloc(reinterpret_cast<void**>(&c.sampler), sizeof(SamplerScratch)));
     L2_HIP(hipHostMalloc(reinterpret_cast<void**>(&c.host_token), sizeof(int), hipHostMallocMapped | hipHostMallocCoherent));
     c.device = device;
