@@ -123,3 +123,32 @@ class DeviceArena:
         v.copy_to_device(a)
         self.used += (a.nbytes + self.ALIGN - 1) // self.ALIGN * self.ALIGN
         return v
+
+
+class PagedCache:
+    """Keys and values of one layer in blocks of `blockSize` rows, for the operators of a step of several requests."""
+
+    def __init__(self, numBlocks, blockSize, numKVHeads, headSize):
+        self.numBlocks, self.blockSize, self.numKVHeads, self.headSize = numBlocks, blockSize, numKVHeads, headSize
+        n = numBlocks * blockSize * numKVHeads * headSize
+        self.key, self.value = DeviceVariable.zeros(np.float16, n), DeviceVariable.zeros(np.float16, n)
+
+    def struct(self):
+        return capi.PagedCache(self.key.ptr, self.value.ptr, 0, self.numBlocks, self.blockSize, self.numKVHeads, self.headSize)
+
+
+class RequestBatch:
+    """Device arrays of a step of up to `numTokens` tokens of `numRequests` requests, each of up to tableStride blocks of
+    own rows: what llama2_batch_tables writes and the other two operators read.  maxLength: a bound of the own rows."""
+
+    def __init__(self, numRequests, numTokens, tableStride, maxLength, prefixTable=None, prefixLength=0):
+        self.numRequests, self.numTokens, self.tableStride, self.maxLength = numRequests, numTokens, tableStride, maxLength
+        self.prefixTable, self.prefixLength = prefixTable, prefixLength
+        ints = lambda n: DeviceVariable.zeros(np.int32, n)  # noqa: E731
+        self.blockTables, self.lengths, self.queryStarts = ints(numRequests * tableStride), ints(numRequests), ints(numRequests + 1)
+        self.positions, self.slots, self.taken = ints(numTokens), ints(numTokens), ints(1)
+
+    def struct(self):
+        return capi.Batch(self.blockTables.ptr, self.lengths.ptr, self.queryStarts.ptr, self.positions.ptr, self.slots.ptr,
+                          self.prefixTable.ptr if self.prefixTable else None, self.numRequests, self.numTokens, self.tableStride,
+                          self.prefixLength, self.maxLength)

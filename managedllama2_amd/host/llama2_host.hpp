@@ -438,6 +438,43 @@ struct Argmax : Module { // src/Argmax.cs
     }
 };
 
+// Steps of several requests at once (no counterpart in the reference, whose cache holds one sequence): thin callers of
+// the three operators; the batch and the cache are plain structs of device pointers that the application keeps.
+struct BatchTables : Module {
+    using Module::Module;
+    // batch.lengths and `taken` count on in place
+    void Forward(const llama2_batch& batch, DeviceVariable<int>& counts, DeviceVariable<int>& freeBlocks, DeviceVariable<int>& taken,
+                 int blockSize)
+    {
+        Check(llama2_batch_tables(&batch, batch.lengths, counts.DevicePointer(), freeBlocks.DevicePointer(),
+                                  static_cast<int>(freeBlocks.Size()), taken.DevicePointer(), taken.DevicePointer(), blockSize));
+    }
+};
+
+struct BatchQKNormRoPE : Module {
+    using Module::Module;
+    // rows side by side without gaps; qGamma, kGamma: null for models that do not norm queries and keys
+    void Forward(DeviceVariable<Half>& queryOutput, DeviceVariable<Half>& query, DeviceVariable<Half>& key, DeviceVariable<Half>& value,
+                 DeviceVariable<Half>* qGamma, DeviceVariable<Half>* kGamma, const llama2_batch& batch, const llama2_paged_cache& cache,
+                 int numHeads, float theta, float eps = 1e-5f)
+    {
+        const int row = numHeads * cache.head_size, kvRow = cache.n_kv_heads * cache.head_size;
+        Check(llama2_batch_qk_norm_rope(queryOutput.DevicePointer(), query.DevicePointer(), key.DevicePointer(), value.DevicePointer(),
+                                        qGamma ? qGamma->DevicePointer() : nullptr, kGamma ? kGamma->DevicePointer() : nullptr, &batch,
+                                        &cache, numHeads, row, row, kvRow, eps, theta));
+    }
+};
+
+struct BatchAttention : Module {
+    using Module::Module;
+    void Forward(DeviceVariable<Half>& output, DeviceVariable<Half>& query, const llama2_batch& batch, const llama2_paged_cache& cache,
+                 int numHeads, float scale)
+    {
+        const int row = numHeads * cache.head_size;
+        Check(llama2_batch_attention(output.DevicePointer(), query.DevicePointer(), &batch, &cache, numHeads, row, row, scale));
+    }
+};
+
 struct Embedding : Module { // src/Embedding.cs
     using Module::Module;
     void Forward(DeviceVariable<Half>& output, DeviceVariable<Half>& table, int size, DeviceVariable<int>& tokens, int pos)

@@ -160,3 +160,34 @@ class SampleTopP(Module):
 
     def Forward(self, logits, indices, size, threshold, tokens, nextPos):
         capi.call("llama2_sample_top_p", logits.ptr, indices.ptr, size, threshold, tokens.ptr, nextPos)
+
+
+# ---- steps of several requests at once (no counterpart in the reference, whose cache holds one sequence)
+
+class BatchTables(Module):
+    """Block tables, slots and positions of a step from the requests' lengths (llama2_batch_tables).  batch.lengths and
+    batch.taken count on in place; counts and freeBlocks are the caller's device variables."""
+
+    def Forward(self, batch, counts, freeBlocks, blockSize):
+        capi.call("llama2_batch_tables", batch.struct(), batch.lengths.ptr, counts.ptr, freeBlocks.ptr, freeBlocks.size,
+                  batch.taken.ptr, batch.taken.ptr, blockSize)
+
+
+class BatchQKNormRoPE(Module):
+    """Norm of every query and key head (qGamma, kGamma; None: no norm), rotation by the tokens' positions, and keys and
+    values to the tokens' slots (llama2_batch_qk_norm_rope).  Rows are `strides` = (queryOutput, query, key and value) elements
+    apart, by default as wide as they are; queryOutput may be query."""
+
+    def Forward(self, queryOutput, query, key, value, batch, cache, numHeads, theta, qGamma=None, kGamma=None, eps=1e-5, strides=None):
+        row, kv_row = numHeads * cache.headSize, cache.numKVHeads * cache.headSize
+        capi.call("llama2_batch_qk_norm_rope", queryOutput.ptr, query.ptr, key.ptr, value.ptr, qGamma.ptr if qGamma else None,
+                  kGamma.ptr if kGamma else None, batch.struct(), cache.struct(), numHeads, *(strides or (row, row, kv_row)), eps, theta)
+
+
+class BatchAttention(Module):
+    """Causal attention of all tokens of a step over the shared prefix and each request's own rows (llama2_batch_attention)."""
+
+    def Forward(self, output, query, batch, cache, numHeads, scale, strides=None):
+        row = numHeads * cache.headSize
+        capi.call("llama2_batch_attention", output.ptr, query.ptr, batch.struct(), cache.struct(), numHeads,
+                  *(strides or (row, row)), scale)

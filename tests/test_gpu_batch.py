@@ -285,6 +285,21 @@ def test_attention_prefix_lengths(prefix, new):
     step(prefix, ctx, new, heads=2, kv_heads=1, prefix=prefix, fill=np.nan, pad=3).check("prefix")
 
 
+@pytest.mark.parametrize("prefix", [13, 31, 32, 33, 63, 64, 65, 127, 128, 200, 1025])
+@pytest.mark.parametrize("requests,heads,kv_heads", [(70, 40, 40), (16, 80, 40), (30, 32, 32), (300, 8, 8)])
+def test_attention_shared_prefixes(prefix, requests, heads, kv_heads):
+    """Enough requests and heads that the prefix is shared: in narrow tiles (bounds for long own rows) and in wide ones, with
+    several tokens per request among them."""
+    prefix = max(prefix, -(-(1 << 15) // ((requests - 1) * kv_heads)))
+    rng = synth.rng_for(1405, prefix, requests)
+    ctx, ones = rng.integers(0, 40, requests), np.ones(requests, int)
+    step(prefix, ctx, ones, 8, heads=heads, kv_heads=kv_heads, d=64, prefix=prefix, pad=2, extra=5000, fill=np.nan).check("narrow")
+    new = np.where(rng.random(requests) < 0.2, rng.integers(0, 6, requests), 1)
+    step(prefix, ctx, new, 16, heads=heads, kv_heads=kv_heads, d=64, prefix=prefix, pad=2, fill=np.nan).check("turns")
+    if prefix in (65, 200):
+        step(prefix, ctx, ones, 8, heads=heads, kv_heads=kv_heads, d=128, prefix=prefix, fill=np.nan).check("d 128")
+
+
 @pytest.mark.parametrize("requests", [2, 16, 17, 65, 130, 300])
 def test_attention_many_requests(requests):
     """Columns of the shared rows: a narrow tile, several of them, wide tiles; requests without tokens among them."""
@@ -344,6 +359,30 @@ def test_attention_later_rows_have_no_influence(bad, d):
                 t = slice(s.starts[b], s.starts[b] + first)
                 assert np.array_equal(got[t], clean[t]) or np.abs(got[t].astype(np.float32) - clean[t]).max() <= 2.0 ** -10 * np.abs(
                     clean[t]).max(), (new, heads, b)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [[6, 1], [100, 3], [200, 70]])
+def test_attention_values_that_are_not_finite(new, d):
+    """An infinite value reaches the tokens that attend its row, at its element; the others do not notice."""
+    s = step(12, [20, 50], new, heads=2, kv_heads=1, d=d, prefix=30)
+    clean = s.check()
+    own = s.ctx[0] + new[0] // 2 # row of the token in the middle
+    rows = s.rows_of(s.value)
+    at = s.table[0, own // s.size], own % s.size
+    for value, elements in ((np.inf, (0, 5)), (-np.inf, (d // 2,)), (np.nan, (d - 1,))):
+        for e in elements:
+            rows[at[0], at[1], e] = value
+    s.upload()
+    got = s.run().astype(np.float32)
+    sees = np.zeros(len(got), bool)
+    sees[new[0] // 2:new[0]] = True
+    assert np.abs(got[~sees] - clean[~sees]).max() <= 2.0 ** -10 * np.abs(clean).max()
+    for h in (0, d):
+        g = got[sees][:, h:h + d]
+        assert (g[:, [0, 5]] == np.inf).all() and (g[:, d // 2] == -np.inf).all() and np.isnan(g[:, d - 1]).all()
+        others = np.setdiff1d(np.arange(d), [0, 5, d // 2, d - 1])
+        assert np.abs(g[:, others] - clean[sees][:, h:h + d][:, others]).max() <= 2.0 ** -10 * np.abs(clean).max()
 
 
 def test_attention_without_rows_and_without_blocks():

@@ -1,0 +1,192 @@
+"""The operators of a step of several requests as a server runs them: a prefix read once, prompts behind it, then steps of
+one token each, captured once and replayed while lengths, tables and free blocks count on on the device.  Every step is
+compared with a 64-bit restatement over the cache as it lies there, and the decode steps of every request with the
+framework's modules of one sequence (llama2_rope, llama2_multi_head_attention) over a contiguous cache."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import batch_util as bu
+from managedllama2_amd import capi, synth
+from managedllama2_amd.device import DeviceVariable, PagedCache, RequestBatch, init
+from managedllama2_amd.modules import BatchAttention, BatchQKNormRoPE, BatchTables
+from gpu_util import up
+
+pytestmark = pytest.mark.gpu
+
+THETA, D = 10000.0, 128
+
+
+class Server:
+    """One layer: tables, rotation with the store, attention; q, k, v come from outside instead of from products."""
+
+    def __init__(self, heads, kv_heads, block_size, n_blocks, requests, tokens, stride, max_length, prefix_rows=0, seed=1):
+        init(0)
+        self.heads, self.kv_heads, self.size, self.tokens, self.requests, self.prefix = heads, kv_heads, block_size, tokens, requests, prefix_rows
+        self.cache = PagedCache(n_blocks, block_size, kv_heads, D)
+        ids = synth.rng_for(1501, seed).permutation(n_blocks).astype(np.int32)
+        n_prefix = -(-prefix_rows // block_size)
+        self.prefix_ids, self.free_ids = ids[:n_prefix], ids[n_prefix:]
+        self.free = up(self.free_ids)
+        self.batch = RequestBatch(requests, tokens, stride, max_length, up(self.prefix_ids) if n_prefix else None, prefix_rows)
+        self.counts = DeviceVariable.zeros(np.int32, requests)
+        self.q, self.out = (DeviceVariable.zeros(np.float16, tokens * heads * D) for _ in range(2))
+        self.k, self.v = (DeviceVariable.zeros(np.float16, tokens * kv_heads * D) for _ in range(2))
+        self.norms = None
+        self.tables, self.rope, self.attention = BatchTables(), BatchQKNormRoPE(), BatchAttention()
+
+    def issue(self):
+        self.tables.Forward(self.batch, self.counts, self.free, self.size)
+        gq, gk = self.norms or (None, None)
+        self.rope.Forward(self.q, self.q, self.k, self.v, self.batch, self.cache, self.heads, THETA, gq, gk)
+        self.attention.Forward(self.out, self.q, self.batch, self.cache, self.heads, D ** -0.5)
+
+    def put(self, counts, q, k, v):
+        self.counts.copy_to_device(np.asarray(counts, np.int32))
+        for dev, host in ((self.q, q), (self.k, k), (self.v, v)):
+            dev.copy_to_device(host)
+
+    def check(self, what):
+        """The outputs of the step that just ran, from the rotated queries and the cache as they are now."""
+        rows = lambda c: c.to_host().reshape(-1, self.kv_heads * D)  # noqa: E731
+        key, value = rows(self.cache.key), rows(self.cache.value)
+        table = self.batch.blockTables.to_host().reshape(self.requests, -1)
+        starts, lengths, positions = self.batch.queryStarts.to_host(), self.batch.lengths.to_host(), self.batch.positions.to_host()
+        q, out = self.q.to_host().reshape(self.tokens, -1), self.out.to_host().reshape(self.tokens, -1)
+        r = np.arange(self.prefix)
+        shared = self.prefix_ids[r // self.size].astype(np.int64) * self.size + r % self.size if self.prefix else r
+        for b in range(self.requests):
+            t = slice(starts[b], starts[b + 1])
+            if t.start == t.stop or positions[t.start] < 0:
+                continue
+            r = np.arange(lengths[b])
+            own = table[b, r // self.size].astype(np.int64) * self.size + r % self.size
+            want, bound = bu.attention(q[t], key, value, shared, own, positions[t], self.prefix, D ** -0.5, self.kv_heads, D)
+            err = np.abs(out[t].astype(np.float64) - want)
+            assert (err <= bound).all(), "%s, request %d: off by %.2e, %.2e allowed" % (what, b, err.max(), bound.flat[np.argmax(err - bound)])
+
+
+def normal(rng, *shape):
+    return rng.standard_normal(shape, np.float32).astype(np.float16)
+
+
+@pytest.mark.parametrize("heads,kv_heads,norms", [(4, 4, False), (8, 2, True)])
+@pytest.mark.parametrize("prefix", [0, 75])
+def test_prompts_then_captured_decode_steps(heads, kv_heads, norms, prefix):
+    rng = synth.rng_for(1502, heads, prefix)
+    size, requests, pad, steps = 16, 9, 3, 40
+    wq, wk = heads * D, kv_heads * D
+    prompts = [1, 20, 7, 33, 16, 0, 64, 2, 15]
+    s = Server(heads, kv_heads, size, 120, requests, sum(prompts) + pad, 12, 190, prefix)
+    if norms:
+        s.norms = [up((1 + 0.1 * rng.standard_normal(D)).astype(np.float16)) for _ in range(2)]
+    history = [[] for _ in range(requests)]  # per request: unrotated k and v of every own row
+    if prefix:  # read as a request of its own, whose blocks are then the shared ones
+        first = Server(heads, kv_heads, size, 120, 1, prefix, 12, prefix)
+        first.cache, first.free, first.norms = s.cache, up(s.prefix_ids), s.norms
+        shared_k, shared_v = normal(rng, prefix, wk), normal(rng, prefix, wk)
+        first.put([prefix], normal(rng, prefix, wq), shared_k, shared_v)
+        first.issue()
+        first.check("prefix")
+        assert np.array_equal(first.batch.blockTables.to_host()[:len(s.prefix_ids)], s.prefix_ids)
+    # the prompts
+    n = s.tokens
+    q, k, v = normal(rng, n, wq), normal(rng, n, wk), normal(rng, n, wk)
+    s.put(prompts, q, k, v)
+    s.issue()
+    s.check("prompts")
+    at = 0
+    for b, m in enumerate(prompts):
+        history[b] += [(k[t], v[t]) for t in range(at, at + m)]
+        at += m
+    # decode, one token each, in buffers of the same size: a padded, captured step
+    d = Server(heads, kv_heads, size, 120, requests, requests + pad, 12, 190, prefix)
+    d.cache, d.free, d.norms, d.free_ids, d.prefix_ids = s.cache, s.free, s.norms, s.free_ids, s.prefix_ids
+    for name in ("blockTables", "lengths", "taken"):
+        setattr(d.batch, name, getattr(s.batch, name))
+    d.batch.prefixTable = s.batch.prefixTable
+    g = C.c_void_p()
+    for step in range(steps):
+        counts = (rng.random(requests) < 0.9).astype(np.int32)
+        q, k, v = normal(rng, d.tokens, wq), normal(rng, d.tokens, wk), normal(rng, d.tokens, wk)
+        d.put(counts, q, k, v)
+        guard = np.full(d.tokens * wq, 9.0, np.float16)
+        d.out.copy_to_device(guard)
+        if step == 0:
+            d.issue()  # eager: the scratch exists from here on
+        elif step == 1:
+            capi.call("llama2_graph_begin_capture")
+            try:
+                d.issue()
+            finally:
+                capi.call("llama2_graph_end_capture", C.byref(g))
+            capi.call("llama2_graph_launch", g)
+        elif step % 7 == 0:
+            d.issue()  # the program's own work between replays
+        else:
+            capi.call("llama2_graph_launch", g)
+        d.check("step %d" % step)
+        total = int(counts.sum())
+        out = d.out.to_host().reshape(d.tokens, wq)
+        assert (out[total:] == 9).all()  # rows behind the last request
+        for b, t in zip(np.flatnonzero(counts), range(total)):
+            history[b].append((k[t], v[t]))
+        assert d.batch.lengths.to_host().tolist() == [len(h) for h in history]
+        if kv_heads == heads and not norms and step % 13 == 0:  # the framework's modules of one sequence
+            for b, t in list(zip(np.flatnonzero(counts), range(total)))[::3]:
+                rows = ([(shared_k[i], shared_v[i]) for i in range(prefix)] if prefix else []) + history[b]
+                ks, vs = (np.stack([r[i] for r in rows]) for i in (0, 1))
+                dk, dv, dq, o, dummy = up(ks), up(vs), up(q[t]), up(np.zeros(wq, np.float16)), up(np.zeros(wq, np.float16))
+                for p in range(len(rows)):
+                    capi.call("llama2_rope", dq.ptr if p == len(rows) - 1 else dummy.ptr, dk.offset_pointer(p * wk), heads, D, p, THETA, heads)
+                capi.call("llama2_multi_head_attention", o.ptr, dq.ptr, dk.ptr, dv.ptr, D, wq, len(rows), D ** -0.5, heads)
+                # that one stores scores as fp16: |score| < 8 off by 2^-9, a weight by 2^-8 of itself
+                assert np.abs(o.to_host().astype(np.float32) - out[t]).max() <= 2.0 ** -8 * np.abs(vs).max(), (step, b)
+    capi.call("llama2_graph_destroy", g)
+    assert int(d.batch.taken[0]) == sum(-(-len(h) // size) for h in history)
+
+
+def test_a_pool_that_runs_dry_stops_requests_one_by_one():
+    rng = synth.rng_for(1503)
+    s = Server(2, 1, 8, 7, 5, 5, 6, 48, 0)  # 7 blocks for 5 requests
+    lengths = np.zeros(5, np.int64)
+    for step in range(30):
+        s.put([1] * 5, normal(rng, 5, 256), normal(rng, 5, 128), normal(rng, 5, 128))
+        before = s.cache.key.to_host()
+        s.out.copy_to_device(np.full(5 * 256, 3.0, np.float16))
+        s.issue()
+        slots = s.batch.slots.to_host()
+        now = s.batch.lengths.to_host()
+        assert ((now - lengths == 1) == (slots >= 0)).all()
+        assert (s.out.to_host().reshape(5, 256)[slots < 0] == 3).all()
+        if (slots < 0).all():
+            assert np.array_equal(before.view(np.uint16), s.cache.key.to_host().view(np.uint16))
+        s.check("step %d" % step)
+        lengths = now
+    assert int(s.batch.taken[0]) == 7 and lengths.max() == 16 and lengths.min() == 8
+
+
+def test_large_tables_in_place():
+    """More tokens than one workgroup takes, lengths and taken blocks updated in place, also when replayed."""
+    import test_gpu_batch as tb
+    for odd, n, new_hi in ((False, 60, 400), (True, 1500, 30)):
+        c = tb.tables_case(21 + n, n, 16, 300, new_hi, 40, 30, odd=odd, prefix=9, stride=80)
+        table, lengths, counts, free, taken, size, prefix, n_tokens = c.host
+        assert n_tokens > 4096
+        c.batch.lengths = c.cached.ptr
+        run = lambda: capi.call("llama2_batch_tables", c.batch, c.cached.ptr, c.counts.ptr, c.free.ptr, c.n_free, c.taken.ptr, c.taken.ptr, size)  # noqa: E731
+        run()
+        g = C.c_void_p()
+        capi.call("llama2_graph_begin_capture")
+        try:
+            run()
+        finally:
+            capi.call("llama2_graph_end_capture", C.byref(g))
+        for rep in range(4):
+            table, lengths, starts, positions, slots, taken = bu.tables(table, lengths, counts, free, taken, size, prefix, n_tokens)
+            assert np.array_equal(c.cached.to_host(), lengths) and int(c.taken[0]) == taken, rep
+            assert np.array_equal(c.table.to_host().reshape(table.shape), table) and np.array_equal(c.slots.to_host(), slots), rep
+            assert np.array_equal(c.positions.to_host(), positions) and np.array_equal(c.starts.to_host(), starts), rep
+            capi.call("llama2_graph_launch", g)
+        capi.call("llama2_graph_destroy", g)
