@@ -58,7 +58,7 @@ struct Item {
     int r0, r1;                 // own rows
     const int* table;           // of the own rows
     int slot;
-    int split;                  // which piece of the own rows, -1: of the shared ones
+    int split;                  // which piece of the own rows
 };
 
 __device__ __forceinline__ f4_t mfma16(h8_t x, h8_t y, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
@@ -175,12 +175,11 @@ __device__ __forceinline__ void join_lanes(const BatchAttnArgs& a, int token, in
 
 // One token's head by a wavefront: D / 8 lanes side by side (8 elements each), the others with every 512 / D-th piece.
 template <int D>
-__device__ void join_pieces(const BatchAttnArgs& a, int token, int head, __amdgpu_buffer_rsrc_t parts)
+__device__ void join_pieces(const BatchAttnArgs& a, int token, int head, int slots, __amdgpu_buffer_rsrc_t parts)
 {
     constexpr int SIDE = D / 8, DEEP = 64 / SIDE;
     const int lane = threadIdx.x & 63, x = lane % SIDE, deep = lane / SIDE;
     const int heads = a.n_kv_heads * a.group, rows = a.n_tokens * heads;
-    const int slots = a.shared_splits + (a.own_prefix + own_rows_of(a, a.positions[token]) + a.own_piece - 1) / a.own_piece;
     float m = -INFINITY, sum = 0.0f, o[8] = {};
     for (int s = deep; s < slots; s += DEEP) {
         const int part = s * rows + token * heads + head; // parts_bytes < 2^31
@@ -420,35 +419,31 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
     if (!a.counters)
         return;
 
-    // Tokens whose last piece this was (their columns lie in one tile each: the group divides 16).
+    // Tokens whose last piece this was; nothing is shared, and their columns lie in one tile each: the group divides 16.
     wait_agent_stores();
     __syncthreads();
-    unsigned* const done = reinterpret_cast<unsigned*>(lds);
+    int* const slots_of = reinterpret_cast<int*>(lds); // per token of the tile: pieces to join, 0: not by this workgroup
     if (wave == 0) {
-        bool last = false;
-        if (lane * a.group < it.rows) {
-            const int t = it.token + it.row0 / a.group + lane, p = a.positions[t];
+        const int p = __shfl(position, (lane * a.group) & 15, 64); // of token `lane` of the tile: that of its first column
+        int slots = 0;
+        if (lane * a.group < it.rows && p >= 0) {
             const int pieces = (a.own_prefix + own_rows_of(a, p) + a.own_piece - 1) / a.own_piece;
-            if (p >= 0 && it.split < pieces) {
-                unsigned* const counter = a.counters + t * a.n_kv_heads + it.kv_head;
-                last = add_agent(counter, 1) + 1 == static_cast<unsigned>(a.shared_splits + pieces);
-                if (last)
-                    store_agent(counter, 0);
+            unsigned* const counter = a.counters + (it.token + it.row0 / a.group + lane) * a.n_kv_heads + it.kv_head;
+            if (it.split < pieces && add_agent(counter, 1) + 1 == static_cast<unsigned>(pieces)) {
+                store_agent(counter, 0);
+                slots = pieces;
             }
         }
-        const unsigned mask = static_cast<unsigned>(__ballot(last));
-        if (lane == 0)
-            *done = mask;
+        if (lane < 16)
+            slots_of[lane] = slots;
     }
     __syncthreads();
-    unsigned left = __builtin_amdgcn_readfirstlane(*done);
     const __amdgpu_buffer_rsrc_t parts = make_rsrc(a.parts, a.parts_bytes);
-    for (int k = 0; left; left &= left - 1)
-        for (int h = 0; h < a.group; ++h, ++k)
-            if ((k & 3) == wave) {
-                const int t = it.token + it.row0 / a.group + __builtin_ctz(left);
-                join_pieces<D>(a, t, it.kv_head * a.group + h, parts);
-            }
+    for (int k = wave; k < it.rows; k += 4) {
+        const int t = k / a.group, slots = __builtin_amdgcn_readfirstlane(slots_of[t]);
+        if (slots)
+            join_pieces<D>(a, it.token + it.row0 / a.group + t, it.kv_head * a.group + k % a.group, slots, parts);
+    }
 }
 
 // ---------------------------------------------------------------- many columns
@@ -750,7 +745,6 @@ __global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttn
         it.row0 = tile * kTileRows;
         it.rows = min(a.n_tokens * a.group - it.row0, kTileRows);
         it.tokens = 1; // all see the same rows
-        it.split = -1;
     } else {
         index -= shared_items;
         const int of_heads = index / a.n_kv_heads;
