@@ -748,7 +748,9 @@ __global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttn
     } else {
         index -= shared_items;
         const int of_heads = index / a.n_kv_heads;
-        const int tile = of_heads % a.own_tiles, split = of_heads / a.own_tiles;
+        const int split = of_heads / a.own_tiles, turn = of_heads % a.own_tiles;
+        // wide tiles from the last one on: of a prompt, later tiles see more rows (3827 prompt tokens 102 -> 92 us)
+        const int tile = MANY ? a.own_tiles - 1 - turn : turn;
         // An XCD gets every eighth workgroup.  Wide tiles: a head's tiles all go to one, whose L2 then serves the rows to
         // all of them.  Narrow ones read every row once: an XCD takes all heads in turn, because the rows of one head
         // alone lie in few channels of its L2.
