@@ -62,7 +62,8 @@ int llama2_init(int device);
 /* Releases the stream and internal scratch.  Caller-owned buffers and decoders
  * stay valid and work again after the next llama2_init on the same device; graphs
  * that the caller captured from modules with scratch (llama2_vec_mat,
- * llama2_multi_head_attention, the sampler modules) hold its address and do not. */
+ * llama2_multi_head_attention, the sampler modules, llama2_batch_tables, llama2_batch_attention)
+ * hold its address and do not. */
 int llama2_shutdown(void);
 /* Text of the calling thread's last error ("" if none).  Never NULL. */
 const char* llama2_last_error(void);
@@ -101,8 +102,8 @@ int llama2_event_destroy(void* event);
  * llama2_graph_launch replays with a single submission (no counterpart in the
  * reference, which pays one cuLaunchKernel per module call, src/Module.cs:21-22).
  * Only kernel entry points may be called while capturing: no malloc / free /
- * memcpy / sync, and llama2_vec_mat / llama2_multi_head_attention only for
- * shapes whose scratch already exists (call them once eagerly first).  The captured calls keep the argument
+ * memcpy / sync, and llama2_vec_mat / llama2_multi_head_attention /
+ * llama2_batch_attention only for shapes whose scratch already exists (call them once eagerly first).  The captured calls keep the argument
  * values they were made with, the scratch address included: the library never
  * frees a scratch buffer before llama2_shutdown, so a later eager call that
  * needs a larger one leaves earlier graphs valid. */

@@ -391,7 +391,7 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
         }
     }
     const bool live = c < it.rows && position >= 0;
-    const int rows = a.n_tokens * a.n_kv_heads * a.group, d = (g * 4 + wave) * VE; // rows < 2^29
+    const int rows = a.n_tokens * a.n_kv_heads * a.group, d = (g * 4 + wave) * VE; // rows < 2^26
     const size_t part = static_cast<size_t>(it.slot) * rows + static_cast<size_t>(token) * a.n_kv_heads * a.group + head;
     if (live && !a.parts) {
         typedef _Float16 Halfs __attribute__((ext_vector_type(VE)));
@@ -822,7 +822,7 @@ __global__ __launch_bounds__(256) void batch_attn_merge_kernel(BatchAttnArgs a)
     constexpr int SIDE = D / 8, DEEP = LANES / SIDE;
     __shared__ float lds[LANES > 64 ? DEEP * SIDE * 8 : 1];
     __shared__ float2 stat[LANES > 64 ? DEEP : 1];
-    const int heads = a.n_kv_heads * a.group, rows = a.n_tokens * heads; // < 2^29: checked on the host
+    const int heads = a.n_kv_heads * a.group, rows = a.n_tokens * heads; // < 2^26: checked on the host
     const int row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     const int lane = threadIdx.x % LANES, x = lane % SIDE, deep = lane / SIDE;
     const int token = min(row, rows - 1) / heads, head = row % heads;
@@ -881,7 +881,7 @@ static void batch_attn_launch(const BatchAttnArgs& a, bool many, int items, int 
     if (!a.parts || a.counters)
         return;
     const int rows = a.n_tokens * a.n_kv_heads * a.group;
-    if (slots <= 16)
+    if (slots <= 16 || rows >= 1 << 24) // of threads there are less than 2^32
         hipLaunchKernelGGL((batch_attn_merge_kernel<D, 64>), dim3(ceil_div(rows, 4)), dim3(256), 0, ctx().stream, a);
     else
         hipLaunchKernelGGL((batch_attn_merge_kernel<D, 256>), dim3(rows), dim3(256), 0, ctx().stream, a);
@@ -901,12 +901,11 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
     if (int rc = check_batch_attention(output, query, batch, cache, n_heads, output_stride, query_stride, scale))
         return rc;
     const llama2_batch& b = *batch;
-    const long long table_rows = static_cast<long long>(b.table_stride) * cache->block_size;
-    const int max_rows = table_rows < b.max_length ? static_cast<int>(table_rows) : b.max_length, group = n_heads / cache->n_kv_heads;
+    const int max_rows = batch_own_rows(b, cache->block_size), group = n_heads / cache->n_kv_heads;
     const BatchAttnPlan p = batch_attn_plan(b, cache->n_kv_heads, group, max_rows, ctx().num_cus > 0 ? ctx().num_cus : 256);
+    if (int rc = check_batch_attn_plan(p, b.n_tokens, n_heads, cache->n_kv_heads))
+        return rc;
     const long long rows = static_cast<long long>(b.n_tokens) * n_heads, items = p.items(cache->n_kv_heads);
-    if (rows > 0x7FFFFFFF / 4 || items > 0x7FFFFFFF)
-        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: %d tokens of %d heads in %d pieces are too many", fn, b.n_tokens, n_heads, p.slots());
     BatchAttnArgs a = {};
     a.out = output;
     a.q = query;

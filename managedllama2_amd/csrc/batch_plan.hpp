@@ -11,6 +11,7 @@ namespace l2 {
 
 constexpr int kMaxBatchTokens = 1 << 20; // tokens and requests of a step
 constexpr int kMaxBatchHeads = 1024;
+constexpr int kMaxBatchRows = 1 << 29; // that a token attends: sums of two such numbers are ints
 
 constexpr int kManyRows = 128; // columns (token, head of the group) of a workgroup's widest tile
 constexpr int kFewRows = 16;   // at most this many: the wavefronts split the cache rows instead of the columns
@@ -148,6 +149,13 @@ inline int check_batch_rope(const llama2_half* q_output, const llama2_half* q, c
     return LLAMA2_OK;
 }
 
+// The most own rows that a request can have.
+inline int batch_own_rows(const llama2_batch& b, int block_size)
+{
+    const long long rows = static_cast<long long>(b.table_stride) * block_size;
+    return rows < b.max_length ? static_cast<int>(rows) : b.max_length;
+}
+
 inline int check_batch_attention(const llama2_half* output, const llama2_half* query, const llama2_batch* batch,
                                  const llama2_paged_cache* cache, int n_heads, int output_stride, int query_stride, float scale)
 {
@@ -168,9 +176,11 @@ inline int check_batch_attention(const llama2_half* output, const llama2_half* q
     L2_CHECK(!overlap(output, out_bytes, query, rows_bytes(b.n_tokens, query_stride, row)) &&
                  !overlap(output, out_bytes, cache->key, cache_bytes(*cache)) && !overlap(output, out_bytes, cache->value, cache_bytes(*cache)),
              "%s: output overlaps query or the cache", fn);
-    L2_CHECK(b.table_stride > 0 && b.max_length > 0 && b.max_length <= 0x7FFFFFFF - 4096 - b.prefix_length,
-             "%s: table_stride=%d and max_length=%d must be positive, and max_length with prefix_length=%d below 2^31", fn,
-             b.table_stride, b.max_length, b.prefix_length);
+    L2_CHECK(b.table_stride > 0 && b.max_length > 0, "%s: table_stride=%d and max_length=%d must be positive", fn, b.table_stride,
+             b.max_length);
+    if (b.prefix_length > kMaxBatchRows || batch_own_rows(b, cache->block_size) > kMaxBatchRows - b.prefix_length)
+        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: prefix_length=%d and %d own rows exceed %d", fn, b.prefix_length,
+                    batch_own_rows(b, cache->block_size), kMaxBatchRows);
     return LLAMA2_OK;
 }
 
@@ -238,6 +248,15 @@ inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int 
         p.shared_splits = ceil_div(b.prefix_length, p.shared_piece);
     }
     return p;
+}
+
+// Launches hold less than 2^32 threads.
+inline int check_batch_attn_plan(const BatchAttnPlan& p, int n_tokens, int n_heads, int n_kv_heads)
+{
+    if (p.items(n_kv_heads) >= 1 << 24 || static_cast<long long>(n_tokens) * n_heads >= 1 << 26)
+        return fail(LLAMA2_ERR_UNSUPPORTED, "llama2_batch_attention: %d tokens of %d heads in %lld pieces are too many", n_tokens, n_heads,
+                    p.items(n_kv_heads));
+    return LLAMA2_OK;
 }
 
 } // namespace l2

@@ -53,6 +53,10 @@ int attention(const llama2_half* o, const llama2_half* q, const llama2_batch* b,
 {
     return l2::check_batch_attention(o, q, b, c, h, so, sq, scale);
 }
+int fits(const llama2_batch* b, int n_kv_heads, int group, int max_rows)
+{
+    return l2::check_batch_attn_plan(l2::batch_attn_plan(*b, n_kv_heads, group, max_rows, 256), b->n_tokens, n_kv_heads * group, n_kv_heads);
+}
 void plan(const llama2_batch* b, int n_kv_heads, int group, int max_rows, int* out)
 {
     const l2::BatchAttnPlan p = l2::batch_attn_plan(*b, n_kv_heads, group, max_rows, 256);
@@ -77,6 +81,7 @@ def lib(tmp_path_factory):
     for ours, name in (("tables", "llama2_batch_tables"), ("rope", "llama2_batch_qk_norm_rope"), ("attention", "llama2_batch_attention")):
         getattr(lib, ours).argtypes = capi._SIGNATURES[name]
     lib.plan.argtypes = [C.POINTER(capi.Batch), C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int)]
+    lib.fits.argtypes = [C.POINTER(capi.Batch), C.c_int, C.c_int, C.c_int]
     lib.last.restype = C.c_char_p
     return lib
 
@@ -210,9 +215,12 @@ def test_attention_refusals(lib):
     for name in ("block_tables", "query_starts", "positions"):
         assert call_attention(lib, batch(**{name: None}), cache()) == INVALID, name
     for name, values in dict(n_requests=(0, (1 << 20) + 1), n_tokens=(0, (1 << 20) + 1), prefix_length=(-1,), table_stride=(0,),
-                             max_length=(0, -1, 0x7FFFFFFF - 4096)).items():
+                             max_length=(0, -1)).items():
         for v in values:
             assert call_attention(lib, batch(**{name: v}), cache()) == INVALID, (name, v)
+    assert call_attention(lib, batch(max_length=0x7FFFFFFF), cache()) == 0  # no more than the tables hold
+    assert call_attention(lib, batch(max_length=0x7FFFFFFF, table_stride=1 << 25), cache()) == UNSUPPORTED
+    assert call_attention(lib, batch(prefix_length=(1 << 29) - 100), cache()) == UNSUPPORTED
     for name in ("o", "q"):
         assert call_attention(lib, batch(), cache(), **{name: None}) == INVALID
         assert call_attention(lib, batch(), cache(), **{name: ATTENTION[name] + 2}) == INVALID
@@ -262,6 +270,14 @@ def test_plan_shares_a_prefix_among_narrow_requests_only(lib):
     assert out[2] == 0 and out[7] == 512 and out[0] and out[5] == 1
     lib.plan(batch(n_requests=1, n_tokens=1, prefix_length=512), 32, 1, 300, out)  # nobody to share with
     assert out[2] == 0 and out[7] == 512 and not out[0]
+
+
+def test_plan_refuses_more_workgroups_than_a_launch_holds(lib):
+    assert lib.fits(batch(n_requests=100000, n_tokens=100000), 32, 1, 4000) == 0
+    assert lib.fits(batch(n_requests=1 << 20, n_tokens=1 << 20), 32, 1, 4000) == UNSUPPORTED
+    assert lib.fits(batch(n_requests=1, n_tokens=1 << 20), 1, 128, 4000) == UNSUPPORTED
+    assert lib.fits(batch(n_requests=1, n_tokens=1 << 20), 8, 4, 1 << 20) == 0
+    assert b"too many" in lib.last()
 
 
 def test_entry_points_refuse_before_init():
