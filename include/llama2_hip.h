@@ -346,13 +346,17 @@ typedef struct llama2_batch {
  * rows and brings counts[b] tokens (none is allowed).  It gets the blocks that its new rows
  * need from free_blocks[taken ..), in the order of the requests; batch->block_tables is
  * extended in place, lengths, query_starts, positions and slots are written, and
- * new_taken[0] is the number of free blocks taken so far.  lengths may be
- * `cached` and new_taken may be `taken`; other arrays must not overlap.
+ * new_taken[0] is taken[0] plus the blocks that the requests up to the last one that is
+ * not refused ask for.  lengths may be `cached` and new_taken may be `taken`; other arrays
+ * must not overlap.
  * A request is refused -- its tokens get position and slot -1, its table and
  * length stay as they are, it takes no block -- if the free blocks left do not suffice for
  * it and all in front of it, if its rows would not fit into table_stride blocks, if its tokens
  * reach beyond n_tokens, or if its count or length is negative.  A request that needs no
- * block is not refused for want of blocks.
+ * block is not refused for want of blocks; where one goes on behind a request that was,
+ * new_taken[0] is above n_free.  With taken[0] above n_free (or negative) the list counts as
+ * empty and new_taken[0] is taken[0]: nobody gets a block until the caller, who has to find blocks
+ * or pause requests then, gives a new list.
  * Block ids are copied, not looked at; free_blocks and the tables must not hold an id twice.
  * prefix_table and max_length are not read. */
 int llama2_batch_tables(const llama2_batch* batch, const int* cached, const int* counts,

@@ -61,14 +61,15 @@ __global__ __launch_bounds__(kTablesBlock) void batch_tables_kernel(TablesArgs a
     const int size = 1 << a.shift, tid = threadIdx.x;
     const int limit = a.table_stride > (0x7FFFFFFF >> a.shift) ? 0x7FFFFFFF : a.table_stride << a.shift;
     const int taken = a.taken[0];
-    const int left = taken >= 0 && taken <= a.n_free ? a.n_free - taken : 0;
+    const bool list = taken >= 0 && taken <= a.n_free; // else it counts as empty
+    const int left = list ? a.n_free - taken : 0;
     const int every = static_cast<int>(gridDim.x) * kTablesBlock;
     int t = static_cast<int>(blockIdx.x) * kTablesBlock + tid; // this thread's next token
     bool lengths = gridDim.x == 1 || (a.apart && blockIdx.x == 0), starts = blockIdx.x == 0;
     for (;;) {
         if (tid == 0)
             most_taken = 0;
-        int tokens_before = 0, need_before = 0; // both cut off one above what can be granted
+        int tokens_before = 0, need_before = 0; // the tokens cut off one above what there is
         for (int first = 0; first < a.n_requests; first += kTablesBlock) {
             const int b = first + tid, in_block = min(a.n_requests - first, kTablesBlock);
             const int c = b < a.n_requests ? a.cached[b] : 0, n = b < a.n_requests ? a.counts[b] : 0;
@@ -78,12 +79,12 @@ __global__ __launch_bounds__(kTablesBlock) void batch_tables_kernel(TablesArgs a
             const int have = fits ? (c >> a.shift) + ((c & (size - 1)) != 0) : 0;
             const int total = fits ? ((c + n) >> a.shift) + (((c + n) & (size - 1)) != 0) : 0;
             const int need = total - have;
-            const int upto = min(block_scan(min(need, left + 1), left + 1, sums) + need_before, left + 1);
+            const int upto = block_scan(need, kMaxBatchTokens, sums) + need_before; // a new block holds a new token: no more of them
             const bool admitted = fits && (need == 0 || upto <= left);
             begin[tid] = end;
             rows[tid] = c;
             from[tid] = !admitted ? -1 : need > 0 ? taken + upto - need : 0;
-            if (admitted && need > 0)
+            if (admitted && upto > 0)
                 atomicMax(&most_taken, upto);
             if (b < a.n_requests) {
                 if (starts)
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(kTablesBlock) void batch_tables_kernel(TablesArgs a
         }
         if (lengths) {
             if (tid == 0)
-                a.new_taken[0] = taken + most_taken;
+                a.new_taken[0] = list ? taken + most_taken : taken;
             return;
         }
         if (a.apart)

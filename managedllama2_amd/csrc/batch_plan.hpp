@@ -90,7 +90,7 @@ inline int check_batch_tables(const llama2_batch* batch, const int* cached, cons
              "%s: null pointer", fn);
     L2_CHECK(aligned(cached, 4) && aligned(counts, 4) && aligned(free_blocks, 4) && aligned(taken, 4) && aligned(new_taken, 4),
              "%s: misaligned pointer", fn);
-    L2_CHECK(n_free >= 0 && n_free < 0x7FFFFFFF && (free_blocks || n_free == 0), "%s: n_free=%d free_blocks=%p", fn, n_free,
+    L2_CHECK(n_free >= 0 && n_free < 0x7FFFFFFF - kMaxBatchTokens && (free_blocks || n_free == 0), "%s: n_free=%d free_blocks=%p", fn, n_free,
              static_cast<const void*>(free_blocks));
     if (int rc = check_block_size(fn, block_size))
         return rc;

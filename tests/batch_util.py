@@ -13,7 +13,7 @@ def tables(block_tables, cached, counts, free, taken, size, prefix, n_tokens):
     lengths, starts = cached.copy(), np.zeros(len(cached) + 1, np.int64)
     positions, slots = np.full(n_tokens, -1, np.int32), np.full(n_tokens, -1, np.int32)
     left = len(free) - taken if 0 <= taken <= len(free) else 0
-    used, begin, blocked = 0, 0, 0  # blocked: what the requests so far asked for
+    used, begin, blocked = 0, 0, 0  # blocked: what the requests so far asked for; used: up to the last one that goes on
     for b, (c, n) in enumerate(zip(cached.tolist(), counts.tolist())):
         end = begin + max(n, 0)
         fits = c >= 0 and n >= 0 and c + n <= stride * size and end <= n_tokens
@@ -22,16 +22,15 @@ def tables(block_tables, cached, counts, free, taken, size, prefix, n_tokens):
             need = -(-(c + n) // size) - first
             blocked += need
             if need == 0 or blocked <= left:
-                table[b, first:first + need] = free[taken + blocked - need:taken + blocked]
-                if need:
-                    used = blocked
+                table[b, first:first + need] = free[taken + blocked - need:taken + blocked] if need else []
+                used = blocked
                 lengths[b] = c + n
                 rows = np.arange(c, c + n)
                 positions[begin:end] = prefix + rows
                 slots[begin:end] = table[b, rows // size] * size + rows % size
         starts[b + 1] = end
         begin = end
-    return table, lengths, np.minimum(starts, n_tokens).astype(np.int32), positions, slots, taken + used
+    return table, lengths, np.minimum(starts, n_tokens).astype(np.int32), positions, slots, taken + used if 0 <= taken <= len(free) else taken
 
 
 def rope(x, positions, gamma, eps, theta, d):

@@ -103,6 +103,20 @@ def test_tables_with_a_count_of_taken_blocks_that_cannot_be(taken):
     TablesCall(table, cached, counts, free[:0], 0, size, prefix, n_tokens).check("no free blocks")
 
 
+def test_tables_of_a_request_that_goes_on_behind_a_refused_one():
+    """One needs two blocks where one is left, the next none, the last one: the second goes on, and the count says that the list is
+    exhausted; from then on nobody gets a block and the count stays."""
+    size = 8
+    table = np.array([[0, -5, -5], [1, -5, -5], [2, -5, -5]], np.int32)
+    cached, counts, free = np.array([8, 3, 8], np.int32), np.array([9, 2, 1], np.int32), np.array([9, 7, 6, 5], np.int32)
+    c = TablesCall(table, cached, counts, free, 3, size, 0, 12)
+    c.check("dry")
+    assert c.lengths.to_host().tolist() == [8, 5, 8] and int(c.new_taken[0]) == 3 + 2 > len(free)
+    c = TablesCall(table, np.array([8, 5, 8], np.int32), counts, free, 5, size, 0, 12)
+    c.check("still dry")
+    assert c.lengths.to_host().tolist() == [8, 7, 8] and int(c.new_taken[0]) == 5
+
+
 def test_tables_in_place_and_replayed():
     """Lengths and the number of taken blocks updated in place: a captured step counts on by itself."""
     c = tables_case(12, 40, 8, 50, 1, pad=4, short=-200, stride=30)
