@@ -201,11 +201,12 @@ __device__ void join_pieces(const BatchAttnArgs& a, int token, int head, int slo
 // memory into the operands' registers.  Lane (g, c), g = lane / 16: keys of row 16 t + c, elements 32 j + 8 g .. + 7
 // (64 consecutive bytes of a row per load and row); values of the rows 16 t + 4 g .. + 3, whose scores the same lane holds, 1/16 of a
 // row each (4 whole rows per load), turned by byte permutations into columns: operand i holds elements c * D/16 + i.
-template <int D>
+template <int D, int WAVES>
 __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
 {
+    constexpr int kStep = 32 * WAVES;
     constexpr int KS = D / 32, VE = D / 16, VW = VE / 2; // k steps; elements and words of a value row per lane
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
     const int r = min(c, it.rows - 1);
     const int token = it.token + (it.row0 + r) / a.group, head = it.kv_head * a.group + (it.row0 + r) % a.group;
@@ -237,7 +238,7 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
             kid[t] = block_of(begin + wave * 32 + 16 * t + (c & ~3));
             vid[t] = block_of(begin + wave * 32 + 16 * t + 4 * g);
         }
-        for (int tb = begin + wave * 32; tb < end; tb += 128) {
+        for (int tb = begin + wave * 32; tb < end; tb += kStep) {
             h8_t kf[2][KS];
             uint32_t vr[8][VW];
             bool ok[2];
@@ -269,11 +270,11 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
                     }
                 }
             }
-            if (tb + 128 < end) {
+            if (tb + kStep < end) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    kid[t] = block_of(tb + 128 + 16 * t + (c & ~3));
-                    vid[t] = block_of(tb + 128 + 16 * t + 4 * g);
+                    kid[t] = block_of(tb + kStep + 16 * t + (c & ~3));
+                    vid[t] = block_of(tb + kStep + 16 * t + 4 * g);
                 }
             }
             f4_t s[2] = {};
@@ -354,6 +355,22 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
         }
     }
     sum = add_xor32(add_xor16(sum));
+
+    if constexpr (WAVES == 1) { // the whole of the rows: the output
+        if (c >= it.rows || position < 0)
+            return;
+        typedef _Float16 Halfs __attribute__((ext_vector_type(VE)));
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            Halfs h;
+#pragma unroll
+            for (int x = 0; x < VE; ++x)
+                h[x] = __builtin_bit_cast(_Float16, float_to_half_bits(o[x][k] * inv));
+            *reinterpret_cast<Halfs*>(a.out + static_cast<size_t>(token) * a.out_stride + head * D + (g * 4 + k) * VE) = h;
+        }
+        return;
+    }
 
     // The four wavefronts' sums through LDS, then each adds up a quarter of the elements: those with k == wave, which are
     // VE neighbours in each lane.
@@ -721,18 +738,26 @@ constexpr int kFewLds = 4 * (D / 16) * 1024 + 512;
 template <int D>
 constexpr int kAttnLds = ManyLds<D>::kTotal > kFewLds<D> ? ManyLds<D>::kTotal : kFewLds<D>;
 
-template <int D, bool MANY>
-__global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttnArgs a)
+// kNarrow: a workgroup per tile of up to 16 columns.  kSingle: a wavefront per tile, for many tiles of few rows, where most
+// of a workgroup would have no rows; no sharing and no pieces.  kWide: a workgroup per tile of up to 128 columns.
+template <int D, BatchAttnKernel KIND>
+__global__ __launch_bounds__(256, KIND == BatchAttnKernel::kWide ? 2 : 3) void batch_attn_kernel(BatchAttnArgs a)
 {
+    constexpr bool MANY = KIND == BatchAttnKernel::kWide, SINGLE = KIND == BatchAttnKernel::kSingle;
     constexpr int kTileRows = MANY ? kManyRows : kFewRows;
-    __shared__ __align__(16) char lds[MANY ? kAttnLds<D> : kFewLds<D>];
+    __shared__ __align__(16) char lds[MANY ? kAttnLds<D> : SINGLE ? 16 : kFewLds<D>];
     Item it = {};
     const int shared_items = a.shared_items;
     // Wide tiles of shared rows first, they take longest; narrow ones last, to fill up what long requests leave idle (64
     // conversations 133 -> 125 us).
     int index = blockIdx.x;
-    if (!MANY)
+    if (KIND == BatchAttnKernel::kNarrow)
         index = index < a.own_items ? index + shared_items : index - a.own_items;
+    if (SINGLE) {
+        index = index * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (index >= a.own_items)
+            return;
+    }
     if (index < shared_items) {
         // The tiles of a piece to one XCD: they read the same rows.
         const int eight = index / (8 * a.shared_tiles), tile = index % (8 * a.shared_tiles) / 8, rest = eight * 8 + index % 8;
@@ -811,7 +836,7 @@ __global__ __launch_bounds__(256, MANY ? 2 : 3) void batch_attn_kernel(BatchAttn
             return;
         }
     }
-    few_rows<D>(a, it, lds);
+    few_rows<D, SINGLE ? 1 : 4>(a, it, lds);
 }
 
 // Joins the pieces of a token's head, in order, where no workgroup of the attention does: LANES lanes per row, D / 8 of
@@ -872,12 +897,14 @@ __global__ __launch_bounds__(256) void batch_attn_merge_kernel(BatchAttnArgs a)
 }
 
 template <int D>
-static void batch_attn_launch(const BatchAttnArgs& a, bool many, int items, int slots)
+static void batch_attn_launch(const BatchAttnArgs& a, BatchAttnKernel kind, int items, int slots)
 {
-    if (many)
-        hipLaunchKernelGGL((batch_attn_kernel<D, true>), dim3(items), dim3(256), 0, ctx().stream, a);
+    if (kind == BatchAttnKernel::kWide)
+        hipLaunchKernelGGL((batch_attn_kernel<D, BatchAttnKernel::kWide>), dim3(items), dim3(256), 0, ctx().stream, a);
+    else if (kind == BatchAttnKernel::kSingle)
+        hipLaunchKernelGGL((batch_attn_kernel<D, BatchAttnKernel::kSingle>), dim3(ceil_div(items, 4)), dim3(256), 0, ctx().stream, a);
     else
-        hipLaunchKernelGGL((batch_attn_kernel<D, false>), dim3(items), dim3(256), 0, ctx().stream, a);
+        hipLaunchKernelGGL((batch_attn_kernel<D, BatchAttnKernel::kNarrow>), dim3(items), dim3(256), 0, ctx().stream, a);
     if (!a.parts || a.counters)
         return;
     const int rows = a.n_tokens * a.n_kv_heads * a.group;
@@ -947,15 +974,15 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
         // Joined in the same launch: few pieces of few columns, which one wavefront per column has done sooner than another
         // launch begins.
         const size_t bytes = part * cache->head_size * sizeof(float);
-        if (!p.many && p.shared_splits == 0 && p.slots() <= 16 && kFewRows % group == 0 && rows / group <= kMaxBatchCounters && bytes < (1u << 31)) {
+        if (p.kernel == BatchAttnKernel::kNarrow && p.shared_splits == 0 && p.slots() <= 16 && kFewRows % group == 0 && rows / group <= kMaxBatchCounters && bytes < (1u << 31)) {
             a.counters = ctx().batch_counters;
             a.parts_bytes = static_cast<uint32_t>(bytes);
         }
     }
     if (cache->head_size == 128)
-        batch_attn_launch<128>(a, p.many, static_cast<int>(items), p.slots());
+        batch_attn_launch<128>(a, p.kernel, static_cast<int>(items), p.slots());
     else
-        batch_attn_launch<64>(a, p.many, static_cast<int>(items), p.slots());
+        batch_attn_launch<64>(a, p.kernel, static_cast<int>(items), p.slots());
     L2_LAUNCH_CHECK(fn);
     return LLAMA2_OK;
 }

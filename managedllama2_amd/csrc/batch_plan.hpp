@@ -185,8 +185,10 @@ inline int check_batch_attention(const llama2_half* output, const llama2_half* q
 }
 
 // ---------------------------------------------------------------- how the attention is cut
+enum class BatchAttnKernel { kNarrow, kSingle, kWide };
+
 struct BatchAttnPlan {
-    bool many = false; // the kernel with wide tiles
+    BatchAttnKernel kernel = BatchAttnKernel::kNarrow;
     int shared_tiles = 0, shared_splits = 0, shared_piece = kPass;
     int own_tiles = 0, own_splits = 1, own_piece = kPass;
     int own_prefix = 0; // prefix rows in front of a request's own, a multiple of kPass; 0: none, or shared
@@ -209,7 +211,8 @@ inline int batch_attn_piece(long long items, int rows, int shortest, int longest
 
 // Sharing pays while a request has fewer than 64 columns of its own (more fill a workgroup's columns anyway, and the
 // prefix becomes the front of every request's rows), and where the prefix, read once more for every other request, is
-// more than joining the pieces costs: about 2^15 rows of a head.
+// more than joining the pieces costs: about 2^15 rows of a head, and a pass at least (98 requests of 40 heads behind 10
+// rows: shared 36 us, not 30; 19 of 8 heads behind 333: 13.1, 15.6).
 //
 // Narrow tiles: pieces so that every compute unit has 4 workgroups, of 128 rows at least (one round of the 4 wavefronts;
 // 777 rows of 32 heads: 64 rows 11.5 us, 128 9.9, 256 11.0) and 1024 at most, so that a long request ends with the others
@@ -221,25 +224,31 @@ inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int 
     BatchAttnPlan p;
     const long long columns = static_cast<long long>(b.n_tokens) * group;
     const bool fill = columns >= 64LL * b.n_requests;
-    const bool shared = !fill && static_cast<long long>(b.n_requests - 1) * b.prefix_length * n_kv_heads >= 1 << 15;
+    const bool shared = !fill && static_cast<long long>(b.n_requests - 1) * b.prefix_length * n_kv_heads >= 1 << 15 && b.prefix_length >= kPass;
     // Up to 128 shared columns are cheaper as tiles of 16 that read the prefix out of the L2 again, if that is little next to
     // the requests' own rows: the kernel without the wide tiles has 3 wavefronts per SIMD instead of 2 (72 columns, 1024
     // shared rows, up to 4000 own ones: 121 us, 130; 75 columns, 2558 and 84: 54, 42).
     const long long again = (columns + kFewRows - 1) / kFewRows - 1;
     const bool wide = columns > 128 || again * b.prefix_length * 16 > static_cast<long long>(b.n_requests) * max_rows;
-    p.many = columns > static_cast<long long>(kFewRows) * b.n_requests || (shared && wide);
-    const int tile = p.many ? kManyRows : kFewRows;
+    const bool many = columns > static_cast<long long>(kFewRows) * b.n_requests || (shared && wide);
+    const int tile = many ? kManyRows : kFewRows;
     p.own_tiles = static_cast<int>(columns / tile) + b.n_requests;
     p.own_prefix = shared ? 0 : round_up(b.prefix_length, kPass);
     const int own_rows = p.own_prefix + max_rows;
     const long long items = static_cast<long long>(p.own_tiles) * n_kv_heads;
     if (fill)
         p.own_piece = batch_attn_piece(items, own_rows, 1024, own_rows, 2LL * cus);
-    else if (p.many && items >= cus)
+    else if (many && items >= cus)
         p.own_piece = batch_attn_piece(items, own_rows, 512, 1024, 4LL * cus);
     else
-        p.own_piece = batch_attn_piece(items, own_rows, 128, 1024, p.many ? cus : 4LL * cus);
+        p.own_piece = batch_attn_piece(items, own_rows, 128, 1024, many ? cus : 4LL * cus);
     p.own_splits = ceil_div(own_rows, p.own_piece);
+    // More tiles than the GPU holds workgroups, of few rows each: a wavefront per tile (98 requests of 40 heads, 10 shared and 6 own
+    // rows: 31.1 us, 16.6; 64 of 32 heads: 60 rows 16.9, 16.5; 120 rows 22.9, 27.4).
+    if (many)
+        p.kernel = BatchAttnKernel::kWide;
+    else if (!shared && p.own_splits == 1 && b.prefix_length + max_rows <= kPass && items >= 3LL * cus)
+        p.kernel = BatchAttnKernel::kSingle;
     if (shared) {
         p.shared_tiles = static_cast<int>((columns + tile - 1) / tile);
         // half a workgroup per compute unit: a shared piece has more columns than an own one (16 samples behind 2048 rows: a

@@ -60,7 +60,7 @@ int fits(const llama2_batch* b, int n_kv_heads, int group, int max_rows)
 void plan(const llama2_batch* b, int n_kv_heads, int group, int max_rows, int* out)
 {
     const l2::BatchAttnPlan p = l2::batch_attn_plan(*b, n_kv_heads, group, max_rows, 256);
-    out[0] = p.many, out[1] = p.shared_tiles, out[2] = p.shared_splits, out[3] = p.shared_piece;
+    out[0] = static_cast<int>(p.kernel), out[1] = p.shared_tiles, out[2] = p.shared_splits, out[3] = p.shared_piece;
     out[4] = p.own_tiles, out[5] = p.own_splits, out[6] = p.own_piece, out[7] = p.own_prefix;
 }
 }
@@ -248,9 +248,10 @@ def test_plan_covers_every_row_and_column(lib, requests):
                 for rows in SIZES:
                     b = batch(n_requests=requests, n_tokens=tokens, prefix_length=prefix)
                     lib.plan(b, kv_heads, group, rows, out)
-                    many, tiles, splits, piece, own_tiles, own_splits, own_piece, own_prefix = out
+                    kernel, tiles, splits, piece, own_tiles, own_splits, own_piece, own_prefix = out
                     what = (requests, kv_heads, group, per, prefix, rows, list(out))
-                    tile = 128 if many else 16
+                    tile = 128 if kernel == 2 else 16
+                    assert kernel != 1 or (splits == 0 and own_splits == 1), what  # a wavefront per tile: no pieces
                     assert own_piece % 64 == 0 and own_piece > 0 and 1 <= own_splits <= 256, what
                     assert own_splits * own_piece >= own_prefix + rows > (own_splits - 1) * own_piece, what
                     assert own_tiles >= tokens * group // tile + requests, what
@@ -265,11 +266,13 @@ def test_plan_covers_every_row_and_column(lib, requests):
 def test_plan_shares_a_prefix_among_narrow_requests_only(lib):
     out = (C.c_int * 8)()
     lib.plan(batch(n_requests=16, n_tokens=16, prefix_length=2048), 32, 1, 256, out)
-    assert out[2] > 0 and out[7] == 0 and not out[0]
+    assert out[2] > 0 and out[7] == 0 and out[0] == 0
     lib.plan(batch(n_requests=8, n_tokens=4000, prefix_length=512), 32, 1, 1500, out)
-    assert out[2] == 0 and out[7] == 512 and out[0] and out[5] == 1
+    assert out[2] == 0 and out[7] == 512 and out[0] == 2 and out[5] == 1
     lib.plan(batch(n_requests=1, n_tokens=1, prefix_length=512), 32, 1, 300, out)  # nobody to share with
-    assert out[2] == 0 and out[7] == 512 and not out[0]
+    assert out[2] == 0 and out[7] == 512 and out[0] == 0
+    lib.plan(batch(n_requests=100, n_tokens=100, prefix_length=10), 32, 1, 54, out)
+    assert out[0] == 1 and out[7] == 64
 
 
 def test_plan_refuses_more_workgroups_than_a_launch_holds(lib):

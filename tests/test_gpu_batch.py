@@ -325,6 +325,18 @@ def test_attention_many_requests(requests):
         step(requests, ctx, new, heads=2, kv_heads=2, prefix=prefix, pad=5, fill=np.nan).check("prefix %d" % prefix)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(40, 40), (80, 20), (40, 8)])
+@pytest.mark.parametrize("prefix", [0, 10, 33])
+def test_attention_many_short_requests(d, heads, kv_heads, prefix):
+    """A wavefront per tile: more tiles than workgroups fit, a few rows each, some requests with several tokens or none."""
+    rng = synth.rng_for(1406, d, heads, prefix)
+    n = -(-800 // kv_heads)
+    ctx, new = rng.integers(0, 64 - prefix - 4, n), rng.choice([0, 1, 1, 1, 1, 1, 1, 1, 3], n)
+    new[0], ctx[1], new[1] = 1, 0, 1
+    step(n, ctx, new, 8, heads=heads, kv_heads=kv_heads, d=d, prefix=prefix, pad=3, fill=np.nan).check("short")
+
+
 @pytest.mark.parametrize("size", [8, 16, 32, 64, 128, 256, 1024])
 def test_attention_block_sizes(size):
     for kv_heads in (1, 3):
