@@ -50,7 +50,7 @@ __device__ __forceinline__ int block_scan(int v, int most, int* lds /* 16 */)
 // table entry.  Latency bounds it: lengths, sums, entries and stores follow each other.
 //
 // Workgroups of several compute the same sums and take every so many thousandth token each (14579 tokens: one workgroup 15.6
-// us, 15 workgroups 7.0).  Where lengths or the number of taken blocks are updated in place, the last workgroup to have
+// us, 15 workgroups 5.8).  Where lengths or the number of taken blocks are updated in place, the last workgroup to have
 // read them writes them.
 __global__ __launch_bounds__(kTablesBlock) void batch_tables_kernel(TablesArgs a)
 {
@@ -84,7 +84,8 @@ __global__ __launch_bounds__(kTablesBlock) void batch_tables_kernel(TablesArgs a
             begin[tid] = end;
             rows[tid] = c;
             from[tid] = !admitted ? -1 : need > 0 ? taken + upto - need : 0;
-            if (admitted && upto > 0)
+            const unsigned long long who = __ballot(admitted); // the sums never fall: a wavefront's last one has its largest
+            if (admitted && (who >> (tid & 63)) == 1)
                 atomicMax(&most_taken, upto);
             if (b < a.n_requests) {
                 if (starts)
