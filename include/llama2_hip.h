@@ -385,13 +385,17 @@ int llama2_batch_qk_norm_rope(llama2_half* q_output, const llama2_half* q, const
  * prefix_length rows of the prefix table and the own rows 0 .. p - prefix_length
  * of the request (row r: block_tables[b][r / block_size]); query head h
  * uses key/value head h / (n_heads / n_kv_heads).  Scores and softmax stay in fp32,
- * probabilities are rounded to fp16 relative to the largest one so far
- * (llama2_multi_head_attention rounds scores to fp16 instead, as the reference
- * does).  Rows of a block id outside the cache are not attended; a token left
- * without rows gives zeros.  Rows behind a token's own, and the rest of the last block,
- * have no influence whatever they hold.  The shared rows are read once for all requests.
- * `output` must not overlap the other buffers.  Reads query_starts, positions,
- * block_tables and prefix_table of the batch.
+ * probabilities are rounded to fp16 on their way into the products with the values
+ * (llama2_multi_head_attention rounds scores to fp16 instead, as the reference does).
+ * Rows of a block id outside the cache are not attended; a token left without rows gives
+ * zeros.  Rows behind a token's own, and the rest of the last block, have no influence
+ * whatever they hold; an infinite value that a token does attend may reach its output as
+ * NaN.  Where it saves reading, the shared rows are read once for up to 128 query rows
+ * instead of once per request.  The same call gives the same bits every time.
+ * positions of a request must not decrease; max_length bounds the launch, rows beyond it
+ * are not attended; any scale is allowed.  `output` must not overlap the other buffers.
+ * Reads query_starts, positions, block_tables and prefix_table of the batch, as
+ * llama2_batch_tables leaves them.  At most 2^29 rows per token and 2^26 query rows.
  * Scratch: as llama2_multi_head_attention (call once before capturing). */
 int llama2_batch_attention(llama2_half* output, const llama2_half* query, const llama2_batch* batch,
                            const llama2_paged_cache* cache, int n_heads, int output_stride,

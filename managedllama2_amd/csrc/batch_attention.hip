@@ -5,11 +5,15 @@
 //   S^T = K Q^T,   O^T = V^T P^T
 // on the matrix cores: with rows of the cache along the first operand, a lane ends up with the scores of ONE query, and
 // its probabilities are already the second operand of the second product.  A workgroup takes one item:
-//   shared   up to 128 columns out of all tokens (of any request) x a piece of the prefix: every shared row is read
-//            once per 128 columns instead of once per request;
-//   own      up to 128 columns of one request x a piece of its own rows (behind the prefix where a request has so many
-//            columns of its own that sharing would not save any reading).
-// Pieces leave fp32 sums, maximum and denominator; batch_attn_merge_kernel joins them in order.
+//   own      a tile of columns of one request x a piece of its own rows, behind the prefix where that is not shared;
+//   shared   a tile of columns out of all tokens, of any request, x a piece of the prefix: a shared row is read once per
+//            tile instead of once per request.
+// Pieces leave fp32 sums, maximum and denominator, which are joined in order.
+//
+// Tiles of up to 16 columns (few_rows) are bound by reading the cache: 979 MB of four long documents in 194 us, 5.0 TB/s, HBM
+// traffic 1.00 times that; 594 MB of 64 conversations in 118 us, 1.02 times (a plain read of 1 GiB reaches 6.0 .. 6.3).  Tiles of
+// up to 128 columns (many_rows) are bound by the chain of a pass, products and exponentials side by side only as far as two
+// wavefronts per SIMD allow: 16384 tokens of 8 heads 840 TFLOP/s, where a library product of 8192^3 reaches 1235.
 #include "common.hpp"
 #include "batch_plan.hpp"
 
@@ -197,10 +201,13 @@ __device__ void join_pieces(const BatchAttnArgs& a, int token, int head, int slo
 }
 
 // ---------------------------------------------------------------- few columns
-// Up to 16 columns: bound by reading the cache.  Each of the 4 wavefronts takes every fourth tile of 32 rows, straight from
-// memory into the operands' registers.  Lane (g, c), g = lane / 16: keys of row 16 t + c, elements 32 j + 8 g .. + 7
-// (64 consecutive bytes of a row per load and row); values of the rows 16 t + 4 g .. + 3, whose scores the same lane holds, 1/16 of a
-// row each (4 whole rows per load), turned by byte permutations into columns: operand i holds elements c * D/16 + i.
+// Up to 16 columns.  Each of 4 wavefronts takes every fourth tile of 32 rows (or one wavefront all of them), straight from
+// memory into the operands' registers: no row is used twice, so LDS would only be a detour.  Lane (g, c), g = lane / 16: keys of
+// row 16 t + c, elements 32 j + 8 g .. + 7 (64 consecutive bytes of a row per load and row); values of the rows 16 t + 4 g .. + 3,
+// whose scores the same lane holds, 1/16 of a row each (4 whole rows per load), turned by byte permutations into columns:
+// operand i holds elements c * D/16 + i.  16 KB are on their way per wavefront, 12 wavefronts per compute unit; with the
+// next tile requested ahead the registers allow fewer of them, and it was slower (64 conversations 136 -> 162 us), with 16
+// wavefronts registers spill (123 -> 162).
 template <int D, int WAVES>
 __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
 {
@@ -424,7 +431,7 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
         for (int x = 0; x < QUADS; ++x) {
             float* to = a.parts + part * D + d + 4 * x;
             if (a.counters) // written through, for the workgroup that joins the pieces in this launch
-                asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(to), "v"(e[x]) : "memory");
+                asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 0" : : "v"(to), "v"(e[x]) : "memory"); // s_nop: e may be overwritten next
             else
                 *reinterpret_cast<f4_t*>(to) = e[x];
         }

@@ -198,11 +198,11 @@ struct BatchAttnPlan {
     long long items(int n_kv_heads) const { return shared_items(n_kv_heads) + static_cast<long long>(own_tiles) * own_splits * n_kv_heads; }
 };
 
-// Pieces of `rows` cache rows, for `items` of them in each piece: `want` workgroups altogether, but pieces not shorter than
-// `shortest` nor longer than `longest`.
+// Pieces of `rows` cache rows, for `items` of them in each piece: up to `want` workgroups altogether, but pieces not shorter
+// than `shortest` nor longer than `longest`.
 inline int batch_attn_piece(long long items, int rows, int shortest, int longest, long long want)
 {
-    const long long enough = (want + items - 1) / items, most = ceil_div(rows, shortest), least = ceil_div(rows, longest);
+    const long long enough = want > items ? want / items : 1, most = ceil_div(rows, shortest), least = ceil_div(rows, longest);
     long long n = enough < most ? enough : most;
     n = n > least ? n : least;
     n = n < kMaxPieces ? n : kMaxPieces;
@@ -217,8 +217,9 @@ inline int batch_attn_piece(long long items, int rows, int shortest, int longest
 // Narrow tiles: pieces so that every compute unit has 4 workgroups, of 128 rows at least (one round of the 4 wavefronts;
 // 777 rows of 32 heads: 64 rows 11.5 us, 128 9.9, 256 11.0) and 1024 at most, so that a long request ends with the others
 // (64 conversations: 512 rows 133 us, 1024 133, 4096 170; four documents of up to 131000 rows: 215, 203, 218).
-// Wide tiles are bound by the matrix cores, and the sums of their pieces weigh more than the cache: 2 workgroups per
-// compute unit, of 512 rows at least.
+// Wide tiles are bound by the matrix cores, and the sums of their pieces weigh more than the cache: 2 workgroups per compute
+// unit, of 1024 rows at least for prompts, of 128 to 512 where prompts and single tokens mix (a mixed step: 1 workgroup per
+// compute unit 76 us, 2 60, 3 69; another one: 44, 53, 53).
 inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int group, int max_rows, int cus)
 {
     BatchAttnPlan p;
@@ -241,7 +242,7 @@ inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int 
     else if (many && items >= cus)
         p.own_piece = batch_attn_piece(items, own_rows, 512, 1024, 4LL * cus);
     else
-        p.own_piece = batch_attn_piece(items, own_rows, 128, 1024, many ? cus : 4LL * cus);
+        p.own_piece = batch_attn_piece(items, own_rows, 128, 1024, many ? 2LL * cus : 4LL * cus);
     p.own_splits = ceil_div(own_rows, p.own_piece);
     // More tiles than the GPU holds workgroups, of few rows each: a wavefront per tile (98 requests of 40 heads, 10 shared and 6 own
     // rows: 31.1 us, 16.6; 64 of 32 heads: 60 rows 16.9, 16.5; 120 rows 22.9, 27.4).
@@ -251,9 +252,10 @@ inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int 
         p.kernel = BatchAttnKernel::kSingle;
     if (shared) {
         p.shared_tiles = static_cast<int>((columns + tile - 1) / tile);
-        // half a workgroup per compute unit: a shared piece has more columns than an own one (16 samples behind 2048 rows: a
-        // whole one 20.8 us, half a one 19.4)
-        p.shared_piece = batch_attn_piece(static_cast<long long>(p.shared_tiles) * n_kv_heads, b.prefix_length, 128, 1024, cus / 2);
+        // a workgroup per compute unit, half a one of wide tiles: the rest is for the requests' own rows (16 samples behind 2048
+        // rows 17.2 us, twice as many workgroups 20.8)
+        p.shared_piece = batch_attn_piece(static_cast<long long>(p.shared_tiles) * n_kv_heads, b.prefix_length, 128, 1024,
+                                          many ? cus / 2 : cus);
         p.shared_splits = ceil_div(b.prefix_length, p.shared_piece);
     }
     return p;

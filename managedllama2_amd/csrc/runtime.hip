@@ -108,6 +108,7 @@ int llama2_init(int device)
     L2_HIP(hipMemset(c.attn_counters, 0, kMaxAttnHeads * sizeof(unsigned)));
     L2_HIP(hipMalloc(reinterpret_cast<void**>(&c.batch_counters), (kMaxBatchCounters + 1) * sizeof(unsigned)));
     L2_HIP(hipMemset(c.batch_counters, 0, (kMaxBatchCounters + 1) * sizeof(unsigned)));
+    L2_HIP(hipStreamSynchronize(nullptr)); // the library's stream does not wait for the null stream's fills
     L2_HIP(hipMalloc(reinterpret_cast<void**>(&c.sampler), sizeof(SamplerScratch)));
     L2_HIP(hipHostMalloc(reinterpret_cast<void**>(&c.host_token), sizeof(int), hipHostMallocMapped | hipHostMallocCoherent));
     c.device = device;

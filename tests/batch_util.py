@@ -72,10 +72,11 @@ def attention(q, key, value, prefix_rows, own_rows, positions, prefix, scale, kv
             y, size = p @ vh[use] / p.sum(), p @ np.abs(vh[use]) / p.sum()
             m = use.sum()
             # fp16 result; probabilities as fp16 (half a step each), their exponents: d terms in fp32, the scale and the base
-            # (|s| 2^-24 each), exp2 itself 2^-22; sums over m rows in fp32 in any order; what fp16 drops below 2^-39
+            # (|s| 2^-24 each), exp2 itself 2^-22; sums over m rows in fp32 in any order; below fp16's normal numbers half a step is
+            # 2^-25, of probabilities that enter times 2^6: 2^-31 of the largest
             eps = 2.0 ** -11 + 2 * ((d + 4) * 2.0 ** -24 * reach + 4 * 2.0 ** -24 * np.abs(s).max() + 2.0 ** -22) + 2 * m * 2.0 ** -24
             out[t, h * d:(h + 1) * d] = y
-            bound[t, h * d:(h + 1) * d] = 2.0 ** -11 * np.abs(y) + 2.0 ** -25 + eps * size + m * 2.0 ** -38 * np.abs(vh[use]).max()
+            bound[t, h * d:(h + 1) * d] = 2.0 ** -11 * np.abs(y) + 2.0 ** -25 + eps * size + m * 2.0 ** -31 * np.abs(vh[use]).max()
     return out, bound
 
 
