@@ -13,7 +13,7 @@
 // Tiles of up to 16 columns (few_rows) are bound by reading the cache: 979 MB of four long documents in 194 us, 5.0 TB/s, HBM
 // traffic 1.00 times that; 594 MB of 64 conversations in 118 us, 1.02 times (a plain read of 1 GiB reaches 6.0 .. 6.3).  Tiles of
 // up to 128 columns (many_rows) are bound by the chain of a pass, products and exponentials side by side only as far as two
-// wavefronts per SIMD allow: 16384 tokens of 8 heads 840 TFLOP/s, where a library product of 8192^3 reaches 1235.
+// wavefronts per SIMD allow: 16384 tokens of 8 heads 815 TFLOP/s, where a library product of 8192^3 reaches 1235.
 #include "common.hpp"
 #include "batch_plan.hpp"
 
