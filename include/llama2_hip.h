@@ -357,7 +357,8 @@ typedef struct llama2_batch {
  * new_taken[0] is above n_free.  With taken[0] above n_free (or negative) the list counts as
  * empty and new_taken[0] is taken[0]: nobody gets a block until the caller, who has to find blocks
  * or pause requests then, gives a new list.
- * Block ids are copied, not looked at; free_blocks and the tables must not hold an id twice.
+ * Block ids are copied, not looked at; free_blocks and the tables must not hold an id twice.  An id whose
+ * slots would be negative or pass 2^31 gives slot -1.
  * prefix_table and max_length are not read. */
 int llama2_batch_tables(const llama2_batch* batch, const int* cached, const int* counts,
                         const int* free_blocks, int n_free, const int* taken, int* new_taken,

@@ -120,7 +120,8 @@ __global__ __launch_bounds__(kTablesBlock) void batch_tables_kernel(TablesArgs a
                     if ((row & (size - 1)) == 0)
                         *entry = block;
                     position = a.prefix_length + row;
-                    slot = (block << a.shift) + (row & (size - 1));
+                    if (block >= 0 && block <= 0x7FFFFFFF >> a.shift) // else its slots are no ints, and would alias others
+                        slot = (block << a.shift) + (row & (size - 1));
                 }
                 a.positions[t] = position;
                 a.slots[t] = slot;

@@ -117,6 +117,20 @@ def test_tables_of_a_request_that_goes_on_behind_a_refused_one():
     assert c.lengths.to_host().tolist() == [8, 7, 8] and int(c.new_taken[0]) == 5
 
 
+def test_tables_of_block_ids_that_have_no_slots():
+    # 16 rows per block: 2^27 - 1 is the last id whose slots are ints; 2^28 would come out as block 0 again
+    ids = [(1 << 27) - 1, 1 << 27, 1 << 28, (1 << 28) + 3, -1, -(1 << 31), 5]
+    n = len(ids)
+    table, cached, counts = up(np.zeros((n, 2), np.int32)), zeros(n), up(np.full(n, 2, np.int32))
+    lengths, starts, positions, slots = zeros(n), zeros(n + 1), zeros(2 * n), zeros(2 * n)
+    b = capi.Batch(table.ptr, lengths.ptr, starts.ptr, positions.ptr, slots.ptr, None, n, 2 * n, 2, 0, 0)
+    free, taken = up(np.array(ids, np.int32)), zeros(1)
+    capi.call("llama2_batch_tables", b, cached.ptr, counts.ptr, free.ptr, n, taken.ptr, taken.ptr, 16)
+    first = [i * 16 if 0 <= i < 1 << 27 else -1 for i in ids]
+    assert slots.to_host().tolist() == [v for s in first for v in (s, s + 1 if s >= 0 else -1)]
+    assert positions.to_host().tolist() == [0, 1] * n and table.to_host().reshape(n, 2)[:, 0].tolist() == ids
+
+
 def test_tables_in_place_and_replayed():
     """Lengths and the number of taken blocks updated in place: a captured step counts on by itself."""
     c = tables_case(12, 40, 8, 50, 1, pad=4, short=-200, stride=30)
