@@ -369,11 +369,12 @@ int llama2_batch_tables(const llama2_batch* batch, const int* cached, const int*
  * of `head_size` elements: y = x / sqrt(mean(x^2) + eps) * gamma if gamma (q_gamma
  * for queries, k_gamma for keys; head_size halfs, null: no norm), then pairs (i, i +
  * head_size/2) rotated by position * theta^(-2 i / head_size) as llama2_rope does, one rounding at the
- * end.  The angle is exact to 2^-32 of a turn at every position (llama2_rope's,
+ * end.  The angle is good to 2^-25 of a turn at every position (llama2_rope's,
  * like the reference's, loses bits as positions grow: the two differ by roundings).
  * Rows of q, k, v and q_output are q_stride, kv_stride and q_output_stride halfs
  * apart (multiples of 8, pointers 16-byte aligned), so that they may be parts of one buffer.
- * q_output may be q with the same stride; it must not overlap otherwise.  No two tokens may
+ * q_output may be q with the same stride (rows of k and v between q's must have that stride
+ * too); it must not overlap otherwise.  Keys and values of the cache must not overlap.  No two tokens may
  * have the same slot.  A token whose slot is not one of the cache's is not stored.
  * Reads positions and slots of the batch.  1 <= theta. */
 int llama2_batch_qk_norm_rope(llama2_half* q_output, const llama2_half* q, const llama2_half* k,

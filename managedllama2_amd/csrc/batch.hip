@@ -173,7 +173,8 @@ struct RopeArgs {
 };
 
 // Turns per position of pair i, theta^(-2 i / head_size) / 2 pi, in 64 bits of fixed point: times a position, the bits above are
-// whole turns and drop out by themselves.  2^31 positions times six products off by 2^-64 each leave 2^-30 of a turn.
+// whole turns and drop out by themselves.  Six products, and powers that are off by
+// up to 2^-59 after their squarings, leave less than 2^-28 of a turn at 2^31 positions; the rounding to fp32 behind it is 2^-26.
 __device__ __forceinline__ unsigned long long turns_of(const unsigned long long (&powers)[6], int i)
 {
     unsigned long long v = 0x28BE60DB9391054Bull; // 1 / 2 pi

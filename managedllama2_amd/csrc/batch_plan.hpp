@@ -4,6 +4,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <utility>
 
 #include "../../include/llama2_hip.h"
 
@@ -77,6 +78,20 @@ inline int check_paged_cache(const char* fn, const llama2_paged_cache* c, int n_
     return LLAMA2_OK;
 }
 
+// `n` rows of a_width halfs from `a` on and as many of b_width from `b` on, both `stride` halfs apart (no less than the
+// widths): does one of the first overlap one of the others?
+inline bool rows_overlap(const void* a, long long a_width, const void* b, long long b_width, long long n, long long stride)
+{
+    uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    if (x > y) {
+        std::swap(x, y);
+        std::swap(a_width, b_width);
+    }
+    const uintptr_t s = static_cast<uintptr_t>(stride) * 2, of = (y - x) / s, rest = (y - x) % s; // only these two rows of the first can
+    const uintptr_t last = static_cast<uintptr_t>(n - 1);
+    return (of <= last && rest < static_cast<uintptr_t>(a_width) * 2) || (of + 1 <= last && s - rest < static_cast<uintptr_t>(b_width) * 2);
+}
+
 inline size_t rows_bytes(int rows, int stride, int width) { return (static_cast<size_t>(rows - 1) * stride + width) * 2; }
 
 inline int check_batch_tables(const llama2_batch* batch, const int* cached, const int* counts, const int* free_blocks, int n_free,
@@ -138,9 +153,14 @@ inline int check_batch_rope(const llama2_half* q_output, const llama2_half* q, c
     const size_t out_bytes = rows_bytes(t, q_output_stride, q_row), kv_bytes = rows_bytes(t, kv_stride, kv_row);
     const bool in_place = q_output == q && q_output_stride == q_stride;
     L2_CHECK(in_place || !overlap(q_output, out_bytes, q, rows_bytes(t, q_stride, q_row)), "%s: q_output overlaps q without being it", fn);
-    // in place, the rows of k and v may lie between those of q
-    L2_CHECK(in_place || (!overlap(q_output, out_bytes, k, kv_bytes) && !overlap(q_output, out_bytes, v, kv_bytes)),
-             "%s: q_output overlaps k or v", fn);
+    for (const llama2_half* x : {k, v}) { // in place, their rows may lie between those of q
+        const bool between = in_place && kv_stride == q_stride && !rows_overlap(q, q_row, x, kv_row, t, q_stride);
+        L2_CHECK(between || !overlap(q_output, out_bytes, x, kv_bytes), "%s: q_output overlaps k or v", fn);
+    }
+    // blocks of keys and values may take turns
+    L2_CHECK(!rows_overlap(cache->key, static_cast<long long>(cache->block_size) * kv_row, cache->value,
+                           static_cast<long long>(cache->block_size) * kv_row, cache->n_blocks, block_halfs(*cache)),
+             "%s: the cache's keys and values overlap", fn);
     const void* written[] = {cache->key, cache->value};
     for (const void* c : written)
         L2_CHECK(!overlap(c, cache_bytes(*cache), q, rows_bytes(t, q_stride, q_row)) && !overlap(c, cache_bytes(*cache), k, kv_bytes) &&

@@ -162,6 +162,14 @@ def test_rope_refusals(lib):
     assert call_rope(lib, batch(), cache(), **dict(fused, o=310 * MIB, so=1536)) == 0  # in place
     assert call_rope(lib, batch(), cache(), **dict(fused, o=310 * MIB, so=1024)) == INVALID
     assert call_rope(lib, batch(), cache(), **dict(fused, o=310 * MIB + 2048, so=1536)) == INVALID
+    # in place, rows of k and v only between those of q: 1024 of q, 256 of k, 256 of v in 1536
+    place = dict(fused, o=310 * MIB, so=1536)
+    for name in ("k", "v"):
+        for at in (0, 16, 2048 - 16, 2560 + 16, 2 * 1536 * 8, -16):
+            assert call_rope(lib, batch(), cache(), **dict(place, **{name: 310 * MIB + at})) == INVALID, (name, at)
+        for at in (2048, 2560, 2048 + 2 * 1536 * 8, -512, -1024):  # of the same row, of the last one, in front
+            assert call_rope(lib, batch(), cache(), **dict(place, **{name: 310 * MIB + at})) == 0, (name, at)
+        assert call_rope(lib, batch(), cache(), **dict(place, skv=1528)) == INVALID
     for name in ("o", "q", "k", "v"):
         assert call_rope(lib, batch(), cache(), **{name: None}) == INVALID, name
     for name in ("o", "q", "k", "v", "gq", "gk"):
@@ -178,6 +186,23 @@ def test_rope_refusals(lib):
     for name in ("o", "q", "k", "v"):  # inside the cache
         assert call_rope(lib, batch(), cache(), **{name: 100 * MIB + 4096}) == INVALID, name
     assert call_rope(lib, None, cache()) == INVALID and call_rope(lib, batch(), None) == INVALID
+
+
+def test_rope_refuses_keys_over_values(lib):
+    block = 16 * 256  # halfs of a block, 2 bytes each; 50 blocks
+    for at in (0, 16, 2 * block - 16, 2 * block, 50 * 2 * block - 16):
+        assert call_rope(lib, batch(), cache(value=100 * MIB + at)) == INVALID, at
+        assert call_rope(lib, batch(), cache(key=200 * MIB + at, value=200 * MIB)) == INVALID, at
+    assert call_rope(lib, batch(), cache(value=100 * MIB + 50 * 2 * block)) == 0
+    turns = dict(block_stride=2 * block)  # blocks of keys and values in turn
+    for at, want in ((2 * block, 0), (2 * block - 16, INVALID), (2 * block + 16, INVALID), (6 * block, 0), (4 * block, INVALID),
+                     (49 * 4 * block + 2 * block + 16, 0), (49 * 4 * block + 2 * block - 16, INVALID)):
+        assert call_rope(lib, batch(), cache(value=100 * MIB + at, **turns)) == want, at
+        assert call_rope(lib, batch(), cache(key=200 * MIB + at, value=200 * MIB, **turns)) == want, at
+    one = cache(n_blocks=1, value=100 * MIB + 2 * block - 16, block_stride=2 * block)
+    assert call_rope(lib, batch(), one) == INVALID
+    assert call_rope(lib, batch(), cache(n_blocks=1, value=100 * MIB + 2 * block + 16, block_stride=2 * block)) == 0
+    assert call_attention(lib, batch(), cache(value=100 * MIB)) == 0  # which only reads them
 
 
 def test_cache_refusals(lib):
