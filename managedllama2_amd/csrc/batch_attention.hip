@@ -50,7 +50,7 @@ struct BatchAttnArgs {
     uint32_t q_sign; // what turns the queries over where the scale is negative
     // items: [shared_splits x n_kv_heads, by eights][shared_tiles][of the eight], and [own_splits][own_tiles][n_kv_heads]
     int shared_items, shared_tiles, shared_splits, shared_piece;
-    int own_items, own_tiles, own_piece, own_prefix; // own_prefix: prefix rows in front of a request's own, a multiple of kPass, or 0
+    int own_items, own_tiles, own_piece, own_prefix, spread; // own_prefix: prefix rows in front of a request's own, a multiple of kPass, or 0
 };
 
 // What a workgroup computes; the same in all its lanes.
@@ -201,7 +201,7 @@ __device__ void join_pieces(const BatchAttnArgs& a, int token, int head, int slo
 }
 
 // ---------------------------------------------------------------- few columns
-// Up to 16 columns.  Each of 4 wavefronts takes every fourth tile of 32 rows (or one wavefront all of them), straight from
+// Up to 16 columns.  Each of 4 wavefronts takes every fourth tile of 32 rows (each of 8 every eighth, or one wavefront all of them), straight from
 // memory into the operands' registers: no row is used twice, so LDS would only be a detour.  Lane (g, c), g = lane / 16: keys of
 // row 16 t + c, elements 32 j + 8 g .. + 7 (64 consecutive bytes of a row per load and row); values of the rows 16 t + 4 g .. + 3,
 // whose scores the same lane holds, 1/16 of a row each (4 whole rows per load), turned by byte permutations into columns:
@@ -379,11 +379,11 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
         return;
     }
 
-    // The four wavefronts' sums through LDS, then each adds up a quarter of the elements: those with k == wave, which are
+    // The wavefronts' sums through LDS, then each of the first four adds up a quarter of the elements: those with k == wave, which are
     // VE neighbours in each lane.
     constexpr int QUADS = VE / 4;
     f4_t* all = reinterpret_cast<f4_t*>(lds);
-    float2* stat = reinterpret_cast<float2*>(lds + 4 * VE * 64 * 16);
+    float2* stat = reinterpret_cast<float2*>(lds + WAVES * VE * 64 * 16);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -392,22 +392,24 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
     if (g == 0)
         stat[wave * 16 + c] = float2{m, sum};
     __syncthreads();
-    float most = -INFINITY, total = 0.0f, weight[4];
+    float most = -INFINITY, total = 0.0f, weight[WAVES];
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
+    for (int w = 0; w < WAVES; ++w)
         most = fmaxf(most, stat[w * 16 + c].x);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
         const float2 st = stat[w * 16 + c];
         weight[w] = weight_of(st.x, most);
         total = fmaf(weight[w], st.y, total);
     }
+    if (WAVES > 4 && wave >= 4)
+        return; // there is no barrier behind this one: a.counters is null
     f4_t e[QUADS];
 #pragma unroll
     for (int x = 0; x < QUADS; ++x) {
         e[x] = f4_t{};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const f4_t y = all[((w * 4 + wave) * QUADS + x) * 64 + lane];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -440,7 +442,7 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
             store_agent(&a.stats[part].y, total);
         }
     }
-    if (!a.counters)
+    if (WAVES != 4 || !a.counters)
         return;
 
     // Tokens whose last piece this was; nothing is shared, and their columns lie in one tile each: the group divides 16.
@@ -473,7 +475,8 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
 // ---------------------------------------------------------------- many columns
 // 17 to 128 columns, 32 per wavefront: passes of 64 rows through LDS, read by all four.  The rows of the next pass go
 // straight from memory into the other of two LDS buffers while this one is computed, so a pass has one barrier and no
-// register holds rows in flight.  Rows lie in LDS as in the cache, their 16-byte pieces exchanged by row so that reads have
+// register holds rows in flight.  With two halves (8 wavefronts, the columns twice) each half has buffers of its own and takes
+// every other pass, and their sums are joined at the end.  Rows lie in LDS as in the cache, their 16-byte pieces exchanged by row so that reads have
 // no bank conflicts; values come out transposed (ds_read_b64_tr_b16: 4 rows of 16 elements per 16 lanes, a column each), in
 // the order in which a lane holds their probabilities (4 rows of one half of the lanes, 4 of the other).
 template <int D>
@@ -500,12 +503,14 @@ __device__ __forceinline__ h4_t read_transposed(const char* p)
     return __builtin_bit_cast(h4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p)));
 }
 
-template <int D>
-__device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
+template <int D, int HALVES>
+__device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* all_lds)
 {
     using L = ManyLds<D>;
     constexpr int QS = D / 16, DT = D / 32; // k steps, tiles of output elements
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    const int half = HALVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8); // takes every other pass
+    char* const lds = all_lds + half * L::kTotal;
     const int hl = lane >> 5, l31 = lane & 31;
     const int r = wave * 32 + l31, rq = min(r, it.rows - 1);
     const bool idle = wave * 32 >= it.rows;
@@ -568,17 +573,20 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
             }
         };
         __syncthreads(); // the last pass of the shared rows has been read
-        look_up(begin);
+        look_up(begin + half * kPass);
         int no_block = (!in_cache(a, block[0]) ? 1 : 0) | (!in_cache(a, block[1]) ? 2 : 0); // of the pass that is on its way
-        request(begin, 0);
-        look_up(begin + kPass);
+        if (HALVES == 1 || begin + half * kPass < end)
+            request(begin + half * kPass, 0);
+        look_up(begin + (half + HALVES) * kPass);
         int buffer = 0;
-        for (int tb = begin; tb < end; tb += kPass, buffer ^= 1) {
+        for (int first = begin; first < end; first += HALVES * kPass, buffer ^= 1) {
+            const int tb = first + half * kPass;
+            const bool here = HALVES == 1 || tb < end;
             char* const ks = lds + buffer * L::kBuffer;
             char* const vs = ks + L::kTensor;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // this wavefront's share of the pass lies in LDS
             int found = 0;
-            if (no_block || tb + kPass > wg_all_see) {
+            if (here && (no_block || tb + kPass > wg_all_see)) {
                 // What lies behind the last row, or in a block that is none, and what is infinite or NaN in rows that some
                 // columns attend and others do not, must not reach a sum through a probability of 0.
                 for (int x = lane; x < 16 * L::kPieces; x += 64) {
@@ -602,12 +610,12 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
             if (lane == 0)
                 flags[buffer * 4 + wave] = no_block | found;
             __syncthreads(); // everybody's share does, and the other buffer has been read
-            if (tb + kPass < end) {
+            if (tb + HALVES * kPass < end) {
                 no_block = (!in_cache(a, block[0]) ? 1 : 0) | (!in_cache(a, block[1]) ? 2 : 0);
-                request(tb + kPass, buffer ^ 1);
-                look_up(tb + 2 * kPass);
+                request(tb + HALVES * kPass, buffer ^ 1);
+                look_up(tb + 2 * HALVES * kPass);
             }
-            if (idle || tb >= any_sees)
+            if (!here || idle || tb >= any_sees)
                 continue;
             int no_rows = 0, said = 0; // no_rows: a bit per 8 rows
 #pragma unroll
@@ -698,6 +706,35 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* lds)
         }
     }
     sum += __shfl_xor(sum, 32, 64);
+    if constexpr (HALVES == 2) { // the other half's sums through LDS
+        f4_t* const others = reinterpret_cast<f4_t*>(all_lds) + wave * DT * 4 * 64;
+        float2* const other = reinterpret_cast<float2*>(all_lds + 4 * DT * 4 * 64 * 16) + wave * 64;
+        __syncthreads();
+        if (half == 1) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    others[(d * 4 + k) * 64 + lane] = f4_t{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+            other[lane] = float2{m, sum};
+        }
+        __syncthreads();
+        if (half == 1)
+            return;
+        const float2 st = other[lane];
+        const float most = fmaxf(m, st.x), wa = weight_of(m, most), wb = weight_of(st.x, most);
+        m = most;
+        sum = fmaf(wb, st.y, sum * wa);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const f4_t y = others[(d * 4 + k) * 64 + lane];
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    o[d][4 * k + x] = fmaf(wb, y[x], o[d][4 * k + x] * wa);
+            }
+    }
     if (r >= it.rows || position < 0)
         return;
     if (a.parts) {
@@ -740,19 +777,20 @@ __device__ __forceinline__ int request_start(const BatchAttnArgs& a, int request
     return min(max(uniform_load(a.query_starts, request), 0), a.n_tokens);
 }
 
-template <int D>
-constexpr int kFewLds = 4 * (D / 16) * 1024 + 512;
-template <int D>
-constexpr int kAttnLds = ManyLds<D>::kTotal > kFewLds<D> ? ManyLds<D>::kTotal : kFewLds<D>;
+template <int D, int WAVES>
+constexpr int kFewLds = WAVES * ((D / 16) * 1024 + 128);
+template <int D, int HALVES>
+constexpr int kManyLds = HALVES * ManyLds<D>::kTotal > kFewLds<D, 4 * HALVES> ? HALVES * ManyLds<D>::kTotal : kFewLds<D, 4 * HALVES>;
 
 // kNarrow: a workgroup per tile of up to 16 columns.  kSingle: a wavefront per tile, for many tiles of few rows, where most
-// of a workgroup would have no rows; no sharing and no pieces.  kWide: a workgroup per tile of up to 128 columns.
+// of a workgroup would have no rows; no sharing and no pieces.  kWide: a workgroup per tile of up to 128 columns.  kTall: the same
+// with two halves of the workgroup that take turns with the passes, where there are no more tiles than compute units.
 template <int D, BatchAttnKernel KIND>
-__global__ __launch_bounds__(256, KIND == BatchAttnKernel::kWide ? 2 : 3) void batch_attn_kernel(BatchAttnArgs a)
+__global__ __launch_bounds__(KIND == BatchAttnKernel::kTall ? 512 : 256, KIND == BatchAttnKernel::kWide || KIND == BatchAttnKernel::kTall ? 2 : 3) void batch_attn_kernel(BatchAttnArgs a)
 {
-    constexpr bool MANY = KIND == BatchAttnKernel::kWide, SINGLE = KIND == BatchAttnKernel::kSingle;
+    constexpr bool TALL = KIND == BatchAttnKernel::kTall, MANY = KIND == BatchAttnKernel::kWide || TALL, SINGLE = KIND == BatchAttnKernel::kSingle;
     constexpr int kTileRows = MANY ? kManyRows : kFewRows;
-    __shared__ __align__(16) char lds[MANY ? kAttnLds<D> : SINGLE ? 16 : kFewLds<D>];
+    __shared__ __align__(16) char lds[MANY ? kManyLds<D, TALL ? 2 : 1> : SINGLE ? 16 : kFewLds<D, 4>];
     Item it = {};
     const int shared_items = a.shared_items;
     // Wide tiles of shared rows first, they take longest; narrow ones last, to fill up what long requests leave idle (64
@@ -783,10 +821,8 @@ __global__ __launch_bounds__(256, KIND == BatchAttnKernel::kWide ? 2 : 3) void b
         const int split = of_heads / a.own_tiles, turn = of_heads % a.own_tiles;
         // wide tiles from the last one on: of a prompt, later tiles see more rows (3827 prompt tokens 102 -> 92 us)
         const int tile = MANY ? a.own_tiles - 1 - turn : turn;
-        // An XCD gets every eighth workgroup.  Wide tiles: a head's tiles all go to one, whose L2 then serves the rows to
-        // all of them.  Narrow ones read every row once: an XCD takes all heads in turn, because the rows of one head
-        // alone lie in few channels of its L2.
-        it.kv_head = (MANY ? index : index + of_heads) % a.n_kv_heads;
+        // An XCD gets every eighth workgroup: the same heads every time, or all of them in turn.
+        it.kv_head = (a.spread ? index + of_heads : index) % a.n_kv_heads;
         // The request: the one it would be if all brought one token, else by counting, 64 at a time.
         int request = min(((tile + 1) * kTileRows - 1) / (kTileRows + a.group), a.n_requests - 1);
         int start = request_start(a, request), stop = request_start(a, request + 1);
@@ -839,11 +875,11 @@ __global__ __launch_bounds__(256, KIND == BatchAttnKernel::kWide ? 2 : 3) void b
     }
     if constexpr (MANY) {
         if (it.rows > kFewRows) {
-            many_rows<D>(a, it, lds);
+            many_rows<D, TALL ? 2 : 1>(a, it, lds);
             return;
         }
     }
-    few_rows<D, SINGLE ? 1 : 4>(a, it, lds);
+    few_rows<D, SINGLE ? 1 : TALL ? 8 : 4>(a, it, lds);
 }
 
 // Joins the pieces of a token's head, in order, where no workgroup of the attention does: LANES lanes per row, D / 8 of
@@ -908,6 +944,8 @@ static void batch_attn_launch(const BatchAttnArgs& a, BatchAttnKernel kind, int 
 {
     if (kind == BatchAttnKernel::kWide)
         hipLaunchKernelGGL((batch_attn_kernel<D, BatchAttnKernel::kWide>), dim3(items), dim3(256), 0, ctx().stream, a);
+    else if (kind == BatchAttnKernel::kTall)
+        hipLaunchKernelGGL((batch_attn_kernel<D, BatchAttnKernel::kTall>), dim3(items), dim3(512), 0, ctx().stream, a);
     else if (kind == BatchAttnKernel::kSingle)
         hipLaunchKernelGGL((batch_attn_kernel<D, BatchAttnKernel::kSingle>), dim3(ceil_div(items, 4)), dim3(256), 0, ctx().stream, a);
     else
@@ -972,6 +1010,7 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
     a.own_tiles = p.own_tiles;
     a.own_piece = p.own_piece;
     a.own_prefix = p.own_prefix;
+    a.spread = p.spread;
     if (p.slots() > 1) {
         const size_t part = static_cast<size_t>(p.slots()) * rows;
         if (int rc = ensure_attn_partials(part * (cache->head_size + 2) * sizeof(float)))

@@ -205,12 +205,13 @@ inline int check_batch_attention(const llama2_half* output, const llama2_half* q
 }
 
 // ---------------------------------------------------------------- how the attention is cut
-enum class BatchAttnKernel { kNarrow, kSingle, kWide };
+enum class BatchAttnKernel { kNarrow, kSingle, kWide, kTall };
 
 struct BatchAttnPlan {
     BatchAttnKernel kernel = BatchAttnKernel::kNarrow;
     int shared_tiles = 0, shared_splits = 0, shared_piece = kPass;
     int own_tiles = 0, own_splits = 1, own_piece = kPass;
+    bool spread = false; // the requests' heads over all XCDs
     int own_prefix = 0; // prefix rows in front of a request's own, a multiple of kPass; 0: none, or shared
     int slots() const { return shared_splits + own_splits; }
     // (piece, key/value head) pairs by eights, one for each XCD
@@ -264,10 +265,17 @@ inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int 
     else
         p.own_piece = batch_attn_piece(items, own_rows, 128, 1024, many ? 2LL * cus : 4LL * cus);
     p.own_splits = ceil_div(own_rows, p.own_piece);
+    // A head's rows lie in few of an XCD's L2 channels: where every row is read once, an XCD takes all heads in turn; where
+    // tiles read the same rows, all of a head go to one XCD, whose L2 then serves them (128 requests of 4 columns beside a wide
+    // prefix: in turn 96 us, 101; 8 prompts: 102, 94).
+    p.spread = columns <= static_cast<long long>(kFewRows) * b.n_requests;
     // More tiles than the GPU holds workgroups, of few rows each: a wavefront per tile (98 requests of 40 heads, 10 shared and 6 own
     // rows: 31.1 us, 16.6; 64 of 32 heads: 60 rows 16.9, 16.5; 120 rows 22.9, 27.4).
     if (many)
-        p.kernel = BatchAttnKernel::kWide;
+        // No more pieces than compute units: twice the wavefronts, which take turns with the passes, from 4 passes on (5 prompts of up
+        // to 609 tokens of 8 heads 24.4 us, 21.9; 17 requests of up to 43 tokens behind 5000 rows 27.2, 23.8; two of 21 behind 388, in
+        // pieces of 2 passes: 12.0, 13.6).
+        p.kernel = !shared && items * p.own_splits <= cus && p.own_piece >= 4 * kPass ? BatchAttnKernel::kTall : BatchAttnKernel::kWide;
     else if (!shared && p.own_splits == 1 && b.prefix_length + max_rows <= kPass && items >= 3LL * cus)
         p.kernel = BatchAttnKernel::kSingle;
     if (shared) {

@@ -275,7 +275,8 @@ def test_plan_covers_every_row_and_column(lib, requests):
                     lib.plan(b, kv_heads, group, rows, out)
                     kernel, tiles, splits, piece, own_tiles, own_splits, own_piece, own_prefix = out
                     what = (requests, kv_heads, group, per, prefix, rows, list(out))
-                    tile = 128 if kernel == 2 else 16
+                    tile = 128 if kernel >= 2 else 16
+                    assert kernel != 3 or (splits == 0 and own_piece >= 256 and own_tiles * own_splits * kv_heads <= 256), what
                     assert kernel != 1 or (splits == 0 and own_splits == 1), what  # a wavefront per tile: no pieces
                     assert own_piece % 64 == 0 and own_piece > 0 and 1 <= own_splits <= 256, what
                     assert own_splits * own_piece >= own_prefix + rows > (own_splits - 1) * own_piece, what
@@ -298,6 +299,10 @@ def test_plan_shares_a_prefix_among_narrow_requests_only(lib):
     assert out[2] == 0 and out[7] == 512 and out[0] == 0
     lib.plan(batch(n_requests=100, n_tokens=100, prefix_length=10), 32, 1, 54, out)
     assert out[0] == 1 and out[7] == 64
+    lib.plan(batch(n_requests=5, n_tokens=1200, prefix_length=134), 8, 1, 609, out)  # fewer tiles than compute units
+    assert out[0] == 3 and out[5] == 1
+    lib.plan(batch(n_requests=5, n_tokens=1200, prefix_length=0), 8, 1, 192, out)  # and few passes
+    assert out[0] == 2 and out[5] == 1
 
 
 def test_plan_refuses_more_workgroups_than_a_launch_holds(lib):

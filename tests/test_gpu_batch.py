@@ -367,6 +367,22 @@ def test_attention_turns(new, heads, kv_heads):
             step(sum(new), [9, 260, 0, 64], new, heads=heads, kv_heads=kv_heads, d=d, prefix=prefix, pad=2, fill=np.nan).check("d %d" % d)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("prefix", [0, 1, 64, 65, 130, 300])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (4, 1)])
+def test_attention_few_tiles_of_many_passes(d, prefix, heads, kv_heads):
+    """Fewer tiles than compute units: the passes go to two halves of a workgroup by turns, odd and even numbers of them, shared
+    rows and own ones; requests of few tokens and of none among them, blocks that are none, and pieces."""
+    for ctx, new in (([0, 256], [300, 64]), ([190, 0, 3], [130, 1, 400]), ([255, 30, 900, 0], [129, 3, 150, 16]), ([0, 9], [700, 0]),
+                     ([1800, 40], [200, 90])):
+        s = step(prefix + len(ctx), ctx, new, heads=heads, kv_heads=kv_heads, d=d, prefix=prefix, pad=3, fill=np.nan)
+        s.check("new %s" % new)
+        for b, r in ((0, 0), (0, 16 * 7), (len(ctx) - 1, 16)):  # these rows' blocks
+            if r < s.lengths[b]:
+                s.table[b, r // s.size] = -1 - r
+        s.check("new %s, blocks that are none" % new)
+
+
 def test_attention_long_requests_in_many_pieces():
     step(1, [9000, 20, 3000], [1, 1, 1], 64, heads=4, kv_heads=1, fill=np.nan).check("decode")
     step(2, [9000, 20, 3000], [2, 30, 1], 64, heads=4, kv_heads=2, prefix=5000, fill=np.nan).check("turns")
