@@ -50,8 +50,12 @@ struct BatchAttnArgs {
     uint32_t q_sign; // what turns the queries over where the scale is negative
     // items: [shared_splits x n_kv_heads, by eights][shared_tiles][of the eight], and [own_splits][own_tiles][n_kv_heads]
     int shared_items, shared_tiles, shared_splits, shared_piece;
+    Divisor by_eights, by_heads, by_tiles, by_group, by_guess; // 8 shared_tiles, n_kv_heads, own_tiles, group, a tile's columns + group
+    Divisor by_piece, by_all; // own_piece, all heads
     int own_items, own_tiles, own_piece, own_prefix, spread; // own_prefix: prefix rows in front of a request's own, a multiple of kPass, or 0
 };
+
+__device__ __forceinline__ int div_by(int n, Divisor d) { return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(n), d.m) >> d.shift); }
 
 // What a workgroup computes; the same in all its lanes.
 struct Item {
@@ -105,6 +109,12 @@ __device__ __forceinline__ int wave_max_int(int v)
 __device__ __forceinline__ int own_rows_of(const BatchAttnArgs& a, int p)
 {
     return p < a.prefix_length ? 0 : min(p - a.prefix_length + 1, a.max_rows);
+}
+
+// The pieces that hold what a token at position p attends of the request's own rows (and of the prefix, where that lies in front).
+__device__ __forceinline__ int pieces_of(const BatchAttnArgs& a, int p)
+{
+    return div_by(a.own_prefix + own_rows_of(a, p) + a.own_piece - 1, a.by_piece);
 }
 
 // exp2(v - base) is the probability times 2^6; without any score above -infinity everything is 0, not NaN.
@@ -216,7 +226,8 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
     const int lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
     const int r = min(c, it.rows - 1);
-    const int token = it.token + (it.row0 + r) / a.group, head = it.kv_head * a.group + (it.row0 + r) % a.group;
+    const int of_tokens = div_by(it.row0 + r, a.by_group), token = it.token + of_tokens;
+    const int head = it.kv_head * a.group + it.row0 + r - of_tokens * a.group;
     const int position = a.positions[token];
     const int limit = own_rows_of(a, position);
     const int least = it.least;
@@ -453,8 +464,8 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
         const int p = __shfl(position, (lane * a.group) & 15, 64); // of token `lane` of the tile: that of its first column
         int slots = 0;
         if (lane * a.group < it.rows && p >= 0) {
-            const int pieces = (a.own_prefix + own_rows_of(a, p) + a.own_piece - 1) / a.own_piece;
-            unsigned* const counter = a.counters + (it.token + it.row0 / a.group + lane) * a.n_kv_heads + it.kv_head;
+            const int pieces = pieces_of(a, p);
+            unsigned* const counter = a.counters + (it.token + div_by(it.row0, a.by_group) + lane) * a.n_kv_heads + it.kv_head;
             if (it.split < pieces && add_agent(counter, 1) + 1 == static_cast<unsigned>(pieces)) {
                 store_agent(counter, 0);
                 slots = pieces;
@@ -466,9 +477,9 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
     __syncthreads();
     const __amdgpu_buffer_rsrc_t parts = make_rsrc(a.parts, a.parts_bytes);
     for (int k = wave; k < it.rows; k += 4) {
-        const int t = k / a.group, slots = __builtin_amdgcn_readfirstlane(slots_of[t]);
+        const int t = div_by(k, a.by_group), slots = __builtin_amdgcn_readfirstlane(slots_of[t]);
         if (slots)
-            join_pieces<D>(a, it.token + it.row0 / a.group + t, it.kv_head * a.group + k % a.group, slots, parts);
+            join_pieces<D>(a, it.token + div_by(it.row0, a.by_group) + t, it.kv_head * a.group + k - t * a.group, slots, parts);
     }
 }
 
@@ -514,14 +525,15 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* all_lds)
     const int hl = lane >> 5, l31 = lane & 31;
     const int r = wave * 32 + l31, rq = min(r, it.rows - 1);
     const bool idle = wave * 32 >= it.rows;
-    const int token = it.token + (it.row0 + rq) / a.group, head = it.kv_head * a.group + (it.row0 + rq) % a.group;
+    const int of_tokens = div_by(it.row0 + rq, a.by_group), token = it.token + of_tokens;
+    const int head = it.kv_head * a.group + it.row0 + rq - of_tokens * a.group;
     h8_t qf[QS];
 #pragma unroll
     for (int j = 0; j < QS; ++j)
         qf[j] = load_query(a, token, head * D + j * 16 + hl * 8);
     const int position = a.positions[token];
-    const int limit = own_rows_of(a, position);
-    const int most_rows = wave_max_int(limit), least = -wave_max_int(-limit);
+    bool first_rows = true; // what follows is computed behind the first request
+    int limit = 0, most_rows = 0, least = 0;
     f16v_t o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -543,7 +555,6 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* all_lds)
         const int begin = seg ? it.r0 : it.p0, end = seg ? it.r1 : it.p1;
         if (begin >= end)
             continue;
-        const int seen = seg ? limit : end, all_see = seg ? least : end, any_sees = seg ? most_rows : end;
         const int wg_all_see = min(seg ? it.least : end, end);
         const int last8 = (end - 1) & ~7;
         auto block_of = [&](int row) { return uniform_load(table, min(row, last8) >> a.shift); };
@@ -578,6 +589,13 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* all_lds)
         if (HALVES == 1 || begin + half * kPass < end)
             request(begin + half * kPass, 0);
         look_up(begin + (half + HALVES) * kPass);
+        if (first_rows) {
+            limit = own_rows_of(a, position);
+            most_rows = wave_max_int(limit);
+            least = -wave_max_int(-limit);
+            first_rows = false;
+        }
+        const int seen = seg ? limit : end, all_see = seg ? least : end, any_sees = seg ? most_rows : end;
         int buffer = 0;
         for (int first = begin; first < end; first += HALVES * kPass, buffer ^= 1) {
             const int tb = first + half * kPass;
@@ -805,11 +823,11 @@ __global__ __launch_bounds__(KIND == BatchAttnKernel::kTall ? 512 : 256, KIND ==
     }
     if (index < shared_items) {
         // The tiles of a piece to one XCD: they read the same rows.
-        const int eight = index / (8 * a.shared_tiles), tile = index % (8 * a.shared_tiles) / 8, rest = eight * 8 + index % 8;
+        const int eight = div_by(index, a.by_eights), tile = (index - eight * 8 * a.shared_tiles) / 8, rest = eight * 8 + index % 8;
         if (rest >= a.shared_splits * a.n_kv_heads)
             return;
-        it.kv_head = rest % a.n_kv_heads;
-        it.slot = rest / a.n_kv_heads;
+        it.slot = div_by(rest, a.by_heads);
+        it.kv_head = rest - it.slot * a.n_kv_heads;
         it.p0 = it.slot * a.shared_piece;
         it.p1 = min(it.p0 + a.shared_piece, a.prefix_length);
         it.row0 = tile * kTileRows;
@@ -817,16 +835,22 @@ __global__ __launch_bounds__(KIND == BatchAttnKernel::kTall ? 512 : 256, KIND ==
         it.tokens = 1; // all see the same rows
     } else {
         index -= shared_items;
-        const int of_heads = index / a.n_kv_heads;
-        const int split = of_heads / a.own_tiles, turn = of_heads % a.own_tiles;
+        const int of_heads = div_by(index, a.by_heads);
+        const int split = div_by(of_heads, a.by_tiles), turn = of_heads - split * a.own_tiles;
         // wide tiles from the last one on: of a prompt, later tiles see more rows (3827 prompt tokens 102 -> 92 us)
         const int tile = MANY ? a.own_tiles - 1 - turn : turn;
         // An XCD gets every eighth workgroup: the same heads every time, or all of them in turn.
-        it.kv_head = (a.spread ? index + of_heads : index) % a.n_kv_heads;
-        // The request: the one it would be if all brought one token, else by counting, 64 at a time.
-        int request = min(((tile + 1) * kTileRows - 1) / (kTileRows + a.group), a.n_requests - 1);
-        int start = request_start(a, request), stop = request_start(a, request + 1);
-        if (first_tile<kTileRows>(a, start, request) > tile || first_tile<kTileRows>(a, stop, request + 1) <= tile) {
+        it.kv_head = a.spread ? index + of_heads : index;
+        it.kv_head -= div_by(it.kv_head, a.by_heads) * a.n_kv_heads;
+        // The request: the one it would be if all brought one token, else (and always among prompts) by counting, 64 at a time.
+        int request = 0, start = 0, stop = 0;
+        const bool guess = !MANY || a.spread;
+        if (guess) {
+            request = min(div_by((tile + 1) * kTileRows - 1, a.by_guess), a.n_requests - 1);
+            start = request_start(a, request);
+            stop = request_start(a, request + 1);
+        }
+        if (!guess || first_tile<kTileRows>(a, start, request) > tile || first_tile<kTileRows>(a, stop, request + 1) <= tile) {
             const int lane = threadIdx.x & 63;
             for (int first = 0; first < a.n_requests; first += 64) { // the last one whose first tile is not behind `tile`
                 const int b = min(first + lane, a.n_requests - 1);
@@ -846,19 +870,16 @@ __global__ __launch_bounds__(KIND == BatchAttnKernel::kTall ? 512 : 256, KIND ==
         if (it.rows <= 0 || it.row0 < 0)
             return;
         it.token = start;
-        const int t0 = start + it.row0 / a.group, t1 = start + (it.row0 + it.rows - 1) / a.group;
-        it.tokens = t1 - t0 + 1;
-        int most = own_rows_of(a, uniform_load(a.positions, t1));
-        it.least = most;
-        if (it.tokens > 1) {
-            int fewest = -most;
-            for (int t = t0 + static_cast<int>(threadIdx.x & 63); t <= t1; t += 64) {
-                const int own = own_rows_of(a, a.positions[t]);
-                most = max(most, own);
-                fewest = max(fewest, -own);
-            }
-            most = wave_max_int(most);
-            it.least = -wave_max_int(fewest);
+        const int t0 = start + div_by(it.row0, a.by_group), t1 = start + div_by(it.row0 + it.rows - 1, a.by_group);
+        it.tokens = t1 - t0 + 1; // 16 at most, 128 of wide tiles
+        int most;
+        if (it.tokens == 1) {
+            it.least = most = own_rows_of(a, uniform_load(a.positions, t1));
+        } else {
+            const int t = t0 + static_cast<int>(threadIdx.x & 63);
+            const int x = own_rows_of(a, a.positions[min(t, t1)]), y = MANY ? own_rows_of(a, a.positions[min(t + 64, t1)]) : x;
+            most = wave_max_int(max(x, y));
+            it.least = -wave_max_int(-min(x, y));
         }
         const int from = split * a.own_piece, to = from + a.own_piece; // of the shared rows in front and its own
         if (a.own_prefix) {
@@ -893,10 +914,10 @@ __global__ __launch_bounds__(256) void batch_attn_merge_kernel(BatchAttnArgs a)
     const int heads = a.n_kv_heads * a.group, rows = a.n_tokens * heads; // < 2^26: checked on the host
     const int row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     const int lane = threadIdx.x % LANES, x = lane % SIDE, deep = lane / SIDE;
-    const int token = min(row, rows - 1) / heads, head = row % heads;
-    if (row >= rows || a.positions[token] < 0)
+    const int token = div_by(min(row, rows - 1), a.by_all), head = row - token * heads, position = a.positions[token];
+    if (row >= rows || position < 0)
         return; // a whole wavefront at least, the whole workgroup where it has barriers
-    const int slots = a.shared_splits + (a.own_prefix + own_rows_of(a, a.positions[token]) + a.own_piece - 1) / a.own_piece;
+    const int slots = a.shared_splits + pieces_of(a, position);
     float m = -INFINITY, sum = 0.0f, o[8] = {};
     for (int s = deep; s < slots; s += DEEP) {
         const size_t part = static_cast<size_t>(s) * rows + row;
@@ -1010,6 +1031,13 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
     a.own_tiles = p.own_tiles;
     a.own_piece = p.own_piece;
     a.own_prefix = p.own_prefix;
+    a.by_eights = divisor(8 * (p.shared_tiles > 0 ? p.shared_tiles : 1));
+    a.by_heads = divisor(a.n_kv_heads);
+    a.by_tiles = divisor(p.own_tiles);
+    a.by_group = divisor(group);
+    a.by_guess = divisor((p.kernel == BatchAttnKernel::kWide || p.kernel == BatchAttnKernel::kTall ? kManyRows : kFewRows) + group);
+    a.by_piece = divisor(p.own_piece);
+    a.by_all = divisor(n_heads);
     a.spread = p.spread;
     if (p.slots() > 1) {
         const size_t part = static_cast<size_t>(p.slots()) * rows;

@@ -29,6 +29,21 @@ inline int log2_of(int power)
     return s;
 }
 
+// n / d for 0 <= n < 2^31 as the upper half of a product (a division by a number known only at run time is 20 instructions
+// that wait for one another, and a workgroup has six in front of its first load): 2 n m / 2^(32 + shift).  m = ceil(2^(31 + shift) / d)
+// is off by less than 1, so the quotient by less than n / 2^(31 + shift) < 2^-shift <= 1 / d.
+struct Divisor {
+    uint32_t m, shift;
+};
+
+inline Divisor divisor(int d)
+{
+    uint32_t shift = 0;
+    while ((1LL << shift) < d)
+        ++shift;
+    return {static_cast<uint32_t>(((1ULL << (31 + shift)) + d - 1) / d), shift};
+}
+
 // ---------------------------------------------------------------- refusals
 inline int check_block_size(const char* fn, int block_size)
 {

@@ -57,6 +57,11 @@ int fits(const llama2_batch* b, int n_kv_heads, int group, int max_rows)
 {
     return l2::check_batch_attn_plan(l2::batch_attn_plan(*b, n_kv_heads, group, max_rows, 256), b->n_tokens, n_kv_heads * group, n_kv_heads);
 }
+unsigned divide(unsigned n, int d) // as a kernel does
+{
+    const l2::Divisor by = l2::divisor(d);
+    return static_cast<unsigned>((static_cast<unsigned long long>(2 * n) * by.m) >> 32) >> by.shift;
+}
 void plan(const llama2_batch* b, int n_kv_heads, int group, int max_rows, int* out)
 {
     const l2::BatchAttnPlan p = l2::batch_attn_plan(*b, n_kv_heads, group, max_rows, 256);
@@ -303,6 +308,16 @@ def test_plan_shares_a_prefix_among_narrow_requests_only(lib):
     assert out[0] == 3 and out[5] == 1
     lib.plan(batch(n_requests=5, n_tokens=1200, prefix_length=0), 8, 1, 192, out)  # and few passes
     assert out[0] == 2 and out[5] == 1
+
+
+def test_division_by_a_product(lib):
+    top = (1 << 31) - 1
+    lib.divide.restype = C.c_uint
+    for d in list(range(1, 70)) + [127, 128, 129, 255, 641, 1023, 1024, 1040, 65535, 65537, 1 << 20, (1 << 20) + 1, (1 << 24) - 1, 1 << 24, top - 1, top]:
+        near = {n for k in (1, 2, 3, 7, 1000, top // d // 2, top // d - 1, top // d) for n in (k * d - 1, k * d, k * d + 1)}
+        for n in near | {0, 1, top, top - 1, 12345678}:
+            if 0 <= n <= top:
+                assert lib.divide(n, d) == n // d, (n, d)
 
 
 def test_plan_refuses_more_workgroups_than_a_launch_holds(lib):
