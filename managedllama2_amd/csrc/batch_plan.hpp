@@ -295,10 +295,12 @@ inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int 
         p.kernel = BatchAttnKernel::kSingle;
     if (shared) {
         p.shared_tiles = static_cast<int>((columns + tile - 1) / tile);
-        // a workgroup per compute unit, half a one of wide tiles: the rest is for the requests' own rows (16 samples behind 2048
-        // rows 17.2 us, twice as many workgroups 20.8)
-        p.shared_piece = batch_attn_piece(static_cast<long long>(p.shared_tiles) * n_kv_heads, b.prefix_length, 128, 1024,
-                                          many ? cus / 2 : cus);
+        // A workgroup per compute unit (16 samples behind 2048 rows 17.2 us, twice as many workgroups 20.8); of wide tiles half a
+        // one beside long rows of the requests' own, which need the rest (128 requests behind 8192 rows, up to 2001 own ones: 92 us,
+        // 98; 25 behind 11736, at most 24 own ones: 25.7, 20.2), and up to 2048 rows, whose sums weigh less (the first case
+        // with 1024: 97; 109 behind 7911 52 -> 46, with up to 4096: 74).
+        p.shared_piece = batch_attn_piece(static_cast<long long>(p.shared_tiles) * n_kv_heads, b.prefix_length, 128, many ? 2048 : 1024,
+                                          many && max_rows > 2 * kPass ? cus / 2 : cus);
         p.shared_splits = ceil_div(b.prefix_length, p.shared_piece);
     }
     return p;
