@@ -190,3 +190,44 @@ def test_large_tables_in_place():
             assert np.array_equal(c.positions.to_host(), positions) and np.array_equal(c.starts.to_host(), starts), rep
             capi.call("llama2_graph_launch", g)
         capi.call("llama2_graph_destroy", g)
+
+
+def test_captured_attentions_share_scratch_and_counters():
+    """Steps of different shapes captured one by one (joined in the launch, by a second one, without pieces), replayed by turns
+    with eager calls between, the last of which needs more scratch than there was at capture."""
+    rng = lambda i: synth.rng_for(1501, i)  # noqa: E731
+    steps = [bu.Step(rng(0), [900], [1], 16, heads=8, kv_heads=8, fill=np.nan),
+             bu.Step(rng(1), [700, 30, 2100], [1, 1, 1], 16, heads=8, kv_heads=2, fill=np.nan, pad=2),
+             bu.Step(rng(2), [300, 0, 64], [40, 130, 1], 32, heads=4, kv_heads=2, d=64, prefix=100, fill=np.nan),
+             bu.Step(rng(3), list(range(40)), [1] * 40, 8, heads=8, kv_heads=8, d=64, prefix=300, fill=np.nan)]
+    large = bu.Step(rng(4), [5000] * 30, [3] * 30, 64, heads=16, kv_heads=16, d=64)
+    graphs, outs, want = [], [], []
+    for s in steps:
+        want.append(s.check())  # also allocates what a capture must not
+    for s in steps:
+        out, g = DeviceVariable.from_host(np.full((s.tokens, s.heads * s.d), 77.0, np.float16)), C.c_void_p()
+        args = (out.ptr, s.dq.ptr, s.batch, s.cache, s.heads, s.heads * s.d, s.heads * s.d, s.scale)
+        capi.call("llama2_graph_begin_capture")
+        try:
+            capi.call("llama2_batch_attention", *args)
+        finally:
+            capi.call("llama2_graph_end_capture", C.byref(g))
+        graphs.append(g)
+        outs.append(out)
+    for turn in range(4):
+        order = synth.rng_for(1502, turn).permutation(len(steps))
+        for i in order:
+            capi.call("llama2_memset", outs[i].ptr, 0x55, outs[i].size * 2)
+            capi.call("llama2_graph_launch", graphs[i])
+        for i in order:
+            live = steps[i].positions >= 0
+            got = outs[i].to_host().reshape(want[i].shape)
+            assert np.array_equal(got[live].view(np.uint16), want[i][live].view(np.uint16)), (turn, i)
+            assert (got[~live].view(np.uint16) == 0x5555).all(), (turn, i)
+        if turn == 1:
+            large.upload()
+            first = large.run()
+            assert np.array_equal(first.view(np.uint16), large.run().view(np.uint16))
+        steps[turn].run()
+    for g in graphs:
+        capi.call("llama2_graph_destroy", g)
