@@ -109,7 +109,7 @@ __device__ __forceinline__ int wave_max_int(int v)
 // Own rows that a token at position p attends.
 __device__ __forceinline__ int own_rows_of(const BatchAttnArgs& a, int p)
 {
-    return p < a.prefix_length ? 0 : min(p - a.prefix_length + 1, a.max_rows);
+    return p < a.prefix_length ? 0 : min(p - a.prefix_length, a.max_rows - 1) + 1;
 }
 
 // The pieces that hold what a token at position p attends of the request's own rows (and of the prefix, where that lies in front).

@@ -461,6 +461,24 @@ def test_attention_without_rows_and_without_blocks():
                 assert not got[:new[0]].any()
 
 
+def test_attention_positions_beyond_the_rows():
+    """A position whose rows max_length (or the table) does not hold attends those that there are, up to the largest int."""
+    for new in ([1, 1], [30, 2], [300, 1]):
+        for prefix in (0, 70):
+            s = step(8, [40, 300], new, heads=2, kv_heads=1, prefix=prefix)
+            s.positions[s.starts[2] - 1] = s.positions[s.starts[1] - 1] = (1 << 31) - 1
+            s.max_length = min(s.lengths)
+            s.upload()
+            got = s.run()
+            for b in (0, 1):  # the others' positions are what they were; max_length cuts all of them
+                t = slice(s.starts[b], s.starts[b + 1])
+                last = np.minimum(s.positions[t], prefix + s.max_length - 1)
+                flat = [np.ascontiguousarray(s.rows_of(c)).reshape(-1, s.width) for c in (s.key, s.value)]
+                want, bound = bu.attention(s.q[t], *flat, s.row_numbers(s.prefix_table, prefix), s.row_numbers(s.table[b], s.lengths[b]),
+                                           last, prefix, s.scale, s.kv_heads, s.d)
+                assert (np.abs(got[t].astype(np.float64) - want) <= bound).all(), (new, prefix, b)
+
+
 def test_attention_large_scores():
     """Scores of thousands, both signs, a negative scale, and keys at the end of the type."""
     for d in (64, 128):
