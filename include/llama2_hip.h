@@ -395,7 +395,8 @@ int llama2_batch_qk_norm_rope(llama2_half* q_output, const llama2_half* q, const
  * NaN.  Where it saves reading, the shared rows are read once for up to 128 query rows
  * instead of once per request.  The same call gives the same bits every time.
  * positions of a request must not decrease; max_length bounds the launch, rows beyond it
- * are not attended; any scale is allowed.  `output` must not overlap the other buffers.
+ * are not attended; any scale is allowed, and scores as large as fp32 holds (a scaled score beyond that gives
+ * NaN, or the row no weight).  `output` must not overlap the other buffers.
  * Reads query_starts, positions, block_tables and prefix_table of the batch, as
  * llama2_batch_tables leaves them.  At most 2^29 rows per token and 2^26 query rows.
  * Scratch: as llama2_multi_head_attention (call once before capturing). */

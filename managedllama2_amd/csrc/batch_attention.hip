@@ -120,6 +120,17 @@ __device__ __forceinline__ int pieces_of(const BatchAttnArgs& a, int p)
 
 // exp2(v - base) is the probability times 2^6; without any score above -infinity everything is 0, not NaN.
 __device__ __forceinline__ float prob_base(float most) { return most == -INFINITY ? 0.0f : most - kProbShift; }
+// Is 2^24 reached, where fp32 numbers are so far apart that the rounding of m and of base alone could take exponents beyond what fp16
+// holds?  Then exponents are those of the rounded scores, cut off at what they are without base's rounding.
+__device__ __forceinline__ bool far_out(float base) { return __any(fabsf(base) >= 0x1p24f); }
+__device__ __forceinline__ float far_exponent(float score, float scale, float base)
+{
+#pragma clang fp contract(off)
+    const float v = score * scale, e = v - base;
+    return e > kProbShift + kSlack ? kProbShift + kSlack : e; // NaN stays
+}
+// Has some column a score so far above its reference that the reference has to follow?  As a difference: m + kSlack would be rounded.
+__device__ __forceinline__ bool has_to_follow(float most, float m) { return __any(most - m > kSlack); }
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ float weight_of(float m, float most) { return m == -INFINITY ? 0.0f : exp2_of(m - most); }
 
@@ -313,7 +324,7 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
                     most = fmaxf(most, s[t][i]);
                 }
             most = max_xor32(max_xor16(most));
-            if (__any(most > m + kSlack)) {
+            if (has_to_follow(most, m)) {
                 most = fmaxf(m, most);
                 const float alpha = weight_of(m, most);
                 sum *= alpha;
@@ -322,7 +333,15 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
                     o[i] *= alpha;
                 m = most;
             }
-            const float base = prob_base(m);
+            float base = prob_base(m);
+            if (far_out(base)) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        s[t][i] = far_exponent(s[t][i], 1.0f, base);
+                base = 0.0f;
+            }
             h8_t p;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -670,7 +689,7 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* all_lds)
                 for (int i = 0; i < 16; ++i)
                     most = fmaxf(most, s[t][i]);
             most = max_xor32(most) * a.scale;
-            if (__any(most > m + kSlack)) {
+            if (has_to_follow(most, m)) {
                 most = fmaxf(m, most);
                 const float alpha = weight_of(m, most);
                 sum *= alpha;
@@ -680,6 +699,17 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* all_lds)
                 m = most;
             }
             const float base = prob_base(m);
+            // Exponents are s * scale - base with one rounding.
+            float factor = a.scale, minus = base;
+            if (far_out(base)) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[t][i] = far_exponent(s[t][i], a.scale, base);
+                factor = 1.0f;
+                minus = 0.0f;
+            }
             h8_t p[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u)
@@ -688,7 +718,7 @@ __device__ void many_rows(const BatchAttnArgs& a, const Item& it, char* all_lds)
                     h2_t e;
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
-                        e[x] = static_cast<_Float16>(exp2_of(__builtin_fmaf(s[u >> 1][8 * (u & 1) + i + x], a.scale, -base)));
+                        e[x] = static_cast<_Float16>(exp2_of(__builtin_fmaf(s[u >> 1][8 * (u & 1) + i + x], factor, -minus)));
                     p[u][i] = e[0];
                     p[u][i + 1] = e[1];
                     sum = dot2(as_u32(e), 0x3C003C00u, sum); // of the rounded ones, in fp32
