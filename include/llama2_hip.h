@@ -386,8 +386,10 @@ int llama2_batch_qk_norm_rope(llama2_half* q_output, const llama2_half* q, const
 /* Causal attention of all tokens: the token at position p of request b attends the
  * prefix_length rows of the prefix table and the own rows 0 .. p - prefix_length
  * of the request (row r: block_tables[b][r / block_size]); query head h
- * uses key/value head h / (n_heads / n_kv_heads).  Scores and softmax stay in fp32,
- * probabilities are rounded to fp16 on their way into the products with the values
+ * uses key/value head h / (n_heads / n_kv_heads).  Scores and softmax stay in fp32; on their
+ * way into the products with the values, probabilities keep 22 bits where up to 16 query rows
+ * are computed at a time (single tokens), and are rounded to fp16 where more are (prompts, a
+ * prefix that many requests share)
  * (llama2_multi_head_attention rounds scores to fp16 instead, as the reference does).
  * Rows of a block id outside the cache are not attended; a token left without rows gives
  * zeros.  Rows behind a token's own, and the rest of the last block, have no influence

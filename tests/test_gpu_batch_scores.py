@@ -117,3 +117,59 @@ def test_many_small_weights_count(d, new, lead, best):
     s.rows_of(s.key)[at][0] = 1
     s.rows_of(s.value)[at][:] = 0
     s.check()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(8, 8), (8, 2), (40, 40)])
+@pytest.mark.parametrize("prefix,ctx", [(0, [2, 16, 59]), (0, [0, 1, 2, 30] * 8), (30, [1, 40, 100]), (70, [0, 3, 20, 9] * 6)])
+def test_tiles_of_single_tokens_keep_the_weights_in_fp32(d, heads, kv_heads, prefix, ctx):
+    """Scores are multiples of 1/4, exact in fp32, so that what is left of an element that nearly cancels is the weights' own error."""
+    rng = synth.rng_for(1425, d, heads, kv_heads, prefix)
+    s = bu.Step(rng, ctx, [1] * len(ctx), 16, heads=heads, kv_heads=kv_heads, d=d, prefix=prefix)
+    s.scale = 0.25
+    for x in (s.key.reshape(-1, kv_heads, d), s.q.reshape(-1, heads, d)):
+        x[...] = 0
+        x[..., :4] = rng.integers(-2, 3, x[..., :4].shape)
+    s.upload()
+    got = s.run().astype(np.float64)
+    keys, values = (s.rows_of(c).reshape(-1, kv_heads, d).astype(np.float64) for c in (s.key, s.value))
+    shared = s.row_numbers(s.prefix_table, prefix)
+    # 24 requests of 40 heads behind 70 rows have these read once for all 24 of them, in wide tiles: weights as fp16, off by half a
+    # step of it (2^-11) each in the one sum and so in the other
+    wide = 2.0 ** -11 if prefix == 70 and kv_heads == 40 else 0.0
+    for b in range(len(ctx)):
+        rows = np.concatenate([shared, s.row_numbers(s.table[b], s.lengths[b])])
+        for h in range(heads):
+            k, v = keys[rows, h // (heads // kv_heads)], values[rows, h // (heads // kv_heads)]
+            x = k @ s.q[b, h * d:(h + 1) * d].astype(np.float64) * 0.25
+            w = np.exp(x - x.max())
+            want, size = w @ v / w.sum(), w @ np.abs(v) / w.sum()
+            # weights as two fp16 numbers (2^-22; what is left below fp16's smallest, 2^-31 of the largest weight), exponents up to 16 from the
+            # constant log2(e), two products and a difference (4 times 2^-24 each), exp2 2^-22; both sums; the result as fp16
+            eps = wide + 2.0 ** -22 + 2 * (4 * 2.0 ** -24 * 16 + 2.0 ** -22) + 2 * len(rows) * 2.0 ** -24
+            bound = 2.0 ** -11 * np.abs(want) + 2.0 ** -25 + eps * size + len(rows) * 2.0 ** -31 * np.abs(v).max()
+            err = np.abs(got[b, h * d:(h + 1) * d] - want)
+            assert (err <= bound).all(), (b, h, (err / bound).max())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("ctx,prefix", [([200, 50], 0), ([0, 31], 0), ([300, 90], 100), ([5, 20], 40)])
+def test_infinite_values_reach_single_tokens(d, ctx, prefix):
+    """A value that is not finite, in a row that every query of its tile attends: its element of the output is that, the others are
+    what they were."""
+    s = bu.Step(synth.rng_for(1426, d, len(ctx), prefix), ctx, [1, 1], 16, heads=4, kv_heads=2, d=d, prefix=prefix)
+    clean = s.check().astype(np.float32)
+    rows = s.rows_of(s.value)
+    own = s.ctx[0] // 2
+    rows[s.table[0, own // 16], own % 16, [0, d // 2, d + 5]] = np.inf, -np.inf, np.nan
+    if prefix:
+        rows[s.prefix_table[prefix // 32], 3, d - 1] = np.inf
+    s.upload()
+    got = s.run().astype(np.float32).reshape(2, 4, d)
+    want = clean.reshape(2, 4, d).copy()
+    want[0, :2, 0], want[0, :2, d // 2], want[0, 2:, 5] = np.inf, -np.inf, np.nan  # two heads of queries to one of keys
+    if prefix:
+        want[:, :2, d - 1] = np.inf
+    same = np.isfinite(want)
+    assert np.array_equal(got[~same], want[~same], equal_nan=True)
+    assert np.array_equal(got[same], want[same])
