@@ -478,14 +478,15 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
             h[x] = __builtin_bit_cast(_Float16, float_to_half_bits(e[x / 4][x % 4] * inv));
         *reinterpret_cast<Halfs*>(a.out + static_cast<size_t>(token) * a.out_stride + head * D + d) = h;
     }
+    const __amdgpu_buffer_rsrc_t parts = make_rsrc(a.parts, a.parts_bytes); // of pieces that are joined in this launch
     if (live && a.parts) {
 #pragma unroll
         for (int x = 0; x < QUADS; ++x) {
-            float* to = a.parts + part * D + d + 4 * x;
-            if (a.counters) // written through, for the workgroup that joins the pieces in this launch
-                asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 0" : : "v"(to), "v"(e[x]) : "memory"); // s_nop: e may be overwritten next
+            if (a.counters) // written through, for the workgroup that joins the pieces; parts_bytes < 2^31
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, e[x]), parts,
+                                                       static_cast<int>((part * D + d + 4 * x) * sizeof(float)), 0, kAuxAgent);
             else
-                *reinterpret_cast<f4_t*>(to) = e[x];
+                *reinterpret_cast<f4_t*>(a.parts + part * D + d + 4 * x) = e[x];
         }
         if (wave == 0 && g == 0) {
             store_agent(&a.stats[part].x, most);
@@ -514,7 +515,6 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
             slots_of[lane] = slots;
     }
     __syncthreads();
-    const __amdgpu_buffer_rsrc_t parts = make_rsrc(a.parts, a.parts_bytes);
     for (int k = wave; k < it.rows; k += 4) {
         const int t = div_by(k, a.by_group), slots = __builtin_amdgcn_readfirstlane(slots_of[t]);
         if (slots)
