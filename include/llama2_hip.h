@@ -401,7 +401,7 @@ int llama2_batch_qk_norm_rope(llama2_half* q_output, const llama2_half* q, const
  * NaN, or the row no weight).  `output` must not overlap the other buffers.
  * Reads query_starts, positions, block_tables and prefix_table of the batch, as
  * llama2_batch_tables leaves them.  At most 2^29 rows per token and 2^26 query rows.
- * Scratch: as llama2_multi_head_attention (call once before capturing). */
+ * Scratch: as llama2_multi_head_attention (call once before capturing), at most 512 MiB for a call. */
 int llama2_batch_attention(llama2_half* output, const llama2_half* query, const llama2_batch* batch,
                            const llama2_paged_cache* cache, int n_heads, int output_stride,
                            int query_stride, float scale);

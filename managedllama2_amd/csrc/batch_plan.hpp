@@ -18,6 +18,7 @@ constexpr int kManyRows = 128; // columns (token, head of the group) of a workgr
 constexpr int kFewRows = 16;   // at most this many: the wavefronts split the cache rows instead of the columns
 constexpr int kPass = 64;      // cache rows per pass of wide tiles; pieces are multiples of it
 constexpr int kMaxPieces = 256; // of a request's rows, and of the prefix
+constexpr long long kMaxBatchScratch = 512LL << 20; // bytes of sums of all pieces
 
 inline int round_up(int v, int to) { return ceil_div(v, to) * to; }
 
@@ -235,13 +236,14 @@ struct BatchAttnPlan {
 };
 
 // Pieces of `rows` cache rows, for `items` of them in each piece: up to `want` workgroups altogether, but pieces not shorter
-// than `shortest` nor longer than `longest`.
-inline int batch_attn_piece(long long items, int rows, int shortest, int longest, long long want)
+// than `shortest` nor longer than `longest`, and no more than `room` of them.
+inline int batch_attn_piece(long long items, int rows, int shortest, int longest, long long want, long long room)
 {
     const long long enough = want > items ? want / items : 1, most = ceil_div(rows, shortest), least = ceil_div(rows, longest);
     long long n = enough < most ? enough : most;
     n = n > least ? n : least;
     n = n < kMaxPieces ? n : kMaxPieces;
+    n = n < room ? n : room;
     return round_up(ceil_div(rows, static_cast<int>(n)), kPass);
 }
 
@@ -261,7 +263,12 @@ inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int 
     BatchAttnPlan p;
     const long long columns = static_cast<long long>(b.n_tokens) * group;
     const bool fill = columns >= 64LL * b.n_requests;
-    const bool shared = !fill && static_cast<long long>(b.n_requests - 1) * b.prefix_length * n_kv_heads >= 1 << 15 && b.prefix_length >= kPass;
+    // Every piece leaves sums, a maximum and a denominator for every query row (room for heads of 128), used or not: there are no more
+    // pieces than kMaxBatchScratch holds, and where it does not hold two, nothing is shared and nothing cut (200 requests of 50 tokens of
+    // 32 heads, up to 8050 own rows: 1.3 GB of sums 1060 us, 0.5 GB 980; with a max_length of 131072 21.3 GB 3100, 0.5 GB 900).
+    const long long room = kMaxBatchScratch / (columns * n_kv_heads * (128 + 2) * 4);
+    const bool shared = !fill && static_cast<long long>(b.n_requests - 1) * b.prefix_length * n_kv_heads >= 1 << 15 && b.prefix_length >= kPass && room >= 2;
+    const long long own_room = shared ? room / 2 : room > 1 ? room : 1;
     // Up to 128 shared columns are cheaper as tiles of 16 that read the prefix out of the L2 again, if that is little next to
     // the requests' own rows: the kernel without the wide tiles has 3 wavefronts per SIMD instead of 2 (72 columns, 1024
     // shared rows, up to 4000 own ones: 121 us, 130; 75 columns, 2558 and 84: 54, 42).
@@ -274,11 +281,11 @@ inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int 
     const int own_rows = p.own_prefix + max_rows;
     const long long items = static_cast<long long>(p.own_tiles) * n_kv_heads;
     if (fill)
-        p.own_piece = batch_attn_piece(items, own_rows, 1024, own_rows, 2LL * cus);
+        p.own_piece = batch_attn_piece(items, own_rows, 1024, own_rows, 2LL * cus, own_room);
     else if (many && items >= cus)
-        p.own_piece = batch_attn_piece(items, own_rows, 512, 1024, 4LL * cus);
+        p.own_piece = batch_attn_piece(items, own_rows, 512, 1024, 4LL * cus, own_room);
     else
-        p.own_piece = batch_attn_piece(items, own_rows, 128, 1024, many ? 2LL * cus : 4LL * cus);
+        p.own_piece = batch_attn_piece(items, own_rows, 128, 1024, many ? 2LL * cus : 4LL * cus, own_room);
     p.own_splits = ceil_div(own_rows, p.own_piece);
     // A head's rows lie in few of an XCD's L2 channels: where every row is read once, an XCD takes all heads in turn; where
     // tiles read the same rows, all of a head go to one XCD, whose L2 then serves them (128 requests of 4 columns beside a wide
@@ -300,7 +307,7 @@ inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int 
         // 98; 25 behind 11736, at most 24 own ones: 25.7, 20.2), and up to 2048 rows, whose sums weigh less (the first case
         // with 1024: 97; 109 behind 7911 52 -> 46, with up to 4096: 74).
         p.shared_piece = batch_attn_piece(static_cast<long long>(p.shared_tiles) * n_kv_heads, b.prefix_length, 128, many ? 2048 : 1024,
-                                          many && max_rows > 2 * kPass ? cus / 2 : cus);
+                                          many && max_rows > 2 * kPass ? cus / 2 : cus, room - p.own_splits);
         p.shared_splits = ceil_div(b.prefix_length, p.shared_piece);
     }
     return p;

@@ -310,6 +310,24 @@ def test_plan_shares_a_prefix_among_narrow_requests_only(lib):
     assert out[0] == 2 and out[5] == 1
 
 
+@pytest.mark.parametrize("requests", [1, 2, 7, 64, 256, 4000])
+def test_plan_needs_a_bounded_scratch(lib, requests):
+    """Sums, maximum and denominator of every piece of every query row: half a GiB at most, whatever the bounds of a call are."""
+    out = (C.c_int * 8)()
+    most = 0
+    for kv_heads, group in ((1, 1), (8, 4), (32, 1), (40, 1), (8, 8)):
+        for tokens in (requests, requests * 3 + 1, requests * 62, requests * 63 // group, 1 << 20):
+            if requests <= tokens <= 1 << 20 and tokens * kv_heads * group < 1 << 26:
+                for prefix in (0, 100, 5000, 1 << 28):
+                    for rows in (1, 100, 4096, 131072, 1 << 28):
+                        lib.plan(batch(n_requests=requests, n_tokens=tokens, prefix_length=prefix), kv_heads, group, rows, out)
+                        slots = out[2] + out[5]
+                        scratch = slots * tokens * kv_heads * group * 130 * 4 if slots > 1 else 0
+                        assert scratch <= 1 << 29, (kv_heads, group, tokens, prefix, rows, list(out))
+                        most = max(most, scratch)
+    assert most > 0
+
+
 def test_division_by_a_product(lib):
     top = (1 << 31) - 1
     lib.divide.restype = C.c_uint
