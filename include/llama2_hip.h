@@ -374,7 +374,7 @@ int llama2_batch_tables(const llama2_batch* batch, const int* cached, const int*
  * Rows of q, k, v and q_output are q_stride, kv_stride and q_output_stride halfs
  * apart (multiples of 8, pointers 16-byte aligned), so that they may be parts of one buffer.
  * q_output may be q with the same stride (rows of k and v between q's must have that stride
- * too); it must not overlap otherwise.  Keys and values of the cache must not overlap.  No two tokens may
+ * too); neither it nor the cache may overlap anything else.  Keys and values of the cache must not overlap.  No two tokens may
  * have the same slot.  A token whose slot is not one of the cache's is not stored.
  * Reads positions and slots of the batch.  1 <= theta. */
 int llama2_batch_qk_norm_rope(llama2_half* q_output, const llama2_half* q, const llama2_half* k,

@@ -108,6 +108,18 @@ inline bool rows_overlap(const void* a, long long a_width, const void* b, long l
     return (of <= last && rest < static_cast<uintptr_t>(a_width) * 2) || (of + 1 <= last && s - rest < static_cast<uintptr_t>(b_width) * 2);
 }
 
+// Does an array of `bytes` at p overlap one of `n` rows of `width` halfs from `a` on, `stride` halfs apart?
+inline bool touches_rows(const void* p, size_t bytes, const void* a, long long width, long long n, long long stride)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(p);
+    if (!p || bytes == 0)
+        return false;
+    if (y < x)
+        return bytes > x - y;
+    const uintptr_t s = static_cast<uintptr_t>(stride) * 2, of = (y - x) / s, rest = (y - x) % s, last = static_cast<uintptr_t>(n - 1);
+    return (of <= last && rest < static_cast<uintptr_t>(width) * 2) || (of < last && bytes > s - rest);
+}
+
 inline size_t rows_bytes(int rows, int stride, int width) { return (static_cast<size_t>(rows - 1) * stride + width) * 2; }
 
 inline int check_batch_tables(const llama2_batch* batch, const int* cached, const int* counts, const int* free_blocks, int n_free,
@@ -182,6 +194,17 @@ inline int check_batch_rope(const llama2_half* q_output, const llama2_half* q, c
         L2_CHECK(!overlap(c, cache_bytes(*cache), q, rows_bytes(t, q_stride, q_row)) && !overlap(c, cache_bytes(*cache), k, kv_bytes) &&
                      !overlap(c, cache_bytes(*cache), v, kv_bytes) && !overlap(c, cache_bytes(*cache), q_output, out_bytes),
                  "%s: the cache overlaps q, k, v or q_output", fn);
+    const struct {
+        const void* p;
+        size_t bytes;
+    } read[] = {{q_gamma, static_cast<size_t>(cache->head_size) * 2}, {k_gamma, static_cast<size_t>(cache->head_size) * 2},
+                {batch->positions, static_cast<size_t>(t) * 4}, {batch->slots, static_cast<size_t>(t) * 4}};
+    for (const auto& r : read) {
+        L2_CHECK(!touches_rows(r.p, r.bytes, q_output, q_row, t, q_output_stride), "%s: q_output overlaps a gamma, positions or slots", fn);
+        for (const void* c : written)
+            L2_CHECK(!touches_rows(r.p, r.bytes, c, static_cast<long long>(cache->block_size) * kv_row, cache->n_blocks, block_halfs(*cache)),
+                     "%s: the cache overlaps a gamma, positions or slots", fn);
+    }
     return LLAMA2_OK;
 }
 
@@ -217,6 +240,15 @@ inline int check_batch_attention(const llama2_half* output, const llama2_half* q
     if (b.prefix_length > kMaxBatchRows || batch_own_rows(b, cache->block_size) > kMaxBatchRows - b.prefix_length)
         return fail(LLAMA2_ERR_UNSUPPORTED, "%s: prefix_length=%d and %d own rows exceed %d", fn, b.prefix_length,
                     batch_own_rows(b, cache->block_size), kMaxBatchRows);
+    const struct {
+        const void* p;
+        size_t ints;
+    } read[] = {{b.positions, static_cast<size_t>(b.n_tokens)}, {b.query_starts, static_cast<size_t>(b.n_requests) + 1},
+                {b.block_tables, static_cast<size_t>(b.n_requests) * b.table_stride},
+                {b.prefix_table, (static_cast<size_t>(b.prefix_length) + cache->block_size - 1) / cache->block_size}};
+    for (const auto& r : read)
+        L2_CHECK(!touches_rows(r.p, r.ints * 4, output, row, b.n_tokens, output_stride),
+                 "%s: output overlaps positions, query_starts or a block table", fn);
     return LLAMA2_OK;
 }
 

@@ -264,6 +264,49 @@ def test_attention_refusals(lib):
         assert call_attention(lib, batch(), cache(), scale=v) == INVALID
 
 
+def around(rows, width, n, stride):
+    """(offsets at which an array of 36 bytes touches one of n rows, offsets at which it does not)"""
+    last = (n - 1) * stride
+    hits = {0, 4, width - 4, -32, last, last + width - 4, stride - 32, stride, last - 32}
+    misses = {-36, last + width, last + stride, last + 2 * stride}
+    if stride > width + 36:
+        misses |= {width, stride - 36, last - 36}
+    return [rows + x for x in hits], [rows + x for x in misses]
+
+
+def test_what_is_written_may_not_lie_over_what_is_read(lib):
+    """9 positions, slots or entries (36 bytes), in front of, behind and between rows of outputs and blocks of the cache."""
+    for stride in (1024, 1032, 1536):
+        hits, misses = around(300 * MIB, 2048, 9, 2 * stride)
+        for name in ("positions", "slots"):
+            assert all(call_rope(lib, batch(**{name: x}), cache(), so=stride) == INVALID for x in hits), (stride, name)
+            assert all(call_rope(lib, batch(**{name: x}), cache(), so=stride) == 0 for x in misses), (stride, name)
+        one = dict(n_requests=8, table_stride=1, max_length=9)  # 9 starts, 8 entries
+        for name in ("positions", "query_starts"):
+            assert all(call_attention(lib, batch(**{name: x}, **one), cache(), so=stride) == INVALID for x in hits), (stride, name)
+            assert all(call_attention(lib, batch(**{name: x}, **one), cache(), so=stride) == 0 for x in misses), (stride, name)
+        for name, more in (("block_tables", dict(n_requests=9, table_stride=1)), ("block_tables", dict(n_requests=3, table_stride=3)),
+                           ("prefix_table", dict(prefix_length=8 * 16 + 1))):
+            assert all(call_attention(lib, batch(**{name: x}, **more), cache(), so=stride) == INVALID for x in hits), (stride, name)
+            assert all(call_attention(lib, batch(**{name: x}, **more), cache(), so=stride) == 0 for x in misses), (stride, name)
+        for name in ("gq", "gk"):
+            assert call_rope(lib, batch(), cache(), **{name: 300 * MIB + 2032}, so=stride) == INVALID
+            assert call_rope(lib, batch(), cache(), **{name: 300 * MIB - 240}, so=stride) == INVALID
+            assert call_rope(lib, batch(), cache(), **{name: 300 * MIB - 256}, so=stride) == 0
+    assert call_rope(lib, batch(), cache(), gq=300 * MIB + 2048, so=1536) == 0  # 256 bytes between two rows
+    block = 16 * 256 * 2  # bytes
+    for base, which in ((100 * MIB, "keys"), (200 * MIB, "values")):
+        for stride in (block, block + 80, 3 * block):
+            hits, misses = around(base, block, 50, stride)
+            for name in ("positions", "slots"):
+                assert all(call_rope(lib, batch(**{name: x}), cache(block_stride=stride // 2)) == INVALID for x in hits), (which, stride)
+                assert all(call_rope(lib, batch(**{name: x}), cache(block_stride=stride // 2)) == 0 for x in misses), (which, stride)
+            for name in ("gq", "gk"):
+                assert call_rope(lib, batch(), cache(block_stride=stride // 2), **{name: base + 49 * stride + block - 16}) == INVALID
+                assert call_rope(lib, batch(), cache(block_stride=stride // 2), **{name: base + 49 * stride + block}) == 0
+    assert call_attention(lib, batch(prefix_table=300 * MIB, prefix_length=0), cache()) == 0  # not read
+
+
 SIZES = (1, 2, 15, 16, 17, 63, 64, 65, 255, 257, 1000, 4096, 131072, 3000001)
 
 
