@@ -356,7 +356,10 @@ typedef struct llama2_batch {
  * block is not refused for want of blocks; where one goes on behind a request that was,
  * new_taken[0] is above n_free.  With taken[0] above n_free (or negative) the list counts as
  * empty and new_taken[0] is taken[0]: nobody gets a block until the caller, who has to find blocks
- * or pause requests then, gives a new list.
+ * or pause requests then, gives a new list, or the number of blocks that really were handed out.  That
+ * can be less than new_taken says (what refused requests asked for is in it where another, a resting
+ * one too, goes on behind them), and is always the sum of ceil(lengths / block_size) over the requests
+ * behind the step, less the same of `cached`.
  * Block ids are copied, not looked at; free_blocks and the tables must not hold an id twice.  An id whose
  * slots would be negative or pass 2^31 gives slot -1.
  * prefix_table and max_length are not read. */

@@ -167,6 +167,46 @@ def test_a_pool_that_runs_dry_stops_requests_one_by_one():
     assert int(s.batch.taken[0]) == 7 and lengths.max() == 16 and lengths.min() == 8
 
 
+def test_blocks_left_behind_a_refused_prompt_are_handed_out_once_taken_is_put_right():
+    """A captured step, updated in place: a prompt that asks for more than is left stands in front of a request in the middle of a
+    block, a resting one and padding, so that `taken` passes the list's end; the host sets it to the blocks that the lengths say were handed
+    out, pauses the prompt, and the others get what is left, no block twice."""
+    size, requests, free = 8, 6, np.array([20, 21, 22, 23, 24, 25], np.int32)
+    b = RequestBatch(requests, 40, 6, 48)
+    table = np.full((requests, 6), -5, np.int32)
+    table[:, 0] = range(requests)
+    lengths = np.array([8, 8, 3, 8, 0, 0], np.int32)
+    b.blockTables.copy_to_device(table)
+    b.lengths.copy_to_device(lengths)
+    dfree, counts = up(free), up(np.zeros(requests, np.int32))
+    BatchTables().Forward(b, counts, dfree, size)  # nobody brings anything
+    assert np.array_equal(b.lengths.to_host(), lengths) and int(b.taken[0]) == 0
+    g = C.c_void_p()
+    capi.call("llama2_graph_begin_capture")
+    try:
+        BatchTables().Forward(b, counts, dfree, size)
+    finally:
+        capi.call("llama2_graph_end_capture", C.byref(g))
+    blocks = lambda n: int((-(-n // size)).sum())  # noqa: E731
+    taken, dry = 0, 0
+    for step, new in enumerate(([9, 1, 1, 9, 0, 0], [1, 25, 1, 1, 0, 0], [0, 1, 1, 8, 0, 0], [30, 0, 8, 0, 0, 0], [0, 9, 1, 0, 1, 0])):
+        counts.copy_to_device(np.array(new, np.int32))
+        capi.call("llama2_graph_launch", g)
+        want = bu.tables(table, lengths, np.array(new, np.int32), free, taken, size, 0, 40)
+        got = b.blockTables.to_host().reshape(table.shape), b.lengths.to_host()
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1]) and int(b.taken[0]) == want[5], step
+        used = taken + blocks(got[1]) - blocks(lengths)
+        assert used <= int(b.taken[0]) and used <= len(free)
+        if int(b.taken[0]) > len(free):  # as the header says
+            dry += 1
+            b.taken.copy_to_device(np.array([used], np.int32))
+        table, lengths, taken = got[0], got[1], used
+        mine = np.concatenate([table[r, :blocks(lengths[r:r + 1])] for r in range(requests)])
+        assert len(set(mine.tolist())) == len(mine)
+    assert dry >= 2 and taken == len(free)
+    capi.call("llama2_graph_destroy", g)
+
+
 def test_large_tables_in_place():
     """More tokens than one workgroup takes, lengths and taken blocks updated in place, also when replayed."""
     import test_gpu_batch as tb
