@@ -69,6 +69,25 @@ __attribute__((visibility("default"))) int l2h_repack_qweight(const uint32_t* qw
     });
 }
 
+// A step of several requests through the three module classes; device pointers throughout, gammas may be null.
+__attribute__((visibility("default"))) int l2h_batch_step(const llama2_batch* batch, const llama2_paged_cache* cache, int* counts,
+                                                          int* free_blocks, int n_free, int* taken, Half* query, Half* key, Half* value,
+                                                          Half* q_gamma, Half* k_gamma, Half* output, int n_heads, float theta, float scale)
+{
+    return guarded([&] {
+        const size_t tokens = batch->n_tokens, row = static_cast<size_t>(n_heads) * cache->head_size,
+                     kvRow = static_cast<size_t>(cache->n_kv_heads) * cache->head_size;
+        auto halfs = [](Half* p, size_t n) { return DeviceVariable<Half>::Window(p, n); };
+        auto q = halfs(query, tokens * row), k = halfs(key, tokens * kvRow), v = halfs(value, tokens * kvRow), out = halfs(output, tokens * row);
+        auto gq = halfs(q_gamma, cache->head_size), gk = halfs(k_gamma, cache->head_size);
+        auto c = DeviceVariable<int>::Window(counts, batch->n_requests), f = DeviceVariable<int>::Window(free_blocks, n_free),
+             t = DeviceVariable<int>::Window(taken, 1);
+        BatchTables().Forward(*batch, c, f, t, cache->block_size);
+        BatchQKNormRoPE().Forward(q, q, k, v, q_gamma ? &gq : nullptr, k_gamma ? &gk : nullptr, *batch, *cache, n_heads, theta);
+        BatchAttention().Forward(out, q, *batch, *cache, n_heads, scale);
+    });
+}
+
 __attribute__((visibility("default"))) int l2h_transformer_open(const char* path, int mode, int stop_on_special, void** handle)
 {
     *handle = nullptr;

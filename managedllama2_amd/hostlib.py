@@ -5,6 +5,8 @@ import os
 
 import numpy as np
 
+from . import capi
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # LLAMA2_HOST_LIB names another build of the facade (the sanitizer build of tests/test_oracle_sanitize.py)
 LIB_PATH = os.environ.get("LLAMA2_HOST_LIB") or os.path.join(_HERE, "libllama2_host.so")
@@ -37,6 +39,9 @@ def load():
         lib.l2h_transformer_logits.argtypes = [C.c_void_p, C.POINTER(C.c_uint16), C.c_int]
         lib.l2h_transformer_seq_len.argtypes = [C.c_void_p]
         lib.l2h_transformer_close.argtypes = [C.c_void_p]
+        vp = C.c_void_p
+        lib.l2h_batch_step.argtypes = [C.POINTER(capi.Batch), C.POINTER(capi.PagedCache), vp, vp, C.c_int, vp, vp, vp, vp, vp, vp, vp,
+                                       C.c_int, C.c_float, C.c_float]
         _lib = lib
     return _lib
 
@@ -82,6 +87,14 @@ class Transformer:
         if self._h:
             _check(load().l2h_transformer_close(self._h))
             self._h = C.c_void_p()
+
+
+def batch_step(batch, cache, counts, free_blocks, taken, query, key, value, output, n_heads, theta, scale, q_gamma=None, k_gamma=None):
+    """libLlama2::{BatchTables, BatchQKNormRoPE, BatchAttention}.Forward one after the other, on DeviceVariables; `query` is rotated
+    in place."""
+    ptr = lambda x: x.ptr if x else None  # noqa: E731
+    _check(load().l2h_batch_step(batch.struct(), cache.struct(), counts.ptr, free_blocks.ptr, free_blocks.size, taken.ptr, query.ptr, key.ptr,
+                                 value.ptr, ptr(q_gamma), ptr(k_gamma), output.ptr, n_heads, theta, scale))
 
 
 def repack_qweight(qweight, qzeros, scales, height, width, fmt=0):

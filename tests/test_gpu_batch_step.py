@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import batch_util as bu
-from managedllama2_amd import capi, synth
+from managedllama2_amd import capi, hostlib, synth
 from managedllama2_amd.device import DeviceVariable, PagedCache, RequestBatch, init
 from managedllama2_amd.modules import BatchAttention, BatchQKNormRoPE, BatchTables
 from gpu_util import up
@@ -145,6 +145,38 @@ def test_prompts_then_captured_decode_steps(heads, kv_heads, norms, prefix):
                 assert np.abs(o.to_host().astype(np.float32) - out[t]).max() <= 2.0 ** -8 * np.abs(vs).max(), (step, b)
     capi.call("llama2_graph_destroy", g)
     assert int(d.batch.taken[0]) == sum(-(-len(h) // size) for h in history)
+
+
+@pytest.mark.parametrize("norms", [False, True])
+def test_cpp_module_classes_do_the_same(norms):
+    """BatchTables, BatchQKNormRoPE and BatchAttention of the C++ host beside those of this one: prompts, then single tokens."""
+    rng = synth.rng_for(1505, int(norms))
+    heads, kv_heads = 8, 2
+    both = [Server(heads, kv_heads, 16, 40, 4, 60, 8, 100, 20) for _ in range(2)]
+    gammas = [up((1 + 0.1 * rng.standard_normal(D)).astype(np.float16)) for _ in range(2)] if norms else None
+    shared = normal(rng, 16 * 2 * kv_heads * D)
+    for s in both:
+        s.norms = gammas
+        for c in (s.cache.key, s.cache.value):  # the prefix's rows
+            for i, block in enumerate(s.prefix_ids):
+                c.copy_to_device(shared[i * 16 * kv_heads * D:(i + 1) * 16 * kv_heads * D], int(block) * 16 * kv_heads * D)
+    for counts in ([30, 1, 0, 17], [1, 1, 1, 1], [0, 2, 40, 1]):
+        q, k, v = normal(rng, 60, heads * D), normal(rng, 60, kv_heads * D), normal(rng, 60, kv_heads * D)
+        for s in both:
+            s.put(counts, q, k, v)
+            s.out.copy_to_device(np.full(60 * heads * D, 5.0, np.float16))
+        both[0].issue()
+        s = both[1]
+        gq, gk = gammas or (None, None)
+        hostlib.batch_step(s.batch, s.cache, s.counts, s.free, s.batch.taken, s.q, s.k, s.v, s.out, heads, THETA, D ** -0.5, gq, gk)
+        for get in (lambda s: s.q, lambda s: s.out, lambda s: s.cache.key, lambda s: s.cache.value, lambda s: s.batch.blockTables,
+                    lambda s: s.batch.lengths, lambda s: s.batch.slots, lambda s: s.batch.positions, lambda s: s.batch.taken):
+            a, b = (get(s).to_host() for s in both)
+            assert np.array_equal(a.view(np.uint8), b.view(np.uint8)), counts
+        both[0].check("%s" % counts)
+    s.cache.headSize = 96
+    with pytest.raises(hostlib.HostError, match="head_size"):
+        hostlib.batch_step(s.batch, s.cache, s.counts, s.free, s.batch.taken, s.q, s.k, s.v, s.out, heads, THETA, D ** -0.5)
 
 
 def test_a_pool_that_runs_dry_stops_requests_one_by_one():
