@@ -29,8 +29,8 @@ typedef float f16v_t __attribute__((ext_vector_type(16)));
 // maximum in nearly every pass): 2^6 exp2(score - m) is at most 2^14, and one of 2^-30 is still a number.  The sum carries
 // the same factors, so that they drop out of the quotient.  Narrow tiles, which wait for
 // the cache, take what that rounding left in a second product: 22 bits in all, and against 64 bits 2.1e-4, which is the output's own
-// rounding, instead of 2.5e-4 .. 2.9e-4 (one request of 777 rows 8.05 -> 8.1 us, 16 samples 16.5 -> 16.8, 64 conversations 121.1 -> 121.8,
-// 128 behind 8192 rows 91.6 -> 92.4, four documents 201.6).  Wide tiles are bound by the matrix cores, which it would give half as many
+// rounding, instead of 2.5e-4 .. 2.9e-4 (one request of 777 rows 8.1 -> 8.2 us, 16 samples 16.9 -> 17.0, 64 conversations 121.4 -> 121.8,
+// 128 behind 8192 rows 92.1 -> 92.6, four documents 201.4).  Wide tiles are bound by the matrix cores, which it would give half as many
 // products again: there the sum is of the rounded ones, so that the weights add up to 1.
 constexpr float kProbShift = 6.0f;
 constexpr float kSlack = 8.0f;
@@ -140,8 +140,6 @@ __device__ __forceinline__ float weight_of(float m, float most) { return m == -I
 
 // Any element infinite or NaN?  (bits 15 and 31 of the sum: all exponent bits set)
 __device__ __forceinline__ uint32_t not_finite(uint32_t v) { return ((v & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
-
-__device__ __forceinline__ bool is_nan(h2_t v) { return v[0] != v[0] || v[1] != v[1]; }
 
 // Elements of a head (D of them) in row `row` of a table; 64-bit offsets: a cache may be larger than 4 GB.
 template <int D>
@@ -349,23 +347,31 @@ __device__ void few_rows(const BatchAttnArgs& a, const Item& it, char* lds)
                 base = 0.0f;
             }
             h8_t p, rest; // the probabilities, and what their rounding left
+            float less = -1.0f; // kept from the compiler: a fused multiply-add takes the fp16 number as it is and rounds to fp16
+            asm volatile("" : "+s"(less));
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = exp2_of(s[t][i] - base);
-                    sum += e;
-                    p[4 * t + i] = static_cast<_Float16>(e);
-                    rest[4 * t + i] = static_cast<_Float16>(e - static_cast<float>(p[4 * t + i]));
+                for (int i = 0; i < 4; i += 2) {
+                    const float e0 = exp2_of(s[t][i] - base), e1 = exp2_of(s[t][i + 1] - base);
+                    sum += e0;
+                    sum += e1;
+                    uint32_t both = as_u32(h2_t{static_cast<_Float16>(e0), static_cast<_Float16>(e1)});
+                    asm volatile("" : "+v"(both)); // rounded once: the compiler would round one by one for the differences, too
+                    const h2_t e = as_h2(both);
+                    p[4 * t + i] = e[0];
+                    p[4 * t + i + 1] = e[1];
+                    rest[4 * t + i] = static_cast<_Float16>(__builtin_fmaf(static_cast<float>(e[0]), less, e0));
+                    rest[4 * t + i + 1] = static_cast<_Float16>(__builtin_fmaf(static_cast<float>(e[1]), less, e1));
                 }
-            h2_t check[2] = {};
+            float check[2] = {}; // sums of products of neighbours, not finite where one of them is not: two words at a time
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int k = 0; k < VW; ++k)
-                    check[k & 1] = __builtin_elementwise_fma(as_h2(vr[i][k]), h2_t{}, check[k & 1]); // NaN of what is not finite
+                for (int k = 0; k < VW; k += 2)
+                    check[i & 1] = dot2(vr[i][k], vr[i][k + 1], check[i & 1]);
             bool special = false;
-            if (!whole || __any(is_nan(check[0]) || is_nan(check[1]))) {
+            if (!whole || __any(!__builtin_isfinite(check[0]) || !__builtin_isfinite(check[1]))) {
                 // What lies behind the last row, or in a block that is none, and what is infinite or NaN (in rows that some
                 // columns attend and others do not, or beside a product of 0 or less), must not reach a sum through the products.
                 uint32_t bad = 0;
