@@ -10,8 +10,8 @@
 //            tile instead of once per request.
 // Pieces leave fp32 sums, maximum and denominator, which are joined in order.
 //
-// Tiles of up to 16 columns (few_rows) are bound by reading the cache: 1059 MB of four long documents in 195 us, 5.4 TB/s, HBM
-// traffic 1.00 times that; 594 MB of 64 conversations in 119 us, 5.0 TB/s, 1.02 times (a plain read of 1 GiB reaches 5.9 .. 6.3).
+// Tiles of up to 16 columns (few_rows) are bound by reading the cache: 1059 MB of four long documents in 201 us, 5.3 TB/s, HBM
+// traffic 1.00 times that; 594 MB of 64 conversations in 119 .. 124 us, 5.0 TB/s, 1.02 times (a plain read of 1 GiB reaches 5.9 .. 6.3).
 // Tiles of up to 128 columns (many_rows) are bound by products and power: with all compute units in their passes two of them
 // take 3200 cycles, 2048 of them matrix products, at a clock that falls from 2.4 to 1.73 GHz; 16384 tokens of 8 heads 830
 // TFLOP/s, where a library product of 8192^3 reaches 1235.

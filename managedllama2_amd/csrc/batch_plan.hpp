@@ -280,16 +280,26 @@ inline int batch_attn_piece(long long items, int rows, int shortest, int longest
 }
 
 // Sharing pays while a request has fewer than 64 columns of its own (more fill a workgroup's columns anyway, and the
-// prefix becomes the front of every request's rows), and where the prefix, read once more for every other request, is
+// prefix becomes the front of every request's rows: 40 requests of 32 heads, up to 2000 own rows behind 1024, 48 tokens each: shared
+// 143 us, not 150; 96 tokens: 223, 178), and where the prefix, read once more for every other request, is
 // more than joining the pieces costs: about 2^15 rows of a head, and a pass at least (98 requests of 40 heads behind 10
 // rows: shared 36 us, not 30; 19 of 8 heads behind 333: 13.1, 15.6).
 //
 // Narrow tiles: pieces so that every compute unit has 4 workgroups, of 128 rows at least (one round of the 4 wavefronts;
 // 777 rows of 32 heads: 64 rows 11.5 us, 128 9.9, 256 11.0) and 1024 at most, so that a long request ends with the others
 // (64 conversations: 512 rows 133 us, 1024 133, 4096 170; four documents of up to 131000 rows: 215, 203, 218).
-// Wide tiles are bound by the matrix cores, and the sums of their pieces weigh more than the cache: 2 workgroups per compute
-// unit, of 1024 rows at least for prompts, of 128 to 512 where prompts and single tokens mix (a mixed step: 1 workgroup per
-// compute unit 76 us, 2 60, 3 69; another one: 44, 53, 53).
+// Wide tiles are bound by the matrix cores, and the sums of their pieces weigh more than the cache.  Of prompts (64 columns
+// per request): 2 workgroups per compute unit, of 1024 rows at least (40 requests of 64 tokens, nothing shared: 81 us, cut as
+// below 114; of 48 tokens, cut as below, 100, so 75).  Where prompts and single tokens mix: 2 per compute unit of 128 to 1024 rows
+// while a piece of all has fewer workgroups than there are compute units (a mixed step: 1 per compute unit 76 us, 2 60, 3 69;
+// another one: 44, 53, 53), else 4 of 512 to 1024 rows.
+//
+// Wide tiles where a request has more than 16 columns on average (40 requests of 32 heads: 12 tokens narrow 60 us, wide 58; 16: 66, 61;
+// 24: 90, 71).  The average stands for all: one prompt of 2048 tokens beside 255 single ones is computed in narrow tiles, 545 us where
+// wide ones take 344.
+//
+// Rows are cut by the bounds that the host knows, not by the lengths: one request of 777 rows 8.2 us, with a max_length of 4096 9.9, of
+// 131072 19.4.
 inline BatchAttnPlan batch_attn_plan(const llama2_batch& b, int n_kv_heads, int group, int max_rows, int cus)
 {
     BatchAttnPlan p;
