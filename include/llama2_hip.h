@@ -125,6 +125,13 @@ int llama2_graph_destroy(void* graph);
  * must be 16-byte aligned.
  */
 
+/* src/QWeight.cs:5-10 */
+typedef struct llama2_qweight {
+    const uint32_t* weight;
+    const uint32_t* zeros;
+    const llama2_half* scales;
+} llama2_qweight;
+
 /* mat_vec_residual_int4_kernel (native/mat_vec_kernel.cuh:58-59), module
  * MatVecResidual.Forward (src/MatVecResidual.cs:15-22):
  *   output[n] = half(float(output[n]) + sum_k input[k]*(w-z)*s).
@@ -410,6 +417,85 @@ int llama2_batch_attention(llama2_half* output, const llama2_half* query, const 
                            const llama2_paged_cache* cache, int n_heads, int output_stride,
                            int query_stride, float scale);
 
+/* Low-rank adapters of one int4 tensor, a pool of which each token may use one: adapter a adds
+ *   scales[a] * sum_{r < ranks[a]} up_a[n][r] * sum_k down_a[r][k] * input[k]
+ * to output n.  Arrays are device memory; nothing beyond an adapter's rank has any influence. */
+typedef struct llama2_adapters {
+    const llama2_half* down; /* element k of rank r of adapter a at a * down_stride + r * rows + k; 16-byte aligned */
+    const llama2_half* up;   /* rank r of output n of adapter a at a * up_stride + n * max_rank + r; 16-byte aligned */
+    const float* scales;     /* [n_adapters] */
+    const int* ranks;        /* [n_adapters]: 0 .. max_rank (values outside count as the nearer of the two) */
+    long long down_stride;   /* halfs between adapters, a multiple of 8; 0: max_rank * rows */
+    long long up_stride;     /* halfs between adapters, a multiple of 8; 0: cols * max_rank */
+    int n_adapters;
+    int max_rank; /* a multiple of 8, 8 .. 128 */
+} llama2_adapters;
+
+/* One int4 tensor of a product of many rows, and where its results go. */
+typedef struct llama2_batch_matrix {
+    llama2_qweight weight;
+    llama2_half* output;             /* 16-byte aligned */
+    const llama2_half* residual;     /* added to the product; null: none; may be output with the same stride */
+    const llama2_adapters* adapters; /* host memory, read during the call; null: none */
+    int cols;                        /* outputs, a multiple of 8 */
+    int output_stride;               /* halfs between rows, a multiple of 8 */
+    int residual_stride;
+} llama2_batch_matrix;
+
+#define LLAMA2_MAX_BATCH_MATRICES 4
+
+/* Products of all tokens of a step with up to LLAMA2_MAX_BATCH_MATRICES int4 tensors that read the same input (q, k and
+ * v; or one):
+ *   output[t][n] = half(residual[t][n] + sum_k input[t][k] * (w - z) * s + adapter's part),
+ * sums in fp32, one rounding at the end; what an adapter's ranks receive of the input keeps 22 bits of the largest of them.
+ * rows % 8 == 0; tensors are laid out as above (ceil(rows/32)*4 words, ceil(rows/128) scales per output).
+ * Token t uses adapter token_adapters[t] of every matrix that has adapters; a value that is not one of 0 .. n_adapters - 1:
+ * none.  What one token or one adapter holds has no influence on the rows of other tokens.  token_adapters may be null where no
+ * matrix has adapters.  Rows of tokens without a position are left as they were.  Reads n_tokens and positions of
+ * the batch.  Outputs must not overlap each other, the input, or anything else that is read.  The same call gives the same bits every
+ * time.  Scratch: as llama2_multi_head_attention (call once before capturing).  Asynchronous, may be captured. */
+int llama2_batch_mat_mul_int4(const llama2_batch_matrix* matrices, int n_matrices, const llama2_half* input, int rows,
+                              int input_stride, const int* token_adapters, const llama2_batch* batch);
+
+/* The first half of the gated feed-forward block for all tokens of a step:
+ *   output[t][n] = half( silu(g) * u ),  silu(v) = v / (1 + exp(-v)),
+ * g and u the sums of llama2_batch_mat_mul_int4 with `gate` and `up` (and their adapters; null: none), in fp32.  The rest
+ * as there. */
+int llama2_batch_mat_mul_swiglu(llama2_half* output, const llama2_half* input, const llama2_qweight* gate,
+                                const llama2_qweight* up, int rows, int cols, int output_stride, int input_stride,
+                                const llama2_adapters* gate_adapters, const llama2_adapters* up_adapters,
+                                const int* token_adapters, const llama2_batch* batch);
+
+/* What stands between two blocks, for all tokens of a step:
+ *   y = input, or norm(input) * input_gamma if input_gamma; y *= gate if gate
+ *   r = residual + residual_scale * y   (r = residual if input is null)
+ *   residual_output = half(r);  output = half(norm(r) * gamma)
+ * with norm(v) = v / sqrt(mean(v^2) + eps), everything in fp32, r not rounded in front of its norm.  gammas and gate:
+ * `size` halfs.  output (with gamma) or residual_output may be null; residual_output may be residual with the same stride,
+ * output may be input with the same stride; otherwise outputs must not overlap anything.
+ * size: a multiple of 8 up to 65536; strides are multiples of 8, pointers 16-byte aligned.  Rows of tokens without a position
+ * are left as they were.  Reads n_tokens and positions of the batch.  Asynchronous, may be captured. */
+int llama2_batch_residual_rmsnorm(llama2_half* output, llama2_half* residual_output, const llama2_half* residual,
+                                  const llama2_half* input, const llama2_half* gamma, const llama2_half* input_gamma,
+                                  const llama2_half* gate, const llama2_batch* batch, int size, int output_stride,
+                                  int residual_output_stride, int residual_stride, int input_stride, float residual_scale,
+                                  float eps);
+
+/* Log probabilities, natural logarithms in fp32, of every row of logits under softmax(logits / temperature):
+ *   log_probs[r][i]  of tokens[r][i] for i < n_tokens; of a token that is not one of 0 .. vocab_size - 1: -infinity
+ *   entropies[r]     -sum p log p
+ *   top_tokens[r][j], top_log_probs[r][j]  for j < n_top: the most likely tokens in order, equal ones by their index; behind the
+ *                    last of a vocabulary smaller than n_top: -1 and -infinity
+ * Any of the four may be null (n_tokens / n_top 0 where theirs are; top_log_probs needs top_tokens).  A logit of -infinity has probability 0; of a row that holds
+ * nothing else all log probabilities are -infinity and the entropy is 0.  A row with NaN or +infinity has NaN for its log probabilities
+ * and its entropy; its top tokens are in the order of the logits, NaN last.  Rows whose position is negative are left as they
+ * were (positions null: none is).  n_tokens <= 1024, n_top <= LLAMA2_MAX_TOP_TOKENS, 0 < temperature; logits need
+ * no alignment beyond their 2 bytes.  Asynchronous, may be captured. */
+#define LLAMA2_MAX_TOP_TOKENS 64
+int llama2_batch_log_probs(float* log_probs, float* entropies, int* top_tokens, float* top_log_probs,
+                           const llama2_half* logits, const int* tokens, const int* positions, int n_rows, int vocab_size,
+                           int logits_stride, int n_tokens, int n_top, float temperature);
+
 /* ------------------------------------------------------- converter repack
  * The tensor transformations of ModelConverter.RepackQWeightByName
  * (src/ModelConverter.cs:196-275) on device buffers: what turns an AWQ
@@ -446,13 +532,6 @@ typedef struct llama2_config {
     int seq_len;
     float rope_theta;
 } llama2_config;
-
-/* src/QWeight.cs:5-10 */
-typedef struct llama2_qweight {
-    const uint32_t* weight;
-    const uint32_t* zeros;
-    const llama2_half* scales;
-} llama2_qweight;
 
 /* src/PerLayerWeight.cs:5-16 */
 typedef struct llama2_layer_weights {

@@ -16,6 +16,8 @@ ERR_NO_DEVICE = -4
 ERR_STEP_FAILED = -5
 MAX_SOFTMAX_SIZE = 8192
 MAX_SAMPLER_SIZE = 65536
+MAX_BATCH_MATRICES = 4
+MAX_TOP_TOKENS = 64
 
 DECODE_MODULES = 0
 DECODE_FUSED = 1
@@ -80,6 +82,18 @@ class Batch(C.Structure):
                 ("max_length", i)]
 
 
+class Adapters(C.Structure):
+    """llama2_adapters: low-rank adapters of one int4 tensor."""
+    _fields_ = [("down", vp), ("up", vp), ("scales", vp), ("ranks", vp), ("down_stride", C.c_longlong), ("up_stride", C.c_longlong),
+                ("n_adapters", i), ("max_rank", i)]
+
+
+class BatchMatrix(C.Structure):
+    """llama2_batch_matrix: one int4 tensor of a product of many rows."""
+    _fields_ = [("weight", QWeight), ("output", vp), ("residual", vp), ("adapters", C.POINTER(Adapters)), ("cols", i),
+                ("output_stride", i), ("residual_stride", i)]
+
+
 _SIGNATURES = {
     "llama2_init": [i],
     "llama2_shutdown": [],
@@ -122,6 +136,11 @@ _SIGNATURES = {
     "llama2_batch_tables": [C.POINTER(Batch), vp, vp, vp, i, vp, vp, i],
     "llama2_batch_qk_norm_rope": [vp, vp, vp, vp, vp, vp, C.POINTER(Batch), C.POINTER(PagedCache), i, i, i, i, f, f],
     "llama2_batch_attention": [vp, vp, C.POINTER(Batch), C.POINTER(PagedCache), i, i, i, f],
+    "llama2_batch_mat_mul_int4": [C.POINTER(BatchMatrix), i, vp, i, i, vp, C.POINTER(Batch)],
+    "llama2_batch_mat_mul_swiglu": [vp, vp, C.POINTER(QWeight), C.POINTER(QWeight), i, i, i, i, C.POINTER(Adapters), C.POINTER(Adapters), vp,
+                                    C.POINTER(Batch)],
+    "llama2_batch_residual_rmsnorm": [vp, vp, vp, vp, vp, vp, vp, C.POINTER(Batch), i, i, i, i, i, f, f],
+    "llama2_batch_log_probs": [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, f],
     "llama2_repack_qdata": [vp, vp, i, i],
     "llama2_repack_scales": [vp, vp, i, i],
     "llama2_compact_scales_v1": [vp, vp, i, i],

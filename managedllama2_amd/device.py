@@ -152,3 +152,21 @@ class RequestBatch:
         return capi.Batch(self.blockTables.ptr, self.lengths.ptr, self.queryStarts.ptr, self.positions.ptr, self.slots.ptr,
                           self.prefixTable.ptr if self.prefixTable else None, self.numRequests, self.numTokens, self.tableStride,
                           self.prefixLength, self.maxLength)
+
+
+class Adapters:
+    """A pool of low-rank adapters of one int4 tensor: down [numAdapters][maxRank][rows] and up [numAdapters][cols][maxRank] in fp16, ranks,
+    and scales in fp32, as device variables."""
+
+    def __init__(self, down, up, ranks, scales, maxRank):
+        self.down, self.up, self.ranks, self.scales, self.maxRank = down, up, ranks, scales, maxRank
+
+    @classmethod
+    def from_host(cls, down, up, ranks, scales):
+        """down: [numAdapters][maxRank][rows], up: [numAdapters][cols][maxRank]."""
+        f = DeviceVariable.from_host
+        return cls(f(np.asarray(down, np.float16)), f(np.asarray(up, np.float16)), f(np.asarray(ranks, np.int32)),
+                   f(np.asarray(scales, np.float32)), down.shape[1])
+
+    def pointer(self):
+        return C.pointer(capi.Adapters(self.down.ptr, self.up.ptr, self.scales.ptr, self.ranks.ptr, 0, 0, self.ranks.size, self.maxRank))

@@ -439,7 +439,7 @@ struct Argmax : Module { // src/Argmax.cs
 };
 
 // Steps of several requests at once (no counterpart in the reference, whose cache holds one sequence): thin callers of
-// the three operators; the batch and the cache are plain structs of device pointers that the application keeps.
+// the operators; the batch and the cache are plain structs of device pointers that the application keeps.
 struct BatchTables : Module {
     using Module::Module;
     // batch.lengths and `taken` count on in place
@@ -472,6 +472,58 @@ struct BatchAttention : Module {
     {
         const int row = numHeads * cache.head_size;
         Check(llama2_batch_attention(output.DevicePointer(), query.DevicePointer(), &batch, &cache, numHeads, row, row, scale));
+    }
+};
+
+// The products of all tokens with up to four int4 tensors that read the same input; the application fills the matrices (outputs,
+// residuals, adapters).  tokenAdapters: the adapter of every token, null where no matrix has any.
+struct BatchMatMulInt4 : Module {
+    using Module::Module;
+    void Forward(const std::vector<llama2_batch_matrix>& matrices, DeviceVariable<Half>& input, int rows, const llama2_batch& batch,
+                 DeviceVariable<int>* tokenAdapters = nullptr)
+    {
+        Check(llama2_batch_mat_mul_int4(matrices.data(), static_cast<int>(matrices.size()), input.DevicePointer(), rows, rows,
+                                        tokenAdapters ? tokenAdapters->DevicePointer() : nullptr, &batch));
+    }
+};
+
+struct BatchMatMulSwiGLU : Module {
+    using Module::Module;
+    // rows side by side without gaps
+    void Forward(DeviceVariable<Half>& output, DeviceVariable<Half>& input, const llama2_qweight& gate, const llama2_qweight& up, int rows,
+                 int cols, const llama2_batch& batch, DeviceVariable<int>* tokenAdapters = nullptr,
+                 const llama2_adapters* gateAdapters = nullptr, const llama2_adapters* upAdapters = nullptr)
+    {
+        Check(llama2_batch_mat_mul_swiglu(output.DevicePointer(), input.DevicePointer(), &gate, &up, rows, cols, cols, rows, gateAdapters,
+                                          upAdapters, tokenAdapters ? tokenAdapters->DevicePointer() : nullptr, &batch));
+    }
+};
+
+struct BatchResidualRMSNorm : Module {
+    using Module::Module;
+    // residual counts on in place; input, inputGamma, gate: null leaves them out
+    void Forward(DeviceVariable<Half>& output, DeviceVariable<Half>& residual, DeviceVariable<Half>* input, DeviceVariable<Half>& gamma,
+                 int size, const llama2_batch& batch, DeviceVariable<Half>* inputGamma = nullptr, DeviceVariable<Half>* gate = nullptr,
+                 float scale = 1.0f, float eps = 1e-5f)
+    {
+        auto pointer = [](DeviceVariable<Half>* v) { return v ? v->DevicePointer() : nullptr; };
+        Check(llama2_batch_residual_rmsnorm(output.DevicePointer(), input ? residual.DevicePointer() : nullptr, residual.DevicePointer(),
+                                            pointer(input), gamma.DevicePointer(), pointer(inputGamma), pointer(gate), &batch, size, size,
+                                            size, size, size, scale, eps));
+    }
+};
+
+struct BatchLogProbs : Module {
+    using Module::Module;
+    // `given` tokens of each row, `top` most likely ones; null: not computed
+    void Forward(DeviceVariable<float>* logProbs, DeviceVariable<float>* entropies, DeviceVariable<int>* topTokens,
+                 DeviceVariable<float>* topLogProbs, DeviceVariable<Half>& logits, int numRows, int vocabSize,
+                 DeviceVariable<int>* tokens = nullptr, int given = 0, int top = 0, float temperature = 1.0f,
+                 DeviceVariable<int>* positions = nullptr)
+    {
+        auto pointer = [](auto* v) { return v ? v->DevicePointer() : nullptr; };
+        Check(llama2_batch_log_probs(pointer(logProbs), pointer(entropies), pointer(topTokens), pointer(topLogProbs), logits.DevicePointer(),
+                                     pointer(tokens), pointer(positions), numRows, vocabSize, vocabSize, given, top, temperature));
     }
 };
 

@@ -88,6 +88,32 @@ __attribute__((visibility("default"))) int l2h_batch_step(const llama2_batch* ba
     });
 }
 
+// The rest of a layer's step, from the attention's output on, and the answers from a row of logits per token, through the module
+// classes: o = output projection onto x, norm, gated block, down projection, x += norm(that) * post_gamma, norm into xb; log
+// probabilities of `given`.  Device pointers throughout, adapters may be null.
+__attribute__((visibility("default"))) int l2h_batch_block(const llama2_batch* batch, const llama2_layer_weights* w, Half* attention, Half* x,
+                                                           Half* xb, Half* h, Half* y, int dim, int hidden, const llama2_adapters* adapters,
+                                                           int* token_adapters, Half* post_gamma, Half* next_gamma, Half* logits, int vocab,
+                                                           int* given, float* log_probs, float* entropies, int* top_tokens, int n_top)
+{
+    return guarded([&] {
+        const size_t tokens = batch->n_tokens;
+        auto halfs = [](Half* p, size_t n) { return DeviceVariable<Half>::Window(p, n); };
+        auto a = halfs(attention, tokens * dim), res = halfs(x, tokens * dim), normed = halfs(xb, tokens * dim), mid = halfs(h, tokens * hidden),
+             out = halfs(y, tokens * dim), ff = halfs(const_cast<Half*>(w->rms_feed_forward), dim), post = halfs(post_gamma, dim),
+             next = halfs(next_gamma, dim), l = halfs(logits, tokens * vocab);
+        auto ids = DeviceVariable<int>::Window(token_adapters, tokens), g = DeviceVariable<int>::Window(given, tokens),
+             top = DeviceVariable<int>::Window(top_tokens, tokens * n_top), pos = DeviceVariable<int>::Window(batch->positions, tokens);
+        auto lp = DeviceVariable<float>::Window(log_probs, tokens), e = DeviceVariable<float>::Window(entropies, tokens);
+        BatchMatMulInt4().Forward({{w->output, x, x, adapters, dim, dim, dim}}, a, dim, *batch, &ids);
+        BatchResidualRMSNorm().Forward(normed, res, nullptr, ff, dim, *batch);
+        BatchMatMulSwiGLU().Forward(mid, normed, w->gate, w->up, dim, hidden, *batch);
+        BatchMatMulInt4().Forward({{w->down, y, nullptr, nullptr, dim, dim, 0}}, mid, hidden, *batch);
+        BatchResidualRMSNorm().Forward(normed, res, &out, next, dim, *batch, &post);
+        BatchLogProbs().Forward(&lp, &e, &top, nullptr, l, static_cast<int>(tokens), vocab, &g, 1, n_top, 1.0f, &pos);
+    });
+}
+
 __attribute__((visibility("default"))) int l2h_transformer_open(const char* path, int mode, int stop_on_special, void** handle)
 {
     *handle = nullptr;

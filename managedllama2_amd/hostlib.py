@@ -42,6 +42,8 @@ def load():
         vp = C.c_void_p
         lib.l2h_batch_step.argtypes = [C.POINTER(capi.Batch), C.POINTER(capi.PagedCache), vp, vp, C.c_int, vp, vp, vp, vp, vp, vp, vp,
                                        C.c_int, C.c_float, C.c_float]
+        lib.l2h_batch_block.argtypes = [C.POINTER(capi.Batch), C.POINTER(capi.LayerWeights), vp, vp, vp, vp, vp, C.c_int, C.c_int,
+                                        C.POINTER(capi.Adapters), vp, vp, vp, vp, C.c_int, vp, vp, vp, vp, C.c_int]
         _lib = lib
     return _lib
 
@@ -95,6 +97,15 @@ def batch_step(batch, cache, counts, free_blocks, taken, query, key, value, outp
     ptr = lambda x: x.ptr if x else None  # noqa: E731
     _check(load().l2h_batch_step(batch.struct(), cache.struct(), counts.ptr, free_blocks.ptr, free_blocks.size, taken.ptr, query.ptr, key.ptr,
                                  value.ptr, ptr(q_gamma), ptr(k_gamma), output.ptr, n_heads, theta, scale))
+
+
+def batch_block(batch, weights, attention, x, xb, h, y, dim, hidden, adapters, token_adapters, post_gamma, next_gamma, logits, vocab, given,
+                log_probs, entropies, top_tokens, n_top):
+    """libLlama2::{BatchMatMulInt4, BatchMatMulSwiGLU, BatchResidualRMSNorm, BatchLogProbs}.Forward: the rest of a layer's step behind
+    the attention and the answers from a row of logits per token, on DeviceVariables; x counts on in place."""
+    _check(load().l2h_batch_block(batch.struct(), weights, attention.ptr, x.ptr, xb.ptr, h.ptr, y.ptr, dim, hidden,
+                                  adapters.pointer() if adapters else None, token_adapters.ptr, post_gamma.ptr, next_gamma.ptr, logits.ptr, vocab,
+                                  given.ptr, log_probs.ptr, entropies.ptr, top_tokens.ptr, n_top))
 
 
 def repack_qweight(qweight, qzeros, scales, height, width, fmt=0):

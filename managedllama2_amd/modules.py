@@ -191,3 +191,48 @@ class BatchAttention(Module):
         row = numHeads * cache.headSize
         capi.call("llama2_batch_attention", output.ptr, query.ptr, batch.struct(), cache.struct(), numHeads,
                   *(strides or (row, row)), scale)
+
+
+class BatchMatMulInt4(Module):
+    """Products of all tokens of a step with up to four int4 tensors that read the same input (llama2_batch_mat_mul_int4).  Each of
+    `matrices` is (output, QWeight, cols) or (output, QWeight, cols, residual, adapters): residual a device variable whose rows are added (it may be
+    the output), adapters a device.Adapters; tokenAdapters: the adapter of every token.  Rows side by side without gaps."""
+
+    def Forward(self, matrices, input, rows, batch, tokenAdapters=None):
+        m = (capi.BatchMatrix * len(matrices))()
+        for i, (output, weight, cols, *more) in enumerate(matrices):
+            residual, adapters = (more + [None, None])[:2]
+            m[i] = capi.BatchMatrix(weight=weight.struct(), output=output.ptr, residual=residual.ptr if residual else None,
+                                    adapters=adapters.pointer() if adapters else None, cols=cols, output_stride=cols, residual_stride=cols)
+        capi.call("llama2_batch_mat_mul_int4", m, len(matrices), input.ptr, rows, rows, tokenAdapters.ptr if tokenAdapters else None,
+                  batch.struct())
+
+
+class BatchMatMulSwiGLU(Module):
+    """silu(gate) * up of all tokens of a step (llama2_batch_mat_mul_swiglu)."""
+
+    def Forward(self, output, input, gate, up, rows, cols, batch, tokenAdapters=None, gateAdapters=None, upAdapters=None):
+        capi.call("llama2_batch_mat_mul_swiglu", output.ptr, input.ptr, gate.struct(), up.struct(), rows, cols, cols, rows,
+                  gateAdapters.pointer() if gateAdapters else None, upAdapters.pointer() if upAdapters else None,
+                  tokenAdapters.ptr if tokenAdapters else None, batch.struct())
+
+
+class BatchResidualRMSNorm(Module):
+    """residual += scale * gate * norm(input) * inputGamma (gate, inputGamma, input: None leaves them out), output = norm(residual) *
+    gamma, for all tokens of a step (llama2_batch_residual_rmsnorm).  Without an input the residual stays as it is."""
+
+    def Forward(self, output, residual, input, gamma, size, batch, inputGamma=None, gate=None, scale=1.0, eps=1e-5):
+        ptr = lambda v: v.ptr if v else None  # noqa: E731
+        capi.call("llama2_batch_residual_rmsnorm", ptr(output), residual.ptr if input else None, residual.ptr, ptr(input), ptr(gamma),
+                  ptr(inputGamma), ptr(gate), batch.struct(), size, size, size, size, size, scale, eps)
+
+
+class BatchLogProbs(Module):
+    """Log probabilities of given tokens, entropies and the most likely tokens of rows of logits (llama2_batch_log_probs).  What is
+    None is not computed; tokens: numTokens of each row; positions: rows with a negative one are left as they were."""
+
+    def Forward(self, logProbs, entropies, topTokens, topLogProbs, logits, numRows, vocabSize, tokens=None, numTokens=0, numTop=0,
+                temperature=1.0, positions=None):
+        ptr = lambda v: v.ptr if v else None  # noqa: E731
+        capi.call("llama2_batch_log_probs", ptr(logProbs), ptr(entropies), ptr(topTokens), ptr(topLogProbs), logits.ptr, ptr(tokens),
+                  ptr(positions), numRows, vocabSize, vocabSize, numTokens, numTop, temperature)

@@ -1,0 +1,175 @@
+"""Products of the rows of many tokens with int4 tensors, low-rank adapters beside them, and the gated block's first half,
+against 64-bit restatements (product_util.py)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import product_util as pu
+from managedllama2_amd import capi, synth
+from managedllama2_amd.device import init
+
+pytestmark = pytest.mark.gpu
+
+RANKS = [16, 0, 1, 5, 8, 13, 24, 32]
+
+
+@pytest.fixture(autouse=True, scope="module")
+def ready():
+    init(0)
+
+
+def rng(*stream):
+    return synth.rng_for(1700, *stream)
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 15, 16, 17, 31, 33, 48, 64, 65, 100, 130, 257])
+@pytest.mark.parametrize("gated", [False, True])
+def test_numbers_of_tokens(tokens, gated):
+    pu.Product(rng(1, tokens, gated), tokens, 264, [88], gated, RANKS, 32, pad=tokens % 5, residual=not gated).upload().check()
+
+
+@pytest.mark.parametrize("K", [8, 24, 120, 128, 136, 256, 1000, 1032, 4096, 11008])
+@pytest.mark.parametrize("tokens", [3, 70, 140])
+def test_lengths_of_a_row(K, tokens):
+    pu.Product(rng(2, K, tokens), tokens, K, [40], False, [8, 3], 8, x_extra=16, extra=8).upload().check()
+    pu.Product(rng(3, K, tokens), tokens, K, [24], True, [8, 3], 8, x_extra=8, extra=24).upload().check()
+
+
+@pytest.mark.parametrize("cols", [[8], [16], [24, 8], [1000], [264, 40, 8, 520], [512, 512, 512], [1376]])
+@pytest.mark.parametrize("tokens", [1, 20, 50, 200])
+def test_widths(cols, tokens):
+    pu.Product(rng(4, tokens, *cols), tokens, 384, cols, False, [4, 16, 7], 16, residual=len(cols) % 2 == 1, extra=16).upload().check()
+    pu.Product(rng(5, tokens, *cols), tokens, 384, cols[:1], True).upload().check()
+
+
+@pytest.mark.parametrize("max_rank", [8, 16, 24, 64, 72, 128])
+@pytest.mark.parametrize("tokens", [1, 16, 40, 150])
+@pytest.mark.parametrize("gated", [False, True])
+def test_ranks(max_rank, tokens, gated):
+    """Adapters of every rank, infinities and NaN beyond each rank and between them, and every way that tokens can use them."""
+    ranks = sorted({0, 1, 7, max_rank // 2, max_rank - 1, max_rank})
+    for i, junk in enumerate((np.nan, -np.inf)):
+        g = rng(6, max_rank, tokens, gated, i)
+        pu.Product(g, tokens, 520, [72], gated, ranks + [max_rank + 50, -3], max_rank, pool_stride=(0, 24)[i], junk=junk).upload().check("any")
+    one = pu.Product(rng(7, max_rank, tokens), tokens, 520, [72], gated, [max_rank] * 3, max_rank, ids=1).upload()
+    one.check("one for all")
+    each = pu.Product(rng(8, max_rank, tokens), tokens, 136, [72], gated, [max_rank] * tokens, max_rank, ids=np.arange(tokens)[::-1]).upload()
+    each.check("one for each")
+
+
+def test_only_some_matrices_have_adapters():
+    p = pu.Product(rng(9), 37, 256, [64, 128, 64], False, [8, 16], 16)
+    p.pools[1] = None
+    p.upload().check()
+    for keep in (0, 1):
+        s = pu.Product(rng(10, keep), 37, 256, [64], True, [8, 16], 16)
+        s.pools[1 - keep] = None
+        s.upload().check()
+
+
+@pytest.mark.parametrize("tokens", [5, 60, 300])
+def test_residual_in_place_and_outputs_side_by_side(tokens):
+    p = pu.Product(rng(11, tokens), tokens, 640, [256], residual=True, in_place=True, pad=3).upload()
+    p.check()
+    q = pu.Product(rng(12, tokens), tokens, 256, [64, 32, 40], ranks=[8], max_rank=8, pad=2).upload()
+    want = q.run()
+    wide = pu.up(np.full((q.tokens, 64 + 32 + 40 + 8), pu.GUARD, np.float16))
+    name, m, *rest = q.args([wide] * 3)
+    at = 0
+    for i, n in enumerate(q.cols):
+        m[i].output, m[i].output_stride = wide.ptr + 2 * at, 144
+        at += n
+    capi.call(name, m, *rest)
+    got = wide.to_host().reshape(q.tokens, -1)
+    assert np.array_equal(got[:, :136].view(np.uint16), np.concatenate(want, 1).view(np.uint16)) and (got[:, 136:] == pu.GUARD).all()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("tokens", [6, 90, 200])
+def test_what_one_token_or_adapter_holds_stays_with_it(gated, tokens):
+    p = pu.Product(rng(13, tokens, gated), tokens, 264, [48], gated, [8, 12, 16], 16, ids=np.arange(tokens) % 4 - 1).upload()
+    want = p.run()[0]
+    for pool in p.pools:
+        pool.down_of(1)[:12, ::7] = np.inf
+        pool.up_of(1)[::3, :12] = np.nan
+    p.x[4, 5] = np.inf
+    p.upload()
+    got = p.run()[0]
+    hit = (p.ids == 1) | (np.arange(tokens) == 4)
+    assert np.array_equal(got[~hit].view(np.uint16), want[~hit].view(np.uint16))
+    assert not np.isfinite(got[hit]).all(1).any()
+
+
+@pytest.mark.parametrize("tokens", [20, 200])
+def test_sizes_of_what_the_ranks_receive(tokens):
+    """Adapters whose inner values lie far outside fp16's range, or far below it, lose nothing."""
+    for i, (d, u) in enumerate(((3.0e4, 1.0e-6), (2.0 ** -14, 200.0), (60000.0, 2.0 ** -20))):
+        p = pu.Product(rng(14, tokens, i), tokens, 512, [64], False, [16, 5], 16, junk=0.0)
+        for pool in p.pools:
+            pool.down[:] = (pool.down.astype(np.float32) * d).clip(-65504, 65504).astype(np.float16)
+            pool.up[:] = (pool.up.astype(np.float32) * u).astype(np.float16)
+        p.upload().check()
+    p.x[:, :512] = 0
+    p.upload().check("zeros")
+
+
+@pytest.mark.parametrize("tokens", [1, 48, 300])
+@pytest.mark.parametrize("gated", [False, True])
+def test_captured_steps_replayed(tokens, gated):
+    """Inputs, adapters of the tokens and tokens without a position change between replays; eager calls of other sizes stand between."""
+    p = pu.Product(rng(15, tokens, gated), tokens, 512, [96], gated, RANKS, 32).upload()
+    other = pu.Product(rng(16, tokens, gated), tokens + 70, 640, [104], gated, RANKS, 32).upload()
+    other.run()
+    outs = p.outputs()
+    capi.call(*p.args(outs))
+    g = C.c_void_p()
+    capi.call("llama2_graph_begin_capture")
+    try:
+        capi.call(*p.args(outs))
+    finally:
+        capi.call("llama2_graph_end_capture", C.byref(g))
+    r = rng(17, tokens)
+    for turn in range(4):
+        p.x[:, :512] = r.standard_normal((p.tokens, 512))
+        p.ids[:] = r.integers(-1, len(RANKS), p.tokens)
+        p.positions[:] = np.where(r.random(p.tokens) < 0.3, -1, 7)
+        for dev, host in ((p.dx, p.x), (p.di, p.ids), (p.dp, p.positions)):
+            dev.copy_to_device(host)
+        outs[0].copy_to_device(np.full((p.tokens, 96), pu.GUARD, np.float16))
+        capi.call("llama2_graph_launch", g)
+        other.run()
+        got = outs[0].to_host().reshape(p.tokens, -1)
+        eager = p.run()[0]
+        assert np.array_equal(got.view(np.uint16), eager.view(np.uint16)), turn
+        dead = p.positions < 0
+        assert (got[dead] == pu.GUARD).all()
+        want, bound = p.reference()[0]
+        assert (np.abs(got.astype(np.float64) - want) <= bound)[~dead].all(), turn
+    capi.call("llama2_graph_destroy", g)
+
+
+def test_a_call_that_would_need_scratch_in_a_capture_is_refused():
+    p = pu.Product(rng(18), 1 << 18, 8, [8], False, [128], 128, ids=0, junk=0.0).upload()
+    outs, g = p.outputs(), C.c_void_p()
+    capi.call("llama2_graph_begin_capture")
+    try:
+        rc = capi.raw(*p.args(outs))
+    finally:
+        capi.call("llama2_graph_end_capture", C.byref(g))
+    assert rc == capi.ERR_INVALID_ARGUMENT and "capture" in capi.last_error()
+    capi.call("llama2_graph_destroy", g)
+    p.check()
+
+
+def test_one_token_beside_the_module_of_one_token():
+    """llama2_mat_vec_int4 and llama2_mat_vec_swiglu round the same sums, added in another order."""
+    for gated, K, N in ((False, 4096, 512), (True, 2048, 352)):
+        p = pu.Product(rng(19, gated), 1, K, [N], gated).upload()
+        out = p.outputs()[0]
+        ws, ss, zs = synth.qweight_sizes(K)
+        w = [v for q in p.weights for v in (q.Weight.ptr, q.Zeros.ptr, q.Scales.ptr)]
+        capi.call("llama2_mat_vec_swiglu" if gated else "llama2_mat_vec_int4", out.ptr, p.dx.ptr, *w, K, N, zs, ss, ws)
+        one, (want, bound) = out.to_host().astype(np.float64), p.reference()[0]
+        assert (np.abs(one - want[0]) <= bound[0]).all()
+        p.check()
