@@ -15,181 +15,291 @@ namespace l2 {
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-struct ProductTensor {
+// What a tensor's adapters leave for its product, per token and 16 ranks (a block): the scale of the adapter with the block's power of
+// two, and the adapter's rank.
+struct TokenAdapter {
+    float factor;
+    int rank;
+};
+constexpr int kRankBlocks = kMaxRank / 16;
+
+// Arguments lie in memory, and a kernel that asks for them one after the other waits for each: a tensor's are neighbours, chosen by
+// an index that the first cache line holds.
+struct alignas(64) LowTensor {
+    const uint16_t* down; // null: no adapters
+    const float* scales;
+    const int* ranks;
+    uint16_t* low;      // [n_tokens][blocks][2][16]: what the ranks received, upper and lower part
+    TokenAdapter* info; // [n_tokens][blocks]
+    long long down_stride;
+    int n_adapters, max_rank;
+};
+
+struct alignas(64) LowArgs {
+    const uint16_t* x;
+    const int* positions;
+    const int* token_adapters;
+    int K, x_stride, n_tokens, most_adapters;
+    LowTensor t[LLAMA2_MAX_BATCH_MATRICES];
+};
+
+struct alignas(64) ProductTensor {
     const uint32_t* w;
     const uint32_t* z;
     const uint16_t* s;
     uint16_t* out;
     const uint16_t* residual;
-    const uint16_t* down; // null: no adapters
-    const uint16_t* up;
-    const float* scales;
-    const int* ranks;
-    long long down_stride, up_stride;
-    uint16_t* low;  // [n_tokens][max_rank / 8][2][8]: what the ranks received, upper and lower part
-    float* factors; // [n_tokens]: scale of the adapter and power of two of the token
-    int n_adapters, max_rank, cols, out_stride, residual_stride;
-    int first; // first block of rows of this tensor
+    const uint16_t* up; // null: no adapters
+    const uint16_t* low;
+    const TokenAdapter* info;
+    long long up_stride;
+    int cols, out_stride, residual_stride, n_adapters, max_rank;
 };
 
-struct ProductArgs {
-    ProductTensor m[LLAMA2_MAX_BATCH_MATRICES];
+struct alignas(64) ProductArgs {
     const uint16_t* x;
     const int* positions;
     const int* token_adapters;
-    int n_matrices, K, groups, ws, ss, zs, x_stride, n_tokens, row_blocks, token_blocks;
+    int K, x_stride, n_tokens, most_adapters; // of any tensor
+    int row_blocks, token_blocks;
+    int first[LLAMA2_MAX_BATCH_MATRICES]; // first block of rows of a tensor
+    ProductTensor t[LLAMA2_MAX_BATCH_MATRICES];
 };
 
-// The arguments as they lie in memory: a tensor chosen by an index is then a scalar load (chosen among registers it is a hundred
+// The arguments as they lie in memory: a tensor chosen by an index is then a few scalar loads (chosen among registers it is a hundred
 // instructions).
-typedef __attribute__((address_space(4))) const ProductArgs KernelArgs;
-__device__ __forceinline__ KernelArgs& kernel_args()
+template <class A>
+using Constant = __attribute__((address_space(4))) const A;
+
+template <class A>
+__device__ __forceinline__ Constant<A>& kernel_args()
 {
-    return *(KernelArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    return *(Constant<A>*)__builtin_amdgcn_kernarg_segment_ptr();
+}
+
+template <class V>
+__device__ __forceinline__ void needed(const V& v)
+{
+    asm volatile("" : : "s"(v));
+}
+
+template <class... V>
+__device__ __forceinline__ void loaded(const V&... v) // here, together
+{
+    (needed(v), ...);
 }
 
 constexpr int kNoAdapter = -1, kNoToken = -2;
 
-// Adapter of token t: one of 0 .. n - 1, kNoAdapter, or kNoToken where there is no token.
-__device__ __forceinline__ int adapter_of(KernelArgs& a, int t)
+// Adapter of token t: one that some tensor has, kNoAdapter, or kNoToken where there is no token.
+__device__ __forceinline__ int adapter_of(const int* positions, const int* token_adapters, int t, int n_tokens, int most_adapters)
 {
-    if (t >= a.n_tokens || a.positions[t] < 0)
-        return kNoToken;
-    const int id = a.token_adapters ? a.token_adapters[t] : kNoAdapter;
-    return id < 0 ? kNoAdapter : id;
+    t = min(t, n_tokens);
+    int position = -1, id = kNoAdapter;
+    if (t < n_tokens) {
+        position = positions[t];
+        if (token_adapters)
+            id = token_adapters[t];
+    }
+    return position < 0 ? kNoToken : id < 0 || id >= most_adapters ? kNoAdapter : id;
 }
 
-// Which of 16 tokens in LDS are the first with their adapter, as bits; the same in every wavefront.
-__device__ __forceinline__ unsigned first_of_adapter(const int* ids, int n_adapters)
-{
-    const int l = threadIdx.x & 15, id = ids[l];
-    bool first = id >= 0 && id < n_adapters;
-#pragma unroll
-    for (int j = 0; j < 15; ++j)
-        first = first && !(j < l && ids[j] == id);
-    return static_cast<unsigned>(__ballot(first)) & 0xFFFFu;
-}
+// Tokens of a block of up to 64 that use the same adapter, by up to 16 of them: an item.  Items are numbered in the order of their
+// first tokens.
+struct Items {
+    int ids[64];            // adapter of a token, kNoAdapter, kNoToken
+    int adapter[64];        // of an item
+    uint8_t tokens[64][16]; // of an item, kNobody behind the last
+    int count;
+};
+constexpr uint8_t kNobody = 255;
 
-__device__ __forceinline__ int nth_bit(unsigned mask, int n) // of the set ones
+// By one wavefront, from the first `tokens` of items.ids; everyone may read the items after the next barrier.
+__device__ __forceinline__ void find_items(Items& items, int tokens)
 {
-    for (; n > 0; --n)
-        mask &= mask - 1;
-    return __builtin_ctz(mask);
-}
-
-__device__ __forceinline__ int rank_of(const int* ranks, int a, int max_rank)
-{
-    const int r = __builtin_amdgcn_readfirstlane(ranks[a]);
-    return r < 0 ? 0 : r > max_rank ? max_rank : r;
+    const int lane = threadIdx.x & 63, id = lane < tokens ? items.ids[lane] : kNoToken;
+    int before = 0, lead = -1; // tokens with this adapter in front of this one, and the first of its sixteen
+    for (int j = 0; j < tokens; ++j) {
+        const bool same = __builtin_amdgcn_readlane(id, j) == id && j <= lane;
+        lead = same && (before & 15) == 0 ? j : lead;
+        before += same;
+    }
+    const unsigned long long leads = __ballot(id >= 0 && lead == lane);
+    reinterpret_cast<u32x4*>(items.tokens)[lane] = u32x4{~0u, ~0u, ~0u, ~0u};
+    if (id >= 0) {
+        const int item = __builtin_popcountll(leads & ((1ULL << lead) - 1));
+        items.tokens[item][(before - 1) & 15] = static_cast<uint8_t>(lane);
+        if (lead == lane)
+            items.adapter[item] = id;
+    }
+    if (lane == 0)
+        items.count = __builtin_popcountll(leads);
 }
 
 __device__ __forceinline__ f4_t mfma16(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// Elements k .. k + 7 of a row of which n exist.
-__device__ __forceinline__ h8_t load8(const uint16_t* row, int k, int n)
+// A buffer whose reads beyond `bytes` return zero.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void* p, size_t bytes)
 {
-    u32x4 v = {};
-    if (k < n)
-        v = *reinterpret_cast<const u32x4*>(row + k);
-    return __builtin_bit_cast(h8_t, v);
+    return make_rsrc(p, bytes > 0x7FFFFFFFu ? 0x7FFFFFFFu : static_cast<uint32_t>(bytes));
+}
+
+constexpr int kBehind = static_cast<int>(0x80000000u); // an offset behind the end of every buffer: reads zero, moves nothing
+
+// 16 rows of 128 halfs, requested in the order of memory (a compute unit looks up 64 bytes at a time, and only neighbouring lanes share a
+// lookup: lanes that read 16 bytes of a row each, as the matrix cores want them, cost four times as many) and turned around through
+// LDS that belongs to the wavefront.  Load i: rows 4 i + lane / 16, elements 8 (lane % 16) on.
+struct HalfTile {
+    u32x4 v[4];
+};
+
+// Lane's place in a row of the tile, or kBehind where the row of n elements has ended; k0: first element of the tile.
+__device__ __forceinline__ int tile_column(int k0, int n)
+{
+    const int k = k0 + 8 * (threadIdx.x & 15);
+    return k < n ? 2 * k : kBehind;
+}
+
+constexpr int kTileBytes = 16 * 256;
+
+__device__ __forceinline__ void put_tile(char* lds, const HalfTile& t)
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = 4 * i + (lane >> 4);
+        *reinterpret_cast<u32x4*>(lds + row * 256 + ((lane & 15) ^ row) * 16) = t.v[i];
+    }
+}
+
+// Operand m of four: lane group c holds elements 32 c + 8 m on of row lane % 16.
+__device__ __forceinline__ h8_t tile_operand(const char* lds, int m)
+{
+    const int row = threadIdx.x & 15, c = (threadIdx.x & 63) >> 4;
+    return *reinterpret_cast<const h8_t*>(lds + row * 256 + ((4 * c + m) ^ row) * 16);
 }
 
 // ---------------------------------------------------------------- what the ranks receive
-// A workgroup takes 16 tokens and one of the adapters that they use; its wavefronts split the inputs.  Columns of other tokens are
-// computed with it and dropped: columns of a matrix product do not mix.
-constexpr int kLowWaves = 8, kLowTiles = 4; // rank tiles of 16 at a time
+// A workgroup takes 16 ranks of one item of a block of 64 tokens, so that an adapter is read once for up to 16 tokens that use it; its
+// wavefronts split the inputs.  Ranks and scales of small pools are requested together with the tokens' adapters.
+constexpr int kLowWaves = 16, kLowTable = kLowWaves * 64;
 
-__global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(ProductArgs)
+__global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
 {
-    constexpr int kStride = kLowTiles * 16 + 4;
-    __shared__ int ids[16];
+    constexpr int kStride = 16 + 4;
+    __shared__ __align__(16) Items items;
+    __shared__ int table[kLowTable];
+    __shared__ float scale_table[kLowTable];
+    __shared__ __align__(16) char tiles[kLowWaves * kTileBytes];
     __shared__ __align__(16) float red[kLowWaves * 16 * kStride];
-    __shared__ __align__(16) float sums[16 * (kMaxRank + 4)];
-    KernelArgs& a = kernel_args();
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, c = lane >> 4;
-    const int t0 = blockIdx.x * 16;
-    __attribute__((address_space(4))) const ProductTensor& m = a.m[blockIdx.z];
-    if (!m.down)
+    auto& a = kernel_args<LowArgs>();
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, c = lane >> 4;
+    const int t0 = blockIdx.x * 64, K = a.K, x_stride = a.x_stride, n_tokens = a.n_tokens, most_adapters = a.most_adapters;
+    const uint16_t* const x = a.x;
+    const int *const positions = a.positions, *const token_adapters = a.token_adapters;
+    auto& t = a.t[blockIdx.z / kRankBlocks];
+    const int block = blockIdx.z % kRankBlocks, r0 = block * 16;
+    const uint16_t* down = t.down;
+    const float* const scales = t.scales;
+    const int* const ranks = t.ranks;
+    uint16_t* const low = t.low;
+    TokenAdapter* const info = t.info;
+    const long long down_stride = t.down_stride;
+    const int n_adapters = t.n_adapters, max_rank = t.max_rank;
+    loaded(K, x_stride, n_tokens, most_adapters, x, positions, token_adapters, down, scales, ranks, low, info, down_stride, n_adapters, max_rank);
+    if (!down || r0 >= max_rank)
         return;
-    if (threadIdx.x < 16)
-        ids[threadIdx.x] = adapter_of(a, t0 + threadIdx.x);
+    int mine = 0;
+    float mine_scale = 0.0f;
+    if (tid < n_adapters) {
+        mine = ranks[tid];
+        mine_scale = scales[tid];
+    }
+    if (wave == 0) {
+        items.ids[lane] = adapter_of(positions, token_adapters, t0 + lane, n_tokens, most_adapters);
+        find_items(items, min(64, n_tokens - t0));
+    }
+    table[tid] = mine;
+    scale_table[tid] = mine_scale;
     __syncthreads();
-    const unsigned firsts = first_of_adapter(ids, m.n_adapters);
-    if (static_cast<int>(blockIdx.y) >= __builtin_popcount(firsts))
+    const int item = blockIdx.y;
+    if (item >= items.count)
         return;
-    const int id = __builtin_amdgcn_readfirstlane(ids[nth_bit(firsts, blockIdx.y)]);
-    const int rank = rank_of(m.ranks, id, m.max_rank);
-    const int token = t0 + l15 < a.n_tokens ? t0 + l15 : a.n_tokens - 1;
-    const uint16_t* x = a.x + static_cast<size_t>(token) * a.x_stride;
-    const uint16_t* down = m.down + id * m.down_stride;
-    for (int r0 = 0; r0 < rank; r0 += kLowTiles * 16) {
-        f4_t acc[kLowTiles] = {};
-        const int tiles = min((rank - r0 + 15) / 16, kLowTiles);
-        for (int k0 = wave * 128; k0 < a.K; k0 += kLowWaves * 128) {
-            h8_t xf[4];
+    const int id = __builtin_amdgcn_readfirstlane(items.adapter[item]);
+    if (id >= n_adapters)
+        return;
+    const int rank = min(max(__builtin_amdgcn_readfirstlane(id < kLowTable ? table[id] : ranks[id]), 0), max_rank);
+    if (r0 >= rank && r0 > 0) // the first block says that there are no ranks at all
+        return;
+    const float scale = id < kLowTable ? scale_table[id] : scales[id];
+    const __amdgpu_buffer_rsrc_t rx = rows_buffer(x + static_cast<size_t>(t0) * x_stride,
+                                                  (static_cast<size_t>(min(64, n_tokens - t0) - 1) * x_stride + K) * 2);
+    const __amdgpu_buffer_rsrc_t rd = rows_buffer(down + id * down_stride, static_cast<size_t>(rank) * K * 2); // ranks beyond are zero
+    int xoff[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int own = items.tokens[item][4 * i + c];
+        xoff[i] = own == kNobody ? kBehind : own * x_stride * 2;
+    }
+    constexpr int kAhead = 2; // tiles of both that a wavefront has requested
+    HalfTile xt[kAhead], dt[kAhead];
+    auto request = [&](int q, int k0) {
+        const int column = tile_column(k0, K);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            xt[q].v[i] = __builtin_amdgcn_raw_buffer_load_b128(rx, column < 0 || xoff[i] < 0 ? kBehind : xoff[i] + column, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            dt[q].v[i] = __builtin_amdgcn_raw_buffer_load_b128(rd, column < 0 ? kBehind : (r0 + 4 * i + c) * K * 2 + column, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+        request(q, (wave + q * kLowWaves) * 128);
+    char* const lds = tiles + wave * kTileBytes;
+    f4_t acc = {};
+    for (int k0 = wave * 128; k0 < K; k0 += kAhead * kLowWaves * 128)
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) { // behind the last elements both are zero
+            h8_t xf[4], df[4];
+            put_tile(lds, xt[q]);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                xf[j] = load8(x, k0 + 32 * j + 8 * c, a.K);
+                xf[j] = tile_operand(lds, j);
+            put_tile(lds, dt[q]);
 #pragma unroll
-            for (int i = 0; i < kLowTiles; ++i)
-                if (i < tiles) {
-                    const int r = r0 + i * 16 + l15;
-                    const uint16_t* row = down + static_cast<size_t>(r < rank ? r : rank - 1) * a.K;
+            for (int j = 0; j < 4; ++j)
+                df[j] = tile_operand(lds, j);
+            request(q, k0 + (q + kAhead) * kLowWaves * 128);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[i] = mfma16(xf[j], load8(row, k0 + 32 * j + 8 * c, a.K), acc[i]);
-                }
+            for (int j = 0; j < 4; ++j)
+                acc = mfma16(xf[j], df[j], acc);
         }
 #pragma unroll
-        for (int i = 0; i < kLowTiles; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                red[(wave * 16 + 4 * c + e) * kStride + i * 16 + l15] = acc[i][e];
-        __syncthreads();
-        for (int e = threadIdx.x; e < 16 * kLowTiles * 16; e += kLowWaves * 64) {
-            const int t = e / (kLowTiles * 16), r = e % (kLowTiles * 16);
-            float v = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kLowWaves; ++w)
-                v += red[(w * 16 + t) * kStride + r];
-            sums[t * (kMaxRank + 4) + r0 + r] = r0 + r < rank ? v : 0.0f;
-        }
-        __syncthreads();
-    }
-    // 32 threads a token, 4 ranks a thread
-    const int t = threadIdx.x >> 5, r = (threadIdx.x & 31) * 4;
-    if (ids[t] != id)
+    for (int e = 0; e < 4; ++e)
+        red[(wave * 16 + 4 * c + e) * kStride + l15] = acc[e];
+    __syncthreads();
+    if (wave >= 4)
         return;
-    float v[4] = {}, most = 0.0f;
-    if (r < rank) {
+    // 16 lanes a token, a rank each
+    const int place = tid >> 4, m = items.tokens[item][place];
+    float v = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[e] = sums[t * (kMaxRank + 4) + r + e];
-            most = fmaxf(most, fabsf(v[e]));
-        }
-    }
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1)
-        most = fmaxf(most, __shfl_xor(most, d, 64));
+    for (int w = 0; w < kLowWaves; ++w)
+        v += red[(w * 16 + place) * kStride + l15];
+    v = r0 + l15 < rank ? v : 0.0f;
+    const float most = row16_max(fabsf(v));
     // the largest between 2^14 and 2^15; nothing to scale where all are 0 or one is infinite
-    int e2 = 0;
-    if (most > 0.0f && most < INFINITY)
-        e2 = 14 - ilogbf(most);
-    if (r < (rank + 7) / 8 * 8) {
-        uint32_t hi[2] = {}, lo[2] = {};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float s = ldexpf(v[e], e2);
-            const uint16_t h = float_to_half_bits(s);
-            hi[e >> 1] |= static_cast<uint32_t>(h) << (16 * (e & 1));
-            lo[e >> 1] |= static_cast<uint32_t>(float_to_half_bits(s - half_bits_to_float(h))) << (16 * (e & 1));
-        }
-        uint16_t* to = m.low + (static_cast<size_t>(t0 + t) * m.max_rank + r / 8 * 8) * 2 + (r & 4);
-        *reinterpret_cast<u32x2*>(to) = u32x2{hi[0], hi[1]};
-        *reinterpret_cast<u32x2*>(to + 8) = u32x2{lo[0], lo[1]};
-    }
-    if (r == 0)
-        m.factors[t0 + t] = ldexpf(m.scales[id], -e2);
+    const int e2 = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
+    const float scaled = ldexpf(v, e2);
+    const uint16_t h = float_to_half_bits(scaled);
+    if (m == kNobody)
+        return;
+    const size_t to = static_cast<size_t>(t0 + m) * ((max_rank + 15) / 16) + block;
+    low[to * 32 + l15] = h;
+    low[to * 32 + 16 + l15] = float_to_half_bits(scaled - half_bits_to_float(h));
+    if (l15 == 0)
+        info[to] = TokenAdapter{ldexpf(scale, -e2), rank};
 }
 
 // ---------------------------------------------------------------- the products
@@ -207,270 +317,395 @@ __device__ __forceinline__ h8_t weights_of(uint32_t w, h2_t minus)
     return __builtin_bit_cast(h8_t, v);
 }
 
-// Lane group c of 16 holds words 4 c .. 4 c + 3 of a group's 16 in v; afterwards words c, 4 + c, 8 + c and 12 + c.
-__device__ __forceinline__ u32x4 words_by_product(u32x4 v)
+// 16 rows of the 16 words of a group, requested in the order of memory (row lane / 4, words 4 (lane % 4) on) and turned around through
+// LDS: afterwards lane group c holds words 4 c .. 4 c + 3 of row lane % 16, which go with operand m of a tile of inputs word by word.
+__device__ __forceinline__ u32x4 turned_words(char* lds, u32x4 v)
 {
-    const auto a = __builtin_amdgcn_permlane32_swap(v[0], v[2], false, false);
-    const auto b = __builtin_amdgcn_permlane32_swap(v[1], v[3], false, false);
-    const auto lo = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
-    const auto hi = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    const int lane = threadIdx.x & 63, row = lane & 15, c = lane >> 4;
+    *reinterpret_cast<u32x4*>(lds + (lane >> 2) * 64 + ((lane & 3) ^ (lane >> 4)) * 16) = v;
+    return *reinterpret_cast<const u32x4*>(lds + row * 64 + (c ^ (row >> 2)) * 16);
 }
 
 constexpr int kProductWaves = 8;
+constexpr int kScaleBytes = 20480; // of LDS for the scales and zero points of a workgroup's rows
 
 // A workgroup takes R tiles of 16 outputs (GATED: half of them of the gate, half of the up projection) and T tiles of 16
-// tokens; its wavefronts take the groups of 128 inputs in turn and add up through LDS.
-template <int R, int T, bool GATED>
+// tokens; its wavefronts take the groups of 128 inputs in turn, D of them requested ahead, and add up through LDS.
+template <int R, int T, int D, bool GATED, bool ADAPTERS>
 __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(ProductArgs)
 {
-    constexpr int kTokens = T * 16, kRows = R * 16, kStride = kRows + 4;
-    __shared__ __align__(16) float red[kProductWaves * kTokens * kStride];
-    __shared__ int ids[kTokens];
-    __shared__ __align__(16) float factors[2][kTokens];
-    KernelArgs& a = kernel_args();
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, c = lane >> 4;
+    constexpr int kTokens = T * 16, kRows = R * 16, kStride = kRows + 4, kTensors = GATED ? 2 : 1, RT = R / kTensors;
+    constexpr int kRing = T * D <= 4 ? T * D : 2; // tiles of tokens whose inputs are on their way or in use
+    static_assert(T * D % kRing == 0 && kRing <= T * D, "a tile has one place in the ring");
+    constexpr int kWaveBytes = kTileBytes + R * 1024, kSums = kProductWaves * kTokens * kStride * 4, kExtra = ADAPTERS ? kTokens * kStride * 4 : 0;
+    constexpr int kFront = kProductWaves * kWaveBytes + kScaleBytes;
+    __shared__ __align__(16) char pool[(kFront > kSums ? kFront : kSums) + kExtra]; // the sums come where tiles and scales were
+    __shared__ __align__(16) Items items;
+    auto& a = kernel_args<ProductArgs>();
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, c = lane >> 4;
+    const int K = a.K, x_stride = a.x_stride, n_tokens = a.n_tokens, most_adapters = a.most_adapters, row_blocks = a.row_blocks,
+              token_blocks = a.token_blocks, first1 = a.first[1], first2 = a.first[2], first3 = a.first[3];
+    const uint16_t* const x = a.x;
+    const int *const positions = a.positions, *const token_adapters = a.token_adapters;
+    loaded(K, x_stride, n_tokens, most_adapters, row_blocks, token_blocks, first1, first2, first3, x, positions, token_adapters);
     // the token blocks of one block of rows follow each other on one XCD
-    const int slot = blockIdx.x >> 3, rb = slot / a.token_blocks * 8 + (blockIdx.x & 7), t0 = slot % a.token_blocks * kTokens;
-    if (rb >= a.row_blocks)
+    const int slot = blockIdx.x >> 3, rb = slot / token_blocks * 8 + (blockIdx.x & 7), t0 = slot % token_blocks * kTokens;
+    if (rb >= row_blocks)
         return;
-    int which = 0;
-    if (!GATED)
-        while (which + 1 < a.n_matrices && rb >= a.m[which + 1].first)
-            ++which;
-    auto& m0 = a.m[which];
-    auto& m1 = a.m[GATED ? 1 : which];
-    const int n0 = (rb - (GATED ? 0 : m0.first)) * (GATED ? kRows / 2 : kRows);
-    auto row_of = [&](int r) { return n0 + (GATED ? r % (R / 2) : r) * 16; };
-    if (threadIdx.x < kTokens) {
-        const int t = t0 + threadIdx.x, id = adapter_of(a, t);
-        ids[threadIdx.x] = id;
-        factors[0][threadIdx.x] = m0.down && id >= 0 && id < m0.n_adapters ? m0.factors[t] : 0.0f;
-        if (GATED)
-            factors[1][threadIdx.x] = m1.down && id >= 0 && id < m1.n_adapters ? m1.factors[t] : 0.0f;
+    const int which = GATED ? 0 : (rb >= first1) + (rb >= first2) + (rb >= first3);
+    const int ws = (K + 31) / 32 * 4, groups = (K + 127) / 128, zs = (groups + 7) / 8;
+    struct Tensor {
+        const uint32_t* w;
+        const uint32_t* z;
+        const uint16_t* s;
+        const uint16_t* up;
+        const uint16_t* low;
+        const TokenAdapter* info;
+        long long up_stride;
+        int n_adapters, max_rank;
+    } m[kTensors];
+#pragma unroll
+    for (int h = 0; h < kTensors; ++h) {
+        auto& t = a.t[which + h];
+        m[h] = {t.w, t.z, t.s, t.up, t.low, t.info, t.up_stride, t.n_adapters, t.max_rank};
     }
-
-    const uint32_t* w[R];
-    const uint32_t* z[R];
-    const uint16_t* s[R];
+    auto& t = a.t[which];
+    const int cols = t.cols, out_stride = t.out_stride, residual_stride = t.residual_stride;
+    uint16_t* const out = t.out;
+    const uint16_t* const residual_rows = t.residual;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        auto& m = GATED && r >= R / 2 ? m1 : m0;
-        const int n = min(row_of(r) + l15, m.cols - 1);
-        w[r] = m.w + static_cast<size_t>(n) * a.ws;
-        z[r] = m.z + static_cast<size_t>(n) * a.zs;
-        s[r] = m.s + static_cast<size_t>(n) * a.ss;
+    for (int h = 0; h < kTensors; ++h) {
+        loaded(m[h].w, m[h].z, m[h].s);
+        if (ADAPTERS)
+            loaded(m[h].up, m[h].low, m[h].info, m[h].up_stride, m[h].n_adapters, m[h].max_rank);
     }
-    const uint16_t* x[T];
-#pragma unroll
-    for (int t = 0; t < T; ++t)
-        x[t] = a.x + static_cast<size_t>(min(t0 + t * 16 + l15, a.n_tokens - 1)) * a.x_stride;
+    loaded(cols, out_stride, residual_stride, out, residual_rows);
+    const int n0 = (rb - (which == 0 ? 0 : which == 1 ? first1 : which == 2 ? first2 : first3)) * RT * 16;
 
-    f4_t acc[T][R] = {};
-    for (int g = wave; g < a.groups; g += kProductWaves) {
-        h8_t wf[R][4];
-        float sc[R];
+    // Rows and tokens that do not exist lie behind the ends of the buffers.
+    const int rows = min(RT * 16, cols - n0), here = min(kTokens, n_tokens - t0);
+    __amdgpu_buffer_rsrc_t rw[kTensors];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            // words behind the end of a row meet zeros of x
-            const u32x4 v = words_by_product(*reinterpret_cast<const u32x4*>(w[r] + min(16 * g + 4 * c, a.ws - 4)));
-            const float zero = static_cast<float>(z[r][g >> 3] >> (4 * (g & 7)) & 15u);
-            const h2_t minus = {static_cast<_Float16>(-1024.0f - zero), static_cast<_Float16>(-64.0f - zero)};
-            sc[r] = half_bits_to_float(s[r][g]);
+    for (int h = 0; h < kTensors; ++h)
+        rw[h] = rows_buffer(m[h].w + static_cast<size_t>(n0) * ws, static_cast<size_t>(rows) * ws * 4);
+    const __amdgpu_buffer_rsrc_t rx = rows_buffer(x + static_cast<size_t>(t0) * x_stride, (static_cast<size_t>(here - 1) * x_stride + K) * 2);
+    const int woff = (lane >> 2) * ws * 4 + 16 * (lane & 3), xoff = c * x_stride * 2;
+
+    // A group's weights and inputs.  A group that does not exist is requested behind the ends too: loads that come and go would make
+    // every wait one for all of them.
+    u32x4 raw[D][R];
+    HalfTile xt[kRing];
+    auto load_w = [&](int d, int g) {
+        const int k = g < groups ? 64 * g : kBehind;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                wf[r][j] = weights_of(v[j], minus);
-        }
+        for (int r = 0; r < R; ++r)
+            raw[d][r] = __builtin_amdgcn_raw_buffer_load_b128(rw[r / RT], woff + (r % RT) * ws * 64 + k, 0, 0);
+        __builtin_amdgcn_sched_barrier(0); // loads keep one order from the first group on: waits count them
+    };
+    auto load_x = [&](int q, int i, int g) { // tile i into place q
+        const int column = tile_column(128 * g, K), at = column < 0 ? kBehind : column + xoff;
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            h8_t xf[4];
+        for (int e = 0; e < 4; ++e)
+            xt[q].v[e] = __builtin_amdgcn_raw_buffer_load_b128(rx, at + (i * 16 + 4 * e) * x_stride * 2, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                xf[j] = load8(x[t], 128 * g + 32 * j + 8 * c, a.K);
-            f4_t p[R] = {};
+    for (int d = 0; d < D; ++d) {
+        load_w(d, wave + d * kProductWaves);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int i = 0; i < T; ++i)
+            if (d * T + i < kRing)
+                load_x(d * T + i, i, wave + d * kProductWaves);
+    }
+    // Scales and zero points of all rows: they are neighbours in memory.
+    char* const lds = pool + wave * kWaveBytes; // of this wavefront
+    uint16_t* const scales = reinterpret_cast<uint16_t*>(pool + kProductWaves * kWaveBytes);
+    uint32_t* const zeros = reinterpret_cast<uint32_t*>(scales + (kRows * groups + 7) / 8 * 8);
 #pragma unroll
-                for (int r = 0; r < R; ++r)
-                    p[r] = mfma16(xf[j], wf[r][j], p[r]);
+    for (int h = 0; h < kTensors; ++h) {
+        const uint16_t* const s = m[h].s + static_cast<size_t>(n0) * groups;
+        const uint32_t* const z = m[h].z + static_cast<size_t>(n0) * zs;
+        for (int i = tid; i < rows * groups; i += kProductWaves * 64)
+            scales[h * RT * 16 * groups + i] = s[i];
+        for (int i = tid; i < rows * zs; i += kProductWaves * 64)
+            zeros[h * RT * 16 * zs + i] = z[i];
+    }
+    if (tid < kTokens)
+        items.ids[tid] = adapter_of(positions, token_adapters, t0 + tid, n_tokens, most_adapters);
+    float* const extra = reinterpret_cast<float*>(pool + (kFront > kSums ? kFront : kSums));
+    if (ADAPTERS && wave == 0)
+        find_items(items, here);
+    __syncthreads();
+    if constexpr (ADAPTERS) {
+        // The adapters' part of each item, straight to where the sums of the wavefronts meet: a token has one adapter.
+        for (int i = wave; i < items.count * kTensors; i += kProductWaves) {
+            const int item = i / kTensors, h = i % kTensors;
+            auto& m0 = m[0];
+            auto& m1 = m[kTensors - 1];
+            const uint16_t *up = h ? m1.up : m0.up, *low = h ? m1.low : m0.low;
+            const int max_rank = h ? m1.max_rank : m0.max_rank, id = __builtin_amdgcn_readfirstlane(items.adapter[item]);
+            if (!up || id >= (h ? m1.n_adapters : m0.n_adapters))
+                continue;
+            // tokens of the places that this lane's row of inputs, and its four rows of results, stand for
+            const int own = items.tokens[item][l15], lead = items.tokens[item][0];
+            const size_t blocks = (max_rank + 15) / 16, mine = (t0 + (own == kNobody ? lead : own)) * blocks;
+            const TokenAdapter* const info = h ? m1.info : m0.info;
+            const __amdgpu_buffer_rsrc_t ru = rows_buffer(up + id * (h ? m1.up_stride : m0.up_stride) + static_cast<size_t>(n0) * max_rank,
+                                                          static_cast<size_t>(rows) * max_rank * 2);
+            int of[4];
 #pragma unroll
-            for (int r = 0; r < R; ++r)
+            for (int e = 0; e < 4; ++e)
+                of[e] = items.tokens[item][4 * c + e];
+            const int rank = __builtin_amdgcn_readfirstlane(info[(t0 + lead) * blocks].rank);
+            f4_t sum[RT] = {};
+            for (int b = 0; b * 16 < rank; ++b) {
+                // lane groups 0 and 1: the upper parts of ranks 0 .. 7 and 8 .. 15 of the block; 2 and 3: the lower ones
+                const int have = rank - b * 16 - (c & 1) * 8;
+                const u32x4 hf = *reinterpret_cast<const u32x4*>(low + (mine + b) * 32 + c * 8);
+                float f[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    acc[t][r][e] = __builtin_fmaf(p[r][e], sc[r], acc[t][r][e]);
+                    f[e] = info[(t0 + (of[e] == kNobody ? lead : of[e])) * blocks + b].factor;
+                u32x4 u[(RT + 1) / 2];
+#pragma unroll
+                for (int r = 0; r < (RT + 1) / 2; ++r) { // 32 rows of 16 ranks, a row by two lanes
+                    const int row = r * 32 + (lane >> 1), r8 = b * 16 + (lane & 1) * 8;
+                    u[r] = __builtin_amdgcn_raw_buffer_load_b128(ru, r8 < rank && row < RT * 16 ? (row * max_rank + r8) * 2 : kBehind, 0, 0);
+                }
+#pragma unroll
+                for (int r = 0; r < (RT + 1) / 2; ++r)
+                    *reinterpret_cast<u32x4*>(lds + r * 1024 + lane * 16) = u[r];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    u32x4 v = *reinterpret_cast<const u32x4*>(lds + (r * 16 + l15) * 32 + (c & 1) * 16);
+                    if (rank & 7)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            v[k] &= have >= 2 * k + 2 ? ~0u : have == 2 * k + 1 ? 0xFFFFu : 0u;
+                    const f4_t p = mfma16(__builtin_bit_cast(h8_t, hf), __builtin_bit_cast(h8_t, v), f4_t{});
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sum[r][e] = __builtin_fmaf(p[e], f[e], sum[r][e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (of[e] != kNobody)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+                        extra[of[e] * kStride + (h * RT + r) * 16 + l15] = sum[r][e];
         }
     }
-    __syncthreads(); // ids and factors
-    // The adapters, each added to the tokens that use it (an adapter with infinite weights must not reach the others).
+
+    f4_t acc[T][R] = {};
+    for (int g0 = wave; g0 < groups; g0 += kProductWaves * D) {
 #pragma unroll
-    for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-        auto& m = h ? m1 : m0;
-        if (!m.down)
-            continue;
+        for (int d = 0; d < D; ++d) { // groups that do not exist are zeros
+            const int g = g0 + d * kProductWaves, gs = min(g, groups - 1);
+            h8_t wf[R][4];
+            float sc[R];
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const unsigned firsts = first_of_adapter(ids + t * 16, m.n_adapters);
-            const int count = __builtin_popcount(firsts);
-            for (int i = wave; i < count; i += kProductWaves) {
-                const int id = __builtin_amdgcn_readfirstlane(ids[t * 16 + nth_bit(firsts, i)]);
-                const int rank = rank_of(m.ranks, id, m.max_rank), token = min(t0 + t * 16 + l15, a.n_tokens - 1);
+            for (int r = 0; r < R; ++r) {
+                const u32x4 v = turned_words(lds + kTileBytes + r * 1024, raw[d][r]);
+                const int row = r * 16 + l15;
+                const float zero = static_cast<float>(zeros[row * zs + (gs >> 3)] >> (4 * (gs & 7)) & 15u);
+                const h2_t minus = {static_cast<_Float16>(-1024.0f - zero), static_cast<_Float16>(-64.0f - zero)};
+                sc[r] = half_bits_to_float(scales[row * groups + gs]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    wf[r][j] = weights_of(v[j], minus);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_w(d, g + kProductWaves * D);
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                const int q = (d * T + i) % kRing, next = d * T + i + kRing; // the tile that comes into this place
+                put_tile(lds, xt[q]);
+                h8_t xf[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    xf[j] = tile_operand(lds, j);
+                load_x(q, next % T, g0 + next / T * kProductWaves);
                 f4_t p[R] = {};
-                for (int r0 = 0; r0 < rank; r0 += 16) {
-                    // lane groups 0 and 1: the upper parts of ranks 0 .. 7 and 8 .. 15; 2 and 3: the lower ones
-                    const int at = r0 + (c & 1) * 8, have = rank - at;
-                    u32x4 h4 = {};
-                    if (have > 0)
-                        h4 = *reinterpret_cast<const u32x4*>(m.low + (static_cast<size_t>(token) * m.max_rank + at) * 2 + (c >> 1) * 8);
 #pragma unroll
-                    for (int r = h * (R / 2); r < (GATED && !h ? R / 2 : R); ++r) {
-                        u32x4 u = {};
-                        if (have > 0)
-                            u = *reinterpret_cast<const u32x4*>(m.up + id * m.up_stride +
-                                                                static_cast<size_t>(min(row_of(r) + l15, m.cols - 1)) * m.max_rank + at);
-                        if (rank & 7)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                u[k] &= have >= 2 * k + 2 ? ~0u : have == 2 * k + 1 ? 0xFFFFu : 0u;
-                        p[r] = mfma16(__builtin_bit_cast(h8_t, h4), __builtin_bit_cast(h8_t, u), p[r]);
-                    }
-                }
+                    for (int r = 0; r < R; ++r)
+                        p[r] = mfma16(xf[j], wf[r][j], p[r]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool own = ids[t * 16 + 4 * c + e] == id;
-                    const float f = factors[h][t * 16 + 4 * c + e];
+                for (int r = 0; r < R; ++r)
 #pragma unroll
-                    for (int r = h * (R / 2); r < (GATED && !h ? R / 2 : R); ++r)
-                        acc[t][r][e] = own ? __builtin_fmaf(p[r][e], f, acc[t][r][e]) : acc[t][r][e];
-                }
+                    for (int e = 0; e < 4; ++e)
+                        acc[i][r][e] = __builtin_fmaf(p[r][e], sc[r], acc[i][r][e]);
             }
         }
     }
+    __syncthreads(); // everyone is through with tiles and scales
+    float* const red = reinterpret_cast<float*>(pool);
 #pragma unroll
-    for (int t = 0; t < T; ++t)
+    for (int i = 0; i < T; ++i)
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                red[(wave * kTokens + t * 16 + 4 * c + e) * kStride + r * 16 + l15] = acc[t][r][e];
+                red[(wave * kTokens + i * 16 + 4 * c + e) * kStride + r * 16 + l15] = acc[i][r][e];
     __syncthreads();
-    constexpr int kOut = GATED ? kRows / 2 : kRows, kPieces = kOut / 8;
-    for (int i = threadIdx.x; i < kTokens * kPieces; i += kProductWaves * 64) {
-        const int t = i / kPieces, piece = i % kPieces * 8, n = n0 + piece;
-        if (ids[t] == kNoToken || n >= m0.cols)
+    constexpr int kPieces = RT * 2; // of 8 outputs
+    for (int i = tid; i < kTokens * kPieces; i += kProductWaves * 64) {
+        const int token = i / kPieces, piece = i % kPieces * 8, n = n0 + piece, id = items.ids[token];
+        if (id == kNoToken || n >= cols)
             continue;
-        float v[2][8] = {};
+        u32x4 residual = {};
+        if (!GATED && residual_rows)
+            residual = *reinterpret_cast<const u32x4*>(residual_rows + static_cast<size_t>(t0 + token) * residual_stride + n);
+        float v[kTensors][8] = {};
 #pragma unroll
-        for (int h = 0; h < (GATED ? 2 : 1); ++h)
-            for (int q = 0; q < kProductWaves; ++q)
+        for (int h = 0; h < kTensors; ++h) {
+            auto add = [&](const float* from) {
 #pragma unroll
                 for (int k = 0; k < 8; k += 4) {
-                    const f4_t y = *reinterpret_cast<const f4_t*>(red + (q * kTokens + t) * kStride + h * kOut + piece + k);
+                    const f4_t y = *reinterpret_cast<const f4_t*>(from + token * kStride + h * RT * 16 + piece + k);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         v[h][k + e] += y[e];
                 }
+            };
+#pragma unroll
+            for (int q = 0; q < kProductWaves; ++q)
+                add(red + q * kTokens * kStride);
+            if (ADAPTERS && m[h].up && id >= 0 && id < m[h].n_adapters)
+                add(extra);
+        }
         u32x4 o;
-        if (GATED) {
+        if constexpr (GATED) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 v[0][k] = v[0][k] / (1.0f + expf(-v[0][k])) * v[1][k];
-        } else if (m0.residual) {
-            const u32x4 y = *reinterpret_cast<const u32x4*>(m0.residual + static_cast<size_t>(t0 + t) * m0.residual_stride + n);
+        } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                v[0][k] += half_bits_to_float(static_cast<uint16_t>(y[k >> 1] >> (16 * (k & 1))));
+                v[0][k] += half_bits_to_float(static_cast<uint16_t>(residual[k >> 1] >> (16 * (k & 1))));
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             o[k] = static_cast<uint32_t>(float_to_half_bits(v[0][2 * k])) | static_cast<uint32_t>(float_to_half_bits(v[0][2 * k + 1])) << 16;
-        *reinterpret_cast<u32x4*>(m0.out + static_cast<size_t>(t0 + t) * m0.out_stride + n) = o;
+        *reinterpret_cast<u32x4*>(out + static_cast<size_t>(t0 + token) * out_stride + n) = o;
     }
 }
 
-template <int R, int T, bool GATED>
-static void launch_product(ProductArgs& a)
+// ---------------------------------------------------------------- host side
+struct Product { // a call of either entry point
+    ProductArgs a;
+    LowArgs low;
+    int n_matrices;
+    bool adapters;
+};
+
+template <int R, int T, int D, bool GATED>
+static void launch_product(Product& p)
 {
     constexpr int kRows = GATED ? R * 8 : R * 16;
+    ProductArgs& a = p.a;
     a.row_blocks = 0;
-    for (int i = 0; i < (GATED ? 1 : a.n_matrices); ++i) {
-        a.m[i].first = a.row_blocks;
-        a.row_blocks += ceil_div(a.m[i].cols, kRows);
+    for (int i = 0; i < LLAMA2_MAX_BATCH_MATRICES; ++i) {
+        a.first[i] = i < (GATED ? 1 : p.n_matrices) ? a.row_blocks : 0x7FFFFFFF;
+        if (i < (GATED ? 1 : p.n_matrices))
+            a.row_blocks += ceil_div(a.t[i].cols, kRows);
     }
     a.token_blocks = ceil_div(a.n_tokens, T * 16);
-    const dim3 grid(static_cast<unsigned>(ceil_div(a.row_blocks, 8)) * 8 * a.token_blocks);
-    hipLaunchKernelGGL((batch_product_kernel<R, T, GATED>), grid, dim3(kProductWaves * 64), 0, ctx().stream, a);
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.row_blocks, 8)) * 8 * a.token_blocks), block(kProductWaves * 64);
+    if (p.adapters)
+        hipLaunchKernelGGL((batch_product_kernel<R, T, D, GATED, true>), grid, block, 0, ctx().stream, a);
+    else
+        hipLaunchKernelGGL((batch_product_kernel<R, T, D, GATED, false>), grid, block, 0, ctx().stream, a);
 }
 
 template <bool GATED>
-static int run_product(const char* fn, ProductArgs& a)
+static int run_product(const char* fn, Product& p)
 {
+    ProductArgs& a = p.a;
+    LowArgs& l = p.low;
     size_t bytes = 0;
-    int most = 0;
-    for (int i = 0; i < a.n_matrices; ++i)
-        if (a.m[i].down) {
-            bytes += static_cast<size_t>(a.n_tokens) * (a.m[i].max_rank * 4 + 4);
-            most = a.m[i].n_adapters > most ? a.m[i].n_adapters : most;
+    for (int i = 0; i < p.n_matrices; ++i)
+        if (l.t[i].down) {
+            bytes += static_cast<size_t>(a.n_tokens) * ceil_div(l.t[i].max_rank, 16) * (64 + sizeof(TokenAdapter));
+            a.most_adapters = l.t[i].n_adapters > a.most_adapters ? l.t[i].n_adapters : a.most_adapters;
         }
-    if (bytes) {
+    p.adapters = bytes > 0;
+    if (p.adapters) {
         if (int rc = ensure_attn_partials(bytes))
             return rc;
-        char* p = reinterpret_cast<char*>(ctx().attn_partials);
-        for (int i = 0; i < a.n_matrices; ++i)
-            if (a.m[i].down) {
-                a.m[i].low = reinterpret_cast<uint16_t*>(p);
-                p += static_cast<size_t>(a.n_tokens) * a.m[i].max_rank * 4;
-            }
-        for (int i = 0; i < a.n_matrices; ++i)
-            if (a.m[i].down) {
-                a.m[i].factors = reinterpret_cast<float*>(p);
-                p += static_cast<size_t>(a.n_tokens) * 4;
-            }
-        hipLaunchKernelGGL(batch_low_kernel, dim3(ceil_div(a.n_tokens, 16), most < 16 ? most : 16, a.n_matrices), dim3(kLowWaves * 64), 0,
-                           ctx().stream, a);
+        char* at = reinterpret_cast<char*>(ctx().attn_partials);
+        for (int i = 0; i < p.n_matrices; ++i) {
+            LowTensor& t = l.t[i];
+            if (!t.down)
+                continue;
+            t.low = reinterpret_cast<uint16_t*>(at);
+            at += static_cast<size_t>(a.n_tokens) * ceil_div(t.max_rank, 16) * 64;
+        }
+        for (int i = 0; i < p.n_matrices; ++i) {
+            LowTensor& t = l.t[i];
+            if (!t.down)
+                continue;
+            t.info = reinterpret_cast<TokenAdapter*>(at);
+            at += static_cast<size_t>(a.n_tokens) * ceil_div(t.max_rank, 16) * sizeof(TokenAdapter);
+            a.t[i].low = t.low;
+            a.t[i].info = t.info;
+            a.t[i].n_adapters = t.n_adapters;
+            a.t[i].max_rank = t.max_rank;
+        }
+        l.x = a.x;
+        l.positions = a.positions;
+        l.token_adapters = a.token_adapters;
+        l.K = a.K;
+        l.x_stride = a.x_stride;
+        l.n_tokens = a.n_tokens;
+        l.most_adapters = a.most_adapters;
+        // items of a block of 64 tokens: one for each adapter in use, and one more for every 16 tokens
+        const int tokens = a.n_tokens < 64 ? a.n_tokens : 64, items = a.most_adapters + 3 < tokens ? a.most_adapters + 3 : tokens;
+        hipLaunchKernelGGL(batch_low_kernel, dim3(ceil_div(a.n_tokens, 64), items, p.n_matrices * kRankBlocks), dim3(kLowWaves * 64), 0, ctx().stream, l);
         L2_LAUNCH_CHECK(fn);
     }
     if (a.n_tokens <= 16)
-        launch_product<2, 1, GATED>(a);
+        launch_product<2, 1, 4, GATED>(p);
     else if (a.n_tokens <= 32)
-        launch_product<2, 2, GATED>(a);
+        launch_product<2, 2, 2, GATED>(p);
     else
-        launch_product<2, 4, GATED>(a);
+        launch_product<4, 4, 1, GATED>(p);
     L2_LAUNCH_CHECK(fn);
     return LLAMA2_OK;
 }
 
-static ProductArgs product_args(const llama2_half* input, int rows, int input_stride, const int* token_adapters, const llama2_batch& batch)
+static Product product_of(const llama2_half* input, int rows, int input_stride, const int* token_adapters, const llama2_batch& batch)
 {
-    ProductArgs a = {};
-    a.x = input;
-    a.positions = batch.positions;
-    a.token_adapters = token_adapters;
-    a.K = rows;
-    a.groups = weight_groups(rows);
-    a.ws = weight_words(rows);
-    a.ss = a.groups;
-    a.zs = zero_words(rows);
-    a.x_stride = input_stride;
-    a.n_tokens = batch.n_tokens;
-    return a;
+    Product p = {};
+    p.a.x = input;
+    p.a.positions = batch.positions;
+    p.a.token_adapters = token_adapters;
+    p.a.K = rows;
+    p.a.x_stride = input_stride;
+    p.a.n_tokens = batch.n_tokens;
+    return p;
 }
 
-static void put_tensor(ProductTensor& m, const llama2_qweight& w, const llama2_adapters* a, int rows, int cols)
+static void put_tensor(Product& p, int i, const llama2_qweight& w, const llama2_adapters* a, int cols)
 {
-    m.w = w.weight;
-    m.z = w.zeros;
-    m.s = w.scales;
-    m.cols = cols;
-    if (a) {
-        m.down = a->down;
-        m.up = a->up;
-        m.scales = a->scales;
-        m.ranks = a->ranks;
-        m.down_stride = down_halfs(*a, rows);
-        m.up_stride = up_halfs(*a, cols);
-        m.n_adapters = a->n_adapters;
-        m.max_rank = a->max_rank;
-    }
+    ProductTensor& t = p.a.t[i];
+    t.w = w.weight;
+    t.z = w.zeros;
+    t.s = w.scales;
+    t.cols = cols;
+    if (!a)
+        return;
+    t.up = a->up;
+    t.up_stride = up_halfs(*a, cols);
+    LowTensor& l = p.low.t[i];
+    l.down = a->down;
+    l.scales = a->scales;
+    l.ranks = a->ranks;
+    l.down_stride = down_halfs(*a, p.a.K);
+    l.n_adapters = a->n_adapters;
+    l.max_rank = a->max_rank;
 }
 
 } // namespace l2
@@ -485,17 +720,17 @@ int llama2_batch_mat_mul_int4(const llama2_batch_matrix* matrices, int n_matrice
     L2_REQUIRE_INIT();
     if (int rc = check_batch_mat_mul(matrices, n_matrices, input, rows, input_stride, token_adapters, batch))
         return rc;
-    ProductArgs a = product_args(input, rows, input_stride, token_adapters, *batch);
-    a.n_matrices = n_matrices;
+    Product p = product_of(input, rows, input_stride, token_adapters, *batch);
+    p.n_matrices = n_matrices;
     for (int i = 0; i < n_matrices; ++i) {
         const llama2_batch_matrix& m = matrices[i];
-        put_tensor(a.m[i], m.weight, m.adapters, rows, m.cols);
-        a.m[i].out = m.output;
-        a.m[i].residual = m.residual;
-        a.m[i].out_stride = m.output_stride;
-        a.m[i].residual_stride = m.residual_stride;
+        put_tensor(p, i, m.weight, m.adapters, m.cols);
+        p.a.t[i].out = m.output;
+        p.a.t[i].residual = m.residual;
+        p.a.t[i].out_stride = m.output_stride;
+        p.a.t[i].residual_stride = m.residual_stride;
     }
-    return run_product<false>("llama2_batch_mat_mul_int4", a);
+    return run_product<false>("llama2_batch_mat_mul_int4", p);
 }
 
 int llama2_batch_mat_mul_swiglu(llama2_half* output, const llama2_half* input, const llama2_qweight* gate, const llama2_qweight* up, int rows,
@@ -506,13 +741,13 @@ int llama2_batch_mat_mul_swiglu(llama2_half* output, const llama2_half* input, c
     if (int rc = check_batch_swiglu(output, input, gate, up, rows, cols, output_stride, input_stride, gate_adapters, up_adapters,
                                     token_adapters, batch))
         return rc;
-    ProductArgs a = product_args(input, rows, input_stride, token_adapters, *batch);
-    a.n_matrices = 2;
-    put_tensor(a.m[0], *gate, gate_adapters, rows, cols);
-    put_tensor(a.m[1], *up, up_adapters, rows, cols);
-    a.m[0].out = output;
-    a.m[0].out_stride = output_stride;
-    return run_product<true>("llama2_batch_mat_mul_swiglu", a);
+    Product p = product_of(input, rows, input_stride, token_adapters, *batch);
+    p.n_matrices = 2;
+    put_tensor(p, 0, *gate, gate_adapters, cols);
+    put_tensor(p, 1, *up, up_adapters, cols);
+    p.a.t[0].out = output;
+    p.a.t[0].out_stride = output_stride;
+    return run_product<true>("llama2_batch_mat_mul_swiglu", p);
 }
 
 } // extern "C"

@@ -7,8 +7,9 @@
 
 namespace l2 {
 
-constexpr int kMaxProductRows = 1 << 17; // inputs of a tensor
+constexpr int kMaxProductRows = 1 << 16; // inputs of a tensor
 constexpr int kMaxProductCols = 1 << 20; // outputs of a tensor
+constexpr int kMaxStride = 1 << 24; // of the input: offsets within 64 rows are ints
 constexpr int kMaxAdapters = 1 << 20;
 constexpr int kMaxRank = 128;
 constexpr int kMaxNormSize = 1 << 16;
@@ -73,6 +74,8 @@ inline int check_product_input(const char* fn, const llama2_half* input, int row
         return fail(LLAMA2_ERR_UNSUPPORTED, "%s: rows=%d exceeds %d", fn, rows, kMaxProductRows);
     L2_CHECK(input_stride >= rows && input_stride % 8 == 0, "%s: input_stride=%d must be a multiple of 8 and hold a row of %d", fn,
              input_stride, rows);
+    if (input_stride > kMaxStride)
+        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: input_stride=%d exceeds %d", fn, input_stride, kMaxStride);
     return LLAMA2_OK;
 }
 

@@ -115,7 +115,7 @@ def test_products_that_are_allowed(lib):
 @pytest.mark.parametrize("bad,code", [
     (dict(m=[], n=0), INVALID), (dict(n=5), INVALID), (dict(n=-1), INVALID), (dict(x=None), INVALID), (dict(x=7 * MIB + 8), INVALID),
     (dict(rows=0), INVALID), (dict(rows=12), INVALID), (dict(rows=-8), INVALID), (dict(rows=1 << 18, stride=1 << 18), UNSUPPORTED),
-    (dict(stride=1016), INVALID), (dict(stride=1028), INVALID), (dict(ids=8 * MIB + 2), INVALID),
+    (dict(stride=1016), INVALID), (dict(stride=(1 << 24) + 8), UNSUPPORTED), (dict(stride=1028), INVALID), (dict(ids=8 * MIB + 2), INVALID),
     (dict(m=[matrix(output=None)]), INVALID), (dict(m=[matrix(output=130 * MIB + 2)]), INVALID), (dict(m=[matrix(residual=140 * MIB + 4)]), INVALID),
     (dict(m=[matrix(cols=0)]), INVALID), (dict(m=[matrix(cols=12)]), INVALID), (dict(m=[matrix(cols=1 << 21, output_stride=1 << 21)]), UNSUPPORTED),
     (dict(m=[matrix(output_stride=504)]), INVALID), (dict(m=[matrix(output_stride=516)]), INVALID),
