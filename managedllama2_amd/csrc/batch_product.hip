@@ -5,23 +5,13 @@
 //
 // w - z is an exact fp16 integer, its products with x are summed in fp32 over a group of 128 and scaled in fp32.  h is summed in
 // fp32 and leaves as two fp16 numbers and a power of two (22 bits of the token's largest), which the matrix cores take as 16 ranks a product.
-#include "common.hpp"
-#include "batch_product_plan.hpp"
+#include "batch_adapters.hpp"
+#include "prefill.hpp"
 
 #include <cmath>
+#include <type_traits>
 
 namespace l2 {
-
-typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
-typedef float f4_t __attribute__((ext_vector_type(4)));
-
-// What a tensor's adapters leave for its product, per token and 16 ranks (a block): the scale of the adapter with the block's power of
-// two, and the adapter's rank.
-struct TokenAdapter {
-    float factor;
-    int rank;
-};
-constexpr int kRankBlocks = kMaxRank / 16;
 
 // Arguments lie in memory, and a kernel that asks for them one after the other waits for each: a tensor's are neighbours, chosen by
 // an index that the first cache line holds.
@@ -42,109 +32,6 @@ struct alignas(64) LowArgs {
     int K, x_stride, n_tokens, most_adapters;
     LowTensor t[LLAMA2_MAX_BATCH_MATRICES];
 };
-
-struct alignas(64) ProductTensor {
-    const uint32_t* w;
-    const uint32_t* z;
-    const uint16_t* s;
-    uint16_t* out;
-    const uint16_t* residual;
-    const uint16_t* up; // null: no adapters
-    const uint16_t* low;
-    const TokenAdapter* info;
-    long long up_stride;
-    int cols, out_stride, residual_stride, n_adapters, max_rank;
-};
-
-struct alignas(64) ProductArgs {
-    const uint16_t* x;
-    const int* positions;
-    const int* token_adapters;
-    int K, x_stride, n_tokens, most_adapters; // of any tensor
-    int row_blocks, token_blocks;
-    int first[LLAMA2_MAX_BATCH_MATRICES]; // first block of rows of a tensor
-    ProductTensor t[LLAMA2_MAX_BATCH_MATRICES];
-};
-
-// The arguments as they lie in memory: a tensor chosen by an index is then a few scalar loads (chosen among registers it is a hundred
-// instructions).
-template <class A>
-using Constant = __attribute__((address_space(4))) const A;
-
-template <class A>
-__device__ __forceinline__ Constant<A>& kernel_args()
-{
-    return *(Constant<A>*)__builtin_amdgcn_kernarg_segment_ptr();
-}
-
-template <class V>
-__device__ __forceinline__ void needed(const V& v)
-{
-    asm volatile("" : : "s"(v));
-}
-
-template <class... V>
-__device__ __forceinline__ void loaded(const V&... v) // here, together
-{
-    (needed(v), ...);
-}
-
-constexpr int kNoAdapter = -1, kNoToken = -2;
-
-// Adapter of token t: one that some tensor has, kNoAdapter, or kNoToken where there is no token.
-__device__ __forceinline__ int adapter_of(const int* positions, const int* token_adapters, int t, int n_tokens, int most_adapters)
-{
-    t = min(t, n_tokens);
-    int position = -1, id = kNoAdapter;
-    if (t < n_tokens) {
-        position = positions[t];
-        if (token_adapters)
-            id = token_adapters[t];
-    }
-    return position < 0 ? kNoToken : id < 0 || id >= most_adapters ? kNoAdapter : id;
-}
-
-// Tokens of a block of up to 64 that use the same adapter, by up to 16 of them: an item.  Items are numbered in the order of their
-// first tokens.
-struct Items {
-    int ids[64];            // adapter of a token, kNoAdapter, kNoToken
-    int adapter[64];        // of an item
-    uint8_t tokens[64][16]; // of an item, kNobody behind the last
-    int count;
-};
-constexpr uint8_t kNobody = 255;
-
-// By one wavefront, from the first `tokens` of items.ids; everyone may read the items after the next barrier.
-__device__ __forceinline__ void find_items(Items& items, int tokens)
-{
-    const int lane = threadIdx.x & 63, id = lane < tokens ? items.ids[lane] : kNoToken;
-    int before = 0, lead = -1; // tokens with this adapter in front of this one, and the first of its sixteen
-    for (int j = 0; j < tokens; ++j) {
-        const bool same = __builtin_amdgcn_readlane(id, j) == id && j <= lane;
-        lead = same && (before & 15) == 0 ? j : lead;
-        before += same;
-    }
-    const unsigned long long leads = __ballot(id >= 0 && lead == lane);
-    reinterpret_cast<u32x4*>(items.tokens)[lane] = u32x4{~0u, ~0u, ~0u, ~0u};
-    if (id >= 0) {
-        const int item = __builtin_popcountll(leads & ((1ULL << lead) - 1));
-        items.tokens[item][(before - 1) & 15] = static_cast<uint8_t>(lane);
-        if (lead == lane)
-            items.adapter[item] = id;
-    }
-    if (lane == 0)
-        items.count = __builtin_popcountll(leads);
-}
-
-__device__ __forceinline__ f4_t mfma16(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-
-// A buffer whose reads beyond `bytes` return zero.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void* p, size_t bytes)
-{
-    return make_rsrc(p, bytes > 0x7FFFFFFFu ? 0x7FFFFFFFu : static_cast<uint32_t>(bytes));
-}
-
-constexpr int kBehind = static_cast<int>(0x80000000u); // an offset behind the end of every buffer: reads zero, moves nothing
 
 // 16 rows of 128 halfs, requested in the order of memory (a compute unit looks up 64 bytes at a time, and only neighbouring lanes share a
 // lookup: lanes that read 16 bytes of a row each, as the matrix cores want them, cost four times as many) and turned around through
@@ -354,20 +241,15 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
         return;
     const int which = GATED ? 0 : (rb >= first1) + (rb >= first2) + (rb >= first3);
     const int ws = (K + 31) / 32 * 4, groups = (K + 127) / 128, zs = (groups + 7) / 8;
-    struct Tensor {
+    struct Tensor : AdapterPart {
         const uint32_t* w;
         const uint32_t* z;
         const uint16_t* s;
-        const uint16_t* up;
-        const uint16_t* low;
-        const TokenAdapter* info;
-        long long up_stride;
-        int n_adapters, max_rank;
     } m[kTensors];
 #pragma unroll
     for (int h = 0; h < kTensors; ++h) {
         auto& t = a.t[which + h];
-        m[h] = {t.w, t.z, t.s, t.up, t.low, t.info, t.up_stride, t.n_adapters, t.max_rank};
+        m[h] = {adapter_part(t), t.w, t.z, t.s};
     }
     auto& t = a.t[which];
     const int cols = t.cols, out_stride = t.out_stride, residual_stride = t.residual_stride;
@@ -440,60 +322,10 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
         // The adapters' part of each item, straight to where the sums of the wavefronts meet: a token has one adapter.
         for (int i = wave; i < items.count * kTensors; i += kProductWaves) {
             const int item = i / kTensors, h = i % kTensors;
-            auto& m0 = m[0];
-            auto& m1 = m[kTensors - 1];
-            const uint16_t *up = h ? m1.up : m0.up, *low = h ? m1.low : m0.low;
-            const int max_rank = h ? m1.max_rank : m0.max_rank, id = __builtin_amdgcn_readfirstlane(items.adapter[item]);
-            if (!up || id >= (h ? m1.n_adapters : m0.n_adapters))
-                continue;
-            // tokens of the places that this lane's row of inputs, and its four rows of results, stand for
-            const int own = items.tokens[item][l15], lead = items.tokens[item][0];
-            const size_t blocks = (max_rank + 15) / 16, mine = (t0 + (own == kNobody ? lead : own)) * blocks;
-            const TokenAdapter* const info = h ? m1.info : m0.info;
-            const __amdgpu_buffer_rsrc_t ru = rows_buffer(up + id * (h ? m1.up_stride : m0.up_stride) + static_cast<size_t>(n0) * max_rank,
-                                                          static_cast<size_t>(rows) * max_rank * 2);
-            int of[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                of[e] = items.tokens[item][4 * c + e];
-            const int rank = __builtin_amdgcn_readfirstlane(info[(t0 + lead) * blocks].rank);
-            f4_t sum[RT] = {};
-            for (int b = 0; b * 16 < rank; ++b) {
-                // lane groups 0 and 1: the upper parts of ranks 0 .. 7 and 8 .. 15 of the block; 2 and 3: the lower ones
-                const int have = rank - b * 16 - (c & 1) * 8;
-                const u32x4 hf = *reinterpret_cast<const u32x4*>(low + (mine + b) * 32 + c * 8);
-                float f[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    f[e] = info[(t0 + (of[e] == kNobody ? lead : of[e])) * blocks + b].factor;
-                u32x4 u[(RT + 1) / 2];
-#pragma unroll
-                for (int r = 0; r < (RT + 1) / 2; ++r) { // 32 rows of 16 ranks, a row by two lanes
-                    const int row = r * 32 + (lane >> 1), r8 = b * 16 + (lane & 1) * 8;
-                    u[r] = __builtin_amdgcn_raw_buffer_load_b128(ru, r8 < rank && row < RT * 16 ? (row * max_rank + r8) * 2 : kBehind, 0, 0);
-                }
-#pragma unroll
-                for (int r = 0; r < (RT + 1) / 2; ++r)
-                    *reinterpret_cast<u32x4*>(lds + r * 1024 + lane * 16) = u[r];
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    u32x4 v = *reinterpret_cast<const u32x4*>(lds + (r * 16 + l15) * 32 + (c & 1) * 16);
-                    if (rank & 7)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            v[k] &= have >= 2 * k + 2 ? ~0u : have == 2 * k + 1 ? 0xFFFFu : 0u;
-                    const f4_t p = mfma16(__builtin_bit_cast(h8_t, hf), __builtin_bit_cast(h8_t, v), f4_t{});
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        sum[r][e] = __builtin_fmaf(p[e], f[e], sum[r][e]);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (of[e] != kNobody)
-#pragma unroll
-                    for (int r = 0; r < RT; ++r)
-                        extra[of[e] * kStride + (h * RT + r) * 16 + l15] = sum[r][e];
+            auto& m1 = m[h ? kTensors - 1 : 0];
+            add_item<RT>(items, item, m1, t0, n0, rows, lds, [&](int token, int r, float v) {
+                extra[token * kStride + (h * RT + r) * 16 + l15] = v;
+            });
         }
     }
 
@@ -620,59 +452,88 @@ static void launch_product(Product& p)
         hipLaunchKernelGGL((batch_product_kernel<R, T, D, GATED, false>), grid, block, 0, ctx().stream, a);
 }
 
+// Rows of more than 32768 inputs: tiles so low that their scales fit.
+static void launch_tall(Product& p, std::false_type) { launch_product<1, 1, 4, false>(p); }
+static void launch_tall(Product& p, std::true_type) { launch_product<2, 1, 4, true>(p); }
+
+constexpr int kWideTokens = 64; // more go through the kernels of the prompt's products
+constexpr int kMostTokens = 4096; // of a launch
+
 template <bool GATED>
 static int run_product(const char* fn, Product& p)
 {
     ProductArgs& a = p.a;
     LowArgs& l = p.low;
-    size_t bytes = 0;
+    const int all = a.n_tokens, most = all < kMostTokens ? all : kMostTokens, groups = weight_groups(a.K);
+    bool fits = true; // the prompt's products hold a tensor's offsets in 31 bits
+    for (int i = 0; i < p.n_matrices; ++i)
+        fits = fits && static_cast<long long>(a.t[i].cols) * weight_words(a.K) * 4 <= 0x7FFFFFFFLL;
+    const bool wide = all > kWideTokens && fits;
+    const size_t fragments = wide ? batch_gemm_bytes(most, a.K) : 0;
+    size_t bytes = fragments;
     for (int i = 0; i < p.n_matrices; ++i)
         if (l.t[i].down) {
-            bytes += static_cast<size_t>(a.n_tokens) * ceil_div(l.t[i].max_rank, 16) * (64 + sizeof(TokenAdapter));
+            p.adapters = true;
+            bytes += static_cast<size_t>(most) * ceil_div(l.t[i].max_rank, 16) * (64 + sizeof(TokenAdapter));
             a.most_adapters = l.t[i].n_adapters > a.most_adapters ? l.t[i].n_adapters : a.most_adapters;
         }
-    p.adapters = bytes > 0;
-    if (p.adapters) {
+    if (bytes)
         if (int rc = ensure_attn_partials(bytes))
             return rc;
-        char* at = reinterpret_cast<char*>(ctx().attn_partials);
-        for (int i = 0; i < p.n_matrices; ++i) {
-            LowTensor& t = l.t[i];
-            if (!t.down)
-                continue;
-            t.low = reinterpret_cast<uint16_t*>(at);
-            at += static_cast<size_t>(a.n_tokens) * ceil_div(t.max_rank, 16) * 64;
-        }
-        for (int i = 0; i < p.n_matrices; ++i) {
-            LowTensor& t = l.t[i];
-            if (!t.down)
-                continue;
-            t.info = reinterpret_cast<TokenAdapter*>(at);
-            at += static_cast<size_t>(a.n_tokens) * ceil_div(t.max_rank, 16) * sizeof(TokenAdapter);
-            a.t[i].low = t.low;
-            a.t[i].info = t.info;
-            a.t[i].n_adapters = t.n_adapters;
-            a.t[i].max_rank = t.max_rank;
-        }
-        l.x = a.x;
-        l.positions = a.positions;
-        l.token_adapters = a.token_adapters;
-        l.K = a.K;
-        l.x_stride = a.x_stride;
-        l.n_tokens = a.n_tokens;
-        l.most_adapters = a.most_adapters;
-        // items of a block of 64 tokens: one for each adapter in use, and one more for every 16 tokens
-        const int tokens = a.n_tokens < 64 ? a.n_tokens : 64, items = a.most_adapters + 3 < tokens ? a.most_adapters + 3 : tokens;
-        hipLaunchKernelGGL(batch_low_kernel, dim3(ceil_div(a.n_tokens, 64), items, p.n_matrices * kRankBlocks), dim3(kLowWaves * 64), 0, ctx().stream, l);
-        L2_LAUNCH_CHECK(fn);
+    char* const base = reinterpret_cast<char*>(ctx().attn_partials);
+    char* at = base + fragments;
+    for (int i = 0; i < p.n_matrices; ++i) {
+        LowTensor& t = l.t[i];
+        if (!t.down)
+            continue;
+        t.low = reinterpret_cast<uint16_t*>(at);
+        at += static_cast<size_t>(most) * ceil_div(t.max_rank, 16) * 64;
+        t.info = reinterpret_cast<TokenAdapter*>(at);
+        at += static_cast<size_t>(most) * ceil_div(t.max_rank, 16) * sizeof(TokenAdapter);
+        a.t[i].low = t.low;
+        a.t[i].info = t.info;
+        a.t[i].n_adapters = t.n_adapters;
+        a.t[i].max_rank = t.max_rank;
     }
-    if (a.n_tokens <= 16)
-        launch_product<2, 1, 4, GATED>(p);
-    else if (a.n_tokens <= 32)
-        launch_product<2, 2, 2, GATED>(p);
-    else
-        launch_product<4, 4, 1, GATED>(p);
-    L2_LAUNCH_CHECK(fn);
+    for (int done = 0; done < all; done += kMostTokens) {
+        a.n_tokens = all - done < kMostTokens ? all - done : kMostTokens;
+        if (p.adapters) {
+            l.x = a.x;
+            l.positions = a.positions;
+            l.token_adapters = a.token_adapters;
+            l.K = a.K;
+            l.x_stride = a.x_stride;
+            l.n_tokens = a.n_tokens;
+            l.most_adapters = a.most_adapters;
+            // items of a block of 64 tokens: one for each adapter in use, and one more for every 16 tokens
+            const int tokens = a.n_tokens < 64 ? a.n_tokens : 64, items = a.most_adapters + 3 < tokens ? a.most_adapters + 3 : tokens;
+            hipLaunchKernelGGL(batch_low_kernel, dim3(ceil_div(a.n_tokens, 64), items, p.n_matrices * kRankBlocks), dim3(kLowWaves * 64), 0,
+                               ctx().stream, l);
+            L2_LAUNCH_CHECK(fn);
+        }
+        if (wide) {
+            if (int rc = launch_batch_gemm(fn, a, p.n_matrices, GATED, p.adapters, base))
+                return rc;
+        } else {
+            // scales and zero points of a workgroup's rows: R * groups <= 512
+            if (a.n_tokens <= 16)
+                groups <= 256 ? launch_product<2, 1, 4, GATED>(p) : launch_tall(p, std::integral_constant<bool, GATED>());
+            else if (a.n_tokens <= 32)
+                groups <= 256 ? launch_product<2, 2, 2, GATED>(p) : launch_tall(p, std::integral_constant<bool, GATED>());
+            else
+                groups <= 128 ? launch_product<4, 4, 1, GATED>(p) : launch_tall(p, std::integral_constant<bool, GATED>());
+            L2_LAUNCH_CHECK(fn);
+        }
+        a.x += static_cast<size_t>(a.n_tokens) * a.x_stride;
+        a.positions += a.n_tokens;
+        if (a.token_adapters)
+            a.token_adapters += a.n_tokens;
+        for (int i = 0; i < (GATED ? 1 : p.n_matrices); ++i) {
+            a.t[i].out += static_cast<size_t>(a.n_tokens) * a.t[i].out_stride;
+            if (a.t[i].residual)
+                a.t[i].residual += static_cast<size_t>(a.n_tokens) * a.t[i].residual_stride;
+        }
+    }
     return LLAMA2_OK;
 }
 

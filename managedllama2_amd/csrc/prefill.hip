@@ -17,6 +17,7 @@
 #include "int4_kernels.hpp"
 #include "gemm_shape.hpp"
 #include "prefill.hpp"
+#include "batch_adapters.hpp"
 
 #include <cmath>
 #include <cstdlib>
@@ -25,7 +26,6 @@
 
 namespace l2 {
 
-typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f16v_t __attribute__((ext_vector_type(16)));
 
 constexpr int kGroup = 128;       // quantisation group along K
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256) void prefill_norm_kernel(NormArgs a)
 }
 
 // ---------------------------------------------------------------- int4 matrix product
-enum PrefillEpi { EPI_QKV, EPI_PARTIAL, EPI_SWIGLU };
+enum PrefillEpi { EPI_QKV, EPI_PARTIAL, EPI_SWIGLU, EPI_ROWS, EPI_GATED }; // the last two: products of many tokens for their own sake
 
 struct GemmArgs {
     QW m[3];
@@ -163,6 +163,17 @@ struct GemmArgs {
     int part_rows;
     int out_groups; // SWIGLU: groups of hf
     const float* rope;
+};
+
+// EPI_ROWS, EPI_GATED: several tensors, or gate and up, with adapters; results to plain rows.
+struct BatchGemmArgs {
+    GemmArgs g;
+    const int* positions;
+    const int* token_adapters;
+    int most_adapters;
+    int first[LLAMA2_MAX_BATCH_MATRICES]; // first pair of a tensor
+    bool adapters;
+    ProductTensor t[LLAMA2_MAX_BATCH_MATRICES];
 };
 
 // Pair k of the 8 nibbles of a word as fp16 n - z, exact: n sits in the mantissa of 1024 + n (bits 0-3 of a half) or
@@ -243,13 +254,17 @@ struct GemmLds {
     static constexpr int kWAt = 3 * kXStage, kZAt = kWAt + 3 * kWStage, kAll = kZAt + 3 * kZStage;
     static constexpr int kRedRow = kTile + 4, kRed = 8 * MT * kTile * kRedRow * 4;
     static constexpr int kBytes = kAll > kRed ? kAll : kRed;
+    static constexpr int kTurnAt = kRed + MT * static_cast<int>(sizeof(Items)), kItems = kTurnAt + 8 * 1024; // EPI_ROWS, EPI_GATED
+    static constexpr int kRowsBytes = kAll > kItems ? kAll : kItems;
+    static_assert(kRowsBytes <= 160 * 1024, "LDS of a compute unit");
     static_assert(kBytes <= 160 * 1024, "LDS of a compute unit");
 };
 
 // Block `unit` of weights (and piece of K) with block `mb` of MT token tiles.
 template <int MT, int WN, int WK, int EPI>
-__device__ __forceinline__ void gemm_block(const GemmArgs& a, char* lds, int unit, int mb)
+__device__ __forceinline__ void gemm_block(const GemmArgs& a, char* lds, int unit, int mb, Constant<BatchGemmArgs>* rows = nullptr)
 {
+    constexpr bool ROWS = EPI == EPI_ROWS || EPI == EPI_GATED;
     static_assert(WN * WK == 4, "8 wavefronts");
     using Lds = GemmLds<MT, WN, WK>;
     constexpr int kXStage = Lds::kXStage, kWRow = Lds::kWRow, kWStage = Lds::kWStage, kZStage = Lds::kZStage;
@@ -265,9 +280,13 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& a, char* lds, int uni
             const int per = a.N >> 6, r = pair % per;
             tensor = pair / per;
             row = (r >> 1) * kRopeHeadSize + (r & 1) * kTile + tile * 64;
-        } else if (EPI == EPI_SWIGLU) {
+        } else if (EPI == EPI_SWIGLU || EPI == EPI_GATED) {
             tensor = tile;
             row = pair * kTile;
+        } else if (EPI == EPI_ROWS) {
+            const int f1 = rows->first[1], f2 = rows->first[2], f3 = rows->first[3];
+            tensor = (pair >= f1) + (pair >= f2) + (pair >= f3);
+            row = ((pair - (tensor == 0 ? 0 : tensor == 1 ? f1 : tensor == 2 ? f2 : f3)) * 2 + tile) * kTile;
         } else {
             tensor = 0;
             row = (pair * 2 + tile) * kTile;
@@ -276,8 +295,15 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& a, char* lds, int uni
     // by value: a choice among the arguments themselves puts them into scratch memory
     auto choose = [](int i, auto first, auto second, auto third) { return i == 0 ? first : (i == 1 ? second : third); };
     auto tensor_of = [&](int i) {
+        if constexpr (ROWS)
+            return QW{rows->t[i].w, rows->t[i].z, rows->t[i].s};
         return QW{choose(i, a.m[0].w, a.m[1].w, a.m[2].w), choose(i, a.m[0].z, a.m[1].z, a.m[2].z),
                   choose(i, a.m[0].s, a.m[1].s, a.m[2].s)};
+    };
+    auto rows_of = [&](int i) {
+        if constexpr (ROWS)
+            return static_cast<int>(rows->t[i].cols);
+        return a.N;
     };
     auto rsrc_of = [](const void* p, uint32_t bytes) {
         const unsigned long long v = reinterpret_cast<unsigned long long>(p);
@@ -323,18 +349,19 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& a, char* lds, int uni
     int wt, wrow;
     tile_of(nb * WN + wr0 / 64, (wr0 / kTile) & 1, wt, wrow);
     wrow += wr0 & (kTile - 1);
-    const u32x4 rw = rsrc_of(tensor_of(wt).w, static_cast<uint32_t>(a.N) * a.ws * 4);
+    const int wN = rows_of(wt);
+    const u32x4 rw = rsrc_of(tensor_of(wt).w, static_cast<uint32_t>(wN) * a.ws * 4);
     int wvoff[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int r = i * RPI + lane / LPR, row = wrow + r < a.N ? wrow + r : a.N - 1;
+        const int r = i * RPI + lane / LPR, row = wrow + r < wN ? wrow + r : wN - 1;
         wvoff[i] = row * a.ws * 4 + ((lane % LPR) ^ swizzle(wr0 + r)) * 16;
     }
     // Scales and zero points of this wavefront's tile and group, by the two halves of the lanes.  Scales need not be
     // aligned to more than their 2 bytes: the word that holds one is fetched.
     int tensor, r0;
     tile_of(nb * WN + wn, t, tensor, r0);
-    const int row = r0 + l31 < a.N ? r0 + l31 : a.N - 1;
+    const int sN = rows_of(tensor), row = r0 + l31 < sN ? r0 + l31 : sN - 1;
     const QW q = tensor_of(tensor);
     const int s_odd = static_cast<int>(reinterpret_cast<uintptr_t>(q.s) & 2) + row * a.ss * 2; // from the first word
     const char* zs_base = h ? reinterpret_cast<const char*>(q.z + static_cast<size_t>(row) * a.zs)
@@ -380,6 +407,15 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& a, char* lds, int uni
         const _Float16 lo = static_cast<_Float16>(1024.0f + z), hi = static_cast<_Float16>(-64.0f - z);
         zlo = h2_t{lo, lo}, zhi = h2_t{hi, hi};
     };
+    int position = -1, adapter = kNoAdapter; // ROWS: of a token of tile `wave`, looked at after the products
+    if constexpr (ROWS) {
+        const int m = (mt0 + wave) * kTile + l31;
+        if (wave < MT && m < a.M) {
+            position = rows->positions[m];
+            if (rows->token_adapters)
+                adapter = rows->token_adapters[m];
+        }
+    }
     constexpr int kLoads = MT * kXPer + 3; // of a step
     auto wait_all_but = [](auto n) {
         __builtin_amdgcn_s_waitcnt(wait_vm(decltype(n)::value));
@@ -490,12 +526,37 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& a, char* lds, int uni
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             red_at(wk, t, mt * kTile + 8 * (i >> 2) + 4 * h + (i & 3))[l31] = acc[mt][i];
-    __syncthreads();
+    Items* const items = reinterpret_cast<Items*>(lds + Lds::kRed);
+    if constexpr (ROWS) {
+        const bool adapters = rows->adapters;
+        if (wave < MT) {
+            if (lane < kTile)
+                items[wave].ids[lane] = known_adapter(position, adapter, rows->most_adapters);
+            if (adapters)
+                find_items(items[wave], kTile);
+        }
+        __syncthreads();
+        if (adapters) { // onto the first group's sums, every wavefront for the outputs of its own tile
+            const AdapterPart part = adapter_part(rows->t[tensor]);
+            float* const to = red_at(0, t, 0);
+            if (mine && r0 < sN)
+                for (int mt = wk; mt < MT; mt += WK)
+                    for (int i = 0; i < items[mt].count; ++i)
+                        add_item<2>(items[mt], i, part, (mt0 + mt) * kTile, r0, min(kTile, sN - r0), lds + Lds::kTurnAt + wave * 1024,
+                                    [&](int token, int r, float v) { to[(mt * kTile + token) * kRedRow + r * 16 + (lane & 15)] += v; });
+            __syncthreads();
+        }
+    } else {
+        __syncthreads();
+    }
 #pragma unroll
     for (int pass = 0; pass < kPasses; ++pass) {
         const int row = row_of(pass), m = mt0 * kTile + row;
         if (row >= MT * kTile || m >= a.M || !mine)
             continue;
+        if constexpr (ROWS)
+            if (items[row / kTile].ids[row % kTile] == kNoToken)
+                continue;
         float v0[8] = {}, v1[8] = {};
 #pragma unroll
         for (int w = 0; w < WK; ++w)
@@ -523,6 +584,38 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& a, char* lds, int uni
             uint16_t* o = choose(tensor0, a.out[0], a.out[1], a.out[2]) + static_cast<size_t>(m) * a.N + n8;
             *reinterpret_cast<u32x4*>(o + row_a) = oa;
             *reinterpret_cast<u32x4*>(o + row_b) = ob;
+        } else if constexpr (ROWS) {
+            auto& to = rows->t[EPI == EPI_GATED ? 0 : tensor0];
+            auto put = [&](int n, const float (&v)[8]) {
+                if (n >= sN) // a multiple of 8
+                    return;
+                u32x4 o;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    o[k] = static_cast<uint32_t>(float_to_half_bits(v[2 * k])) | static_cast<uint32_t>(float_to_half_bits(v[2 * k + 1])) << 16;
+                *reinterpret_cast<u32x4*>(to.out + static_cast<size_t>(m) * to.out_stride + n) = o;
+            };
+            if constexpr (EPI == EPI_GATED) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    v0[k] = v0[k] / (1.0f + expf(-v0[k])) * v1[k];
+                put(row_a + n8, v0);
+            } else {
+                auto add = [&](int n, float (&v)[8]) {
+                    if (n >= sN)
+                        return;
+                    const u32x4 y = *reinterpret_cast<const u32x4*>(to.residual + static_cast<size_t>(m) * to.residual_stride + n);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        v[k] += half_bits_to_float(static_cast<uint16_t>(y[k >> 1] >> (16 * (k & 1))));
+                };
+                if (to.residual) {
+                    add(row_a + n8, v0);
+                    add(row_b + n8, v1);
+                }
+                put(row_a + n8, v0);
+                put(row_b + n8, v1);
+            }
         } else if (EPI == EPI_PARTIAL) {
             float* o = a.parts + (static_cast<size_t>(split) * a.part_rows + m) * a.N + n8;
 #pragma unroll
@@ -571,6 +664,43 @@ __global__ __launch_bounds__(512, 2) void prefill_gemm_kernel(GemmArgs a)
         }
     }
     gemm_block<MT, WN, WK, EPI>(a, lds, unit, mb);
+}
+
+template <int MT, int MT2, int WN, int WK, int EPI>
+__global__ __launch_bounds__(512, 2) void batch_gemm_kernel(BatchGemmArgs b)
+{
+    constexpr int kBytes = GemmLds<MT, WN, WK>::kRowsBytes, kBytes2 = GemmLds<MT2, WN, WK>::kRowsBytes;
+    __shared__ __align__(1024) char lds[kBytes > kBytes2 ? kBytes : kBytes2];
+    const GemmArgs& a = b.g;
+    Constant<BatchGemmArgs>* const rows = &kernel_args<BatchGemmArgs>();
+    int slot = blockIdx.x >> 3, mblocks = a.mblocks, row = 0; // as above
+    const bool second = MT2 != MT && slot >= a.first * a.mblocks;
+    if (second)
+        slot -= a.first * a.mblocks, mblocks = a.mblocks2, row = a.first;
+    const int unit = (row + slot / mblocks) * 8 + (blockIdx.x & 7), mb = slot % mblocks;
+    if (unit >= a.nblocks)
+        return;
+    if constexpr (MT2 != MT) {
+        if (second) {
+            gemm_block<MT2, WN, WK, EPI>(a, lds, unit, mb, rows);
+            return;
+        }
+    }
+    gemm_block<MT, WN, WK, EPI>(a, lds, unit, mb, rows);
+}
+
+// Rows of fp16 into fragment order, zeros behind the end of a row: a workgroup per token tile and group.
+__global__ __launch_bounds__(256) void batch_fragments_kernel(uint16_t* xf, const uint16_t* x, int M, int K, int x_stride, int groups)
+{
+    const int g = blockIdx.x, tile = blockIdx.y;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int m = tile * kTile + i * 16 + (threadIdx.x >> 4), k = g * kGroup + (threadIdx.x & 15) * 8;
+        u32x4 v = {};
+        if (m < M && k < K)
+            v = *reinterpret_cast<const u32x4*>(x + static_cast<size_t>(m) * x_stride + k);
+        *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(xf) + frag_offset(m, k, groups)) = frag_order(v);
+    }
 }
 
 static GemmShape gemm_shape(int tiles, int pairs, int groups, bool may_split)
@@ -623,6 +753,72 @@ int launch_gemm(const char* name, GemmArgs a, int pairs)
     }
     L2_LAUNCH_CHECK(name);
     return LLAMA2_OK;
+}
+
+template <int MT, int WN, int EPI, int MT2 = MT>
+void launch_batch_gemm_as(BatchGemmArgs& b)
+{
+    GemmArgs& a = b.g;
+    a.mblocks = ceil_div(a.M, MT * kTile);
+    a.mblocks2 = ceil_div(a.M, MT2 * kTile);
+    a.nblocks = ceil_div(a.pairs, WN);
+    const int rows = ceil_div(a.nblocks, 8);
+    if (MT2 == MT)
+        a.first = rows;
+    const dim3 grid(8 * (a.first * a.mblocks + (rows - a.first) * a.mblocks2));
+    hipLaunchKernelGGL((batch_gemm_kernel<MT, MT2, WN, 4 / WN, EPI>), grid, dim3(512), 0, ctx().stream, b);
+}
+
+template <int EPI>
+static int launch_batch_gemm_epi(const char* name, BatchGemmArgs& b)
+{
+    const GemmShape s = gemm_shape(ceil_div(b.g.M, kTile), b.g.pairs, b.g.groups, false);
+    b.g.splits = 1;
+    b.g.first = s.first;
+    if (s.mt2 != s.mt) {
+        if (s.mt == 4 && s.mt2 == 3)
+            launch_batch_gemm_as<4, 4, EPI, 3>(b);
+        else if (s.mt == 4)
+            launch_batch_gemm_as<4, 4, EPI, 2>(b);
+        else
+            launch_batch_gemm_as<3, 4, EPI, 2>(b);
+    } else {
+        switch (s.wn * 10 + s.mt) {
+        case 44: launch_batch_gemm_as<4, 4, EPI>(b); break;
+        case 43: launch_batch_gemm_as<3, 4, EPI>(b); break;
+        case 42: launch_batch_gemm_as<2, 4, EPI>(b); break;
+        case 41: launch_batch_gemm_as<1, 4, EPI>(b); break;
+        case 22: launch_batch_gemm_as<2, 2, EPI>(b); break;
+        case 21: launch_batch_gemm_as<1, 2, EPI>(b); break;
+        default: launch_batch_gemm_as<1, 1, EPI>(b); break;
+        }
+    }
+    L2_LAUNCH_CHECK(name);
+    return LLAMA2_OK;
+}
+
+size_t batch_gemm_bytes(int n_tokens, int K) { return static_cast<size_t>(ceil_div(n_tokens, kTile)) * ceil_div(K, kGroup) * kBlockBytes; }
+
+int launch_batch_gemm(const char* name, const ProductArgs& call, int n_matrices, bool gated, bool adapters, void* fragments)
+{
+    BatchGemmArgs b{};
+    const int groups = ceil_div(call.K, kGroup), tiles = ceil_div(call.n_tokens, kTile);
+    b.g.xf = static_cast<const uint16_t*>(fragments);
+    b.g.xf_bytes = static_cast<uint32_t>(batch_gemm_bytes(call.n_tokens, call.K));
+    b.g.groups = groups, b.g.ws = weight_words(call.K), b.g.ss = groups, b.g.zs = zero_words(call.K), b.g.M = call.n_tokens;
+    b.positions = call.positions, b.token_adapters = call.token_adapters, b.most_adapters = call.most_adapters, b.adapters = adapters;
+    for (int i = 0; i < LLAMA2_MAX_BATCH_MATRICES; ++i) {
+        b.t[i] = call.t[i];
+        b.first[i] = i < n_matrices ? b.g.pairs : 0x7FFFFFFF;
+        if (i < n_matrices && !gated)
+            b.g.pairs += ceil_div(call.t[i].cols, 2 * kTile);
+    }
+    if (gated)
+        b.g.pairs = ceil_div(call.t[0].cols, kTile);
+    hipLaunchKernelGGL(batch_fragments_kernel, dim3(groups, tiles), dim3(256), 0, ctx().stream, static_cast<uint16_t*>(fragments), call.x,
+                       call.n_tokens, call.K, call.x_stride, groups);
+    L2_LAUNCH_CHECK(name);
+    return gated ? launch_batch_gemm_epi<EPI_GATED>(name, b) : launch_batch_gemm_epi<EPI_ROWS>(name, b);
 }
 
 // ---------------------------------------------------------------- causal attention

@@ -1,6 +1,9 @@
 """Products of the rows of many tokens with int4 tensors, low-rank adapters beside them, and the gated block's first half,
 against 64-bit restatements (product_util.py)."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -149,17 +152,33 @@ def test_captured_steps_replayed(tokens, gated):
     capi.call("llama2_graph_destroy", g)
 
 
+CAPTURE = """
+import ctypes as C, sys
+sys.path[:0] = [%r, %r]
+import product_util as pu
+from managedllama2_amd import capi, synth
+from managedllama2_amd.device import init
+init(0)
+p = pu.Product(synth.rng_for(1718), 1000, 4096, [8], False, [128], 128, ids=0, junk=0.0).upload()
+outs, g = p.outputs(), C.c_void_p()
+capi.call("llama2_graph_begin_capture")
+try:
+    rc = capi.raw(*p.args(outs))
+    said = capi.last_error()
+finally:
+    capi.call("llama2_graph_end_capture", C.byref(g))
+assert rc == capi.ERR_INVALID_ARGUMENT and "capture" in said, (rc, said)
+capi.call("llama2_graph_destroy", g)
+p.check()
+print("refused, then done")
+"""
+
+
 def test_a_call_that_would_need_scratch_in_a_capture_is_refused():
-    p = pu.Product(rng(18), 1 << 18, 8, [8], False, [128], 128, ids=0, junk=0.0).upload()
-    outs, g = p.outputs(), C.c_void_p()
-    capi.call("llama2_graph_begin_capture")
-    try:
-        rc = capi.raw(*p.args(outs))
-    finally:
-        capi.call("llama2_graph_end_capture", C.byref(g))
-    assert rc == capi.ERR_INVALID_ARGUMENT and "capture" in capi.last_error()
-    capi.call("llama2_graph_destroy", g)
-    p.check()
+    """In a process of its own, whose library has no scratch yet from other calls."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    out = subprocess.run([sys.executable, "-c", CAPTURE % (here, os.path.dirname(here))], capture_output=True, text=True, timeout=100)
+    assert out.returncode == 0 and "refused, then done" in out.stdout, out.stderr[-2000:]
 
 
 def test_one_token_beside_the_module_of_one_token():
