@@ -27,7 +27,7 @@ struct alignas(64) ProductTensor {
     uint16_t* out;
     const uint16_t* residual;
     const uint16_t* up; // null: no adapters
-    const uint16_t* low;
+    const void* low;
     const TokenAdapter* info;
     long long up_stride;
     int cols, out_stride, residual_stride, n_adapters, max_rank;
@@ -130,7 +130,7 @@ constexpr int kBehind = static_cast<int>(0x80000000u); // an offset behind the e
 // What a product needs of a tensor's adapters.
 struct AdapterPart {
     const uint16_t* up; // null: no adapters
-    const uint16_t* low;
+    const void* low;
     const TokenAdapter* info;
     long long up_stride;
     int n_adapters, max_rank;
@@ -164,7 +164,7 @@ __device__ __forceinline__ void add_item(const Items& items, int item, const Ada
     for (int b = 0; b * 16 < rank; ++b) {
         // lane groups 0 and 1: the upper parts of ranks 0 .. 7 and 8 .. 15 of the block; 2 and 3: the lower ones
         const int have = rank - b * 16 - (c & 1) * 8;
-        const u32x4 hf = *reinterpret_cast<const u32x4*>(m.low + (mine + b) * 32 + c * 8);
+        const u32x4 hf = static_cast<const u32x4*>(m.low)[(mine + b) * 4 + c];
         float f[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)

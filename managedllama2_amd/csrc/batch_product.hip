@@ -19,7 +19,7 @@ struct alignas(64) LowTensor {
     const uint16_t* down; // null: no adapters
     const float* scales;
     const int* ranks;
-    uint16_t* low;      // [n_tokens][blocks][2][16]: what the ranks received, upper and lower part
+    void* low;          // [n_tokens][blocks] of 64 bytes: what the ranks received, 16 floats or the upper and lower parts of 16 numbers
     TokenAdapter* info; // [n_tokens][blocks]
     long long down_stride;
     int n_adapters, max_rank;
@@ -69,8 +69,10 @@ __device__ __forceinline__ h8_t tile_operand(const char* lds, int m)
 // ---------------------------------------------------------------- what the ranks receive
 // A workgroup takes 16 ranks of one item of a block of 64 tokens, so that an adapter is read once for up to 16 tokens that use it; its
 // wavefronts split the inputs.  Ranks and scales of small pools are requested together with the tokens' adapters.
-constexpr int kLowWaves = 16, kLowTable = kLowWaves * 64;
+// WIDE: as two fp16 numbers and a power of two (what the matrix cores take), else in fp32, the adapter's scale with it.
+constexpr int kLowWaves = 8, kLowTable = kLowWaves * 64;
 
+template <bool WIDE>
 __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
 {
     constexpr int kStride = 16 + 4;
@@ -89,11 +91,11 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
     const uint16_t* down = t.down;
     const float* const scales = t.scales;
     const int* const ranks = t.ranks;
-    uint16_t* const low = t.low;
+    void* const lows = t.low;
     TokenAdapter* const info = t.info;
     const long long down_stride = t.down_stride;
     const int n_adapters = t.n_adapters, max_rank = t.max_rank;
-    loaded(K, x_stride, n_tokens, most_adapters, x, positions, token_adapters, down, scales, ranks, low, info, down_stride, n_adapters, max_rank);
+    loaded(K, x_stride, n_tokens, most_adapters, x, positions, token_adapters, down, scales, ranks, lows, info, down_stride, n_adapters, max_rank);
     if (!down || r0 >= max_rank)
         return;
     int mine = 0;
@@ -128,7 +130,7 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
         const int own = items.tokens[item][4 * i + c];
         xoff[i] = own == kNobody ? kBehind : own * x_stride * 2;
     }
-    constexpr int kAhead = 2; // tiles of both that a wavefront has requested
+    constexpr int kAhead = 4; // tiles of both that a wavefront has requested
     HalfTile xt[kAhead], dt[kAhead];
     auto request = [&](int q, int k0) {
         const int column = tile_column(k0, K);
@@ -175,18 +177,25 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
     for (int w = 0; w < kLowWaves; ++w)
         v += red[(w * 16 + place) * kStride + l15];
     v = r0 + l15 < rank ? v : 0.0f;
-    const float most = row16_max(fabsf(v));
-    // the largest between 2^14 and 2^15; nothing to scale where all are 0 or one is infinite
-    const int e2 = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
-    const float scaled = ldexpf(v, e2);
-    const uint16_t h = float_to_half_bits(scaled);
-    if (m == kNobody)
-        return;
-    const size_t to = static_cast<size_t>(t0 + m) * ((max_rank + 15) / 16) + block;
-    low[to * 32 + l15] = h;
-    low[to * 32 + 16 + l15] = float_to_half_bits(scaled - half_bits_to_float(h));
-    if (l15 == 0)
-        info[to] = TokenAdapter{ldexpf(scale, -e2), rank};
+    const size_t to = static_cast<size_t>(t0 + (m == kNobody ? 0 : m)) * ((max_rank + 15) / 16) + block;
+    if constexpr (WIDE) {
+        const float most = row16_max(fabsf(v));
+        // the largest between 2^14 and 2^15; nothing to scale where all are 0 or one is infinite
+        const int e2 = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
+        const float scaled = ldexpf(v, e2);
+        const uint16_t h = float_to_half_bits(scaled);
+        if (m == kNobody)
+            return;
+        uint16_t* const low = static_cast<uint16_t*>(lows);
+        low[to * 32 + l15] = h;
+        low[to * 32 + 16 + l15] = float_to_half_bits(scaled - half_bits_to_float(h));
+        if (l15 == 0)
+            info[to] = TokenAdapter{ldexpf(scale, -e2), rank};
+    } else if (m != kNobody) {
+        static_cast<float*>(lows)[to * 16 + l15] = v * scale;
+        if (l15 == 0)
+            info[to] = TokenAdapter{scale, rank};
+    }
 }
 
 // ---------------------------------------------------------------- the products
@@ -213,6 +222,14 @@ __device__ __forceinline__ u32x4 turned_words(char* lds, u32x4 v)
     return *reinterpret_cast<const u32x4*>(lds + row * 64 + (c ^ (row >> 2)) * 16);
 }
 
+// 16 bytes that are aligned as halfs, or as words
+struct __attribute__((packed, aligned(2))) AnyHalfs {
+    u32x4 v;
+};
+struct __attribute__((packed, aligned(4))) AnyWords {
+    u32x4 v;
+};
+
 constexpr int kProductWaves = 8;
 constexpr int kScaleBytes = 20480; // of LDS for the scales and zero points of a workgroup's rows
 
@@ -227,7 +244,8 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
     constexpr int kWaveBytes = kTileBytes + R * 1024, kSums = kProductWaves * kTokens * kStride * 4, kExtra = ADAPTERS ? kTokens * kStride * 4 : 0;
     constexpr int kFront = kProductWaves * kWaveBytes + kScaleBytes;
     __shared__ __align__(16) char pool[(kFront > kSums ? kFront : kSums) + kExtra]; // the sums come where tiles and scales were
-    __shared__ __align__(16) Items items;
+    __shared__ int ids[kTokens];
+    __shared__ int ranks[kTensors][kTokens];
     auto& a = kernel_args<ProductArgs>();
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, c = lane >> 4;
     const int K = a.K, x_stride = a.x_stride, n_tokens = a.n_tokens, most_adapters = a.most_adapters, row_blocks = a.row_blocks,
@@ -299,33 +317,83 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
             if (d * T + i < kRing)
                 load_x(d * T + i, i, wave + d * kProductWaves);
     }
-    // Scales and zero points of all rows: they are neighbours in memory.
+    // Scales and zero points of all rows: they are neighbours in memory, and multiples of 8.
     char* const lds = pool + wave * kWaveBytes; // of this wavefront
     uint16_t* const scales = reinterpret_cast<uint16_t*>(pool + kProductWaves * kWaveBytes);
-    uint32_t* const zeros = reinterpret_cast<uint32_t*>(scales + (kRows * groups + 7) / 8 * 8);
+    uint32_t* const zeros = reinterpret_cast<uint32_t*>(scales + kRows * groups);
 #pragma unroll
     for (int h = 0; h < kTensors; ++h) {
-        const uint16_t* const s = m[h].s + static_cast<size_t>(n0) * groups;
-        const uint32_t* const z = m[h].z + static_cast<size_t>(n0) * zs;
-        for (int i = tid; i < rows * groups; i += kProductWaves * 64)
-            scales[h * RT * 16 * groups + i] = s[i];
-        for (int i = tid; i < rows * zs; i += kProductWaves * 64)
-            zeros[h * RT * 16 * zs + i] = z[i];
+        const AnyHalfs* const s = reinterpret_cast<const AnyHalfs*>(m[h].s + static_cast<size_t>(n0) * groups);
+        const AnyWords* const z = reinterpret_cast<const AnyWords*>(m[h].z + static_cast<size_t>(n0) * zs);
+        const int ns = rows * groups / 8, nz = rows * zs / 4;
+        for (int i = tid; i < ns + nz; i += kProductWaves * 64)
+            if (i < ns)
+                reinterpret_cast<u32x4*>(scales + h * RT * 16 * groups)[i] = s[i].v;
+            else
+                reinterpret_cast<u32x4*>(zeros + h * RT * 16 * zs)[i - ns] = z[i - ns].v;
     }
-    if (tid < kTokens)
-        items.ids[tid] = adapter_of(positions, token_adapters, t0 + tid, n_tokens, most_adapters);
+    if (tid < kTokens) {
+        const int token = t0 + tid;
+        int rank[kTensors] = {};
+        if (ADAPTERS && token < n_tokens)
+#pragma unroll
+            for (int h = 0; h < kTensors; ++h)
+                if (m[h].up)
+                    rank[h] = m[h].info[static_cast<size_t>(token) * ((m[h].max_rank + 15) / 16)].rank; // of no adapter: not used
+        ids[tid] = adapter_of(positions, token_adapters, token, n_tokens, most_adapters);
+#pragma unroll
+        for (int h = 0; h < kTensors; ++h)
+            ranks[h][tid] = rank[h];
+    }
     float* const extra = reinterpret_cast<float*>(pool + (kFront > kSums ? kFront : kSums));
-    if (ADAPTERS && wave == 0)
-        find_items(items, here);
     __syncthreads();
     if constexpr (ADAPTERS) {
-        // The adapters' part of each item, straight to where the sums of the wavefronts meet: a token has one adapter.
-        for (int i = wave; i < items.count * kTensors; i += kProductWaves) {
-            const int item = i / kTensors, h = i % kTensors;
-            auto& m1 = m[h ? kTensors - 1 : 0];
-            add_item<RT>(items, item, m1, t0, n0, rows, lds, [&](int token, int r, float v) {
-                extra[token * kStride + (h * RT + r) * 16 + l15] = v;
-            });
+        // The adapters' part, straight to where the sums of the wavefronts meet.  A thread takes every so many outputs of one token: with
+        // few tokens of an adapter the matrix cores would compute 16 for one.
+        constexpr int kThreads = kProductWaves * 64 / kTokens, kOwn = kRows > kThreads ? kRows / kThreads : 1, kPer = kOwn / kTensors ? kOwn / kTensors : 1;
+        static_assert(kOwn * kThreads >= kRows, "all outputs of a token");
+        const int token = tid / kThreads, id = ids[token];
+#pragma unroll
+        for (int h = 0; h < (kOwn < kTensors ? 1 : kTensors); ++h) {
+            // rows `first` + i * kThreads of a tensor's RT * 16; where a token has as many threads as outputs, they are one of either tensor's
+            const int of = kOwn < kTensors ? tid % kThreads / (RT * 16) : h, first = kOwn < kTensors ? tid % kThreads % (RT * 16) : tid % kThreads;
+            const AdapterPart part = of == 0 ? AdapterPart(m[0]) : AdapterPart(m[kTensors - 1]);
+            const int rank = id >= 0 && id < part.n_adapters && of < kTensors ? ranks[of][token] : 0;
+            const uint16_t* up = part.up + id * part.up_stride + static_cast<size_t>(n0 + first) * part.max_rank;
+            const f4_t* low = static_cast<const f4_t*>(part.low) + static_cast<size_t>(t0 + token) * ((part.max_rank + 15) / 16) * 4;
+            float sum[kPer] = {};
+            for (int r0 = 0; r0 < rank; r0 += 16) {
+                f4_t x[4];
+                u32x4 u[kPer][2] = {};
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    x[k] = low[r0 / 4 + k]; // zeros behind the rank
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        if (first + i * kThreads < rows && r0 + 8 * k < rank)
+                            u[i][k] = *reinterpret_cast<const u32x4*>(up + static_cast<size_t>(i) * kThreads * part.max_rank + r0 + 8 * k);
+                if (rank - r0 < 16 && (rank & 7))
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int have = rank - r0 - 2 * k;
+                        const uint32_t mask = have >= 2 ? ~0u : have == 1 ? 0xFFFFu : 0u;
+#pragma unroll
+                        for (int i = 0; i < kPer; ++i)
+                            u[i][k >> 2][k & 3] &= mask;
+                    }
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        sum[i] = __builtin_fmaf(half_bits_to_float(static_cast<uint16_t>(u[i][k >> 3][(k & 7) >> 1] >> (16 * (k & 1)))), x[k >> 2][k & 3], sum[i]);
+            }
+            if (rank > 0)
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+                    if (first + i * kThreads < RT * 16)
+                        extra[token * kStride + of * RT * 16 + first + i * kThreads] = sum[i];
         }
     }
 
@@ -353,11 +421,12 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
             for (int i = 0; i < T; ++i) {
                 const int q = (d * T + i) % kRing, next = d * T + i + kRing; // the tile that comes into this place
                 put_tile(lds, xt[q]);
+                __builtin_amdgcn_sched_barrier(0);
+                load_x(q, next % T, g0 + next / T * kProductWaves);
                 h8_t xf[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     xf[j] = tile_operand(lds, j);
-                load_x(q, next % T, g0 + next / T * kProductWaves);
                 f4_t p[R] = {};
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -384,7 +453,7 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
     __syncthreads();
     constexpr int kPieces = RT * 2; // of 8 outputs
     for (int i = tid; i < kTokens * kPieces; i += kProductWaves * 64) {
-        const int token = i / kPieces, piece = i % kPieces * 8, n = n0 + piece, id = items.ids[token];
+        const int token = i / kPieces, piece = i % kPieces * 8, n = n0 + piece, id = ids[token];
         if (id == kNoToken || n >= cols)
             continue;
         u32x4 residual = {};
@@ -405,7 +474,7 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
 #pragma unroll
             for (int q = 0; q < kProductWaves; ++q)
                 add(red + q * kTokens * kStride);
-            if (ADAPTERS && m[h].up && id >= 0 && id < m[h].n_adapters)
+            if (ADAPTERS && id >= 0 && id < m[h].n_adapters && ranks[h][token] > 0)
                 add(extra);
         }
         u32x4 o;
@@ -453,8 +522,8 @@ static void launch_product(Product& p)
 }
 
 // Rows of more than 32768 inputs: tiles so low that their scales fit.
-static void launch_tall(Product& p, std::false_type) { launch_product<1, 1, 4, false>(p); }
-static void launch_tall(Product& p, std::true_type) { launch_product<2, 1, 4, true>(p); }
+static void launch_tall(Product& p, std::false_type) { launch_product<1, 1, 2, false>(p); }
+static void launch_tall(Product& p, std::true_type) { launch_product<2, 1, 2, true>(p); }
 
 constexpr int kWideTokens = 64; // more go through the kernels of the prompt's products
 constexpr int kMostTokens = 4096; // of a launch
@@ -486,7 +555,7 @@ static int run_product(const char* fn, Product& p)
         LowTensor& t = l.t[i];
         if (!t.down)
             continue;
-        t.low = reinterpret_cast<uint16_t*>(at);
+        t.low = at;
         at += static_cast<size_t>(most) * ceil_div(t.max_rank, 16) * 64;
         t.info = reinterpret_cast<TokenAdapter*>(at);
         at += static_cast<size_t>(most) * ceil_div(t.max_rank, 16) * sizeof(TokenAdapter);
@@ -507,8 +576,11 @@ static int run_product(const char* fn, Product& p)
             l.most_adapters = a.most_adapters;
             // items of a block of 64 tokens: one for each adapter in use, and one more for every 16 tokens
             const int tokens = a.n_tokens < 64 ? a.n_tokens : 64, items = a.most_adapters + 3 < tokens ? a.most_adapters + 3 : tokens;
-            hipLaunchKernelGGL(batch_low_kernel, dim3(ceil_div(a.n_tokens, 64), items, p.n_matrices * kRankBlocks), dim3(kLowWaves * 64), 0,
-                               ctx().stream, l);
+            const dim3 grid(ceil_div(a.n_tokens, 64), items, p.n_matrices * kRankBlocks);
+            if (wide)
+                hipLaunchKernelGGL(batch_low_kernel<true>, grid, dim3(kLowWaves * 64), 0, ctx().stream, l);
+            else
+                hipLaunchKernelGGL(batch_low_kernel<false>, grid, dim3(kLowWaves * 64), 0, ctx().stream, l);
             L2_LAUNCH_CHECK(fn);
         }
         if (wide) {
@@ -517,7 +589,7 @@ static int run_product(const char* fn, Product& p)
         } else {
             // scales and zero points of a workgroup's rows: R * groups <= 512
             if (a.n_tokens <= 16)
-                groups <= 256 ? launch_product<2, 1, 4, GATED>(p) : launch_tall(p, std::integral_constant<bool, GATED>());
+                groups <= 256 ? launch_product<2, 1, 2, GATED>(p) : launch_tall(p, std::integral_constant<bool, GATED>());
             else if (a.n_tokens <= 32)
                 groups <= 256 ? launch_product<2, 2, 2, GATED>(p) : launch_tall(p, std::integral_constant<bool, GATED>());
             else
