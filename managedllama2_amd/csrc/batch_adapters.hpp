@@ -95,21 +95,24 @@ struct Items {
 };
 constexpr uint8_t kNobody = 255;
 
-// By one wavefront, from the first `tokens` of items.ids; everyone may read the items after the next barrier.
-__device__ __forceinline__ void find_items(Items& items, int tokens)
+// By one wavefront, from the first `tokens` of items.ids, which are below `most`; everyone may read the items after the next barrier.
+__device__ __forceinline__ void find_items(Items& items, int tokens, int most)
 {
     const int lane = threadIdx.x & 63, id = lane < tokens ? items.ids[lane] : kNoToken;
-    int before = 0, lead = -1; // tokens with this adapter in front of this one, and the first of its sixteen
-    for (int j = 0; j < tokens; ++j) {
-        const bool same = __builtin_amdgcn_readlane(id, j) == id && j <= lane;
-        lead = same && (before & 15) == 0 ? j : lead;
-        before += same;
+    unsigned long long same = __ballot(id >= 0); // the lanes with this lane's adapter, bit by bit
+    for (int bits = most - 1, b = 0; bits >> b; ++b) {
+        const unsigned long long set = __ballot((id >> b) & 1);
+        same &= (id >> b) & 1 ? set : ~set;
     }
+    const int before = __builtin_popcountll(same & ((1ULL << lane) - 1));
+    for (int n = before & ~15; n > 0; --n) // what the sixteens in front hold
+        same &= same - 1;
+    const int lead = __builtin_ctzll(same | 1ULL << 63); // the first of this lane's sixteen
     const unsigned long long leads = __ballot(id >= 0 && lead == lane);
     reinterpret_cast<u32x4*>(items.tokens)[lane] = u32x4{~0u, ~0u, ~0u, ~0u};
     if (id >= 0) {
         const int item = __builtin_popcountll(leads & ((1ULL << lead) - 1));
-        items.tokens[item][(before - 1) & 15] = static_cast<uint8_t>(lane);
+        items.tokens[item][before & 15] = static_cast<uint8_t>(lane);
         if (lead == lane)
             items.adapter[item] = id;
     }

@@ -30,6 +30,8 @@ struct alignas(64) LowArgs {
     const int* positions;
     const int* token_adapters;
     int K, x_stride, n_tokens, most_adapters;
+    uint16_t* packed; // non-null: the rows as operands, by the workgroups behind those of the tensors
+    int n_matrices;
     LowTensor t[LLAMA2_MAX_BATCH_MATRICES];
 };
 
@@ -66,6 +68,28 @@ __device__ __forceinline__ h8_t tile_operand(const char* lds, int m)
     return *reinterpret_cast<const h8_t*>(lds + row * 256 + ((4 * c + m) ^ row) * 16);
 }
 
+// ---------------------------------------------------------------- rows as operands
+// 16 tokens and a group of 128 inputs are the four operands of 16 x 16 x 32 products, 1 KB each: lane group c of operand m holds elements
+// 32 c + 8 m on of token lane % 16, zeros behind the end of a row.  Tokens behind the last one repeat it.  `worker` of `workers` pairs of
+// such tiles at a time, 512 threads.
+__device__ __forceinline__ void pack_rows(uint16_t* packed, const uint16_t* x, int K, int x_stride, int n_tokens, int worker, int workers)
+{
+    const int groups = (K + 127) / 128, units = (n_tokens + 15) / 16 * groups, lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+    for (int u = worker * 2 + (part >> 2); u < units; u += workers * 2) {
+        const int tile = u / groups, g = u % groups, m = part & 3;
+        const int token = min(tile * 16 + (lane & 15), n_tokens - 1), k = g * 128 + 32 * (lane >> 4) + 8 * m;
+        u32x4 v = {};
+        if (k < K)
+            v = *reinterpret_cast<const u32x4*>(x + static_cast<size_t>(token) * x_stride + k);
+        reinterpret_cast<u32x4*>(packed)[(static_cast<size_t>(u) * 4 + m) * 64 + lane] = v;
+    }
+}
+
+__global__ __launch_bounds__(512) void batch_pack_kernel(uint16_t* packed, const uint16_t* x, int K, int x_stride, int n_tokens)
+{
+    pack_rows(packed, x, K, x_stride, n_tokens, blockIdx.x, gridDim.x);
+}
+
 // ---------------------------------------------------------------- what the ranks receive
 // A workgroup takes 16 ranks of one item of a block of 64 tokens, so that an adapter is read once for up to 16 tokens that use it; its
 // wavefronts split the inputs.  Ranks and scales of small pools are requested together with the tokens' adapters.
@@ -86,6 +110,10 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
     const int t0 = blockIdx.x * 64, K = a.K, x_stride = a.x_stride, n_tokens = a.n_tokens, most_adapters = a.most_adapters;
     const uint16_t* const x = a.x;
     const int *const positions = a.positions, *const token_adapters = a.token_adapters;
+    if (static_cast<int>(blockIdx.z) == a.n_matrices * kRankBlocks) {
+        pack_rows(a.packed, x, K, x_stride, n_tokens, blockIdx.x * gridDim.y + blockIdx.y, gridDim.x * gridDim.y);
+        return;
+    }
     auto& t = a.t[blockIdx.z / kRankBlocks];
     const int block = blockIdx.z % kRankBlocks, r0 = block * 16;
     const uint16_t* down = t.down;
@@ -106,7 +134,7 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
     }
     if (wave == 0) {
         items.ids[lane] = adapter_of(positions, token_adapters, t0 + lane, n_tokens, most_adapters);
-        find_items(items, min(64, n_tokens - t0));
+        find_items(items, min(64, n_tokens - t0), most_adapters);
     }
     table[tid] = mine;
     scale_table[tid] = mine_scale;
@@ -241,7 +269,8 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
     constexpr int kTokens = T * 16, kRows = R * 16, kStride = kRows + 4, kTensors = GATED ? 2 : 1, RT = R / kTensors;
     constexpr int kRing = T * D <= 4 ? T * D : 2; // tiles of tokens whose inputs are on their way or in use
     static_assert(T * D % kRing == 0 && kRing <= T * D, "a tile has one place in the ring");
-    constexpr int kWaveBytes = kTileBytes + R * 1024, kSums = kProductWaves * kTokens * kStride * 4, kExtra = ADAPTERS ? kTokens * kStride * 4 : 0;
+    constexpr bool PACKED = T > 1; // the inputs come as operands; of few tokens in rows, which saves the launch that packs them
+    constexpr int kWaveBytes = (PACKED ? 0 : kTileBytes) + R * 1024, kWordsAt = kWaveBytes - R * 1024, kSums = kProductWaves * kTokens * kStride * 4, kExtra = ADAPTERS ? kTokens * kStride * 4 : 0;
     constexpr int kFront = kProductWaves * kWaveBytes + kScaleBytes;
     __shared__ __align__(16) char pool[(kFront > kSums ? kFront : kSums) + kExtra]; // the sums come where tiles and scales were
     __shared__ int ids[kTokens];
@@ -288,7 +317,9 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
 #pragma unroll
     for (int h = 0; h < kTensors; ++h)
         rw[h] = rows_buffer(m[h].w + static_cast<size_t>(n0) * ws, static_cast<size_t>(rows) * ws * 4);
-    const __amdgpu_buffer_rsrc_t rx = rows_buffer(x + static_cast<size_t>(t0) * x_stride, (static_cast<size_t>(here - 1) * x_stride + K) * 2);
+    const int tiles = (here + 15) / 16;
+    const __amdgpu_buffer_rsrc_t rx = PACKED ? rows_buffer(x + static_cast<size_t>(t0) * groups * 128, static_cast<size_t>(tiles) * groups * 4096)
+                                             : rows_buffer(x + static_cast<size_t>(t0) * x_stride, (static_cast<size_t>(here - 1) * x_stride + K) * 2);
     const int woff = (lane >> 2) * ws * 4 + 16 * (lane & 3), xoff = c * x_stride * 2;
 
     // A group's weights and inputs.  A group that does not exist is requested behind the ends too: loads that come and go would make
@@ -303,10 +334,17 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
         __builtin_amdgcn_sched_barrier(0); // loads keep one order from the first group on: waits count them
     };
     auto load_x = [&](int q, int i, int g) { // tile i into place q
-        const int column = tile_column(128 * g, K), at = column < 0 ? kBehind : column + xoff;
+        if constexpr (PACKED) {
+            const int at = g < groups ? (i * groups + g) * 4096 + lane * 16 : kBehind;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            xt[q].v[e] = __builtin_amdgcn_raw_buffer_load_b128(rx, at + (i * 16 + 4 * e) * x_stride * 2, 0, 0);
+            for (int e = 0; e < 4; ++e)
+                xt[q].v[e] = __builtin_amdgcn_raw_buffer_load_b128(rx, at + e * 1024, 0, 0);
+        } else {
+            const int column = tile_column(128 * g, K), at = column < 0 ? kBehind : column + xoff;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                xt[q].v[e] = __builtin_amdgcn_raw_buffer_load_b128(rx, at + (i * 16 + 4 * e) * x_stride * 2, 0, 0);
+        }
         __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
@@ -406,7 +444,7 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
             float sc[R];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const u32x4 v = turned_words(lds + kTileBytes + r * 1024, raw[d][r]);
+                const u32x4 v = turned_words(lds + kWordsAt + r * 1024, raw[d][r]);
                 const int row = r * 16 + l15;
                 const float zero = static_cast<float>(zeros[row * zs + (gs >> 3)] >> (4 * (gs & 7)) & 15u);
                 const h2_t minus = {static_cast<_Float16>(-1024.0f - zero), static_cast<_Float16>(-64.0f - zero)};
@@ -420,19 +458,29 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
 #pragma unroll
             for (int i = 0; i < T; ++i) {
                 const int q = (d * T + i) % kRing, next = d * T + i + kRing; // the tile that comes into this place
-                put_tile(lds, xt[q]);
-                __builtin_amdgcn_sched_barrier(0);
-                load_x(q, next % T, g0 + next / T * kProductWaves);
                 h8_t xf[4];
+                if constexpr (PACKED) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    xf[j] = tile_operand(lds, j);
+                    for (int j = 0; j < 4; ++j)
+                        xf[j] = __builtin_bit_cast(h8_t, xt[q].v[j]);
+                } else {
+                    put_tile(lds, xt[q]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    load_x(q, next % T, g0 + next / T * kProductWaves);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        xf[j] = tile_operand(lds, j);
+                }
                 f4_t p[R] = {};
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int r = 0; r < R; ++r)
                         p[r] = mfma16(xf[j], wf[r][j], p[r]);
+                if constexpr (PACKED) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    load_x(q, next % T, g0 + next / T * kProductWaves);
+                }
 #pragma unroll
                 for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -538,7 +586,8 @@ static int run_product(const char* fn, Product& p)
     for (int i = 0; i < p.n_matrices; ++i)
         fits = fits && static_cast<long long>(a.t[i].cols) * weight_words(a.K) * 4 <= 0x7FFFFFFFLL;
     const bool wide = all > kWideTokens && fits;
-    const size_t fragments = wide ? batch_gemm_bytes(most, a.K) : 0;
+    const bool packed = !wide && all > 16;
+    const size_t fragments = wide ? batch_gemm_bytes(most, a.K) : packed ? static_cast<size_t>(ceil_div(most, 16)) * groups * 4096 : 0;
     size_t bytes = fragments;
     for (int i = 0; i < p.n_matrices; ++i)
         if (l.t[i].down) {
@@ -576,12 +625,24 @@ static int run_product(const char* fn, Product& p)
             l.most_adapters = a.most_adapters;
             // items of a block of 64 tokens: one for each adapter in use, and one more for every 16 tokens
             const int tokens = a.n_tokens < 64 ? a.n_tokens : 64, items = a.most_adapters + 3 < tokens ? a.most_adapters + 3 : tokens;
-            const dim3 grid(ceil_div(a.n_tokens, 64), items, p.n_matrices * kRankBlocks);
+            l.n_matrices = p.n_matrices;
+            l.packed = packed ? reinterpret_cast<uint16_t*>(base) : nullptr;
+            const dim3 grid(ceil_div(a.n_tokens, 64), items, p.n_matrices * kRankBlocks + packed);
             if (wide)
                 hipLaunchKernelGGL(batch_low_kernel<true>, grid, dim3(kLowWaves * 64), 0, ctx().stream, l);
             else
                 hipLaunchKernelGGL(batch_low_kernel<false>, grid, dim3(kLowWaves * 64), 0, ctx().stream, l);
             L2_LAUNCH_CHECK(fn);
+        }
+        const uint16_t* const rows = a.x;
+        if (packed) {
+            if (!p.adapters) {
+                const int units = ceil_div(a.n_tokens, 16) * groups;
+                hipLaunchKernelGGL(batch_pack_kernel, dim3(ceil_div(units, 2)), dim3(512), 0, ctx().stream, reinterpret_cast<uint16_t*>(base), a.x,
+                                   a.K, a.x_stride, a.n_tokens);
+                L2_LAUNCH_CHECK(fn);
+            }
+            a.x = reinterpret_cast<const uint16_t*>(base);
         }
         if (wide) {
             if (int rc = launch_batch_gemm(fn, a, p.n_matrices, GATED, p.adapters, base))
@@ -596,7 +657,7 @@ static int run_product(const char* fn, Product& p)
                 groups <= 128 ? launch_product<4, 4, 1, GATED>(p) : launch_tall(p, std::integral_constant<bool, GATED>());
             L2_LAUNCH_CHECK(fn);
         }
-        a.x += static_cast<size_t>(a.n_tokens) * a.x_stride;
+        a.x = rows + static_cast<size_t>(a.n_tokens) * a.x_stride;
         a.positions += a.n_tokens;
         if (a.token_adapters)
             a.token_adapters += a.n_tokens;

@@ -533,7 +533,7 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& a, char* lds, int uni
             if (lane < kTile)
                 items[wave].ids[lane] = known_adapter(position, adapter, rows->most_adapters);
             if (adapters)
-                find_items(items[wave], kTile);
+                find_items(items[wave], kTile, rows->most_adapters);
         }
         __syncthreads();
         if (adapters) { // onto the first group's sums, every wavefront for the outputs of its own tile
