@@ -38,8 +38,7 @@ struct alignas(64) ProductArgs {
     const int* positions;
     const int* token_adapters;
     int K, x_stride, n_tokens, most_adapters; // of any tensor
-    int row_blocks, token_blocks;
-    int first[LLAMA2_MAX_BATCH_MATRICES]; // first block of rows of a tensor
+    int token_blocks;
     ProductTensor t[LLAMA2_MAX_BATCH_MATRICES];
 };
 

@@ -9,6 +9,7 @@
 #include "prefill.hpp"
 
 #include <cmath>
+#include <cstdlib>
 #include <type_traits>
 
 namespace l2 {
@@ -258,58 +259,63 @@ struct __attribute__((packed, aligned(4))) AnyWords {
     u32x4 v;
 };
 
-constexpr int kProductWaves = 8;
 constexpr int kScaleBytes = 20480; // of LDS for the scales and zero points of a workgroup's rows
 
 // A workgroup takes R tiles of 16 outputs (GATED: half of them of the gate, half of the up projection) and T tiles of 16
-// tokens; its wavefronts take the groups of 128 inputs in turn, D of them requested ahead, and add up through LDS.
-template <int R, int T, int D, bool GATED, bool ADAPTERS>
-__global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(ProductArgs)
+// tokens; its W wavefronts take the groups of 128 inputs in turn, D of them requested ahead, and add up through LDS.
+template <int W, int R, int T, int D, bool GATED, bool ADAPTERS>
+__global__ __launch_bounds__(W * 64, 2) void batch_product_kernel(ProductArgs)
 {
     constexpr int kTokens = T * 16, kRows = R * 16, kStride = kRows + 4, kTensors = GATED ? 2 : 1, RT = R / kTensors;
     constexpr int kRing = T * D <= 4 ? T * D : 2; // tiles of tokens whose inputs are on their way or in use
     static_assert(T * D % kRing == 0 && kRing <= T * D, "a tile has one place in the ring");
     constexpr bool PACKED = T > 1; // the inputs come as operands; of few tokens in rows, which saves the launch that packs them
-    constexpr int kWaveBytes = (PACKED ? 0 : kTileBytes) + R * 1024, kWordsAt = kWaveBytes - R * 1024, kSums = kProductWaves * kTokens * kStride * 4, kExtra = ADAPTERS ? kTokens * kStride * 4 : 0;
-    constexpr int kFront = kProductWaves * kWaveBytes + kScaleBytes;
-    __shared__ __align__(16) char pool[(kFront > kSums ? kFront : kSums) + kExtra]; // the sums come where tiles and scales were
-    __shared__ int ids[kTokens];
-    __shared__ int ranks[kTensors][kTokens];
+    constexpr int kWaveBytes = (PACKED ? 0 : kTileBytes) + R * 1024, kWordsAt = kWaveBytes - R * 1024;
+    constexpr int kSums = W * kTokens * kStride * 4, kExtraAt = W * kWaveBytes + kScaleBytes, kFront = kExtraAt + (ADAPTERS ? kTokens * kStride * 4 : 0);
+    __shared__ __align__(16) char pool[kFront > kSums ? kFront : kSums]; // the sums come where tiles, scales and the adapters' part were
+    __shared__ int live[kTokens];
     auto& a = kernel_args<ProductArgs>();
+    auto& t = a.t[GATED ? 0 : blockIdx.y];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, c = lane >> 4;
-    const int K = a.K, x_stride = a.x_stride, n_tokens = a.n_tokens, most_adapters = a.most_adapters, row_blocks = a.row_blocks,
-              token_blocks = a.token_blocks, first1 = a.first[1], first2 = a.first[2], first3 = a.first[3];
+    const int K = a.K, x_stride = a.x_stride, n_tokens = a.n_tokens, most_adapters = a.most_adapters, token_blocks = a.token_blocks;
     const uint16_t* const x = a.x;
     const int *const positions = a.positions, *const token_adapters = a.token_adapters;
-    loaded(K, x_stride, n_tokens, most_adapters, row_blocks, token_blocks, first1, first2, first3, x, positions, token_adapters);
-    // the token blocks of one block of rows follow each other on one XCD
-    const int slot = blockIdx.x >> 3, rb = slot / token_blocks * 8 + (blockIdx.x & 7), t0 = slot % token_blocks * kTokens;
-    if (rb >= row_blocks)
-        return;
-    const int which = GATED ? 0 : (rb >= first1) + (rb >= first2) + (rb >= first3);
-    const int ws = (K + 31) / 32 * 4, groups = (K + 127) / 128, zs = (groups + 7) / 8;
     struct Tensor : AdapterPart {
         const uint32_t* w;
         const uint32_t* z;
         const uint16_t* s;
     } m[kTensors];
-#pragma unroll
-    for (int h = 0; h < kTensors; ++h) {
-        auto& t = a.t[which + h];
-        m[h] = {adapter_part(t), t.w, t.z, t.s};
-    }
-    auto& t = a.t[which];
+    m[0] = {adapter_part(t), t.w, t.z, t.s};
+    if constexpr (GATED)
+        m[1] = {adapter_part(a.t[1]), a.t[1].w, a.t[1].z, a.t[1].s};
     const int cols = t.cols, out_stride = t.out_stride, residual_stride = t.residual_stride;
     uint16_t* const out = t.out;
     const uint16_t* const residual_rows = t.residual;
+    loaded(K, x_stride, n_tokens, most_adapters, token_blocks, x, positions, token_adapters, m[0].w, m[0].z, m[0].s, m[kTensors - 1].w,
+           m[kTensors - 1].z, m[kTensors - 1].s, cols, out_stride, residual_stride, out, residual_rows);
+    if (ADAPTERS)
+        loaded(m[0].up, m[0].low, m[0].info, m[0].up_stride, m[0].n_adapters, m[0].max_rank, m[kTensors - 1].up, m[kTensors - 1].low,
+               m[kTensors - 1].info, m[kTensors - 1].up_stride, m[kTensors - 1].n_adapters, m[kTensors - 1].max_rank);
+    // the token blocks of one block of rows follow each other on one XCD
+    const int slot = blockIdx.x >> 3, rb = slot / token_blocks * 8 + (blockIdx.x & 7), t0 = slot % token_blocks * kTokens, n0 = rb * RT * 16;
+    if (n0 >= cols)
+        return;
+    const int ws = (K + 31) / 32 * 4, groups = (K + 127) / 128, zs = (groups + 7) / 8;
+
+    // The threads of a token, its adapter and that one's ranks: asked for first, since more hangs on them.
+    constexpr int kThreads = W * 64 / kTokens;
+    const int my_token = tid / kThreads, token_at = t0 + my_token;
+    int position = -1, adapter = kNoAdapter, rank[kTensors] = {};
+    if (token_at < n_tokens) {
+        position = positions[token_at];
+        if (token_adapters)
+            adapter = token_adapters[token_at];
+        if constexpr (ADAPTERS)
 #pragma unroll
-    for (int h = 0; h < kTensors; ++h) {
-        loaded(m[h].w, m[h].z, m[h].s);
-        if (ADAPTERS)
-            loaded(m[h].up, m[h].low, m[h].info, m[h].up_stride, m[h].n_adapters, m[h].max_rank);
+            for (int h = 0; h < kTensors; ++h)
+                if (m[h].up)
+                    rank[h] = m[h].info[static_cast<size_t>(token_at) * ((m[h].max_rank + 15) / 16)].rank; // of no adapter: not used
     }
-    loaded(cols, out_stride, residual_stride, out, residual_rows);
-    const int n0 = (rb - (which == 0 ? 0 : which == 1 ? first1 : which == 2 ? first2 : first3)) * RT * 16;
 
     // Rows and tokens that do not exist lie behind the ends of the buffers.
     const int rows = min(RT * 16, cols - n0), here = min(kTokens, n_tokens - t0);
@@ -349,97 +355,111 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
     };
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-        load_w(d, wave + d * kProductWaves);
+        load_w(d, wave + d * W);
 #pragma unroll
         for (int i = 0; i < T; ++i)
             if (d * T + i < kRing)
-                load_x(d * T + i, i, wave + d * kProductWaves);
+                load_x(d * T + i, i, wave + d * W);
     }
     // Scales and zero points of all rows: they are neighbours in memory, and multiples of 8.
     char* const lds = pool + wave * kWaveBytes; // of this wavefront
-    uint16_t* const scales = reinterpret_cast<uint16_t*>(pool + kProductWaves * kWaveBytes);
+    uint16_t* const scales = reinterpret_cast<uint16_t*>(pool + W * kWaveBytes);
     uint32_t* const zeros = reinterpret_cast<uint32_t*>(scales + kRows * groups);
 #pragma unroll
     for (int h = 0; h < kTensors; ++h) {
         const AnyHalfs* const s = reinterpret_cast<const AnyHalfs*>(m[h].s + static_cast<size_t>(n0) * groups);
         const AnyWords* const z = reinterpret_cast<const AnyWords*>(m[h].z + static_cast<size_t>(n0) * zs);
         const int ns = rows * groups / 8, nz = rows * zs / 4;
-        for (int i = tid; i < ns + nz; i += kProductWaves * 64)
+        for (int i = tid; i < ns + nz; i += W * 64)
             if (i < ns)
                 reinterpret_cast<u32x4*>(scales + h * RT * 16 * groups)[i] = s[i].v;
             else
                 reinterpret_cast<u32x4*>(zeros + h * RT * 16 * zs)[i - ns] = z[i - ns].v;
     }
-    if (tid < kTokens) {
-        const int token = t0 + tid;
-        int rank[kTensors] = {};
-        if (ADAPTERS && token < n_tokens)
-#pragma unroll
-            for (int h = 0; h < kTensors; ++h)
-                if (m[h].up)
-                    rank[h] = m[h].info[static_cast<size_t>(token) * ((m[h].max_rank + 15) / 16)].rank; // of no adapter: not used
-        ids[tid] = adapter_of(positions, token_adapters, token, n_tokens, most_adapters);
-#pragma unroll
-        for (int h = 0; h < kTensors; ++h)
-            ranks[h][tid] = rank[h];
-    }
-    float* const extra = reinterpret_cast<float*>(pool + (kFront > kSums ? kFront : kSums));
-    __syncthreads();
+    const int id = known_adapter(position, adapter, most_adapters);
+    if (tid % kThreads == 0)
+        live[my_token] = id != kNoToken;
+    f4_t acc[T][R] = {};
     if constexpr (ADAPTERS) {
-        // The adapters' part, straight to where the sums of the wavefronts meet.  A thread takes every so many outputs of one token: with
-        // few tokens of an adapter the matrix cores would compute 16 for one.
-        constexpr int kThreads = kProductWaves * 64 / kTokens, kOwn = kRows > kThreads ? kRows / kThreads : 1, kPer = kOwn / kTensors ? kOwn / kTensors : 1;
+        // The adapters' part, into the first wavefront's sums.  A thread takes every so many outputs of one token: with few tokens of an
+        // adapter the matrix cores would compute 16 for one.
+        float* const extra = reinterpret_cast<float*>(pool + kExtraAt);
+        constexpr int kOwn = kRows > kThreads ? kRows / kThreads : 1, kPer = kOwn / kTensors ? kOwn / kTensors : 1;
+        constexpr int kBoth = kOwn < kTensors ? 1 : kTensors; // tensors of a thread's outputs; a token may have as many threads as outputs
         static_assert(kOwn * kThreads >= kRows, "all outputs of a token");
-        const int token = tid / kThreads, id = ids[token];
+        const int mine = tid % kThreads;
+        AdapterPart part[kBoth];
+        int ranks[kBoth], first[kBoth], column[kBoth], most = 0; // rows first + i * kThreads of a tensor
 #pragma unroll
-        for (int h = 0; h < (kOwn < kTensors ? 1 : kTensors); ++h) {
-            // rows `first` + i * kThreads of a tensor's RT * 16; where a token has as many threads as outputs, they are one of either tensor's
-            const int of = kOwn < kTensors ? tid % kThreads / (RT * 16) : h, first = kOwn < kTensors ? tid % kThreads % (RT * 16) : tid % kThreads;
-            const AdapterPart part = of == 0 ? AdapterPart(m[0]) : AdapterPart(m[kTensors - 1]);
-            const int rank = id >= 0 && id < part.n_adapters && of < kTensors ? ranks[of][token] : 0;
-            const uint16_t* up = part.up + id * part.up_stride + static_cast<size_t>(n0 + first) * part.max_rank;
-            const f4_t* low = static_cast<const f4_t*>(part.low) + static_cast<size_t>(t0 + token) * ((part.max_rank + 15) / 16) * 4;
-            float sum[kPer] = {};
-            for (int r0 = 0; r0 < rank; r0 += 16) {
-                f4_t x[4];
-                u32x4 u[kPer][2] = {};
+        for (int h = 0; h < kBoth; ++h) {
+            const int of = kBoth < kTensors ? min(mine / (RT * 16), kTensors - 1) : h;
+            first[h] = kBoth < kTensors ? mine - of * RT * 16 : mine;
+            column[h] = of * RT * 16 + first[h];
+            part[h] = of == 0 ? AdapterPart(m[0]) : AdapterPart(m[kTensors - 1]);
+            ranks[h] = id >= 0 && id < part[h].n_adapters && first[h] < RT * 16 ? (of == 0 ? rank[0] : rank[kTensors - 1]) : 0;
+            most = max(most, ranks[h]);
+        }
+        float sum[kBoth][kPer] = {};
+        for (int r0 = 0; r0 < most; r0 += 16) {
+            f4_t x[kBoth][4] = {};
+            u32x4 u[kBoth][kPer][2] = {};
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    x[k] = low[r0 / 4 + k]; // zeros behind the rank
+            for (int h = 0; h < kBoth; ++h) {
+                const uint16_t* const up = part[h].up + id * part[h].up_stride + static_cast<size_t>(n0 + first[h]) * part[h].max_rank + r0;
+                const f4_t* const low = static_cast<const f4_t*>(part[h].low) + (static_cast<size_t>(token_at) * ((part[h].max_rank + 15) / 16) * 16 + r0) / 4;
+                if (r0 < ranks[h])
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        x[h][k] = low[k]; // zeros behind the rank
 #pragma unroll
                 for (int i = 0; i < kPer; ++i)
 #pragma unroll
                     for (int k = 0; k < 2; ++k)
-                        if (first + i * kThreads < rows && r0 + 8 * k < rank)
-                            u[i][k] = *reinterpret_cast<const u32x4*>(up + static_cast<size_t>(i) * kThreads * part.max_rank + r0 + 8 * k);
-                if (rank - r0 < 16 && (rank & 7))
+                        if (first[h] + i * kThreads < rows && r0 + 8 * k < ranks[h])
+                            u[h][i][k] = *reinterpret_cast<const u32x4*>(up + static_cast<size_t>(i) * kThreads * part[h].max_rank + 8 * k);
+            }
+#pragma unroll
+            for (int h = 0; h < kBoth; ++h) {
+                if (ranks[h] - r0 < 16 && (ranks[h] & 7))
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        const int have = rank - r0 - 2 * k;
+                        const int have = ranks[h] - r0 - 2 * k;
                         const uint32_t mask = have >= 2 ? ~0u : have == 1 ? 0xFFFFu : 0u;
 #pragma unroll
                         for (int i = 0; i < kPer; ++i)
-                            u[i][k >> 2][k & 3] &= mask;
+                            u[h][i][k >> 2][k & 3] &= mask;
                     }
 #pragma unroll
                 for (int i = 0; i < kPer; ++i)
 #pragma unroll
                     for (int k = 0; k < 16; ++k)
-                        sum[i] = __builtin_fmaf(half_bits_to_float(static_cast<uint16_t>(u[i][k >> 3][(k & 7) >> 1] >> (16 * (k & 1)))), x[k >> 2][k & 3], sum[i]);
+                        sum[h][i] = __builtin_fmaf(half_bits_to_float(static_cast<uint16_t>(u[h][i][k >> 3][(k & 7) >> 1] >> (16 * (k & 1)))),
+                                                   x[h][k >> 2][k & 3], sum[h][i]);
             }
-            if (rank > 0)
-#pragma unroll
-                for (int i = 0; i < kPer; ++i)
-                    if (first + i * kThreads < RT * 16)
-                        extra[token * kStride + of * RT * 16 + first + i * kThreads] = sum[i];
         }
+#pragma unroll
+        for (int h = 0; h < kBoth; ++h)
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (first[h] + i * kThreads < RT * 16)
+                    extra[my_token * kStride + column[h] + i * kThreads] = sum[h][i];
+        __syncthreads();
+        if (wave == 0)
+#pragma unroll
+            for (int i = 0; i < T; ++i)
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[i][r][e] = extra[(i * 16 + 4 * c + e) * kStride + r * 16 + l15];
+    } else {
+        __syncthreads();
     }
 
-    f4_t acc[T][R] = {};
-    for (int g0 = wave; g0 < groups; g0 += kProductWaves * D) {
+    for (int g0 = wave; g0 < groups; g0 += W * D) {
 #pragma unroll
         for (int d = 0; d < D; ++d) { // groups that do not exist are zeros
-            const int g = g0 + d * kProductWaves, gs = min(g, groups - 1);
+            const int g = g0 + d * W, gs = min(g, groups - 1);
             h8_t wf[R][4];
             float sc[R];
 #pragma unroll
@@ -454,7 +474,7 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
                     wf[r][j] = weights_of(v[j], minus);
             }
             __builtin_amdgcn_sched_barrier(0);
-            load_w(d, g + kProductWaves * D);
+            load_w(d, g + W * D);
 #pragma unroll
             for (int i = 0; i < T; ++i) {
                 const int q = (d * T + i) % kRing, next = d * T + i + kRing; // the tile that comes into this place
@@ -466,7 +486,7 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
                 } else {
                     put_tile(lds, xt[q]);
                     __builtin_amdgcn_sched_barrier(0);
-                    load_x(q, next % T, g0 + next / T * kProductWaves);
+                    load_x(q, next % T, g0 + next / T * W);
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         xf[j] = tile_operand(lds, j);
@@ -479,7 +499,7 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
                         p[r] = mfma16(xf[j], wf[r][j], p[r]);
                 if constexpr (PACKED) {
                     __builtin_amdgcn_sched_barrier(0);
-                    load_x(q, next % T, g0 + next / T * kProductWaves);
+                    load_x(q, next % T, g0 + next / T * W);
                 }
 #pragma unroll
                 for (int r = 0; r < R; ++r)
@@ -500,31 +520,25 @@ __global__ __launch_bounds__(kProductWaves * 64) void batch_product_kernel(Produ
                 red[(wave * kTokens + i * 16 + 4 * c + e) * kStride + r * 16 + l15] = acc[i][r][e];
     __syncthreads();
     constexpr int kPieces = RT * 2; // of 8 outputs
-    for (int i = tid; i < kTokens * kPieces; i += kProductWaves * 64) {
-        const int token = i / kPieces, piece = i % kPieces * 8, n = n0 + piece, id = ids[token];
-        if (id == kNoToken || n >= cols)
+    for (int i = tid; i < kTokens * kPieces; i += W * 64) {
+        const int token = i / kPieces, piece = i % kPieces * 8, n = n0 + piece;
+        if (!live[token] || n >= cols)
             continue;
         u32x4 residual = {};
         if (!GATED && residual_rows)
             residual = *reinterpret_cast<const u32x4*>(residual_rows + static_cast<size_t>(t0 + token) * residual_stride + n);
         float v[kTensors][8] = {};
 #pragma unroll
-        for (int h = 0; h < kTensors; ++h) {
-            auto add = [&](const float* from) {
+        for (int h = 0; h < kTensors; ++h)
+#pragma unroll
+            for (int q = 0; q < W; ++q)
 #pragma unroll
                 for (int k = 0; k < 8; k += 4) {
-                    const f4_t y = *reinterpret_cast<const f4_t*>(from + token * kStride + h * RT * 16 + piece + k);
+                    const f4_t y = *reinterpret_cast<const f4_t*>(red + (q * kTokens + token) * kStride + h * RT * 16 + piece + k);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         v[h][k + e] += y[e];
                 }
-            };
-#pragma unroll
-            for (int q = 0; q < kProductWaves; ++q)
-                add(red + q * kTokens * kStride);
-            if (ADAPTERS && id >= 0 && id < m[h].n_adapters && ranks[h][token] > 0)
-                add(extra);
-        }
         u32x4 o;
         if constexpr (GATED) {
 #pragma unroll
@@ -550,28 +564,24 @@ struct Product { // a call of either entry point
     bool adapters;
 };
 
-template <int R, int T, int D, bool GATED>
+template <int W, int R, int T, int D, bool GATED>
 static void launch_product(Product& p)
 {
-    constexpr int kRows = GATED ? R * 8 : R * 16;
     ProductArgs& a = p.a;
-    a.row_blocks = 0;
-    for (int i = 0; i < LLAMA2_MAX_BATCH_MATRICES; ++i) {
-        a.first[i] = i < (GATED ? 1 : p.n_matrices) ? a.row_blocks : 0x7FFFFFFF;
-        if (i < (GATED ? 1 : p.n_matrices))
-            a.row_blocks += ceil_div(a.t[i].cols, kRows);
-    }
+    int cols = 0;
+    for (int i = 0; i < p.n_matrices; ++i)
+        cols = a.t[i].cols > cols ? a.t[i].cols : cols;
     a.token_blocks = ceil_div(a.n_tokens, T * 16);
-    const dim3 grid(static_cast<unsigned>(ceil_div(a.row_blocks, 8)) * 8 * a.token_blocks), block(kProductWaves * 64);
+    const dim3 grid(static_cast<unsigned>(round_up(ceil_div(cols, GATED ? R * 8 : R * 16), 8)) * a.token_blocks, GATED ? 1 : p.n_matrices), block(W * 64);
     if (p.adapters)
-        hipLaunchKernelGGL((batch_product_kernel<R, T, D, GATED, true>), grid, block, 0, ctx().stream, a);
+        hipLaunchKernelGGL((batch_product_kernel<W, R, T, D, GATED, true>), grid, block, 0, ctx().stream, a);
     else
-        hipLaunchKernelGGL((batch_product_kernel<R, T, D, GATED, false>), grid, block, 0, ctx().stream, a);
+        hipLaunchKernelGGL((batch_product_kernel<W, R, T, D, GATED, false>), grid, block, 0, ctx().stream, a);
 }
 
 // Rows of more than 32768 inputs: tiles so low that their scales fit.
-static void launch_tall(Product& p, std::false_type) { launch_product<1, 1, 2, false>(p); }
-static void launch_tall(Product& p, std::true_type) { launch_product<2, 1, 2, true>(p); }
+static void launch_tall(Product& p, std::false_type) { launch_product<8, 1, 1, 2, false>(p); }
+static void launch_tall(Product& p, std::true_type) { launch_product<8, 2, 1, 2, true>(p); }
 
 constexpr int kWideTokens = 64; // more go through the kernels of the prompt's products
 constexpr int kMostTokens = 4096; // of a launch
@@ -649,12 +659,27 @@ static int run_product(const char* fn, Product& p)
                 return rc;
         } else {
             // scales and zero points of a workgroup's rows: R * groups <= 512
-            if (a.n_tokens <= 16)
-                groups <= 256 ? launch_product<2, 1, 2, GATED>(p) : launch_tall(p, std::integral_constant<bool, GATED>());
-            else if (a.n_tokens <= 32)
-                groups <= 256 ? launch_product<2, 2, 2, GATED>(p) : launch_tall(p, std::integral_constant<bool, GATED>());
-            else
-                groups <= 128 ? launch_product<4, 4, 1, GATED>(p) : launch_tall(p, std::integral_constant<bool, GATED>());
+            const int shape = getenv("L2_SHAPE") ? atoi(getenv("L2_SHAPE")) : 0; // XXX
+            if (a.n_tokens <= 16) {
+                if (shape == 1) GATED ? launch_product<4, 2, 1, 2, GATED>(p) : launch_product<8, GATED ? 2 : 1, 1, 2, GATED>(p);
+                else if (shape == 2) launch_product<8, 4, 1, 1, GATED>(p);
+                else if (shape == 3) launch_product<4, 4, 1, 1, GATED>(p);
+                else if (shape == 4) launch_product<4, 2, 1, 2, GATED>(p);
+                else if (shape == 5) launch_product<16, 2, 1, 1, GATED>(p);
+                else launch_product<8, 2, 1, 2, GATED>(p);
+            } else if (a.n_tokens <= 32) {
+                if (shape == 1) launch_product<8, GATED ? 2 : 1, 2, 2, GATED>(p);
+                else if (shape == 2) launch_product<4, 2, 2, 2, GATED>(p);
+                else if (shape == 3) launch_product<4, 4, 2, 1, GATED>(p);
+                else if (shape == 4) launch_product<8, 4, 2, 1, GATED>(p);
+                else launch_product<8, 2, 2, 2, GATED>(p);
+            } else {
+                if (shape == 1) launch_product<4, 4, 4, 1, GATED>(p);
+                else if (shape == 2) launch_product<8, 2, 4, 1, GATED>(p);
+                else if (shape == 3) launch_product<4, 2, 4, 1, GATED>(p);
+                else if (shape == 4) GATED ? launch_product<4, 2, 4, 1, GATED>(p) : launch_product<8, GATED ? 2 : 3, 4, 1, GATED>(p);
+                else launch_product<8, 4, 4, 1, GATED>(p);
+            }
             L2_LAUNCH_CHECK(fn);
         }
         a.x = rows + static_cast<size_t>(a.n_tokens) * a.x_stride;

@@ -13,7 +13,7 @@ constexpr int kMaxStride = 1 << 24; // of the input: offsets within 64 rows are 
 constexpr int kMaxAdapters = 1 << 20;
 constexpr int kMaxRank = 128;
 constexpr int kMaxNormSize = 1 << 16;
-constexpr int kMaxVocab = 1 << 24;
+constexpr int kMaxVocab = 1 << 20; // 32 segments of 32768
 constexpr int kMaxGiven = 1024;
 
 inline int weight_words(int rows) { return ceil_div(rows, 32) * 4; } // of an output
@@ -251,6 +251,29 @@ inline int check_batch_log_probs(const float* log_probs, const float* entropies,
             L2_CHECK(!written[i].bytes || !x.bytes || !overlap(written[i].p, written[i].bytes, x.p, x.bytes), "%s: an output overlaps an input", fn);
     }
     return LLAMA2_OK;
+}
+
+// ---------------------------------------------------------------- how rows of logits are cut
+constexpr int kLogProbRows = 1 << 15; // of a launch
+
+struct LogProbShape {
+    int segments, length, pieces; // length: of a segment; pieces: of 4096 logits that it takes at most, 1, 2, 4 or 8
+};
+
+// A workgroup holds up to 32768 logits.  Few rows are cut until there are as many workgroups as compute units, into pieces of 4096 at
+// least; the likeliest of all segments are ranked by comparison with each other, 512 of them while there is a choice.
+inline LogProbShape log_prob_shape(int rows, int vocab, int n_top, int cus)
+{
+    const int least = ceil_div(vocab, 1 << 15), most = ceil_div(vocab, 1 << 12);
+    int n = cus / rows < most ? cus / rows : most;
+    n = n_top > 0 && n > 512 / n_top ? 512 / n_top : n;
+    n = n > least ? n : least;
+    LogProbShape s;
+    s.length = round_up(ceil_div(vocab, n), 8);
+    s.segments = ceil_div(vocab, s.length);
+    const int pieces = ceil_div(s.length, 1 << 12);
+    s.pieces = pieces <= 2 ? pieces : pieces <= 4 ? 4 : 8;
+    return s;
 }
 
 } // namespace l2

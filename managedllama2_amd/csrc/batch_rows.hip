@@ -23,21 +23,6 @@ __device__ __forceinline__ float block_sum(float v, float* lds /* WAVES */)
     return t;
 }
 
-template <int WAVES>
-__device__ __forceinline__ float block_max(float v, float* lds)
-{
-    v = wave_max(v);
-    if ((threadIdx.x & 63) == 0)
-        lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float t = lds[0];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w)
-        t = fmaxf(t, lds[w]);
-    __syncthreads();
-    return t;
-}
-
 // ---------------------------------------------------------------- residual and norms
 struct NormRowsArgs {
     uint16_t* output;
@@ -157,7 +142,9 @@ struct LogProbArgs {
     const uint16_t* logits;
     const int* tokens;
     const int* positions;
-    int vocab, stride, n_tokens, n_top;
+    float* parts;       // several segments: [row][segment] of 4 floats (largest, sum, moment), then [row][segment][n_top] keys
+    unsigned* counters; // per row, zero between launches
+    int vocab, stride, n_tokens, n_top, segments, length; // length: of a segment, a multiple of 8
     float inverse, per_e; // 1 / temperature, and with log2(e)
 };
 
@@ -168,153 +155,317 @@ __device__ __forceinline__ unsigned order_of(uint16_t h)
         return 0;
     if (h == 0x8000u)
         h = 0;
-    return h & 0x8000u ? 0xFFFFu ^ h : h | 0x8000u; // -infinity: 0x03FF
+    return h & 0x8000u ? 0xFFFFu ^ h : h | 0x8000u;
+}
+constexpr unsigned kOrderOfNothing = 0x03FF; // -infinity
+
+__device__ __forceinline__ float logit_of(unsigned order)
+{
+    return order == 0 ? NAN : half_bits_to_float(static_cast<uint16_t>(order & 0x8000u ? order & 0x7FFFu : 0xFFFFu ^ order));
 }
 
-constexpr int kLogProbThreads = 1024, kCandidates = 2048;
+// Likelier first, equal ones by index.
+__device__ __forceinline__ unsigned long long key_of(unsigned order, int i) { return static_cast<unsigned long long>(order) << 32 | (0xFFFFFFFFu - i); }
 
-// A workgroup per row.  Its threads' largest logits bound the n_top-th largest from below (the n_top-th of 1024 maxima); what
-// reaches that bound is collected and ranked by comparison.  Where more than kCandidates do (rows of equal logits), the bound is
-// found bit by bit, and of the equal ones the first by their index are taken.
-__global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogProbArgs a)
+__device__ __forceinline__ uint16_t element(const u32x4& v, int k) { return static_cast<uint16_t>(v[k >> 1] >> (16 * (k & 1))); }
+
+struct __attribute__((packed, aligned(2))) AnyHalfs { // 16 bytes of halfs
+    u32x4 v;
+};
+
+constexpr int kLogProbWaves = 8, kLogProbThreads = kLogProbWaves * 64, kCandidates = 2048, kQuads = kLogProbThreads / 4;
+constexpr int kLongestSegment = 8 * 8 * kLogProbThreads;
+
+struct LogProbLds {
+    float sums[2][kLogProbWaves], largest[kLogProbWaves];
+    unsigned quads[kQuads];
+    unsigned long long found[kCandidates];
+    int count, bound, scan[kLogProbWaves];
+    unsigned arrived;
+};
+
+// Largest, sum and moment of a segment, or of all of them.
+struct LogProbSums {
+    float top, total, moment; // sum of e = exp((x - top) / T), and of e (x - top)
+};
+
+// What a row answers: by all threads, from its sums and its likeliest tokens in `found` (`have` of them, in any order).
+__device__ __forceinline__ void answer_row(const LogProbArgs& a, int row, const LogProbSums& s, const unsigned long long* found, int have)
 {
-    constexpr int WAVES = kLogProbThreads / 64;
-    __shared__ float lds[WAVES];
-    __shared__ unsigned maxima[kLogProbThreads];
-    __shared__ unsigned long long found[kCandidates];
-    __shared__ int count, bound;
-    const int row = blockIdx.x, tid = threadIdx.x;
-    if (a.positions && a.positions[row] < 0)
-        return;
-    const uint16_t* x = a.logits + static_cast<size_t>(row) * a.stride;
-    float top = -INFINITY;
-    unsigned largest = 0;
-    bool nan = false;
-    for (int i = tid; i < a.vocab; i += kLogProbThreads) {
-        const float v = half_bits_to_float(x[i]);
-        nan = nan || v != v;
-        top = fmaxf(top, v);
-        largest = max(largest, order_of(x[i]));
-    }
-    top = block_max<WAVES>(top, lds);
-    float total = 0.0f, moment = 0.0f;
-    if (top > -INFINITY && top < INFINITY) {
-        for (int i = tid; i < a.vocab; i += kLogProbThreads) {
-            const float d = half_bits_to_float(x[i]) - top;
-            const float e = __builtin_amdgcn_exp2f(d * a.per_e);
-            total += e;
-            moment = e > 0.0f ? __builtin_fmaf(e, d, moment) : moment;
-        }
-    }
-    total = block_sum<WAVES>(total, lds);
-    moment = block_sum<WAVES>(moment, lds);
-    const bool wrong = __syncthreads_or(nan) || top == INFINITY;
-    const float log_total = logf(total);
-    auto log_prob = [&](float v) {
-        return wrong ? NAN : v == -INFINITY ? -INFINITY : (v - top) * a.inverse - log_total;
-    };
+    const uint16_t* const x = a.logits + static_cast<size_t>(row) * a.stride;
+    const bool wrong = s.top == INFINITY || s.total != s.total;
+    const float log_total = logf(s.total);
+    auto log_prob = [&](float v) { return wrong ? NAN : v == -INFINITY ? -INFINITY : (v - s.top) * a.inverse - log_total; };
     if (a.log_probs)
-        for (int i = tid; i < a.n_tokens; i += kLogProbThreads) {
+        for (int i = threadIdx.x; i < a.n_tokens; i += kLogProbThreads) {
             const int token = a.tokens[static_cast<size_t>(row) * a.n_tokens + i];
             const bool there = token >= 0 && token < a.vocab;
             a.log_probs[static_cast<size_t>(row) * a.n_tokens + i] = there ? log_prob(half_bits_to_float(x[token])) : -INFINITY;
         }
-    if (a.entropies && tid == 0)
-        a.entropies[row] = wrong ? NAN : top == -INFINITY ? 0.0f : log_total - moment * a.inverse / total;
-    if (a.n_top == 0)
-        return;
-    // the n_top-th largest of the threads' maxima (threads without a logit have 0, which bounds everything)
-    const int want = min(a.n_top, a.vocab);
-    maxima[tid] = largest;
-    if (tid == 0)
-        count = 0;
-    __syncthreads();
-    int above = 0;
-    for (int j = 0; j < kLogProbThreads; ++j) {
-        const unsigned o = maxima[j];
-        above += o > largest || (o == largest && j < tid);
-    }
-    if (above == want - 1)
-        bound = static_cast<int>(largest);
-    __syncthreads();
-    unsigned least = static_cast<unsigned>(bound);
-    auto key = [&](unsigned order, int i) { return static_cast<unsigned long long>(order) << 32 | (0xFFFFFFFFu - i); };
-    for (int i = tid; i < a.vocab; i += kLogProbThreads) {
-        const unsigned o = order_of(x[i]);
-        if (o >= least) {
-            const int at = atomicAdd(&count, 1);
-            if (at < kCandidates)
-                found[at] = key(o, i);
-        }
-    }
-    __syncthreads();
-    int have = count;
-    if (have > kCandidates) { // uniform
-        // the largest bound that `want` logits reach, bit by bit
-        unsigned reach = 0;
-        for (int bit = 15; bit >= 0; --bit) {
-            const unsigned probe = reach | 1u << bit;
-            int n = 0;
-            for (int i = tid; i < a.vocab; i += kLogProbThreads)
-                n += order_of(x[i]) >= probe;
-            __syncthreads();
-            if (tid == 0)
-                count = 0;
-            __syncthreads();
-            if (n)
-                atomicAdd(&count, n);
-            __syncthreads();
-            if (count >= want)
-                reach = probe;
-        }
-        __syncthreads();
-        if (tid == 0)
-            count = 0;
-        __syncthreads();
-        for (int i = tid; i < a.vocab; i += kLogProbThreads) {
-            const unsigned o = order_of(x[i]);
-            if (o > reach)
-                found[atomicAdd(&count, 1)] = key(o, i); // fewer than `want`
-        }
-        __syncthreads();
-        // the equal ones in order, a thousand at a time
-        for (int first = 0; first < a.vocab; first += kLogProbThreads) {
-            const int before = count;
-            if (before >= want)
-                break;
-            const bool equal = first + tid < a.vocab && order_of(x[first + tid]) == reach;
-            maxima[tid] = equal;
-            __syncthreads();
-            if (equal) {
-                int at = before;
-                for (int j = 0; j < tid; ++j)
-                    at += maxima[j];
-                if (at < want)
-                    found[at] = key(reach, first + tid);
-            }
-            const int n = __syncthreads_count(equal);
-            if (tid == 0)
-                count = min(before + n, want);
-            __syncthreads();
-        }
-        have = want;
-    }
-    for (int i = tid; i < have; i += kLogProbThreads) {
+    if (a.entropies && threadIdx.x == 0)
+        a.entropies[row] = wrong ? NAN : s.top == -INFINITY ? 0.0f : log_total - s.moment * a.inverse / s.total;
+    for (int i = threadIdx.x; i < have; i += kLogProbThreads) {
+        const unsigned long long key = found[i];
         int rank = 0;
         for (int j = 0; j < have; ++j)
-            rank += found[j] > found[i];
+            rank += found[j] > key;
         if (rank >= a.n_top)
             continue;
-        const int token = static_cast<int>(0xFFFFFFFFu - static_cast<unsigned>(found[i]));
-        a.top_tokens[static_cast<size_t>(row) * a.n_top + rank] = token;
+        a.top_tokens[static_cast<size_t>(row) * a.n_top + rank] = static_cast<int>(0xFFFFFFFFu - static_cast<unsigned>(key));
         if (a.top_log_probs)
-            a.top_log_probs[static_cast<size_t>(row) * a.n_top + rank] = log_prob(half_bits_to_float(x[token]));
+            a.top_log_probs[static_cast<size_t>(row) * a.n_top + rank] = log_prob(logit_of(static_cast<unsigned>(key >> 32)));
     }
-    for (int i = want + tid; i < a.n_top; i += kLogProbThreads) {
+    for (int i = a.vocab + threadIdx.x; i < a.n_top; i += kLogProbThreads) { // more asked for than there are
         a.top_tokens[static_cast<size_t>(row) * a.n_top + i] = -1;
         if (a.top_log_probs)
             a.top_log_probs[static_cast<size_t>(row) * a.n_top + i] = -INFINITY;
     }
+}
+
+// Eight logits of a segment from index i on, -infinity behind its end.
+__device__ __forceinline__ u32x4 load_logits(const uint16_t* row, int i, int end)
+{
+    u32x4 v = {0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u};
+    if (i + 8 <= end)
+        return reinterpret_cast<const AnyHalfs*>(row + i)->v;
+    for (int k = 0; k < end - i; ++k) {
+        const uint32_t h = row[i + k];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e == k >> 1)
+                v[e] = k & 1 ? (v[e] & 0xFFFFu) | h << 16 : (v[e] & 0xFFFF0000u) | h;
+    }
+    return v;
+}
+
+// Those of eight logits that are of order `least` at least, with what is there already; the count goes on behind what fits.
+__device__ __forceinline__ void collect(LogProbLds& lds, const u32x4& v, unsigned least, int i, int end)
+{
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const unsigned o = order_of(element(v, k));
+        if (o >= least && i + k < end) {
+            const int at = atomicAdd(&lds.count, 1);
+            if (at < kCandidates)
+                lds.found[at] = key_of(o, i + k);
+        }
+    }
+}
+
+// The likeliest `want` of a segment into lds.found where the bound does not find them: the want-th largest order bit by bit (`reach`, or
+// 0xFFFF: to be found), then what lies above it, then of those equal to it the first by their index.  Returns how many were found.  Reads the
+// segment again for each of these: rows of many equal logits, or with NaN.
+__device__ __noinline__ int likeliest_one_by_one(LogProbLds& lds, const uint16_t* row, int begin, int end, int want, unsigned reach)
+{
+    const int tid = threadIdx.x;
+    auto count = [&](unsigned least) {
+        __syncthreads();
+        if (tid == 0)
+            lds.count = 0;
+        __syncthreads();
+        int n = 0;
+        for (int i = begin + tid * 8; i < end; i += kLogProbThreads * 8) {
+            const u32x4 v = load_logits(row, i, end);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                n += order_of(element(v, k)) >= least && i + k < end;
+        }
+        if (n)
+            atomicAdd(&lds.count, n);
+        __syncthreads();
+        return lds.count;
+    };
+    if (reach == 0xFFFF || count(reach + 1) > kCandidates || count(reach) < want) {
+        reach = 0;
+        for (int bit = 15; bit >= 0; --bit)
+            if (count(reach | 1u << bit) >= want)
+                reach |= 1u << bit;
+    }
+    __syncthreads();
+    if (tid == 0)
+        lds.count = 0;
+    __syncthreads();
+    for (int i = begin + tid * 8; i < end; i += kLogProbThreads * 8)
+        collect(lds, load_logits(row, i, end), reach + 1, i, end);
+    __syncthreads();
+    int have = min(lds.count, kCandidates);
+    for (int first = begin; first < end && have < want; first += kLogProbThreads * 8) {
+        const int i = first + tid * 8, lane = tid & 63;
+        const u32x4 v = load_logits(row, i, end);
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            n += order_of(element(v, k)) == reach && i + k < end;
+        int upto = n;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(upto, d, 64);
+            upto = lane >= d ? upto + o : upto;
+        }
+        __syncthreads();
+        if (lane == 63)
+            lds.scan[tid >> 6] = upto;
+        __syncthreads();
+        int at = have + upto - n, all = 0;
+        for (int w = 0; w < kLogProbWaves; ++w) {
+            at += w < (tid >> 6) ? lds.scan[w] : 0;
+            all += lds.scan[w];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (order_of(element(v, k)) == reach && i + k < end) {
+                if (at < want)
+                    lds.found[at] = key_of(reach, i + k);
+                ++at;
+            }
+        have = min(have + all, want);
+    }
+    __syncthreads();
+    return have;
+}
+
+// A workgroup per segment of a row, which stays in registers.  One reading, packed maxima, one exponential per logit; with few
+// rows a row is cut into segments, which the last one to arrive puts together.
+template <int PIECES>
+__global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogProbArgs a)
+{
+    __shared__ LogProbLds lds;
+    const int row = blockIdx.y, segment = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (a.positions && a.positions[row] < 0)
+        return;
+    const int begin = segment * a.length, end = min(begin + a.length, a.vocab);
+    const uint16_t* const row_at = a.logits + static_cast<size_t>(row) * a.stride;
+    u32x4 x[PIECES];
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int i = begin + (p * kLogProbThreads + tid) * 8;
+        x[p] = load_logits(row_at, i, end);
+    }
+    h2_t m2 = as_h2(0xFC00FC00u);
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p)
+        m2 = max_h2(m2, max_h2(max_h2(as_h2(x[p][0]), as_h2(x[p][1])), max_h2(as_h2(x[p][2]), as_h2(x[p][3]))));
+    const float most = fmaxf(static_cast<float>(m2[0]), static_cast<float>(m2[1]));
+    float quad = fmaxf(most, dpp_f32<DPP_QUAD_XOR1>(most));
+    quad = fmaxf(quad, dpp_f32<DPP_QUAD_XOR2>(quad));
+    if ((lane & 3) == 0)
+        lds.quads[tid >> 2] = order_of(float_to_half_bits(quad));
+    const float of_wave = wave_max(most);
+    if (lane == 0)
+        lds.largest[wave] = of_wave;
+    if (tid == 0)
+        lds.count = 0;
+    __syncthreads();
+    LogProbSums s = {lds.largest[0], 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 1; w < kLogProbWaves; ++w)
+        s.top = fmaxf(s.top, lds.largest[w]);
+    const int want = min(a.n_top, end - begin);
+    if (wave == 0 && want > 0) { // the want-th largest of the quads
+        const unsigned q0 = lds.quads[lane], q1 = lds.quads[lane + 64];
+        unsigned bound = 0;
+#pragma unroll
+        for (int bit = 15; bit >= 0; --bit) {
+            const unsigned probe = bound | 1u << bit;
+            if (__builtin_popcountll(__ballot(q0 >= probe)) + __builtin_popcountll(__ballot(q1 >= probe)) >= want)
+                bound = probe;
+        }
+        if (lane == 0)
+            lds.bound = static_cast<int>(bound);
+    }
+    // of a row that holds nothing above -infinity, nothing; NaN makes its way into the sum
+    const float base = s.top == -INFINITY ? 0.0f : s.top;
+    float total[2] = {}, moment[2] = {};
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float d = half_bits_to_float(element(x[p], k)) - base;
+            const float e = __builtin_amdgcn_exp2f(d * a.per_e);
+            total[k & 1] += e;
+            moment[k & 1] = __builtin_fmaf(e, fmaxf(d, -3.0e38f), moment[k & 1]);
+        }
+    const float t = wave_sum(total[0] + total[1]), m = wave_sum(moment[0] + moment[1]);
+    if (lane == 0) {
+        lds.sums[0][wave] = t;
+        lds.sums[1][wave] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kLogProbWaves; ++w) {
+        s.total += lds.sums[0][w];
+        s.moment += lds.sums[1][w];
+    }
+    int have = 0;
+    if (want > 0) {
+        // The largest of every four threads bound the want-th largest from below (lds.bound, the want-th of these 128), and what reaches
+        // that bound is collected.  Where that is nothing but -infinity, too much (many equal logits) or too little (NaN, which the
+        // maxima leave out), in another way.
+        const unsigned bound = static_cast<unsigned>(lds.bound);
+        if (bound > kOrderOfNothing && order_of(float_to_half_bits(most)) >= bound)
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) {
+                const h2_t m8 = max_h2(max_h2(as_h2(x[p][0]), as_h2(x[p][1])), max_h2(as_h2(x[p][2]), as_h2(x[p][3])));
+                if (order_of(float_to_half_bits(fmaxf(static_cast<float>(m8[0]), static_cast<float>(m8[1])))) >= bound)
+                    collect(lds, x[p], bound, begin + (p * kLogProbThreads + tid) * 8, end);
+            }
+        __syncthreads();
+        have = lds.count;
+        if (have < want || have > kCandidates)
+            have = likeliest_one_by_one(lds, row_at, begin, end, want, bound > kOrderOfNothing ? 0xFFFFu : kOrderOfNothing);
+    }
+    if (a.segments == 1) {
+        answer_row(a, row, s, lds.found, have);
+        return;
+    }
+    // Several segments: sums and the likeliest of each go through memory that every XCD sees.
+    const size_t at = static_cast<size_t>(row) * a.segments;
+    float* const sums = a.parts + at * 4;
+    unsigned* const keys = reinterpret_cast<unsigned*>(a.parts + static_cast<size_t>(gridDim.y) * a.segments * 4) + at * a.n_top * 2;
+    if (tid == 0) {
+        store_agent(sums + segment * 4, s.top);
+        store_agent(sums + segment * 4 + 1, s.total);
+        store_agent(sums + segment * 4 + 2, s.moment);
+    }
+    auto put = [&](int rank, unsigned long long key) {
+        store_agent(keys + (static_cast<size_t>(segment) * a.n_top + rank) * 2, static_cast<unsigned>(key));
+        store_agent(keys + (static_cast<size_t>(segment) * a.n_top + rank) * 2 + 1, static_cast<unsigned>(key >> 32));
+    };
+    for (int i = tid; i < have; i += kLogProbThreads) {
+        const unsigned long long key = lds.found[i];
+        int rank = 0;
+        for (int j = 0; j < have; ++j)
+            rank += lds.found[j] > key;
+        if (rank < a.n_top)
+            put(rank, key);
+    }
+    for (int i = want + tid; i < a.n_top; i += kLogProbThreads) // a segment shorter than that
+        put(i, 0);
+    wait_agent_stores();
+    __syncthreads();
+    if (tid == 0)
+        lds.arrived = add_agent(a.counters + row, 1);
+    __syncthreads();
+    if (lds.arrived + 1 != static_cast<unsigned>(a.segments))
+        return;
+    if (tid == 0)
+        store_agent(a.counters + row, 0u);
+    // A lane per segment (up to 32), and a thread per key.
+    LogProbSums own = {-INFINITY, 0.0f, 0.0f};
+    if (lane < a.segments)
+        own = {load_agent(sums + lane * 4), load_agent(sums + lane * 4 + 1), load_agent(sums + lane * 4 + 2)};
+    const int n = a.segments * a.n_top;
+    for (int i = tid; i < n; i += kLogProbThreads) {
+        const unsigned lo = load_agent(keys + i * 2), hi = load_agent(keys + i * 2 + 1);
+        lds.found[i] = static_cast<unsigned long long>(hi) << 32 | lo;
+    }
+    LogProbSums all = {wave_max(own.top), 0.0f, 0.0f};
+    const float d = own.top - all.top, w = __builtin_amdgcn_exp2f(d * a.per_e);
+    const bool nothing = own.top == -INFINITY; // but NaN, perhaps
+    all.total = wave_sum(nothing ? own.total * 0.0f : own.total * w);
+    all.moment = wave_sum(nothing ? 0.0f : w * __builtin_fmaf(own.total, d, own.moment));
+    __syncthreads();
+    answer_row(a, row, all, lds.found, n);
 }
 
 } // namespace l2
@@ -357,10 +508,35 @@ int llama2_batch_log_probs(float* log_probs, float* entropies, int* top_tokens, 
                                        logits_stride, n_tokens, n_top, temperature))
         return rc;
     const double inverse = 1.0 / static_cast<double>(temperature);
-    const LogProbArgs a = {log_probs, entropies, top_tokens, top_log_probs, logits, tokens, positions, vocab_size, logits_stride, n_tokens,
-                           n_top, static_cast<float>(inverse), static_cast<float>(inverse * 1.4426950408889634)};
-    hipLaunchKernelGGL(batch_log_probs_kernel, dim3(n_rows), dim3(kLogProbThreads), 0, ctx().stream, a);
-    L2_LAUNCH_CHECK("llama2_batch_log_probs");
+    LogProbArgs a = {log_probs, entropies, top_tokens, top_log_probs, logits, tokens, positions, nullptr, ctx().batch_counters, vocab_size,
+                     logits_stride, n_tokens, n_top, 1, vocab_size, static_cast<float>(inverse), static_cast<float>(inverse * 1.4426950408889634)};
+    const LogProbShape shape = log_prob_shape(n_rows, vocab_size, n_top, ctx().num_cus);
+    a.segments = shape.segments;
+    a.length = shape.length;
+    for (int done = 0; done < n_rows; done += kLogProbRows) {
+        const int rows = n_rows - done < kLogProbRows ? n_rows - done : kLogProbRows;
+        if (a.segments > 1) {
+            const size_t parts = static_cast<size_t>(rows) * a.segments;
+            if (int rc = ensure_attn_partials(parts * (16 + 8 * static_cast<size_t>(n_top))))
+                return rc;
+            a.parts = ctx().attn_partials;
+        }
+        const dim3 grid(a.segments, rows), block(kLogProbThreads);
+        switch (shape.pieces) {
+        case 1: hipLaunchKernelGGL(batch_log_probs_kernel<1>, grid, block, 0, ctx().stream, a); break;
+        case 2: hipLaunchKernelGGL(batch_log_probs_kernel<2>, grid, block, 0, ctx().stream, a); break;
+        case 4: hipLaunchKernelGGL(batch_log_probs_kernel<4>, grid, block, 0, ctx().stream, a); break;
+        default: hipLaunchKernelGGL(batch_log_probs_kernel<8>, grid, block, 0, ctx().stream, a); break;
+        }
+        L2_LAUNCH_CHECK("llama2_batch_log_probs");
+        a.logits += static_cast<size_t>(rows) * logits_stride;
+        a.positions += positions ? rows : 0;
+        a.tokens += tokens ? static_cast<size_t>(rows) * n_tokens : 0;
+        a.log_probs += log_probs ? static_cast<size_t>(rows) * n_tokens : 0;
+        a.entropies += entropies ? rows : 0;
+        a.top_tokens += top_tokens ? static_cast<size_t>(rows) * n_top : 0;
+        a.top_log_probs += top_log_probs ? static_cast<size_t>(rows) * n_top : 0;
+    }
     return LLAMA2_OK;
 }
 

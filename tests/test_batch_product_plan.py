@@ -195,7 +195,7 @@ def test_log_probabilities(lib):
                 dict(top=20 * MIB + 64), dict(tlp=30 * MIB), dict(h=31 * MIB)):
         assert call(**bad) == INVALID, (bad, lib.last())
         assert b"llama2_batch_log_probs" in lib.last()
-    assert call(vocab=(1 << 24) + 1, stride=(1 << 24) + 1) == UNSUPPORTED
+    assert call(vocab=(1 << 20) + 1, stride=(1 << 20) + 1) == UNSUPPORTED
 
 
 def test_calls_before_init_are_refused():

@@ -226,6 +226,39 @@ def test_masked_logits(vocab):
     lp_check(x, tokens, 64, 0.1)
 
 
+@pytest.mark.parametrize("vocab", [3, 64, 700, 4097, 32000, 45000])
+def test_few_or_many_logits_beside_masked_and_nan(vocab):
+    """Every number of logits that are left, with NaN among them: the likeliest tokens are found in other ways then."""
+    g = rng(14, vocab)
+    rows = 12
+    x = np.full((rows, vocab), -np.inf, np.float16)
+    for r in range(rows):
+        left = [0, 1, 2, 5, 63, 64, 65, 200, 2047, 2049, 6000, vocab][r]
+        at = g.permutation(vocab)[:left] if r % 2 else np.arange(min(left, vocab)) * 4 % vocab  # spread, or in few places
+        x[r, at] = g.integers(-3, 3, len(at))
+    tokens = g.integers(0, vocab, (rows, 2)).astype(np.int32)
+    lp_check(x, tokens, 64)
+    lp_check(x, tokens, 5)
+    x[::2, g.random(vocab) < 0.5] = np.nan
+    x[1::2, :-2] = np.where(g.random(vocab - 2) < 0.999, np.nan, x[1::2, :-2]) if vocab > 2 else np.nan
+    lp_check(x, tokens, 64)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 30, 130, 300])
+def test_segments_of_rows(rows):
+    """Rows in as many segments as there are compute units for, or in those that they need."""
+    g = rng(15, rows)
+    for vocab in (4100, 32000, 70001):
+        x = logits(g, rows, vocab)
+        x[0, vocab // 2:] = -np.inf  # whole segments of nothing
+        if rows > 2:
+            x[1, -1] = np.nan
+            x[2, 100] = np.inf
+        pos = np.where(np.arange(rows) % 5 == 3, -1, 1).astype(np.int32)
+        for n_top in (1, 64):
+            lp_check(x, g.integers(0, vocab, (rows, 2)).astype(np.int32), n_top, 0.7, pos)
+
+
 @pytest.mark.parametrize("temperature", [1e-3, 0.05, 1.0, 7.0, 1e4])
 def test_temperatures(temperature):
     g = rng(11, int(temperature * 1000))
