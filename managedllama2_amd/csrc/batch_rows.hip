@@ -4,20 +4,20 @@
 #include "batch_product_plan.hpp"
 
 #include <cmath>
+#include <type_traits>
 
 namespace l2 {
 
-// Sum over a workgroup of WAVES wavefronts, in every thread.
-template <int WAVES>
-__device__ __forceinline__ float block_sum(float v, float* lds /* WAVES */)
+// Sum over a workgroup of up to 16 wavefronts, in every thread.
+__device__ __forceinline__ float block_sum(float v, float* lds /* 16 */)
 {
     v = wave_sum(v);
+    const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0)
-        lds[threadIdx.x >> 6] = v;
+        lds[wave] = v;
     __syncthreads();
     float t = lds[0];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w)
+    for (int w = 1; w < waves; ++w)
         t += lds[w];
     __syncthreads();
     return t;
@@ -38,15 +38,19 @@ struct NormRowsArgs {
 };
 
 // A workgroup per row, which stays in registers between its one reading and its writing: PIECES of 8 elements per thread.
-template <int WAVES, int PIECES>
-__global__ __launch_bounds__(WAVES * 64) void batch_norm_kernel(NormRowsArgs a)
+//
+// HBM bounds many rows: 4000 rows of 5120 with both norms and a gate 28 us, 5.8 TB/s; with results that pass through the L2 (which
+// cannot hold them) 39.6, with one piece per thread, and so ten wavefronts to a sum, 34.4.  Few rows are latency: 48 rows of 4096 3.9 us, with two
+// pieces 4.3.
+template <int PIECES, bool THROUGH>
+__global__ __launch_bounds__(1024) void batch_norm_kernel(NormRowsArgs a)
 {
-    __shared__ float lds[WAVES];
+    __shared__ float lds[16];
     const int t = blockIdx.x;
     if (a.positions[t] < 0)
         return;
     const size_t row = static_cast<size_t>(t);
-    auto at = [](int i) { return (threadIdx.x + i * WAVES * 64) * 8; };
+    auto at = [](int i) { return static_cast<int>(threadIdx.x + i * blockDim.x) * 8; };
     auto half_of = [](u32x4 v, int k) { return half_bits_to_float(static_cast<uint16_t>(v[k >> 1] >> (16 * (k & 1)))); };
     float r[PIECES][8];
 #pragma unroll
@@ -72,7 +76,7 @@ __global__ __launch_bounds__(WAVES * 64) void batch_norm_kernel(NormRowsArgs a)
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     ss = __builtin_fmaf(half_of(y[i], k), half_of(y[i], k), ss);
-            norm = 1.0f / sqrtf(block_sum<WAVES>(ss, lds) / static_cast<float>(a.size) + a.eps);
+            norm = 1.0f / sqrtf(block_sum(ss, lds) / static_cast<float>(a.size) + a.eps);
         }
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
@@ -104,7 +108,10 @@ __global__ __launch_bounds__(WAVES * 64) void batch_norm_kernel(NormRowsArgs a)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             o[k] = static_cast<uint32_t>(float_to_half_bits(f[2 * k])) | static_cast<uint32_t>(float_to_half_bits(f[2 * k + 1])) << 16;
-        *reinterpret_cast<u32x4*>(p + at(i)) = o;
+        if constexpr (THROUGH)
+            __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(p + at(i)));
+        else
+            *reinterpret_cast<u32x4*>(p + at(i)) = o;
     };
     if (a.residual_output)
 #pragma unroll
@@ -119,7 +126,7 @@ __global__ __launch_bounds__(WAVES * 64) void batch_norm_kernel(NormRowsArgs a)
 #pragma unroll
         for (int k = 0; k < 8; ++k)
             ss = __builtin_fmaf(r[i][k], r[i][k], ss);
-    const float norm = 1.0f / sqrtf(block_sum<WAVES>(ss, lds) / static_cast<float>(a.size) + a.eps);
+    const float norm = 1.0f / sqrtf(block_sum(ss, lds) / static_cast<float>(a.size) + a.eps);
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
         if (at(i) >= a.size)
@@ -485,16 +492,28 @@ int llama2_batch_residual_rmsnorm(llama2_half* output, llama2_half* residual_out
         return rc;
     const NormRowsArgs a = {output, residual_output, residual, input, gamma, input_gamma, gate, batch->positions, size, output_stride,
                             residual_output_stride, residual_stride, input_stride, residual_scale, eps};
-    const dim3 grid(batch->n_tokens);
+    // Two pieces a thread where there are more rows than the card holds workgroups of one piece a thread.  What the L2 of all XCDs cannot
+    // hold does not go through it.
+    const int pieces_all = size / 8, written = (output != nullptr) + (residual_output != nullptr);
+    int pieces = batch->n_tokens >= 2 * ctx().num_cus ? 2 : 1;
+    while (ceil_div(pieces_all, pieces) > 1024)
+        pieces *= 2;
+    const bool through = static_cast<size_t>(batch->n_tokens) * size * 2 * written >= 32u << 20;
+    const dim3 grid(batch->n_tokens), block(round_up(ceil_div(pieces_all, pieces), 64));
     const hipStream_t st = ctx().stream;
-    if (size <= 2048)
-        hipLaunchKernelGGL((batch_norm_kernel<4, 1>), grid, dim3(256), 0, st, a);
-    else if (size <= 8192)
-        hipLaunchKernelGGL((batch_norm_kernel<16, 1>), grid, dim3(1024), 0, st, a);
-    else if (size <= 16384)
-        hipLaunchKernelGGL((batch_norm_kernel<16, 2>), grid, dim3(1024), 0, st, a);
-    else
-        hipLaunchKernelGGL((batch_norm_kernel<16, 8>), grid, dim3(1024), 0, st, a);
+    auto launch = [&](auto p) {
+        constexpr int P = decltype(p)::value;
+        if (through)
+            hipLaunchKernelGGL((batch_norm_kernel<P, true>), grid, block, 0, st, a);
+        else
+            hipLaunchKernelGGL((batch_norm_kernel<P, false>), grid, block, 0, st, a);
+    };
+    switch (pieces) {
+    case 1: launch(std::integral_constant<int, 1>()); break;
+    case 2: launch(std::integral_constant<int, 2>()); break;
+    case 4: launch(std::integral_constant<int, 4>()); break;
+    default: launch(std::integral_constant<int, 8>()); break;
+    }
     L2_LAUNCH_CHECK("llama2_batch_residual_rmsnorm");
     return LLAMA2_OK;
 }
