@@ -214,6 +214,7 @@ __device__ __forceinline__ void answer_row(const LogProbArgs& a, int row, const 
     for (int i = threadIdx.x; i < have; i += kLogProbThreads) {
         const unsigned long long key = found[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < have; ++j)
             rank += found[j] > key;
         if (rank >= a.n_top)
@@ -384,14 +385,16 @@ __global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogPro
     const float base = s.top == -INFINITY ? 0.0f : s.top;
     float total[2] = {}, moment[2] = {};
 #pragma unroll
-    for (int p = 0; p < PIECES; ++p)
+    for (int p = 0; p < PIECES; ++p) {
+        asm volatile("" : "+v"(x[p]));
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float d = half_bits_to_float(element(x[p], k)) - base;
+            const float d = __builtin_fmaf(half_bits_to_float(element(x[p], k)), 1.0f, -base); // one instruction
             const float e = __builtin_amdgcn_exp2f(d * a.per_e);
             total[k & 1] += e;
-            moment[k & 1] = __builtin_fmaf(e, fmaxf(d, -3.0e38f), moment[k & 1]);
+            moment[k & 1] = __builtin_fmaf(e, __builtin_amdgcn_fmed3f(d, -3.0e38f, 0.0f), moment[k & 1]); // of a masked logit 0
         }
+    }
     const float t = wave_sum(total[0] + total[1]), m = wave_sum(moment[0] + moment[1]);
     if (lane == 0) {
         lds.sums[0][wave] = t;
@@ -409,12 +412,22 @@ __global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogPro
         // that bound is collected.  Where that is nothing but -infinity, too much (many equal logits) or too little (NaN, which the
         // maxima leave out), in another way.
         const unsigned bound = static_cast<unsigned>(lds.bound);
-        if (bound > kOrderOfNothing && order_of(float_to_half_bits(most)) >= bound)
+        const float least = logit_of(bound);
+        if (bound > kOrderOfNothing && most >= least)
 #pragma unroll
             for (int p = 0; p < PIECES; ++p) {
+                asm volatile("" : "+v"(x[p])); // nothing is carried over from the exponentials, which would take a register per logit
                 const h2_t m8 = max_h2(max_h2(as_h2(x[p][0]), as_h2(x[p][1])), max_h2(as_h2(x[p][2]), as_h2(x[p][3])));
-                if (order_of(float_to_half_bits(fmaxf(static_cast<float>(m8[0]), static_cast<float>(m8[1])))) >= bound)
-                    collect(lds, x[p], bound, begin + (p * kLogProbThreads + tid) * 8, end);
+                if (static_cast<float>(m8[0]) >= least || static_cast<float>(m8[1]) >= least)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int i = begin + (p * kLogProbThreads + tid) * 8 + k;
+                        if (half_bits_to_float(element(x[p], k)) >= least && i < end) {
+                            const int at = atomicAdd(&lds.count, 1);
+                            if (at < kCandidates)
+                                lds.found[at] = key_of(order_of(element(x[p], k)), i);
+                        }
+                    }
             }
         __syncthreads();
         have = lds.count;
