@@ -447,8 +447,9 @@ typedef struct llama2_batch_matrix {
 /* Products of all tokens of a step with up to LLAMA2_MAX_BATCH_MATRICES int4 tensors that read the same input (q, k and
  * v; or one):
  *   output[t][n] = half(residual[t][n] + sum_k input[t][k] * (w - z) * s + adapter's part),
- * sums in fp32, one rounding at the end; what an adapter's ranks receive of the input keeps 22 bits of the largest of them.
- * rows % 8 == 0; tensors are laid out as above (ceil(rows/32)*4 words, ceil(rows/128) scales per output).
+ * sums in fp32, one rounding at the end; what an adapter's ranks receive of the input is fp32 too, and above 64 tokens keeps
+ * 22 bits of the largest of them.
+ * rows % 8 == 0, up to 65536; cols up to 2^20, input_stride up to 2^24; tensors are laid out as above (ceil(rows/32)*4 words, ceil(rows/128) scales per output).
  * Token t uses adapter token_adapters[t] of every matrix that has adapters; a value that is not one of 0 .. n_adapters - 1:
  * none.  What one token or one adapter holds has no influence on the rows of other tokens.  token_adapters may be null where no
  * matrix has adapters.  Rows of tokens without a position are left as they were.  Reads n_tokens and positions of
@@ -459,8 +460,8 @@ int llama2_batch_mat_mul_int4(const llama2_batch_matrix* matrices, int n_matrice
 
 /* The first half of the gated feed-forward block for all tokens of a step:
  *   output[t][n] = half( silu(g) * u ),  silu(v) = v / (1 + exp(-v)),
- * g and u the sums of llama2_batch_mat_mul_int4 with `gate` and `up` (and their adapters; null: none), in fp32.  The rest
- * as there. */
+ * g and u the sums of llama2_batch_mat_mul_int4 with `gate` and `up` (and their adapters; null: none), in fp32.  rows up to
+ * 32768, the rest as there. */
 int llama2_batch_mat_mul_swiglu(llama2_half* output, const llama2_half* input, const llama2_qweight* gate,
                                 const llama2_qweight* up, int rows, int cols, int output_stride, int input_stride,
                                 const llama2_adapters* gate_adapters, const llama2_adapters* up_adapters,
@@ -489,8 +490,9 @@ int llama2_batch_residual_rmsnorm(llama2_half* output, llama2_half* residual_out
  * Any of the four may be null (n_tokens / n_top 0 where theirs are; top_log_probs needs top_tokens).  A logit of -infinity has probability 0; of a row that holds
  * nothing else all log probabilities are -infinity and the entropy is 0.  A row with NaN or +infinity has NaN for its log probabilities
  * and its entropy; its top tokens are in the order of the logits, NaN last.  Rows whose position is negative are left as they
- * were (positions null: none is).  n_tokens <= 1024, n_top <= LLAMA2_MAX_TOP_TOKENS, 0 < temperature; logits need
- * no alignment beyond their 2 bytes.  Asynchronous, may be captured. */
+ * were (positions null: none is).  n_tokens <= 1024, n_top <= LLAMA2_MAX_TOP_TOKENS, vocab_size <= 2^20, 0 < temperature; logits
+ * need no alignment beyond their 2 bytes.  Scratch: as llama2_multi_head_attention (call once before capturing).  Asynchronous,
+ * may be captured. */
 #define LLAMA2_MAX_TOP_TOKENS 64
 int llama2_batch_log_probs(float* log_probs, float* entropies, int* top_tokens, float* top_log_probs,
                            const llama2_half* logits, const int* tokens, const int* positions, int n_rows, int vocab_size,

@@ -5,12 +5,10 @@
 //
 // w - z is an exact fp16 integer, its products with x are summed in fp32 over a group of 128 and scaled in fp32.  h is summed in
 // fp32 and leaves as two fp16 numbers and a power of two (22 bits of the token's largest), which the matrix cores take as 16 ranks a product.
-#include "batch_adapters.hpp"
+#include "batch_product.hpp"
 #include "prefill.hpp"
 
 #include <cmath>
-#include <cstdlib>
-#include <type_traits>
 
 namespace l2 {
 
@@ -32,7 +30,7 @@ struct alignas(64) LowArgs {
     const int* token_adapters;
     int K, x_stride, n_tokens, most_adapters;
     uint16_t* packed; // non-null: the rows as operands, by the workgroups behind those of the tensors
-    int n_matrices;
+    int n_matrices, z_blocks; // z_blocks: workgroups that share a matrix's ranks
     LowTensor t[LLAMA2_MAX_BATCH_MATRICES];
 };
 
@@ -52,13 +50,14 @@ __device__ __forceinline__ int tile_column(int k0, int n)
 
 constexpr int kTileBytes = 16 * 256;
 
+template <bool NIBBLES> // eight elements in the order in which nibbles come out of a word
 __device__ __forceinline__ void put_tile(char* lds, const HalfTile& t)
 {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int row = 4 * i + (lane >> 4);
-        *reinterpret_cast<u32x4*>(lds + row * 256 + ((lane & 15) ^ row) * 16) = t.v[i];
+        *reinterpret_cast<u32x4*>(lds + row * 256 + ((lane & 15) ^ row) * 16) = NIBBLES ? frag_order(t.v[i]) : t.v[i];
     }
 }
 
@@ -71,7 +70,7 @@ __device__ __forceinline__ h8_t tile_operand(const char* lds, int m)
 
 // ---------------------------------------------------------------- rows as operands
 // 16 tokens and a group of 128 inputs are the four operands of 16 x 16 x 32 products, 1 KB each: lane group c of operand m holds elements
-// 32 c + 8 m on of token lane % 16, zeros behind the end of a row.  Tokens behind the last one repeat it.  `worker` of `workers` pairs of
+// 32 c + 8 m on of token lane % 16, in the order of a word's nibbles, zeros behind the end of a row.  Tokens behind the last one repeat it.  `worker` of `workers` pairs of
 // such tiles at a time, 512 threads.
 __device__ __forceinline__ void pack_rows(uint16_t* packed, const uint16_t* x, int K, int x_stride, int n_tokens, int worker, int workers)
 {
@@ -82,7 +81,7 @@ __device__ __forceinline__ void pack_rows(uint16_t* packed, const uint16_t* x, i
         u32x4 v = {};
         if (k < K)
             v = *reinterpret_cast<const u32x4*>(x + static_cast<size_t>(token) * x_stride + k);
-        reinterpret_cast<u32x4*>(packed)[(static_cast<size_t>(u) * 4 + m) * 64 + lane] = v;
+        reinterpret_cast<u32x4*>(packed)[(static_cast<size_t>(u) * 4 + m) * 64 + lane] = frag_order(v);
     }
 }
 
@@ -92,12 +91,13 @@ __global__ __launch_bounds__(512) void batch_pack_kernel(uint16_t* packed, const
 }
 
 // ---------------------------------------------------------------- what the ranks receive
-// A workgroup takes 16 ranks of one item of a block of 64 tokens, so that an adapter is read once for up to 16 tokens that use it; its
+// A workgroup takes items of a block of 64 tokens, so that an adapter is read once for up to 16 tokens that use it, and ranks by 16; its
 // wavefronts split the inputs.  Ranks and scales of small pools are requested together with the tokens' adapters.
 // WIDE: as two fp16 numbers and a power of two (what the matrix cores take), else in fp32, the adapter's scale with it.
+// CHUNKS of 128 inputs that a wavefront has requested; KEEP: they are all that there are, and the inputs stay for all ranks.
 constexpr int kLowWaves = 8, kLowTable = kLowWaves * 64;
 
-template <bool WIDE>
+template <bool WIDE, int CHUNKS, bool KEEP>
 __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
 {
     constexpr int kStride = 16 + 4;
@@ -108,16 +108,20 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
     __shared__ __align__(16) float red[kLowWaves * 16 * kStride];
     auto& a = kernel_args<LowArgs>();
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, c = lane >> 4;
-    const int t0 = blockIdx.x * 64, K = a.K, x_stride = a.x_stride, n_tokens = a.n_tokens, most_adapters = a.most_adapters;
+    const int t0 = blockIdx.x * 64, K = a.K, x_stride = a.x_stride, n_tokens = a.n_tokens, most_adapters = a.most_adapters, z_blocks = a.z_blocks;
     const uint16_t* const x = a.x;
     const int *const positions = a.positions, *const token_adapters = a.token_adapters;
-    if (static_cast<int>(blockIdx.z) == a.n_matrices * kRankBlocks) {
-        pack_rows(a.packed, x, K, x_stride, n_tokens, blockIdx.x * gridDim.y + blockIdx.y, gridDim.x * gridDim.y);
+    const int which = blockIdx.z / z_blocks, first_block = blockIdx.z - which * z_blocks;
+    if (which == a.n_matrices) {
+        const int worker = (first_block * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x, workers = gridDim.x * gridDim.y * z_blocks;
+        if constexpr (WIDE)
+            pack_fragments(a.packed, x, K, x_stride, n_tokens, worker, workers);
+        else
+            pack_rows(a.packed, x, K, x_stride, n_tokens, worker, workers);
         return;
     }
-    auto& t = a.t[blockIdx.z / kRankBlocks];
-    const int block = blockIdx.z % kRankBlocks, r0 = block * 16;
-    const uint16_t* down = t.down;
+    auto& t = a.t[which];
+    const uint16_t* const down = t.down;
     const float* const scales = t.scales;
     const int* const ranks = t.ranks;
     void* const lows = t.low;
@@ -125,7 +129,7 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
     const long long down_stride = t.down_stride;
     const int n_adapters = t.n_adapters, max_rank = t.max_rank;
     loaded(K, x_stride, n_tokens, most_adapters, x, positions, token_adapters, down, scales, ranks, lows, info, down_stride, n_adapters, max_rank);
-    if (!down || r0 >= max_rank)
+    if (!down || first_block * 16 >= max_rank)
         return;
     int mine = 0;
     float mine_scale = 0.0f;
@@ -140,108 +144,115 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
     table[tid] = mine;
     scale_table[tid] = mine_scale;
     __syncthreads();
-    const int item = blockIdx.y;
-    if (item >= items.count)
-        return;
-    const int id = __builtin_amdgcn_readfirstlane(items.adapter[item]);
-    if (id >= n_adapters)
-        return;
-    const int rank = min(max(__builtin_amdgcn_readfirstlane(id < kLowTable ? table[id] : ranks[id]), 0), max_rank);
-    if (r0 >= rank && r0 > 0) // the first block says that there are no ranks at all
-        return;
-    const float scale = id < kLowTable ? scale_table[id] : scales[id];
     const __amdgpu_buffer_rsrc_t rx = rows_buffer(x + static_cast<size_t>(t0) * x_stride,
                                                   (static_cast<size_t>(min(64, n_tokens - t0) - 1) * x_stride + K) * 2);
-    const __amdgpu_buffer_rsrc_t rd = rows_buffer(down + id * down_stride, static_cast<size_t>(rank) * K * 2); // ranks beyond are zero
-    int xoff[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int own = items.tokens[item][4 * i + c];
-        xoff[i] = own == kNobody ? kBehind : own * x_stride * 2;
-    }
-    constexpr int kAhead = 4; // tiles of both that a wavefront has requested
-    HalfTile xt[kAhead], dt[kAhead];
-    auto request = [&](int q, int k0) {
-        const int column = tile_column(k0, K);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            xt[q].v[i] = __builtin_amdgcn_raw_buffer_load_b128(rx, column < 0 || xoff[i] < 0 ? kBehind : xoff[i] + column, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            dt[q].v[i] = __builtin_amdgcn_raw_buffer_load_b128(rd, column < 0 ? kBehind : (r0 + 4 * i + c) * K * 2 + column, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-    };
-#pragma unroll
-    for (int q = 0; q < kAhead; ++q)
-        request(q, (wave + q * kLowWaves) * 128);
     char* const lds = tiles + wave * kTileBytes;
-    f4_t acc = {};
-    for (int k0 = wave * 128; k0 < K; k0 += kAhead * kLowWaves * 128)
+    for (int item = blockIdx.y; item < items.count; item += gridDim.y) {
+        const int id = __builtin_amdgcn_readfirstlane(items.adapter[item]);
+        if (id >= n_adapters)
+            continue;
+        const int rank = min(max(__builtin_amdgcn_readfirstlane(id < kLowTable ? table[id] : ranks[id]), 0), max_rank);
+        const float scale = id < kLowTable ? scale_table[id] : scales[id];
+        const __amdgpu_buffer_rsrc_t rd = rows_buffer(down + id * down_stride, static_cast<size_t>(rank) * K * 2); // ranks beyond are zero
+        int xoff[4];
 #pragma unroll
-        for (int q = 0; q < kAhead; ++q) { // behind the last elements both are zero
-            h8_t xf[4], df[4];
-            put_tile(lds, xt[q]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                xf[j] = tile_operand(lds, j);
-            put_tile(lds, dt[q]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                df[j] = tile_operand(lds, j);
-            request(q, k0 + (q + kAhead) * kLowWaves * 128);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                acc = mfma16(xf[j], df[j], acc);
+        for (int i = 0; i < 4; ++i) {
+            const int own = items.tokens[item][4 * i + c];
+            xoff[i] = own == kNobody ? kBehind : own * x_stride * 2;
         }
+        HalfTile xt[CHUNKS], dt[CHUNKS];
+        h8_t xf[KEEP ? CHUNKS : 1][4];
+        auto chunk = [&](int q) { return (wave + q * kLowWaves) * 128; };
+        auto request_x = [&](int q, int k0) {
+            const int column = tile_column(k0, K);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        red[(wave * 16 + 4 * c + e) * kStride + l15] = acc[e];
-    __syncthreads();
-    if (wave >= 4)
-        return;
-    // 16 lanes a token, a rank each
-    const int place = tid >> 4, m = items.tokens[item][place];
-    float v = 0.0f;
+            for (int i = 0; i < 4; ++i)
+                xt[q].v[i] = __builtin_amdgcn_raw_buffer_load_b128(rx, column < 0 || xoff[i] < 0 ? kBehind : xoff[i] + column, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto request_d = [&](int q, int k0, int block) { // blocks behind the rank lie behind the end
+            const int column = tile_column(k0, K);
 #pragma unroll
-    for (int w = 0; w < kLowWaves; ++w)
-        v += red[(w * 16 + place) * kStride + l15];
-    v = r0 + l15 < rank ? v : 0.0f;
-    const size_t to = static_cast<size_t>(t0 + (m == kNobody ? 0 : m)) * ((max_rank + 15) / 16) + block;
-    if constexpr (WIDE) {
-        const float most = row16_max(fabsf(v));
-        // the largest between 2^14 and 2^15; nothing to scale where all are 0 or one is infinite
-        const int e2 = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
-        const float scaled = ldexpf(v, e2);
-        const uint16_t h = float_to_half_bits(scaled);
-        if (m == kNobody)
-            return;
-        uint16_t* const low = static_cast<uint16_t*>(lows);
-        low[to * 32 + l15] = h;
-        low[to * 32 + 16 + l15] = float_to_half_bits(scaled - half_bits_to_float(h));
-        if (l15 == 0)
-            info[to] = TokenAdapter{ldexpf(scale, -e2), rank};
-    } else if (m != kNobody) {
-        static_cast<float*>(lows)[to * 16 + l15] = v * scale;
-        if (l15 == 0)
-            info[to] = TokenAdapter{scale, rank};
+            for (int i = 0; i < 4; ++i)
+                dt[q].v[i] = __builtin_amdgcn_raw_buffer_load_b128(rd, column < 0 ? kBehind : (block * 16 + 4 * i + c) * K * 2 + column, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int q = 0; q < CHUNKS; ++q) {
+            request_x(q, chunk(q));
+            request_d(q, chunk(q), first_block);
+        }
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int q = 0; q < CHUNKS; ++q) {
+                put_tile<false>(lds, xt[q]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    xf[q][j] = tile_operand(lds, j);
+            }
+        }
+        for (int block = first_block; block == 0 || block * 16 < rank; block += z_blocks) { // the first one says that there are no ranks at all
+            f4_t acc = {};
+            for (int k0 = wave * 128; k0 < K; k0 += CHUNKS * kLowWaves * 128) {
+#pragma unroll
+                for (int q = 0; q < CHUNKS; ++q) { // behind the last elements both are zero
+                    const int next = k0 + (q + CHUNKS) * kLowWaves * 128;
+                    const bool on = next - q * kLowWaves * 128 < K; // else the next block from the front
+                    h8_t df[4];
+                    if constexpr (!KEEP) {
+                        put_tile<false>(lds, xt[q]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            xf[0][j] = tile_operand(lds, j);
+                        request_x(q, on ? next : chunk(q));
+                    }
+                    put_tile<false>(lds, dt[q]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        df[j] = tile_operand(lds, j);
+                    request_d(q, on ? next : chunk(q), on ? block : block + z_blocks);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc = mfma16(xf[KEEP ? q : 0][j], df[j], acc);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                red[(wave * 16 + 4 * c + e) * kStride + l15] = acc[e];
+            __syncthreads();
+            if (wave < 4) { // 16 lanes a token, a rank each
+                const int place = tid >> 4, m = items.tokens[item][place];
+                float v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kLowWaves; ++w)
+                    v += red[(w * 16 + place) * kStride + l15];
+                v = block * 16 + l15 < rank ? v : 0.0f;
+                const size_t to = static_cast<size_t>(t0 + (m == kNobody ? 0 : m)) * ((max_rank + 15) / 16) + block;
+                if constexpr (WIDE) {
+                    const float most = row16_max(fabsf(v));
+                    // the largest between 2^14 and 2^15; nothing to scale where all are 0 or one is infinite
+                    const int e2 = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
+                    const float scaled = ldexpf(v, e2);
+                    const uint16_t h = float_to_half_bits(scaled);
+                    if (m != kNobody) {
+                        uint16_t* const low = static_cast<uint16_t*>(lows);
+                        low[to * 32 + l15] = h;
+                        low[to * 32 + 16 + l15] = float_to_half_bits(scaled - half_bits_to_float(h));
+                        if (l15 == 0)
+                            info[to] = TokenAdapter{ldexpf(scale, -e2), rank};
+                    }
+                } else if (m != kNobody) {
+                    static_cast<float*>(lows)[to * 16 + l15] = v * scale;
+                    if (l15 == 0)
+                        info[to] = TokenAdapter{scale, rank};
+                }
+            }
+            __syncthreads();
+        }
     }
 }
 
 // ---------------------------------------------------------------- the products
-// The eight weights of a word as fp16 n - z, in order: a byte into both halves, the lower nibble of one and the upper nibble
-// of the other into the mantissa of 1024, then 1024 + n - (1024 + z) and (1024 + 16 n) / 16 - (64 + z).
-__device__ __forceinline__ h8_t weights_of(uint32_t w, h2_t minus)
-{
-    const h2_t times = {static_cast<_Float16>(1.0f), static_cast<_Float16>(0.0625f)};
-    u32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t u = __builtin_amdgcn_perm(0u, w, 0x0C000C00u | i | i << 16);
-        v[i] = as_u32(__builtin_elementwise_fma(as_h2((u & 0x00F0000Fu) | 0x64006400u), times, minus));
-    }
-    return __builtin_bit_cast(h8_t, v);
-}
-
 // 16 rows of the 16 words of a group, requested in the order of memory (row lane / 4, words 4 (lane % 4) on) and turned around through
 // LDS: afterwards lane group c holds words 4 c .. 4 c + 3 of row lane % 16, which go with operand m of a tile of inputs word by word.
 __device__ __forceinline__ u32x4 turned_words(char* lds, u32x4 v)
@@ -267,7 +278,7 @@ template <int W, int R, int T, int D, bool GATED, bool ADAPTERS>
 __global__ __launch_bounds__(W * 64, 2) void batch_product_kernel(ProductArgs)
 {
     constexpr int kTokens = T * 16, kRows = R * 16, kStride = kRows + 4, kTensors = GATED ? 2 : 1, RT = R / kTensors;
-    constexpr int kRing = T * D <= 4 ? T * D : 2; // tiles of tokens whose inputs are on their way or in use
+    constexpr int kRing = T * D <= 4 && !(R == 4 && T == 4) ? T * D : 2; // tiles of tokens whose inputs are on their way or in use
     static_assert(T * D % kRing == 0 && kRing <= T * D, "a tile has one place in the ring");
     constexpr bool PACKED = T > 1; // the inputs come as operands; of few tokens in rows, which saves the launch that packs them
     constexpr int kWaveBytes = (PACKED ? 0 : kTileBytes) + R * 1024, kWordsAt = kWaveBytes - R * 1024;
@@ -303,10 +314,10 @@ __global__ __launch_bounds__(W * 64, 2) void batch_product_kernel(ProductArgs)
     const int ws = (K + 31) / 32 * 4, groups = (K + 127) / 128, zs = (groups + 7) / 8;
 
     // The threads of a token, its adapter and that one's ranks: asked for first, since more hangs on them.
-    constexpr int kThreads = W * 64 / kTokens;
+    constexpr int kThreads = (W < 8 ? W : 8) * 64 / kTokens; // the other wavefronts take none
     const int my_token = tid / kThreads, token_at = t0 + my_token;
     int position = -1, adapter = kNoAdapter, rank[kTensors] = {};
-    if (token_at < n_tokens) {
+    if (my_token < kTokens && token_at < n_tokens) {
         position = positions[token_at];
         if (token_adapters)
             adapter = token_adapters[token_at];
@@ -377,7 +388,7 @@ __global__ __launch_bounds__(W * 64, 2) void batch_product_kernel(ProductArgs)
                 reinterpret_cast<u32x4*>(zeros + h * RT * 16 * zs)[i - ns] = z[i - ns].v;
     }
     const int id = known_adapter(position, adapter, most_adapters);
-    if (tid % kThreads == 0)
+    if (tid % kThreads == 0 && my_token < kTokens)
         live[my_token] = id != kNoToken;
     f4_t acc[T][R] = {};
     if constexpr (ADAPTERS) {
@@ -441,7 +452,7 @@ __global__ __launch_bounds__(W * 64, 2) void batch_product_kernel(ProductArgs)
         for (int h = 0; h < kBoth; ++h)
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
-                if (first[h] + i * kThreads < RT * 16)
+                if (my_token < kTokens && first[h] + i * kThreads < RT * 16)
                     extra[my_token * kStride + column[h] + i * kThreads] = sum[h][i];
         __syncthreads();
         if (wave == 0)
@@ -467,11 +478,13 @@ __global__ __launch_bounds__(W * 64, 2) void batch_product_kernel(ProductArgs)
                 const u32x4 v = turned_words(lds + kWordsAt + r * 1024, raw[d][r]);
                 const int row = r * 16 + l15;
                 const float zero = static_cast<float>(zeros[row * zs + (gs >> 3)] >> (4 * (gs & 7)) & 15u);
-                const h2_t minus = {static_cast<_Float16>(-1024.0f - zero), static_cast<_Float16>(-64.0f - zero)};
+                const _Float16 lo = static_cast<_Float16>(1024.0f + zero), hi = static_cast<_Float16>(-64.0f - zero);
+                const h2_t zlo = {lo, lo}, zhi = {hi, hi};
                 sc[r] = half_bits_to_float(scales[row * groups + gs]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    wf[r][j] = weights_of(v[j], minus);
+                    wf[r][j] = __builtin_bit_cast(h8_t, u32x4{dequant_pair(v[j], 0, zlo, zhi), dequant_pair(v[j], 1, zlo, zhi),
+                                                               dequant_pair(v[j], 2, zlo, zhi), dequant_pair(v[j], 3, zlo, zhi)});
             }
             __builtin_amdgcn_sched_barrier(0);
             load_w(d, g + W * D);
@@ -484,7 +497,7 @@ __global__ __launch_bounds__(W * 64, 2) void batch_product_kernel(ProductArgs)
                     for (int j = 0; j < 4; ++j)
                         xf[j] = __builtin_bit_cast(h8_t, xt[q].v[j]);
                 } else {
-                    put_tile(lds, xt[q]);
+                    put_tile<true>(lds, xt[q]);
                     __builtin_amdgcn_sched_barrier(0);
                     load_x(q, next % T, g0 + next / T * W);
 #pragma unroll
@@ -579,29 +592,67 @@ static void launch_product(Product& p)
         hipLaunchKernelGGL((batch_product_kernel<W, R, T, D, GATED, false>), grid, block, 0, ctx().stream, a);
 }
 
-// Rows of more than 32768 inputs: tiles so low that their scales fit.
-static void launch_tall(Product& p, std::false_type) { launch_product<8, 1, 1, 2, false>(p); }
-static void launch_tall(Product& p, std::true_type) { launch_product<8, 2, 1, 2, true>(p); }
-
-constexpr int kWideTokens = 64; // more go through the kernels of the prompt's products
 constexpr int kMostTokens = 4096; // of a launch
+constexpr int kMostGroups = 256; // of rows whose inputs are packed; of more one tile of outputs has room for its scales
+
+// Tiles by how many columns all tensors of a call have beside the CUs: as few workgroups as have something for every CU, since every one
+// reads the inputs of its tokens.  Measured in us, without adapters, at 4096 inputs and with 256 CUs (W wavefronts, R tiles of outputs):
+//   tokens  columns          chosen          others
+//   1       4096             W 8, R 1  5.7   W 8, R 2  7.1;  W 4, R 2  7.5
+//   16      12288            W 4, R 2 11.2   W 8, R 1 12.2;  W 8, R 4 10.6, which at 4096 takes 9.1
+//   16      32000            W 4, R 4 17.2   W 4, R 2 18.6;  W 8, R 1 25.4
+//   1       gated 2 * 11008  W 4, R 2 15.2   W 8, R 2 17.0;  W 4, R 4 16.4
+//   32      4096             W 8, R 1  8.3   W 8, R 2  9.5;  W 4, R 4 12.9
+//   32      12288            W 4, R 2 13.6   W 8, R 2 15.8;  W 8, R 1 16.7
+//   64      4096             two blocks of 32 tokens, W 4, R 2 10.6   one of 64, W 8, R 2 12.6, R 4 15.5
+//   64      6144             W 8, R 2 12.8   two blocks 16.2;  R 4 15.4
+//   64      12288            W 8, R 4 17.0   two blocks 17.7;  R 2 20.7
+// Scales and zero points of a workgroup's rows fit up to R * groups = 512.
+template <bool GATED>
+static void launch_shape(Product& p, int columns, int groups)
+{
+    const int n = p.a.n_tokens, per_cu = columns / ctx().num_cus;
+    if constexpr (!GATED) { // a gated tile is one of both tensors
+        if (groups > kMostGroups || (n <= 16 && per_cu <= 24))
+            return launch_product<8, 1, 1, 2, false>(p);
+        if (n > 16 && n <= 32 && per_cu <= 16)
+            return launch_product<8, 1, 2, 2, false>(p);
+    }
+    if (n <= 16)
+        per_cu >= 100 && groups <= kMostGroups / 2 ? launch_product<4, 4, 1, 1, GATED>(p) : launch_product<4, 2, 1, 2, GATED>(p);
+    else if (n <= 32 || per_cu <= 16 || (groups > kMostGroups / 2 && per_cu > 24))
+        launch_product<4, 2, 2, 2, GATED>(p);
+    else if (per_cu <= 24)
+        launch_product<8, 2, 4, 1, GATED>(p);
+    else
+        launch_product<8, 4, 4, 1, GATED>(p);
+}
 
 template <bool GATED>
 static int run_product(const char* fn, Product& p)
 {
     ProductArgs& a = p.a;
     LowArgs& l = p.low;
-    const int all = a.n_tokens, most = all < kMostTokens ? all : kMostTokens, groups = weight_groups(a.K);
-    bool fits = true; // the prompt's products hold a tensor's offsets in 31 bits
-    for (int i = 0; i < p.n_matrices; ++i)
+    const int all = a.n_tokens, groups = weight_groups(a.K);
+    int columns = 0;
+    bool fits = true, adapters = false; // the prompt's products hold a tensor's offsets in 31 bits
+    for (int i = 0; i < p.n_matrices; ++i) {
+        columns += a.t[i].cols; // at most 2^22
         fits = fits && static_cast<long long>(a.t[i].cols) * weight_words(a.K) * 4 <= 0x7FFFFFFFLL;
-    const bool wide = all > kWideTokens && fits;
-    const bool packed = !wide && all > 16;
+        adapters = adapters || l.t[i].down;
+    }
+    // More than 64 tokens go through the kernels of the prompt's products, and more than 16 where these have tiles for every CU and no
+    // adapters, of which each tile reads those of all its tokens one after the other (gated 2 * 11008 columns of 4096 inputs, 32 tokens
+    // 23.2 -> 18.6 us, 64 29.5 -> 24.2; with an adapter each 49 against 122; 2 * 8192 columns, 64 tokens 18.4 against 20.7).
+    const bool wide = fits && (all > 64 || (all > 16 && !adapters && columns >= 80 * ctx().num_cus));
+    const bool packed = !wide && all > 16 && groups <= kMostGroups;
+    const int step = groups <= kMostGroups ? kMostTokens : kMostTokens / 8; // threads of a launch in 32 bits
+    const int most = all < step ? all : step;
     const size_t fragments = wide ? batch_gemm_bytes(most, a.K) : packed ? static_cast<size_t>(ceil_div(most, 16)) * groups * 4096 : 0;
+    p.adapters = adapters;
     size_t bytes = fragments;
     for (int i = 0; i < p.n_matrices; ++i)
         if (l.t[i].down) {
-            p.adapters = true;
             bytes += static_cast<size_t>(most) * ceil_div(l.t[i].max_rank, 16) * (64 + sizeof(TokenAdapter));
             a.most_adapters = l.t[i].n_adapters > a.most_adapters ? l.t[i].n_adapters : a.most_adapters;
         }
@@ -623,8 +674,8 @@ static int run_product(const char* fn, Product& p)
         a.t[i].n_adapters = t.n_adapters;
         a.t[i].max_rank = t.max_rank;
     }
-    for (int done = 0; done < all; done += kMostTokens) {
-        a.n_tokens = all - done < kMostTokens ? all - done : kMostTokens;
+    for (int done = 0; done < all; done += step) {
+        a.n_tokens = all - done < step ? all - done : step;
         if (p.adapters) {
             l.x = a.x;
             l.positions = a.positions;
@@ -633,15 +684,27 @@ static int run_product(const char* fn, Product& p)
             l.x_stride = a.x_stride;
             l.n_tokens = a.n_tokens;
             l.most_adapters = a.most_adapters;
-            // items of a block of 64 tokens: one for each adapter in use, and one more for every 16 tokens
-            const int tokens = a.n_tokens < 64 ? a.n_tokens : 64, items = a.most_adapters + 3 < tokens ? a.most_adapters + 3 : tokens;
             l.n_matrices = p.n_matrices;
-            l.packed = packed ? reinterpret_cast<uint16_t*>(base) : nullptr;
-            const dim3 grid(ceil_div(a.n_tokens, 64), items, p.n_matrices * kRankBlocks + packed);
-            if (wide)
-                hipLaunchKernelGGL(batch_low_kernel<true>, grid, dim3(kLowWaves * 64), 0, ctx().stream, l);
+            l.packed = packed || wide ? reinterpret_cast<uint16_t*>(base) : nullptr;
+            // Items of a block of 64 tokens: one for each adapter in use, and one more for every 16 tokens.  Of few blocks every item and
+            // every 16 ranks have a workgroup; of many a workgroup takes several, since those with nothing to do cost as well.
+            const int blocks = ceil_div(a.n_tokens, 64), tokens = a.n_tokens < 64 ? a.n_tokens : 64;
+            const int items = a.most_adapters + 3 < tokens ? a.most_adapters + 3 : tokens;
+            int rank_blocks = 1;
+            for (int i = 0; i < p.n_matrices; ++i)
+                if (l.t[i].down && ceil_div(l.t[i].max_rank, 16) > rank_blocks)
+                    rank_blocks = ceil_div(l.t[i].max_rank, 16);
+            l.z_blocks = wide ? 1 : rank_blocks;
+            const dim3 grid(blocks, wide && items > 8 ? 8 : items, (p.n_matrices + (l.packed ? 1 : 0)) * l.z_blocks), threads(kLowWaves * 64);
+            const hipStream_t st = ctx().stream;
+            if (!wide)
+                hipLaunchKernelGGL((batch_low_kernel<false, 4, false>), grid, threads, 0, st, l);
+            else if (a.K <= 4 * kLowWaves * 128)
+                hipLaunchKernelGGL((batch_low_kernel<true, 4, true>), grid, threads, 0, st, l);
+            else if (a.K <= 5 * kLowWaves * 128)
+                hipLaunchKernelGGL((batch_low_kernel<true, 5, true>), grid, threads, 0, st, l);
             else
-                hipLaunchKernelGGL(batch_low_kernel<false>, grid, dim3(kLowWaves * 64), 0, ctx().stream, l);
+                hipLaunchKernelGGL((batch_low_kernel<true, 4, false>), grid, threads, 0, st, l);
             L2_LAUNCH_CHECK(fn);
         }
         const uint16_t* const rows = a.x;
@@ -655,31 +718,10 @@ static int run_product(const char* fn, Product& p)
             a.x = reinterpret_cast<const uint16_t*>(base);
         }
         if (wide) {
-            if (int rc = launch_batch_gemm(fn, a, p.n_matrices, GATED, p.adapters, base))
+            if (int rc = launch_batch_gemm(fn, a, p.n_matrices, GATED, p.adapters, p.adapters, base))
                 return rc;
         } else {
-            // scales and zero points of a workgroup's rows: R * groups <= 512
-            const int shape = getenv("L2_SHAPE") ? atoi(getenv("L2_SHAPE")) : 0; // XXX
-            if (a.n_tokens <= 16) {
-                if (shape == 1) GATED ? launch_product<4, 2, 1, 2, GATED>(p) : launch_product<8, GATED ? 2 : 1, 1, 2, GATED>(p);
-                else if (shape == 2) launch_product<8, 4, 1, 1, GATED>(p);
-                else if (shape == 3) launch_product<4, 4, 1, 1, GATED>(p);
-                else if (shape == 4) launch_product<4, 2, 1, 2, GATED>(p);
-                else if (shape == 5) launch_product<16, 2, 1, 1, GATED>(p);
-                else launch_product<8, 2, 1, 2, GATED>(p);
-            } else if (a.n_tokens <= 32) {
-                if (shape == 1) launch_product<8, GATED ? 2 : 1, 2, 2, GATED>(p);
-                else if (shape == 2) launch_product<4, 2, 2, 2, GATED>(p);
-                else if (shape == 3) launch_product<4, 4, 2, 1, GATED>(p);
-                else if (shape == 4) launch_product<8, 4, 2, 1, GATED>(p);
-                else launch_product<8, 2, 2, 2, GATED>(p);
-            } else {
-                if (shape == 1) launch_product<4, 4, 4, 1, GATED>(p);
-                else if (shape == 2) launch_product<8, 2, 4, 1, GATED>(p);
-                else if (shape == 3) launch_product<4, 2, 4, 1, GATED>(p);
-                else if (shape == 4) GATED ? launch_product<4, 2, 4, 1, GATED>(p) : launch_product<8, GATED ? 2 : 3, 4, 1, GATED>(p);
-                else launch_product<8, 4, 4, 1, GATED>(p);
-            }
+            launch_shape<GATED>(p, columns, groups);
             L2_LAUNCH_CHECK(fn);
         }
         a.x = rows + static_cast<size_t>(a.n_tokens) * a.x_stride;

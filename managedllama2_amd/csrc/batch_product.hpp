@@ -1,5 +1,5 @@
-// What the products of many tokens share with the kernels of the prompt's products: the tokens' adapters, in groups that the matrix
-// cores take together, and small device helpers.
+// What the products of many tokens share with the kernels of the prompt's products: operands from nibbles and rows, the tokens' adapters in
+// groups that the matrix cores take together, and small device helpers.
 #pragma once
 
 #include "common.hpp"
@@ -129,6 +129,58 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void* p, siz
 
 constexpr int kBehind = static_cast<int>(0x80000000u); // an offset behind the end of every buffer: reads zero, moves nothing
 
+// ---------------------------------------------------------------- inputs of the prompt's products
+constexpr int kGroup = 128;       // quantisation group along K
+constexpr int kFragBytes = 1024;  // one operand fragment: 64 lanes of 16 bytes
+constexpr int kBlockBytes = 8 * kFragBytes; // a token tile times a group
+
+// Fragment order of an activation matrix [m][k]: the lane (k / 64 % 2) * 32 + m % 32 of fragment
+// (m / 32, k / 128, k / 8 % 8) holds 8 consecutive k, in the order in which the weights' nibbles come out of
+// a word (0 4 1 5 2 6 3 7).  The word of weights that goes with them is word k / 8 of its row, so a lane's 8
+// words of a group are 32 contiguous bytes, and every fragment is one fully coalesced load.
+__device__ __forceinline__ uint32_t frag_offset(int m, int k, int groups)
+{
+    return static_cast<uint32_t>(((m >> 5) * groups + (k >> 7)) * 8 + ((k >> 3) & 7)) * kFragBytes +
+           ((((k >> 6) & 1) << 5) + (m & 31)) * 16;
+}
+
+__device__ __forceinline__ u32x4 frag_order(u32x4 v) // 8 consecutive values -> 0 4 1 5 2 6 3 7
+{
+    u32x4 o;
+    o[0] = (v[0] & 0xFFFFu) | (v[2] << 16);
+    o[1] = (v[0] >> 16) | (v[2] & 0xFFFF0000u);
+    o[2] = (v[1] & 0xFFFFu) | (v[3] << 16);
+    o[3] = (v[1] >> 16) | (v[3] & 0xFFFF0000u);
+    return o;
+}
+
+// Pair k of the 8 nibbles of a word as fp16 n - z, exact: n sits in the mantissa of 1024 + n (bits 0-3 of a half) or
+// 1024 + 16 n (bits 4-7).
+__device__ __forceinline__ uint32_t dequant_pair(uint32_t w, int k, h2_t zlo /* 1024 + z */, h2_t zhi /* -(64 + z) */)
+{
+    const h2_t sixteenth = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
+    uint32_t magic = 0x64006400u; // in a vector register: (w & mask) | magic is one instruction then
+    asm("" : "+v"(magic));
+    const uint32_t v = k >= 2 ? w >> 8 : w;
+    return k & 1 ? as_u32(__builtin_elementwise_fma(as_h2((v & 0x00F000F0u) | magic), sixteenth, zhi))
+                 : as_u32(as_h2((v & 0x000F000Fu) | magic) - zlo);
+}
+
+// Rows into fragment order, zeros behind the end of a row and in rows behind the last: `worker` of `workers`, 512 threads, a token tile and
+// a group at a time.
+__device__ __forceinline__ void pack_fragments(uint16_t* xf, const uint16_t* x, int K, int x_stride, int n_tokens, int worker, int workers)
+{
+    const int groups = (K + kGroup - 1) / kGroup, units = (n_tokens + 31) / 32 * groups;
+    for (int u = worker; u < units; u += workers) {
+        const int m = u / groups * 32 + (threadIdx.x >> 4), k = u % groups * kGroup + (threadIdx.x & 15) * 8;
+        u32x4 v = {};
+        if (m < n_tokens && k < K)
+            v = *reinterpret_cast<const u32x4*>(x + static_cast<size_t>(m) * x_stride + k);
+        *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(xf) + frag_offset(m, k, groups)) = frag_order(v);
+    }
+}
+
+// ---------------------------------------------------------------- adapters beside the prompt's products
 // What a product needs of a tensor's adapters.
 struct AdapterPart {
     const uint16_t* up; // null: no adapters

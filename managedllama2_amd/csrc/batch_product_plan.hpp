@@ -8,6 +8,7 @@
 namespace l2 {
 
 constexpr int kMaxProductRows = 1 << 16; // inputs of a tensor
+constexpr int kMaxGatedRows = 1 << 15; // of a gate and an up projection, whose scales a workgroup holds side by side
 constexpr int kMaxProductCols = 1 << 20; // outputs of a tensor
 constexpr int kMaxStride = 1 << 24; // of the input: offsets within 64 rows are ints
 constexpr int kMaxAdapters = 1 << 20;
@@ -61,8 +62,8 @@ inline int check_adapters(const char* fn, const llama2_adapters* a, int rows, in
 }
 
 // What the products of many rows share: the input, a tensor and its adapters, and that `out` overlaps none of them.
-inline int check_product_input(const char* fn, const llama2_half* input, int rows, int input_stride, const int* token_adapters,
-                               const llama2_batch* batch)
+inline int check_product_input(const char* fn, const llama2_half* input, int rows, int most_rows, int input_stride,
+                               const int* token_adapters, const llama2_batch* batch)
 {
     if (int rc = check_batch(fn, batch))
         return rc;
@@ -70,8 +71,8 @@ inline int check_product_input(const char* fn, const llama2_half* input, int row
     L2_CHECK(aligned(input, 16), "%s: input must be 16-byte aligned", fn);
     L2_CHECK(aligned(token_adapters, 4), "%s: misaligned token_adapters", fn);
     L2_CHECK(rows > 0 && rows % 8 == 0, "%s: rows=%d must be a positive multiple of 8", fn, rows);
-    if (rows > kMaxProductRows)
-        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: rows=%d exceeds %d", fn, rows, kMaxProductRows);
+    if (rows > most_rows)
+        return fail(LLAMA2_ERR_UNSUPPORTED, "%s: rows=%d exceeds %d", fn, rows, most_rows);
     L2_CHECK(input_stride >= rows && input_stride % 8 == 0, "%s: input_stride=%d must be a multiple of 8 and hold a row of %d", fn,
              input_stride, rows);
     if (input_stride > kMaxStride)
@@ -115,7 +116,7 @@ inline int check_batch_mat_mul(const llama2_batch_matrix* m, int n_matrices, con
                                const int* token_adapters, const llama2_batch* batch)
 {
     const char* fn = "llama2_batch_mat_mul_int4";
-    if (int rc = check_product_input(fn, input, rows, input_stride, token_adapters, batch))
+    if (int rc = check_product_input(fn, input, rows, kMaxProductRows, input_stride, token_adapters, batch))
         return rc;
     L2_CHECK(m && n_matrices > 0 && n_matrices <= LLAMA2_MAX_BATCH_MATRICES, "%s: n_matrices=%d must be 1 .. %d, and matrices not null", fn,
              n_matrices, LLAMA2_MAX_BATCH_MATRICES);
@@ -150,7 +151,7 @@ inline int check_batch_swiglu(const llama2_half* output, const llama2_half* inpu
                               const llama2_adapters* up_adapters, const int* token_adapters, const llama2_batch* batch)
 {
     const char* fn = "llama2_batch_mat_mul_swiglu";
-    if (int rc = check_product_input(fn, input, rows, input_stride, token_adapters, batch))
+    if (int rc = check_product_input(fn, input, rows, kMaxGatedRows, input_stride, token_adapters, batch))
         return rc;
     L2_CHECK(output && aligned(output, 16) && gate && up, "%s: null pointer, or misaligned output", fn);
     const llama2_qweight* w[] = {gate, up};

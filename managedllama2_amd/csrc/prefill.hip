@@ -17,7 +17,7 @@
 #include "int4_kernels.hpp"
 #include "gemm_shape.hpp"
 #include "prefill.hpp"
-#include "batch_adapters.hpp"
+#include "batch_product.hpp"
 
 #include <cmath>
 #include <cstdlib>
@@ -27,30 +27,6 @@
 namespace l2 {
 
 typedef float f16v_t __attribute__((ext_vector_type(16)));
-
-constexpr int kGroup = 128;       // quantisation group along K
-constexpr int kFragBytes = 1024;  // one operand fragment: 64 lanes of 16 bytes
-constexpr int kBlockBytes = 8 * kFragBytes; // a token tile times a group
-
-// Fragment order of an activation matrix [m][k]: the lane (k / 64 % 2) * 32 + m % 32 of fragment
-// (m / 32, k / 128, k / 8 % 8) holds 8 consecutive k, in the order in which the weights' nibbles come out of
-// a word (0 4 1 5 2 6 3 7).  The word of weights that goes with them is word k / 8 of its row, so a lane's 8
-// words of a group are 32 contiguous bytes, and every fragment is one fully coalesced load.
-__device__ __forceinline__ uint32_t frag_offset(int m, int k, int groups)
-{
-    return static_cast<uint32_t>(((m >> 5) * groups + (k >> 7)) * 8 + ((k >> 3) & 7)) * kFragBytes +
-           ((((k >> 6) & 1) << 5) + (m & 31)) * 16;
-}
-
-__device__ __forceinline__ u32x4 frag_order(u32x4 v) // 8 consecutive values -> 0 4 1 5 2 6 3 7
-{
-    u32x4 o;
-    o[0] = (v[0] & 0xFFFFu) | (v[2] << 16);
-    o[1] = (v[0] >> 16) | (v[2] & 0xFFFF0000u);
-    o[2] = (v[1] & 0xFFFFu) | (v[3] << 16);
-    o[3] = (v[1] >> 16) | (v[3] & 0xFFFF0000u);
-    return o;
-}
 
 // ---------------------------------------------------------------- RoPE angles
 __global__ __launch_bounds__(256) void prefill_rope_kernel(float* tab, int position, int count, float theta)
@@ -175,18 +151,6 @@ struct BatchGemmArgs {
     bool adapters;
     ProductTensor t[LLAMA2_MAX_BATCH_MATRICES];
 };
-
-// Pair k of the 8 nibbles of a word as fp16 n - z, exact: n sits in the mantissa of 1024 + n (bits 0-3 of a half) or
-// 1024 + 16 n (bits 4-7).
-__device__ __forceinline__ uint32_t dequant_pair(uint32_t w, int k, h2_t zlo /* 1024 + z */, h2_t zhi /* -(64 + z) */)
-{
-    const h2_t sixteenth = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
-    uint32_t magic = 0x64006400u; // in a vector register: (w & mask) | magic is one instruction then
-    asm("" : "+v"(magic));
-    const uint32_t v = k >= 2 ? w >> 8 : w;
-    return k & 1 ? as_u32(__builtin_elementwise_fma(as_h2((v & 0x00F000F0u) | magic), sixteenth, zhi))
-                 : as_u32(as_h2((v & 0x000F000Fu) | magic) - zlo);
-}
 
 __device__ __forceinline__ f16v_t mfma(h8_t a, h8_t b, f16v_t c)
 {
@@ -689,18 +653,9 @@ __global__ __launch_bounds__(512, 2) void batch_gemm_kernel(BatchGemmArgs b)
     gemm_block<MT, WN, WK, EPI>(a, lds, unit, mb, rows);
 }
 
-// Rows of fp16 into fragment order, zeros behind the end of a row: a workgroup per token tile and group.
-__global__ __launch_bounds__(256) void batch_fragments_kernel(uint16_t* xf, const uint16_t* x, int M, int K, int x_stride, int groups)
+__global__ __launch_bounds__(512) void batch_fragments_kernel(uint16_t* xf, const uint16_t* x, int K, int x_stride, int n_tokens)
 {
-    const int g = blockIdx.x, tile = blockIdx.y;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int m = tile * kTile + i * 16 + (threadIdx.x >> 4), k = g * kGroup + (threadIdx.x & 15) * 8;
-        u32x4 v = {};
-        if (m < M && k < K)
-            v = *reinterpret_cast<const u32x4*>(x + static_cast<size_t>(m) * x_stride + k);
-        *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(xf) + frag_offset(m, k, groups)) = frag_order(v);
-    }
+    pack_fragments(xf, x, K, x_stride, n_tokens, blockIdx.x, gridDim.x);
 }
 
 static GemmShape gemm_shape(int tiles, int pairs, int groups, bool may_split)
@@ -799,7 +754,7 @@ static int launch_batch_gemm_epi(const char* name, BatchGemmArgs& b)
 
 size_t batch_gemm_bytes(int n_tokens, int K) { return static_cast<size_t>(ceil_div(n_tokens, kTile)) * ceil_div(K, kGroup) * kBlockBytes; }
 
-int launch_batch_gemm(const char* name, const ProductArgs& call, int n_matrices, bool gated, bool adapters, void* fragments)
+int launch_batch_gemm(const char* name, const ProductArgs& call, int n_matrices, bool gated, bool adapters, bool packed, void* fragments)
 {
     BatchGemmArgs b{};
     const int groups = ceil_div(call.K, kGroup), tiles = ceil_div(call.n_tokens, kTile);
@@ -815,9 +770,11 @@ int launch_batch_gemm(const char* name, const ProductArgs& call, int n_matrices,
     }
     if (gated)
         b.g.pairs = ceil_div(call.t[0].cols, kTile);
-    hipLaunchKernelGGL(batch_fragments_kernel, dim3(groups, tiles), dim3(256), 0, ctx().stream, static_cast<uint16_t*>(fragments), call.x,
-                       call.n_tokens, call.K, call.x_stride, groups);
-    L2_LAUNCH_CHECK(name);
+    if (!packed) {
+        hipLaunchKernelGGL(batch_fragments_kernel, dim3(tiles * groups), dim3(512), 0, ctx().stream, static_cast<uint16_t*>(fragments), call.x,
+                           call.K, call.x_stride, call.n_tokens);
+        L2_LAUNCH_CHECK(name);
+    }
     return gated ? launch_batch_gemm_epi<EPI_GATED>(name, b) : launch_batch_gemm_epi<EPI_ROWS>(name, b);
 }
 

@@ -36,9 +36,9 @@ int prefill_run(const PrefillWorkspace& ws, const llama2_config& cfg, const llam
                 const llama2_transformer_weights& w, const llama2_run_state& s, int position, int count);
 
 // The products of many tokens (llama2_batch_mat_mul_int4, llama2_batch_mat_mul_swiglu) on the same kernels: `fragments` has room for
-// batch_gemm_bytes.  Tensors of less than 2^31 bytes, fragments too.
+// batch_gemm_bytes, and holds the rows already if `packed`.  Tensors of less than 2^31 bytes, fragments too.
 struct ProductArgs;
 size_t batch_gemm_bytes(int n_tokens, int K);
-int launch_batch_gemm(const char* name, const ProductArgs& call, int n_matrices, bool gated, bool adapters, void* fragments);
+int launch_batch_gemm(const char* name, const ProductArgs& call, int n_matrices, bool gated, bool adapters, bool packed, void* fragments);
 
 } // namespace l2

@@ -146,7 +146,7 @@ def test_products_that_are_refused(lib, bad, code):
 
 @pytest.mark.parametrize("bad,code", [
     (dict(o=None), INVALID), (dict(o=30 * MIB + 2), INVALID), (dict(x=None), INVALID), (dict(g=None), INVALID), (dict(u=None), INVALID),
-    (dict(u=(None, 220, 221)), INVALID), (dict(rows=4), INVALID), (dict(cols=4), INVALID), (dict(so=504), INVALID), (dict(so=516), INVALID),
+    (dict(u=(None, 220, 221)), INVALID), (dict(rows=4), INVALID), (dict(rows=32776, sx=32776), UNSUPPORTED), (dict(cols=4), INVALID), (dict(so=504), INVALID), (dict(so=516), INVALID),
     (dict(sx=1000), INVALID), (dict(ga=adapters(), ids=None), INVALID), (dict(ua=adapters(max_rank=4)), INVALID), (dict(o=7 * MIB), INVALID),
     (dict(o=200 * MIB), INVALID), (dict(o=60 * MIB, ua=adapters()), INVALID), (dict(o=4 * MIB), INVALID), (dict(b=batch(n_requests=0)), INVALID)])
 def test_gated_products_that_are_refused(lib, bad, code):

@@ -46,6 +46,29 @@ def test_widths(cols, tokens):
     pu.Product(rng(5, tokens, *cols), tokens, 384, cols[:1], True).upload().check()
 
 
+@pytest.mark.parametrize("columns", [3000, 5000, 8000, 21000, 27000])
+@pytest.mark.parametrize("tokens", [1, 16, 18, 32, 40, 64])
+@pytest.mark.parametrize("adapters", [False, True])
+def test_tiles_of_few_and_many_columns(columns, tokens, adapters):
+    """Every tile that the numbers of columns and tokens choose, with rows and tokens left over at its end."""
+    ranks, max_rank = ([8, 3, 0, 16], 16) if adapters else ([], 0)
+    pu.Product(rng(20, columns, tokens, adapters), tokens, 392, [columns - 1000, 1000], False, ranks, max_rank, residual=True, pad=1).upload().check()
+    pu.Product(rng(21, columns, tokens, adapters), tokens, 392, [columns // 16 * 8], True, ranks, max_rank, pad=1).upload().check()
+
+
+@pytest.mark.parametrize("K,cols,tokens", [(16520, 104, 3), (16520, 24, 40), (16520, 6400, 40), (32768, 40, 1), (32768, 40, 50), (32776, 40, 1),
+                                           (32776, 24, 40), (40000, 24, 100), (65536, 40, 2), (65536, 24, 20)])
+def test_long_rows(K, cols, tokens):
+    pu.Product(rng(22, K, cols, tokens), tokens, K, [cols], False, [16, 5], 16).upload().check()
+    if K <= 32768 and cols < 1000:
+        pu.Product(rng(23, K, cols, tokens), tokens, K, [cols], True, [16, 5], 16).upload().check()
+
+
+def test_more_tokens_than_a_launch_takes():
+    pu.Product(rng(24), 4133, 264, [40, 24], False, RANKS, 32, residual=True, pad=7).upload().check()
+    pu.Product(rng(25), 4133, 264, [24], True, RANKS, 32, pad=7).upload().check()
+
+
 @pytest.mark.parametrize("max_rank", [8, 16, 24, 64, 72, 128])
 @pytest.mark.parametrize("tokens", [1, 16, 40, 150])
 @pytest.mark.parametrize("gated", [False, True])
