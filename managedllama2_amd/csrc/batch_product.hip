@@ -30,7 +30,7 @@ struct alignas(64) LowArgs {
     const int* token_adapters;
     int K, x_stride, n_tokens, most_adapters;
     uint16_t* packed; // non-null: the rows as operands, by the workgroups behind those of the tensors
-    int n_matrices, z_blocks; // z_blocks: workgroups that share a matrix's ranks
+    int n_matrices;
     LowTensor t[LLAMA2_MAX_BATCH_MATRICES];
 };
 
@@ -91,13 +91,85 @@ __global__ __launch_bounds__(512) void batch_pack_kernel(uint16_t* packed, const
 }
 
 // ---------------------------------------------------------------- what the ranks receive
-// A workgroup takes items of a block of 64 tokens, so that an adapter is read once for up to 16 tokens that use it, and ranks by 16; its
+// Few tokens: a wavefront takes a rank of a token's adapter, whose row of the adapter it sums up with the token's inputs in fp32; tokens that
+// share an adapter find it in the caches.  Nothing waits but the adapter's number for the arguments and its row for the number: ranks
+// and scales of small pools and the inputs are requested together with the number.
+constexpr int kRankWaves = 8, kRankLoads = 8;
+
+__global__ __launch_bounds__(kRankWaves * 64) void batch_ranks_kernel(LowArgs)
+{
+    auto& a = kernel_args<LowArgs>();
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), token = blockIdx.x;
+    const int K = a.K, x_stride = a.x_stride, n_tokens = a.n_tokens, most_adapters = a.most_adapters;
+    const uint16_t* const x = a.x;
+    const int *const positions = a.positions, *const token_adapters = a.token_adapters;
+    if (static_cast<int>(blockIdx.z) == a.n_matrices) {
+        pack_rows(a.packed, x, K, x_stride, n_tokens, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
+        return;
+    }
+    auto& t = a.t[blockIdx.z];
+    const uint16_t* const down = t.down;
+    const float* const scales = t.scales;
+    const int* const ranks = t.ranks;
+    float* const low = static_cast<float*>(t.low);
+    TokenAdapter* const info = t.info;
+    const long long down_stride = t.down_stride;
+    const int n_adapters = t.n_adapters, max_rank = t.max_rank;
+    loaded(K, x_stride, n_tokens, most_adapters, x, positions, token_adapters, down, scales, ranks, low, info, down_stride, n_adapters, max_rank);
+    const int r = blockIdx.y * kRankWaves + wave;
+    if (!down || r >= (max_rank + 15) / 16 * 16)
+        return;
+    const int position = positions[token], given = token_adapters[token];
+    int rank_table = 0;
+    float scale_table = 0.0f;
+    if (lane < n_adapters) {
+        rank_table = ranks[lane];
+        scale_table = scales[lane];
+    }
+    const __amdgpu_buffer_rsrc_t rx = rows_buffer(x + static_cast<size_t>(token) * x_stride, static_cast<size_t>(K) * 2);
+    u32x4 xv[kRankLoads], dv[kRankLoads];
+    auto request = [&](u32x4(&v)[kRankLoads], const __amdgpu_buffer_rsrc_t& row, int k0) { // elements behind the end are zero
+#pragma unroll
+        for (int i = 0; i < kRankLoads; ++i)
+            v[i] = __builtin_amdgcn_raw_buffer_load_b128(row, k0 * 2 + i * 1024 + lane * 16, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    request(xv, rx, 0);
+    const int id = __builtin_amdgcn_readfirstlane(known_adapter(position, given, most_adapters));
+    if (id < 0 || id >= n_adapters)
+        return;
+    const int rank = min(max(id < 64 ? __builtin_amdgcn_readlane(rank_table, id) : ranks[id], 0), max_rank);
+    const float scale = id < 64 ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale_table), id)) : scales[id];
+    float sum = 0.0f;
+    if (r < rank) {
+        const __amdgpu_buffer_rsrc_t rd = rows_buffer(down + id * down_stride + static_cast<size_t>(r) * K, static_cast<size_t>(K) * 2);
+        for (int k0 = 0; k0 < K; k0 += kRankLoads * 512) {
+            if (k0 > 0)
+                request(xv, rx, k0);
+            request(dv, rd, k0);
+#pragma unroll
+            for (int i = 0; i < kRankLoads; ++i)
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    sum = __builtin_fmaf(half_bits_to_float(static_cast<uint16_t>(dv[i][k >> 1] >> (16 * (k & 1)))),
+                                         half_bits_to_float(static_cast<uint16_t>(xv[i][k >> 1] >> (16 * (k & 1)))), sum);
+        }
+        sum = wave_sum(sum);
+    }
+    const size_t to = static_cast<size_t>(token) * ((max_rank + 15) / 16) + r / 16;
+    if (lane == 0 && r < (rank + 15) / 16 * 16)
+        low[to * 16 + r % 16] = sum * scale;
+    if (lane == 0 && r % 16 == 0)
+        info[to] = TokenAdapter{scale, rank};
+}
+
+// Many tokens: a workgroup takes items of a block of 64 tokens, so that an adapter is read once for up to 16 tokens that use it, and ranks by 16; its
 // wavefronts split the inputs.  Ranks and scales of small pools are requested together with the tokens' adapters.
-// WIDE: as two fp16 numbers and a power of two (what the matrix cores take), else in fp32, the adapter's scale with it.
+// They leave as two fp16 numbers and a power of two, which the matrix cores take.
 // CHUNKS of 128 inputs that a wavefront has requested; KEEP: they are all that there are, and the inputs stay for all ranks.
 constexpr int kLowWaves = 8, kLowTable = kLowWaves * 64;
 
-template <bool WIDE, int CHUNKS, bool KEEP>
+template <int CHUNKS, bool KEEP>
 __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
 {
     constexpr int kStride = 16 + 4;
@@ -108,19 +180,14 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
     __shared__ __align__(16) float red[kLowWaves * 16 * kStride];
     auto& a = kernel_args<LowArgs>();
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, c = lane >> 4;
-    const int t0 = blockIdx.x * 64, K = a.K, x_stride = a.x_stride, n_tokens = a.n_tokens, most_adapters = a.most_adapters, z_blocks = a.z_blocks;
+    const int t0 = blockIdx.x * 64, K = a.K, x_stride = a.x_stride, n_tokens = a.n_tokens, most_adapters = a.most_adapters;
     const uint16_t* const x = a.x;
     const int *const positions = a.positions, *const token_adapters = a.token_adapters;
-    const int which = blockIdx.z / z_blocks, first_block = blockIdx.z - which * z_blocks;
-    if (which == a.n_matrices) {
-        const int worker = (first_block * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x, workers = gridDim.x * gridDim.y * z_blocks;
-        if constexpr (WIDE)
-            pack_fragments(a.packed, x, K, x_stride, n_tokens, worker, workers);
-        else
-            pack_rows(a.packed, x, K, x_stride, n_tokens, worker, workers);
+    if (static_cast<int>(blockIdx.z) == a.n_matrices) {
+        pack_fragments(a.packed, x, K, x_stride, n_tokens, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
         return;
     }
-    auto& t = a.t[which];
+    auto& t = a.t[blockIdx.z];
     const uint16_t* const down = t.down;
     const float* const scales = t.scales;
     const int* const ranks = t.ranks;
@@ -129,7 +196,7 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
     const long long down_stride = t.down_stride;
     const int n_adapters = t.n_adapters, max_rank = t.max_rank;
     loaded(K, x_stride, n_tokens, most_adapters, x, positions, token_adapters, down, scales, ranks, lows, info, down_stride, n_adapters, max_rank);
-    if (!down || first_block * 16 >= max_rank)
+    if (!down)
         return;
     int mine = 0;
     float mine_scale = 0.0f;
@@ -180,7 +247,7 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
 #pragma unroll
         for (int q = 0; q < CHUNKS; ++q) {
             request_x(q, chunk(q));
-            request_d(q, chunk(q), first_block);
+            request_d(q, chunk(q), 0);
         }
         if constexpr (KEEP) {
 #pragma unroll
@@ -191,7 +258,7 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
                     xf[q][j] = tile_operand(lds, j);
             }
         }
-        for (int block = first_block; block == 0 || block * 16 < rank; block += z_blocks) { // the first one says that there are no ranks at all
+        for (int block = 0; block == 0 || block * 16 < rank; ++block) { // the first one says that there are no ranks at all
             f4_t acc = {};
             for (int k0 = wave * 128; k0 < K; k0 += CHUNKS * kLowWaves * 128) {
 #pragma unroll
@@ -210,7 +277,7 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         df[j] = tile_operand(lds, j);
-                    request_d(q, on ? next : chunk(q), on ? block : block + z_blocks);
+                    request_d(q, on ? next : chunk(q), on ? block : block + 1);
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         acc = mfma16(xf[KEEP ? q : 0][j], df[j], acc);
@@ -228,23 +295,17 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
                     v += red[(w * 16 + place) * kStride + l15];
                 v = block * 16 + l15 < rank ? v : 0.0f;
                 const size_t to = static_cast<size_t>(t0 + (m == kNobody ? 0 : m)) * ((max_rank + 15) / 16) + block;
-                if constexpr (WIDE) {
-                    const float most = row16_max(fabsf(v));
-                    // the largest between 2^14 and 2^15; nothing to scale where all are 0 or one is infinite
-                    const int e2 = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
-                    const float scaled = ldexpf(v, e2);
-                    const uint16_t h = float_to_half_bits(scaled);
-                    if (m != kNobody) {
-                        uint16_t* const low = static_cast<uint16_t*>(lows);
-                        low[to * 32 + l15] = h;
-                        low[to * 32 + 16 + l15] = float_to_half_bits(scaled - half_bits_to_float(h));
-                        if (l15 == 0)
-                            info[to] = TokenAdapter{ldexpf(scale, -e2), rank};
-                    }
-                } else if (m != kNobody) {
-                    static_cast<float*>(lows)[to * 16 + l15] = v * scale;
+                const float most = row16_max(fabsf(v));
+                // the largest between 2^14 and 2^15; nothing to scale where all are 0 or one is infinite
+                const int e2 = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
+                const float scaled = ldexpf(v, e2);
+                const uint16_t h = float_to_half_bits(scaled);
+                if (m != kNobody) {
+                    uint16_t* const low = static_cast<uint16_t*>(lows);
+                    low[to * 32 + l15] = h;
+                    low[to * 32 + 16 + l15] = float_to_half_bits(scaled - half_bits_to_float(h));
                     if (l15 == 0)
-                        info[to] = TokenAdapter{scale, rank};
+                        info[to] = TokenAdapter{ldexpf(scale, -e2), rank};
                 }
             }
             __syncthreads();
@@ -686,25 +747,26 @@ static int run_product(const char* fn, Product& p)
             l.most_adapters = a.most_adapters;
             l.n_matrices = p.n_matrices;
             l.packed = packed || wide ? reinterpret_cast<uint16_t*>(base) : nullptr;
-            // Items of a block of 64 tokens: one for each adapter in use, and one more for every 16 tokens.  Of few blocks every item and
-            // every 16 ranks have a workgroup; of many a workgroup takes several, since those with nothing to do cost as well.
-            const int blocks = ceil_div(a.n_tokens, 64), tokens = a.n_tokens < 64 ? a.n_tokens : 64;
-            const int items = a.most_adapters + 3 < tokens ? a.most_adapters + 3 : tokens;
-            int rank_blocks = 1;
+            int max_rank = 0;
             for (int i = 0; i < p.n_matrices; ++i)
-                if (l.t[i].down && ceil_div(l.t[i].max_rank, 16) > rank_blocks)
-                    rank_blocks = ceil_div(l.t[i].max_rank, 16);
-            l.z_blocks = wide ? 1 : rank_blocks;
-            const dim3 grid(blocks, wide && items > 8 ? 8 : items, (p.n_matrices + (l.packed ? 1 : 0)) * l.z_blocks), threads(kLowWaves * 64);
+                max_rank = l.t[i].down && l.t[i].max_rank > max_rank ? l.t[i].max_rank : max_rank;
             const hipStream_t st = ctx().stream;
-            if (!wide)
-                hipLaunchKernelGGL((batch_low_kernel<false, 4, false>), grid, threads, 0, st, l);
-            else if (a.K <= 4 * kLowWaves * 128)
-                hipLaunchKernelGGL((batch_low_kernel<true, 4, true>), grid, threads, 0, st, l);
-            else if (a.K <= 5 * kLowWaves * 128)
-                hipLaunchKernelGGL((batch_low_kernel<true, 5, true>), grid, threads, 0, st, l);
-            else
-                hipLaunchKernelGGL((batch_low_kernel<true, 4, false>), grid, threads, 0, st, l);
+            const int tensors = p.n_matrices + (l.packed ? 1 : 0);
+            if (!wide) {
+                hipLaunchKernelGGL(batch_ranks_kernel, dim3(a.n_tokens, round_up(max_rank, 16) / kRankWaves, tensors), dim3(kRankWaves * 64), 0, st, l);
+            } else {
+                // Items of a block of 64 tokens: one for each adapter in use, and one more for every 16 tokens.  A workgroup takes several
+                // where there are many, since those with nothing to do cost as well.
+                int items = a.n_tokens < 64 ? a.n_tokens : 64;
+                items = a.most_adapters + 3 < items ? a.most_adapters + 3 : items;
+                const dim3 grid(ceil_div(a.n_tokens, 64), items < 8 ? items : 8, tensors), threads(kLowWaves * 64);
+                if (a.K <= 4 * kLowWaves * 128)
+                    hipLaunchKernelGGL((batch_low_kernel<4, true>), grid, threads, 0, st, l);
+                else if (a.K <= 5 * kLowWaves * 128)
+                    hipLaunchKernelGGL((batch_low_kernel<5, true>), grid, threads, 0, st, l);
+                else
+                    hipLaunchKernelGGL((batch_low_kernel<4, false>), grid, threads, 0, st, l);
+            }
             L2_LAUNCH_CHECK(fn);
         }
         const uint16_t* const rows = a.x;
