@@ -341,7 +341,7 @@ __global__ __launch_bounds__(W * 64, 2) void batch_product_kernel(ProductArgs)
     constexpr int kTokens = T * 16, kRows = R * 16, kStride = kRows + 4, kTensors = GATED ? 2 : 1, RT = R / kTensors;
     constexpr int kRing = T * D <= 4 && !(R == 4 && T == 4) ? T * D : 2; // tiles of tokens whose inputs are on their way or in use
     static_assert(T * D % kRing == 0 && kRing <= T * D, "a tile has one place in the ring");
-    constexpr bool PACKED = T > 1; // the inputs come as operands; of few tokens in rows, which saves the launch that packs them
+    constexpr bool PACKED = T > 2; // the inputs come as operands; of few tokens in rows, which saves the launch that packs them
     constexpr int kWaveBytes = (PACKED ? 0 : kTileBytes) + R * 1024, kWordsAt = kWaveBytes - R * 1024;
     constexpr int kSums = W * kTokens * kStride * 4, kExtraAt = W * kWaveBytes + kScaleBytes, kFront = kExtraAt + (ADAPTERS ? kTokens * kStride * 4 : 0);
     __shared__ __align__(16) char pool[kFront > kSums ? kFront : kSums]; // the sums come where tiles, scales and the adapters' part were
@@ -657,36 +657,47 @@ constexpr int kMostTokens = 4096; // of a launch
 constexpr int kMostGroups = 256; // of rows whose inputs are packed; of more one tile of outputs has room for its scales
 
 // Tiles by how many columns all tensors of a call have beside the CUs: as few workgroups as have something for every CU, since every one
-// reads the inputs of its tokens.  Measured in us, without adapters, at 4096 inputs and with 256 CUs (W wavefronts, R tiles of outputs):
+// reads the inputs of its tokens, and as many wavefronts in them as the CU has room for.  Measured in us with 256 CUs (W wavefronts, R
+// tiles of outputs; 4096 inputs and no adapters where nothing else is said):
 //   tokens  columns          chosen          others
-//   1       4096             W 8, R 1  5.7   W 8, R 2  7.1;  W 4, R 2  7.5
-//   16      12288            W 4, R 2 11.2   W 8, R 1 12.2;  W 8, R 4 10.6, which at 4096 takes 9.1
+//   1       4096             W 8, R 1  5.7   W 12, R 2 6.6;  W 4, R 2  7.5
+//   1       5120 of 13824    W 12, R 2 14.2  W 8, R 1 16.9;  W 4, R 2 18.9
+//   16      12288            W 4, R 2 11.2   W 8, R 1 12.2
 //   16      32000            W 4, R 4 17.2   W 4, R 2 18.6;  W 8, R 1 25.4
 //   1       gated 2 * 11008  W 4, R 2 15.2   W 8, R 2 17.0;  W 4, R 4 16.4
-//   32      4096             W 8, R 1  8.3   W 8, R 2  9.5;  W 4, R 4 12.9
-//   32      12288            W 4, R 2 13.6   W 8, R 2 15.8;  W 8, R 1 16.7
-//   64      4096             two blocks of 32 tokens, W 4, R 2 10.6   one of 64, W 8, R 2 12.6, R 4 15.5
-//   64      6144             W 8, R 2 12.8   two blocks 16.2;  R 4 15.4
-//   64      12288            W 8, R 4 17.0   two blocks 17.7;  R 2 20.7
+//   32      4096             W 8, R 1  7.3   W 12, R 2 8.3;  W 8, R 4 11.7
+//   32      6144             W 12, R 2 9.1   W 8, R 1 11.1;  W 8, R 4 12.2
+//   32      12288            W 8, R 4 13.5   W 4, R 4 14.8;  W 8, R 1 15.6
+//   32      gated 2 * 11008, an adapter each   W 4, R 4 28.0   W 8, R 4 32.6;  W 4, R 2 30.1
+//   64      4096             two blocks of 32 tokens, W 12, R 2 8.5   one of 64, W 8, R 2 12.6;  R 4 15.5
+//   64      6144             W 8, R 2 12.8   R 4 15.4;  two blocks 16.1
+//   64      12288            W 8, R 4 17.0   R 2 20.7;  two blocks (48 tokens) 22.7
+// Inputs that come as operands (a launch more, or workgroups of the adapters' first kernel) pay off in blocks of 64 tokens (48 tokens of 12288
+// columns with adapters 23.8 against 27.2 with inputs in rows), not below (32 tokens of 4096 columns 8.3 against 7.3).
 // Scales and zero points of a workgroup's rows fit up to R * groups = 512.
+constexpr int kFewColumns = 16; // of a CU
+
 template <bool GATED>
-static void launch_shape(Product& p, int columns, int groups)
+static void launch_shape(Product& p, bool packed, int per_cu, int groups)
 {
-    const int n = p.a.n_tokens, per_cu = columns / ctx().num_cus;
+    const int n = p.a.n_tokens;
+    const bool high = groups <= kMostGroups / 2;
+    if (packed)
+        return per_cu > 24 && high ? launch_product<8, 4, 4, 1, GATED>(p) : launch_product<8, 2, 4, 1, GATED>(p);
     if constexpr (!GATED) { // a gated tile is one of both tensors
-        if (groups > kMostGroups || (n <= 16 && per_cu <= 24))
+        if (groups > kMostGroups || (n <= 16 && per_cu <= kFewColumns))
             return launch_product<8, 1, 1, 2, false>(p);
-        if (n > 16 && n <= 32 && per_cu <= 16)
-            return launch_product<8, 1, 2, 2, false>(p);
+        if (n <= 32 && per_cu <= kFewColumns)
+            return launch_product<8, 1, 2, 1, false>(p);
     }
-    if (n <= 16)
-        per_cu >= 100 && groups <= kMostGroups / 2 ? launch_product<4, 4, 1, 1, GATED>(p) : launch_product<4, 2, 1, 2, GATED>(p);
-    else if (n <= 32 || per_cu <= 16 || (groups > kMostGroups / 2 && per_cu > 24))
-        launch_product<4, 2, 2, 2, GATED>(p);
-    else if (per_cu <= 24)
-        launch_product<8, 2, 4, 1, GATED>(p);
+    if (n <= 16 && per_cu <= 32)
+        launch_product<12, 2, 1, 1, GATED>(p);
+    else if (n <= 16)
+        per_cu >= 100 && high ? launch_product<4, 4, 1, 1, GATED>(p) : launch_product<4, 2, 1, 2, GATED>(p);
+    else if (per_cu <= 24 || !high)
+        launch_product<12, 2, 2, 1, GATED>(p);
     else
-        launch_product<8, 4, 4, 1, GATED>(p);
+        per_cu < 64 ? launch_product<8, 4, 2, 1, GATED>(p) : launch_product<4, 4, 2, 1, GATED>(p);
 }
 
 template <bool GATED>
@@ -706,7 +717,8 @@ static int run_product(const char* fn, Product& p)
     // adapters, of which each tile reads those of all its tokens one after the other (gated 2 * 11008 columns of 4096 inputs, 32 tokens
     // 23.2 -> 18.6 us, 64 29.5 -> 24.2; with an adapter each 49 against 122; 2 * 8192 columns, 64 tokens 18.4 against 20.7).
     const bool wide = fits && (all > 64 || (all > 16 && !adapters && columns >= 80 * ctx().num_cus));
-    const bool packed = !wide && all > 16 && groups <= kMostGroups;
+    const int per_cu = columns / ctx().num_cus;
+    const bool packed = !wide && all > 32 && per_cu > kFewColumns && groups <= kMostGroups;
     const int step = groups <= kMostGroups ? kMostTokens : kMostTokens / 8; // threads of a launch in 32 bits
     const int most = all < step ? all : step;
     const size_t fragments = wide ? batch_gemm_bytes(most, a.K) : packed ? static_cast<size_t>(ceil_div(most, 16)) * groups * 4096 : 0;
@@ -783,7 +795,7 @@ static int run_product(const char* fn, Product& p)
             if (int rc = launch_batch_gemm(fn, a, p.n_matrices, GATED, p.adapters, p.adapters, base))
                 return rc;
         } else {
-            launch_shape<GATED>(p, columns, groups);
+            launch_shape<GATED>(p, packed, per_cu, groups);
             L2_LAUNCH_CHECK(fn);
         }
         a.x = rows + static_cast<size_t>(a.n_tokens) * a.x_stride;
