@@ -4,7 +4,8 @@
 //   y[t][n] = sum_g s[n][g] sum_{k in g} x[t][k] (w[n][k] - z[n][g])  +  f_a sum_r up_a[n][r] h[t][r],   h[t][r] = sum_k down_a[r][k] x[t][k]
 //
 // w - z is an exact fp16 integer, its products with x are summed in fp32 over a group of 128 and scaled in fp32.  h is summed in
-// fp32 and leaves as two fp16 numbers and a power of two (22 bits of the token's largest), which the matrix cores take as 16 ranks a product.
+// fp32; up to 64 tokens it meets the adapter's halfs in fp32 too, beyond that it leaves as two fp16 numbers and a power of two (22 bits of the
+// token's largest of 16), which the matrix cores take as 16 ranks a product.
 #include "batch_product.hpp"
 #include "prefill.hpp"
 
@@ -91,32 +92,58 @@ __global__ __launch_bounds__(512) void batch_pack_kernel(uint16_t* packed, const
 }
 
 // ---------------------------------------------------------------- what the ranks receive
+// Block `to` of 16 ranks, one in each of 16 lanes, as two fp16 numbers and a power of two, which the matrix cores take.
+__device__ __forceinline__ void put_parts(void* lows, TokenAdapter* info, size_t to, float v, float scale, int rank, bool write)
+{
+    const int l15 = threadIdx.x & 15;
+    const float most = row16_max(fabsf(v));
+    // the largest between 2^14 and 2^15; nothing to scale where all are 0 or one is infinite
+    const int e2 = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
+    const float scaled = ldexpf(v, e2);
+    const uint16_t h = float_to_half_bits(scaled);
+    if (!write)
+        return;
+    uint16_t* const low = static_cast<uint16_t*>(lows);
+    low[to * 32 + l15] = h;
+    low[to * 32 + 16 + l15] = float_to_half_bits(scaled - half_bits_to_float(h));
+    if (l15 == 0)
+        info[to] = TokenAdapter{ldexpf(scale, -e2), rank};
+}
+
 // Few tokens: a wavefront takes a rank of a token's adapter, whose row of the adapter it sums up with the token's inputs in fp32; tokens that
 // share an adapter find it in the caches.  Nothing waits but the adapter's number for the arguments and its row for the number: ranks
 // and scales of small pools and the inputs are requested together with the number.
-constexpr int kRankWaves = 8, kRankLoads = 8;
+// WIDE: as the prompt's products take them, a block of 16 ranks per workgroup.
+constexpr int kRankLoads = 8;
+constexpr int rank_waves(bool wide) { return wide ? 16 : 8; }
 
-__global__ __launch_bounds__(kRankWaves * 64) void batch_ranks_kernel(LowArgs)
+template <bool WIDE>
+__global__ __launch_bounds__(rank_waves(WIDE) * 64) void batch_ranks_kernel(LowArgs)
 {
+    __shared__ float received[rank_waves(WIDE)];
     auto& a = kernel_args<LowArgs>();
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), token = blockIdx.x;
     const int K = a.K, x_stride = a.x_stride, n_tokens = a.n_tokens, most_adapters = a.most_adapters;
     const uint16_t* const x = a.x;
     const int *const positions = a.positions, *const token_adapters = a.token_adapters;
     if (static_cast<int>(blockIdx.z) == a.n_matrices) {
-        pack_rows(a.packed, x, K, x_stride, n_tokens, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
+        const int worker = blockIdx.y * gridDim.x + blockIdx.x, workers = gridDim.x * gridDim.y;
+        if constexpr (WIDE)
+            pack_fragments(a.packed, x, K, x_stride, n_tokens, worker, workers);
+        else
+            pack_rows(a.packed, x, K, x_stride, n_tokens, worker, workers);
         return;
     }
     auto& t = a.t[blockIdx.z];
     const uint16_t* const down = t.down;
     const float* const scales = t.scales;
     const int* const ranks = t.ranks;
-    float* const low = static_cast<float*>(t.low);
+    void* const low = t.low;
     TokenAdapter* const info = t.info;
     const long long down_stride = t.down_stride;
     const int n_adapters = t.n_adapters, max_rank = t.max_rank;
     loaded(K, x_stride, n_tokens, most_adapters, x, positions, token_adapters, down, scales, ranks, low, info, down_stride, n_adapters, max_rank);
-    const int r = blockIdx.y * kRankWaves + wave;
+    const int r = blockIdx.y * rank_waves(WIDE) + wave;
     if (!down || r >= (max_rank + 15) / 16 * 16)
         return;
     const int position = positions[token], given = token_adapters[token];
@@ -157,15 +184,22 @@ __global__ __launch_bounds__(kRankWaves * 64) void batch_ranks_kernel(LowArgs)
         sum = wave_sum(sum);
     }
     const size_t to = static_cast<size_t>(token) * ((max_rank + 15) / 16) + r / 16;
-    if (lane == 0 && r < (rank + 15) / 16 * 16)
-        low[to * 16 + r % 16] = sum * scale;
-    if (lane == 0 && r % 16 == 0)
-        info[to] = TokenAdapter{scale, rank};
+    if constexpr (WIDE) {
+        if (lane == 0)
+            received[wave] = sum;
+        __syncthreads();
+        if (wave == 0)
+            put_parts(low, info, to, received[lane & 15], scale, rank, lane < 16);
+    } else {
+        if (lane == 0 && r < (rank + 15) / 16 * 16)
+            static_cast<float*>(low)[to * 16 + r % 16] = sum * scale;
+        if (lane == 0 && r % 16 == 0)
+            info[to] = TokenAdapter{scale, rank};
+    }
 }
 
 // Many tokens: a workgroup takes items of a block of 64 tokens, so that an adapter is read once for up to 16 tokens that use it, and ranks by 16; its
 // wavefronts split the inputs.  Ranks and scales of small pools are requested together with the tokens' adapters.
-// They leave as two fp16 numbers and a power of two, which the matrix cores take.
 // CHUNKS of 128 inputs that a wavefront has requested; KEEP: they are all that there are, and the inputs stay for all ranks.
 constexpr int kLowWaves = 8, kLowTable = kLowWaves * 64;
 
@@ -295,18 +329,7 @@ __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
                     v += red[(w * 16 + place) * kStride + l15];
                 v = block * 16 + l15 < rank ? v : 0.0f;
                 const size_t to = static_cast<size_t>(t0 + (m == kNobody ? 0 : m)) * ((max_rank + 15) / 16) + block;
-                const float most = row16_max(fabsf(v));
-                // the largest between 2^14 and 2^15; nothing to scale where all are 0 or one is infinite
-                const int e2 = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
-                const float scaled = ldexpf(v, e2);
-                const uint16_t h = float_to_half_bits(scaled);
-                if (m != kNobody) {
-                    uint16_t* const low = static_cast<uint16_t*>(lows);
-                    low[to * 32 + l15] = h;
-                    low[to * 32 + 16 + l15] = float_to_half_bits(scaled - half_bits_to_float(h));
-                    if (l15 == 0)
-                        info[to] = TokenAdapter{ldexpf(scale, -e2), rank};
-                }
+                put_parts(lows, info, to, v, scale, rank, m != kNobody);
             }
             __syncthreads();
         }
@@ -721,6 +744,16 @@ static int run_product(const char* fn, Product& p)
     const bool packed = !wide && all > 32 && per_cu > kFewColumns && groups <= kMostGroups;
     const int step = groups <= kMostGroups ? kMostTokens : kMostTokens / 8; // threads of a launch in 32 bits
     const int most = all < step ? all : step;
+    // More than 64 tokens: what the ranks receive token by token while that looks up little, else in items of tokens that share an adapter, more
+    // reluctantly where those read their inputs again for every 16 ranks (100 tokens of 16 adapters through gated 2 * 11008 columns of 4096, 16
+    // ranks, 52 MB: 66.3 us against 71.4; 200 through q, k and v of 4096, 32 ranks, 315 MB: 91.4 against 86.7; 128 of 13824 inputs, 64 ranks, 453 MB:
+    // 72.6 against 96.8).
+    const bool keeps = a.K <= 5 * kLowWaves * 128;
+    double looked_up = 0.0; // bytes
+    for (int i = 0; i < p.n_matrices; ++i)
+        if (l.t[i].down)
+            looked_up += 4.0 * all * a.K * l.t[i].max_rank;
+    const bool each = looked_up <= (keeps ? 2e8 : 5e8);
     const size_t fragments = wide ? batch_gemm_bytes(most, a.K) : packed ? static_cast<size_t>(ceil_div(most, 16)) * groups * 4096 : 0;
     p.adapters = adapters;
     size_t bytes = fragments;
@@ -765,7 +798,9 @@ static int run_product(const char* fn, Product& p)
             const hipStream_t st = ctx().stream;
             const int tensors = p.n_matrices + (l.packed ? 1 : 0);
             if (!wide) {
-                hipLaunchKernelGGL(batch_ranks_kernel, dim3(a.n_tokens, round_up(max_rank, 16) / kRankWaves, tensors), dim3(kRankWaves * 64), 0, st, l);
+                hipLaunchKernelGGL(batch_ranks_kernel<false>, dim3(a.n_tokens, round_up(max_rank, 16) / 8, tensors), dim3(512), 0, st, l);
+            } else if (each) {
+                hipLaunchKernelGGL(batch_ranks_kernel<true>, dim3(a.n_tokens, ceil_div(max_rank, 16), tensors), dim3(1024), 0, st, l);
             } else {
                 // Items of a block of 64 tokens: one for each adapter in use, and one more for every 16 tokens.  A workgroup takes several
                 // where there are many, since those with nothing to do cost as well.
@@ -774,7 +809,7 @@ static int run_product(const char* fn, Product& p)
                 const dim3 grid(ceil_div(a.n_tokens, 64), items < 8 ? items : 8, tensors), threads(kLowWaves * 64);
                 if (a.K <= 4 * kLowWaves * 128)
                     hipLaunchKernelGGL((batch_low_kernel<4, true>), grid, threads, 0, st, l);
-                else if (a.K <= 5 * kLowWaves * 128)
+                else if (keeps)
                     hipLaunchKernelGGL((batch_low_kernel<5, true>), grid, threads, 0, st, l);
                 else
                     hipLaunchKernelGGL((batch_low_kernel<4, false>), grid, threads, 0, st, l);

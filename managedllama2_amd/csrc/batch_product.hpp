@@ -166,11 +166,13 @@ __device__ __forceinline__ uint32_t dequant_pair(uint32_t w, int k, h2_t zlo /* 
                  : as_u32(as_h2((v & 0x000F000Fu) | magic) - zlo);
 }
 
-// Rows into fragment order, zeros behind the end of a row and in rows behind the last: `worker` of `workers`, 512 threads, a token tile and
+// Rows into fragment order, zeros behind the end of a row and in rows behind the last: by 512 threads of `worker` of `workers`, a token tile and
 // a group at a time.
 __device__ __forceinline__ void pack_fragments(uint16_t* xf, const uint16_t* x, int K, int x_stride, int n_tokens, int worker, int workers)
 {
     const int groups = (K + kGroup - 1) / kGroup, units = (n_tokens + 31) / 32 * groups;
+    if (threadIdx.x >= 512)
+        return;
     for (int u = worker; u < units; u += workers) {
         const int m = u / groups * 32 + (threadIdx.x >> 4), k = u % groups * kGroup + (threadIdx.x & 15) * 8;
         u32x4 v = {};

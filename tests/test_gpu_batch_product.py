@@ -84,6 +84,22 @@ def test_ranks(max_rank, tokens, gated):
     each.check("one for each")
 
 
+@pytest.mark.parametrize("tokens,K,max_rank", [(2000, 520, 72), (3001, 264, 64), (300, 5000, 64), (1100, 4096, 16), (150, 11008, 128)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_adapters_of_many_tokens(tokens, K, max_rank, gated):
+    """So many that tokens which share an adapter are taken together."""
+    ranks = [max_rank, 0, 1, max_rank // 2, max_rank - 1, 7]
+    for i, (ids, junk) in enumerate(((None, np.nan), (2, np.inf), (np.sort(rng(26, tokens).integers(-1, 7, tokens)), -np.inf))):
+        p = pu.Product(rng(27, tokens, gated, i), tokens, K, [40], gated, ranks, max_rank, pool_stride=16 * i, junk=junk, ids=ids).upload()
+        want = p.check(str(i))[0]
+    for pool in p.pools:
+        pool.up_of(2)[::3, :1] = np.nan
+    p.x[4, 5] = np.inf
+    got = p.upload().run()[0]
+    hit = (p.ids == 2) | (np.arange(tokens) == 4)
+    assert np.array_equal(got[~hit].view(np.uint16), want[~hit].view(np.uint16)) and not np.isfinite(got[hit]).all(1).any()
+
+
 def test_only_some_matrices_have_adapters():
     p = pu.Product(rng(9), 37, 256, [64, 128, 64], False, [8, 16], 16)
     p.pools[1] = None
