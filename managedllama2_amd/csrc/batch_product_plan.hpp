@@ -267,6 +267,7 @@ inline LogProbShape log_prob_shape(int rows, int vocab, int n_top, int cus)
 {
     const int least = ceil_div(vocab, 1 << 15), most = ceil_div(vocab, 1 << 12);
     int n = cus / rows < most ? cus / rows : most;
+    n = n < 64 ? n : 64; // a lane each puts them together
     n = n_top > 0 && n > 512 / n_top ? 512 / n_top : n;
     n = n > least ? n : least;
     LogProbShape s;

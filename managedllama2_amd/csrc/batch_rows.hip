@@ -470,7 +470,7 @@ __global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogPro
         return;
     if (tid == 0)
         store_agent(a.counters + row, 0u);
-    // A lane per segment (up to 32), and a thread per key.
+    // A lane per segment, and a thread per key.
     LogProbSums own = {-INFINITY, 0.0f, 0.0f};
     if (lane < a.segments)
         own = {load_agent(sums + lane * 4), load_agent(sums + lane * 4 + 1), load_agent(sums + lane * 4 + 2)};

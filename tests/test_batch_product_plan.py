@@ -34,6 +34,11 @@ int log_probs(float* lp, float* h, int* top, float* tlp, const llama2_half* x, c
 {
     return l2::check_batch_log_probs(lp, h, top, tlp, x, tokens, positions, rows, vocab, stride, n, n_top, temperature);
 }
+void shape(int rows, int vocab, int n_top, int cus, int* out)
+{
+    const l2::LogProbShape s = l2::log_prob_shape(rows, vocab, n_top, cus);
+    out[0] = s.segments, out[1] = s.length, out[2] = s.pieces;
+}
 }
 """
 NAMES = {"mat_mul": "llama2_batch_mat_mul_int4", "swiglu": "llama2_batch_mat_mul_swiglu", "norm": "llama2_batch_residual_rmsnorm",
@@ -196,6 +201,20 @@ def test_log_probabilities(lib):
         assert call(**bad) == INVALID, (bad, lib.last())
         assert b"llama2_batch_log_probs" in lib.last()
     assert call(vocab=(1 << 20) + 1, stride=(1 << 20) + 1) == UNSUPPORTED
+
+
+def test_how_rows_of_logits_are_cut(lib):
+    out = (C.c_int * 3)()
+    for rows in (1, 2, 3, 40, 255, 256, 300, 1 << 15):
+        for vocab in (1, 7, 8, 4095, 4096, 4097, 32000, 32768, 32769, 128000, 262144, (1 << 20) - 1, 1 << 20):
+            for n_top in (0, 1, 5, 64):
+                lib.shape(rows, vocab, n_top, 256, out)
+                segments, length, pieces = out
+                assert length % 8 == 0 and (segments - 1) * length < vocab <= segments * length, (rows, vocab, n_top)
+                assert length <= 4096 * pieces and pieces in (1, 2, 4, 8)  # what a workgroup's registers hold
+                assert segments <= 64 and segments * n_top <= 2048  # lanes, and keys in its memory
+                assert segments == 1 or vocab > 4096
+                assert segments * rows <= 256 or segments == -(-vocab // 32768) or length == 32768
 
 
 def test_calls_before_init_are_refused():

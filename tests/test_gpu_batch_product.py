@@ -4,6 +4,7 @@ import ctypes as C
 import os
 import subprocess
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -189,6 +190,51 @@ def test_captured_steps_replayed(tokens, gated):
         want, bound = p.reference()[0]
         assert (np.abs(got.astype(np.float64) - want) <= bound)[~dead].all(), turn
     capi.call("llama2_graph_destroy", g)
+
+
+def test_two_graphs_that_share_a_workspace():
+    """Steps of different kernels, captured one after the other and replayed in turn, with their packed inputs and what the ranks receive in
+    the library's scratch."""
+    steps, graphs = [], []
+    for i, (tokens, K, cols, gated) in enumerate(((1, 512, 96, False), (50, 392, 8000, False), (300, 640, 88, True))):
+        steps.append(pu.Product(rng(28, i), tokens, K, [cols], gated, RANKS, 32).upload())
+    want = [p.run()[0] for p in steps]
+    for p in steps:
+        outs, graph = p.outputs(), C.c_void_p()
+        capi.call("llama2_graph_begin_capture")
+        try:
+            capi.call(*p.args(outs))
+        finally:
+            capi.call("llama2_graph_end_capture", C.byref(graph))
+        graphs.append((graph, outs[0]))
+    for order in ((0, 1, 2), (2, 0, 1), (1, 1, 0, 2)):
+        for i in order:
+            graphs[i][1].copy_to_device(np.zeros(want[i].shape, np.float16))
+        for i in order:
+            capi.call("llama2_graph_launch", graphs[i][0])
+        for i in order:
+            assert np.array_equal(graphs[i][1].to_host().view(np.uint16), want[i].ravel().view(np.uint16)), (order, i)
+    for graph, _ in graphs:
+        capi.call("llama2_graph_destroy", graph)
+
+
+def test_threads_that_call_at_once():
+    steps = [pu.Product(rng(29, i), tokens, 392, [cols], bool(i % 2), RANKS, 32).upload()
+             for i, (tokens, cols) in enumerate(((1, 264), (20, 264), (50, 8000), (200, 88)))]
+    want = [p.run()[0] for p in steps]
+    wrong = []
+
+    def work(p, w):
+        for _ in range(20):
+            if not np.array_equal(p.run()[0].view(np.uint16), w.view(np.uint16)):
+                wrong.append(p.tokens)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(steps, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 CAPTURE = """

@@ -78,6 +78,13 @@ def test_numbers_of_rows(tokens):
     norm_check(norm_case(rng(3, tokens), tokens, 4096, pad=1))
 
 
+def test_results_larger_than_the_caches():
+    c = norm_case(rng(16), 2100, 4096, pad=3, input_gamma=True, gate=True, scale=0.5)
+    apart, place = norm_check(c), norm_check(c, in_place=True)
+    for a, b in zip(apart, place):
+        assert np.array_equal(a[:2100].view(np.uint16), b[:2100].view(np.uint16))
+
+
 def test_in_place():
     c = norm_case(rng(4), 40, 4096, pad=4, input_gamma=True, gate=True, extra=8)
     apart, place = norm_check(c), norm_check(c, in_place=True)
@@ -259,6 +266,12 @@ def test_segments_of_rows(rows):
             lp_check(x, g.integers(0, vocab, (rows, 2)).astype(np.int32), n_top, 0.7, pos)
 
 
+@pytest.mark.parametrize("vocab,n_top", [(270000, 1), (1 << 20, 0), (1 << 20, 2), (1000003, 64)])
+def test_vocabularies_of_many_segments(vocab, n_top):
+    g = rng(18, vocab, n_top)
+    lp_check(logits(g, 1, vocab), g.integers(0, vocab, (1, 3)).astype(np.int32), n_top)
+
+
 @pytest.mark.parametrize("temperature", [1e-3, 0.05, 1.0, 7.0, 1e4])
 def test_temperatures(temperature):
     g = rng(11, int(temperature * 1000))
@@ -274,6 +287,35 @@ def test_many_rows():
     got = lp_check(x, g.integers(0, 1001, (700, 2)).astype(np.int32), 5, positions=np.where(np.arange(700) % 7, 3, -1).astype(np.int32))
     again = lp_run(x, np.zeros((700, 2), np.int32), 5, positions=np.where(np.arange(700) % 7, 3, -1).astype(np.int32))
     assert np.array_equal(got["h"].view(np.uint32), again["h"].view(np.uint32))
+
+
+def test_two_graphs_that_share_a_workspace():
+    """Rows in segments, whose parts lie in the library's scratch: two graphs and eager calls take turns."""
+    g = rng(17)
+    shapes, graphs = ((2, 32000, 20), (5, 70001, 7)), []
+    for rows, vocab, n_top in shapes:
+        lp_run(logits(g, rows, vocab), np.zeros((rows, 1), np.int32), n_top)
+        x, h, top = up(logits(g, rows, vocab)), up(np.zeros(rows, np.float32)), up(np.zeros((rows, n_top), np.int32))
+        graph = C.c_void_p()
+        capi.call("llama2_graph_begin_capture")
+        try:
+            capi.call("llama2_batch_log_probs", None, h.ptr, top.ptr, None, x.ptr, None, None, rows, vocab, vocab, 0, n_top, 1.0)
+        finally:
+            capi.call("llama2_graph_end_capture", C.byref(graph))
+        graphs.append((graph, x, h, top))
+    for turn in range(4):
+        new = [logits(g, rows, vocab) for rows, vocab, _ in shapes]
+        for (graph, x, _, _), v in zip(graphs, new):
+            x.copy_to_device(v)
+        for graph, *_ in graphs[::1 - turn % 2 * 2]:
+            capi.call("llama2_graph_launch", graph)
+        lp_check(logits(g, 3, 40000), np.zeros((3, 1), np.int32), 5)
+        for (graph, x, h, top), v, (rows, vocab, n_top) in zip(graphs, new, shapes):
+            again = lp_run(v, np.zeros((rows, 1), np.int32), n_top)
+            assert np.array_equal(h.to_host().view(np.uint32), again["h"].view(np.uint32)), turn
+            assert np.array_equal(top.to_host().reshape(rows, n_top), [pu.top_tokens(r, n_top) for r in v]), turn
+    for graph, *_ in graphs:
+        capi.call("llama2_graph_destroy", graph)
 
 
 def test_both_captured_and_replayed():
