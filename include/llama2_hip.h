@@ -449,7 +449,7 @@ typedef struct llama2_batch_matrix {
  *   output[t][n] = half(residual[t][n] + sum_k input[t][k] * (w - z) * s + adapter's part),
  * sums in fp32, one rounding at the end; what an adapter's ranks receive of the input is fp32 too, and above 64 tokens keeps
  * 22 bits of the largest of them.
- * rows % 8 == 0, up to 65536; cols up to 2^20, input_stride up to 2^24; tensors are laid out as above (ceil(rows/32)*4 words, ceil(rows/128) scales per output).
+ * rows % 8 == 0, up to 65536; cols up to 2^20, input_stride up to 2^24; scales are finite; tensors are laid out as above (ceil(rows/32)*4 words, ceil(rows/128) scales per output).
  * Token t uses adapter token_adapters[t] of every matrix that has adapters; a value that is not one of 0 .. n_adapters - 1:
  * none.  What one token or one adapter holds has no influence on the rows of other tokens.  token_adapters may be null where no
  * matrix has adapters.  Rows of tokens without a position are left as they were.  Reads n_tokens and positions of

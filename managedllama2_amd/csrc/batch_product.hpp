@@ -33,6 +33,10 @@ struct alignas(64) ProductTensor {
     int cols, out_stride, residual_stride, n_adapters, max_rank;
 };
 
+// A step of one token, where the kernels of a decode step take its shape; false where they do not.
+struct ProductArgs;
+bool launch_one_token(const ProductArgs& call, int n_matrices, bool gated);
+
 struct alignas(64) ProductArgs {
     const uint16_t* x;
     const int* positions;

@@ -42,6 +42,9 @@ enum Mode {
     RESIDUAL = 1, // out[0][n] = half(sum + float(out[0][n]))
     SWIGLU = 2,   // out[0][n] = half(silu(gate.x) * (up.x))
     QKV_ROPE = 3, // q/k/v rows (i, i+64) of a head; q and k rotated; k, v written to the cache row of *pos
+    // of OneTokenArgs (span kernel only):
+    ONE_ROWS = 4,  // out[t][n] = half(residual[t][n] + sum + adapter's part)  (1 or 3 tensors)
+    ONE_GATED = 5, // out[0][n] = half(silu(gate) * up), with the adapters' parts
 };
 // Where the staged input comes from.
 enum Stage {
@@ -76,6 +79,21 @@ struct Int4Args {
     // those up to *pos_ptr count
     const float* parts;
     int block_shift;
+};
+
+// A step of one token (batch_one.hip): its position, its adapter, and what that one's ranks received of the input.
+struct OneTokenArgs : Int4Args {
+    const int* positions;
+    const int* token_adapters;
+    int most_adapters;
+    const uint16_t* residual[3];
+    struct {
+        const uint16_t* up; // null: no adapters
+        const float* low;
+        const int* used;
+        long long up_stride;
+        int n_adapters, max_rank;
+    } part[3];
 };
 
 constexpr int kAuxStream = 2; // "nt": weights are touched once
@@ -695,9 +713,10 @@ constexpr int span_scale_words(int J, int ROWS)
     return span_single_scales(J) ? (ROWS * 16 + 63) / 64 : (ROWS * 16 * J + 127) / 128;
 }
 
-template <int J, int MODE, int STAGE, int TN, int WAVES, int ROWS>
-__global__ __launch_bounds__(WAVES * 64) void int4_matvec_span_kernel(Int4Args a, SpanPlan plan)
+template <int J, int MODE, int STAGE, int TN, int WAVES, int ROWS, class Args>
+__global__ __launch_bounds__(WAVES * 64) void int4_matvec_span_kernel(Args a, SpanPlan plan)
 {
+    constexpr bool ONE = MODE == ONE_ROWS || MODE == ONE_GATED;
     // The rows i and i + 64 of a RoPE pair are not neighbours: their scales and zero words are two runs, one to each
     // half of the lanes.
     constexpr bool PAIR = MODE == QKV_ROPE && ROWS == 2;
@@ -772,6 +791,11 @@ __global__ __launch_bounds__(WAVES * 64) void int4_matvec_span_kernel(Int4Args a
         asm volatile("" : "+v"(pos_bits)); // stays where it is written
         return __builtin_amdgcn_readfirstlane(static_cast<int>(pos_bits)); // 0 without pos_ptr: nothing was read
     };
+    uint32_t one_position = 0, one_adapter = 0;
+    if constexpr (ONE) {
+        one_position = __builtin_amdgcn_raw_buffer_load_b32(make_rsrc(a.positions, 4), 0, 0, 0);
+        one_adapter = __builtin_amdgcn_raw_buffer_load_b32(make_rsrc(a.token_adapters, a.token_adapters ? 4 : 0), 0, 0, 0);
+    }
     // input next, then the span's scales / zero words / residuals, then the first row
     const bool stager = WAVES == 4 || threadIdx.x < 256;
     VecPieces<J> xp, gp;
@@ -846,6 +870,12 @@ __global__ __launch_bounds__(WAVES * 64) void int4_matvec_span_kernel(Int4Args a
         const __amdgpu_buffer_rsrc_t ro = make_rsrc(uniform_ptr(a.out[0] + r0), n * 2);
         res = __builtin_amdgcn_raw_buffer_load_b16(ro, lane * 2, 0, 0);
     }
+    uint32_t one_res[TN] = {};
+    if constexpr (MODE == ONE_ROWS)
+#pragma unroll
+        for (int t = 0; t < TN; ++t)
+            one_res[t] = __builtin_amdgcn_raw_buffer_load_b16(
+                make_rsrc(uniform_ptr(a.residual[t] + r0), a.residual[t] ? n * 2 : 0), lane * 2, 0, 0);
     asm volatile("" ::: "memory"); // the small loads stay ahead of the weights in the memory queue
     u32x4 ring[2][J];
     load_w(ring[0], 0);
@@ -917,6 +947,29 @@ __global__ __launch_bounds__(WAVES * 64) void int4_matvec_span_kernel(Int4Args a
     if (J <= 2)
         keep_meta();
 
+    // The adapter's part of a row is two ranks per lane, on top of the lane's share of the row: all rows' requested here, behind the first row of
+    // weights, together with what the ranks received.  Without an adapter from nowhere: loads that come and go would make every wait one for
+    // all of them.
+    uint32_t one_up[ONE ? Q : 1], one_rank[TN];
+    u32x2 one_low[TN];
+    if constexpr (ONE) {
+        const int position = __builtin_amdgcn_readfirstlane(static_cast<int>(one_position));
+        const int id = __builtin_amdgcn_readfirstlane(static_cast<int>(one_adapter));
+        n = position < 0 ? 0 : n; // nothing is written
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+            const auto& p = a.part[t];
+            const bool has = n > 0 && a.token_adapters && id >= 0 && id < p.n_adapters;
+            const __amdgpu_buffer_rsrc_t ru = make_rsrc(uniform_ptr(p.up + (has ? id * p.up_stride + static_cast<size_t>(r0) * p.max_rank : 0)),
+                                                        has ? n * p.max_rank * 2 : 0);
+            one_rank[t] = __builtin_amdgcn_raw_buffer_load_b32(make_rsrc(p.used, has ? 4 : 0), 0, 0, 0);
+            one_low[t] = __builtin_amdgcn_raw_buffer_load_b64(make_rsrc(p.low, has ? (p.max_rank + 15) / 16 * 64 : 0), lane * 8, 0, 0);
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i)
+                one_up[i * TN + t] = __builtin_amdgcn_raw_buffer_load_b32(ru, lane * 2 < p.max_rank ? lane * 4 : kNowhere, i * p.max_rank * 2, 0);
+        }
+    }
+
     const int zshift = ((lane >> 2) & 7) * 4; // nibble of the zero word: group (c/4) % 8, same for every j
     float outv[TN];
 #pragma unroll
@@ -945,6 +998,12 @@ __global__ __launch_bounds__(WAVES * 64) void int4_matvec_span_kernel(Int4Args a
         }
         float acc[1];
         dot_frag<J, 1>(acc, cur, xs, sx, lane, zshift);
+        if constexpr (ONE) { // what lies behind the rank is no number
+            const int have = __builtin_amdgcn_readfirstlane(static_cast<int>(one_rank[t])) - 2 * lane;
+            const uint32_t v = one_up[q] & (have > 1 ? ~0u : have > 0 ? 0xFFFFu : 0u);
+            acc[0] = fmaf(half_bits_to_float(static_cast<uint16_t>(v)), __uint_as_float(have > 0 ? one_low[t][0] : 0u), acc[0]);
+            acc[0] = fmaf(half_bits_to_float(static_cast<uint16_t>(v >> 16)), __uint_as_float(have > 1 ? one_low[t][1] : 0u), acc[0]);
+        }
         const float s = wave_sum(acc[0]);
         outv[t] = lane == i ? s : outv[t];
     }
@@ -999,7 +1058,11 @@ __global__ __launch_bounds__(WAVES * 64) void int4_matvec_span_kernel(Int4Args a
             vdst[r0] = float_to_half_bits(outv[TN > 2 ? 2 : 0]);
         }
     } else if (lane < n) {
-        if (MODE == SWIGLU) {
+        if constexpr (MODE == ONE_ROWS) {
+#pragma unroll
+            for (int t = 0; t < TN; ++t)
+                a.out[t][r0 + lane] = float_to_half_bits(outv[t] + half_bits_to_float(static_cast<uint16_t>(one_res[t])));
+        } else if (MODE == SWIGLU || MODE == ONE_GATED) {
             float v = outv[0];
             v *= 1.0f / (1.0f + expf(-v)); // native/mat_vec_kernel.cu:219-221
             v *= outv[TN - 1];
@@ -1113,10 +1176,10 @@ inline int resident_waves()
 
 // The span kernel for this launch, if the shape suits it: scales readable 4 bytes at a time, and
 // all wavefronts resident at once with ROWS rows each.
-template <int J, int MODE, int STAGE, int TN, int WAVES, int ROWS>
-inline bool try_span(const Int4Args& a, bool launch = true)
+template <int J, int MODE, int STAGE, int TN, int WAVES, int ROWS, class Args>
+inline bool try_span(const Args& a, bool launch = true)
 {
-    constexpr auto kernel = int4_matvec_span_kernel<J, MODE, STAGE, TN, WAVES, ROWS>;
+    constexpr auto kernel = int4_matvec_span_kernel<J, MODE, STAGE, TN, WAVES, ROWS, Args>;
     SpanPlan plan{};
     if (MODE == QKV_ROPE) {
         if (a.N % kRopeHeadSize)
@@ -1151,10 +1214,10 @@ inline bool span_allowed(const Int4Args& a, int tensors)
     return span_single_scales(J) || scales_in_pairs(a, tensors);
 }
 
-template <int J, int MODE, int STAGE>
-inline bool launch_span(const Int4Args& a)
+template <int J, int MODE, int STAGE, class Args>
+inline bool launch_span(const Args& a)
 {
-    if (!span_allowed<J>(a, MODE == SWIGLU ? 2 : a.n_tensors))
+    if (!span_allowed<J>(a, MODE == SWIGLU || MODE == ONE_GATED ? 2 : a.n_tensors))
         return false;
     // Rows per wavefront and wavefronts per workgroup as measured on the 7B / 13B shapes: one row per
     // wavefront where that many wavefronts fit, three for the SwiGLU pair of tensors.
@@ -1169,7 +1232,7 @@ inline bool launch_span(const Int4Args& a)
             return a.n_tensors == 3 && ceil_div(a.N / 2, 12) <= cus && try_span<J, MODE, STAGE, 3, 12, 2>(a);
         else
             return a.n_tensors == 3 && try_span<J, MODE, STAGE, 3, 8, 1>(a);
-    } else if constexpr (MODE == SWIGLU) {
+    } else if constexpr (MODE == SWIGLU || MODE == ONE_GATED) {
         // 13824 rows 14.9 us (8 wavefronts of four rows) -> 14.2, 14336 15.0 -> 14.3; three rows keep what they fit: 12288
         // rows 12.9 us, 13.4 with seven
         if constexpr (J == 3) {
@@ -1188,7 +1251,7 @@ inline bool launch_span(const Int4Args& a)
                 return true;
         }
         return try_span<J, MODE, STAGE, 2, 8, 3>(a) || try_span<J, MODE, STAGE, 2, 8, 4>(a);
-    } else if constexpr (MODE == PLAIN) {
+    } else if constexpr (MODE == PLAIN || MODE == ONE_ROWS) {
         // 4224 / 5120 / 6144 rows 10.2 / 10.7 / 11.2 us (8 wavefronts of two rows) -> 8.6 / 9.3 / 10.4; up to 4096 rows two
         // workgroups per compute unit hold 8 wavefronts of one row: 2048 / 4096 rows 6.1 / 8.3 us, 8.2 / 8.6 with 12 of two
         if constexpr (J == 3) {
@@ -1207,7 +1270,7 @@ inline bool launch_span(const Int4Args& a)
         if (a.n_tensors != 1)
             return false;
     }
-    if constexpr (MODE == PLAIN || MODE == RESIDUAL) {
+    if constexpr (MODE == PLAIN || MODE == RESIDUAL || MODE == ONE_ROWS) {
         // One tensor whose rows fill one workgroup of 16 wavefronts on every compute unit: a quarter of the staging, and nobody waits
         // for a second workgroup.  4096 rows of 4096 / 2560 inputs 3.87 / 3.61 us (4 wavefronts) -> 3.77 / 3.44, in the step of 7B behind
         // 255 rows 0.3 %; 3072 rows, which leave compute units empty, are 3.46 with 4 wavefronts and 3.69 with 16.  2304 .. 4096 inputs by

@@ -47,6 +47,45 @@ def test_widths(cols, tokens):
     pu.Product(rng(5, tokens, *cols), tokens, 384, cols[:1], True).upload().check()
 
 
+@pytest.mark.parametrize("K", [8, 120, 512, 1032, 2048, 4096, 5120, 8192, 10240, 11008, 13824, 14336, 14344])
+@pytest.mark.parametrize("max_rank", [0, 16, 128])
+def test_one_token(K, max_rank):
+    """One tensor, three of one width, gate and up: on the kernels of a decode step where they take the shape."""
+    for i, (cols, gated) in enumerate((([72], False), ([136] * 3, False), ([1000], True), ([520], False))):
+        ranks = [max_rank, 0, 3, max_rank - 1] if max_rank else ()
+        for id in (0, 2, 3, 1, -1) if max_rank else (-1,):
+            p = pu.Product(rng(30, K, max_rank, i, id + 1), 1, K, cols, gated, ranks, max_rank, residual=not gated and i != 1, pool_stride=8 * i, extra=8,
+                           x_extra=8, ids=id)
+            if i == 1:
+                p.pools[1] = None
+                p.residual = [p.x[:, :8].repeat(18, 1)] * 3
+            p.upload().check(str((i, id)))
+    p.positions[:] = -1
+    p.live = 0
+    got = p.upload().run()[0]
+    assert (got == pu.GUARD).all()
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 50, 70])
+def test_scales_and_zero_points_at_odd_places(tokens):
+    for gated in (False, True):
+        p = pu.Product(rng(31, tokens, gated), tokens, 520, [88], gated).upload()
+        want = p.run()[0]
+        moved = []
+        for (_, Z, S), w in zip(p.q, p.weights):
+            s, z = pu.up(np.concatenate([np.full(1, np.nan, np.float16), S.ravel()])), pu.up(np.concatenate([np.full(1, 77, np.uint32), Z.ravel()]))
+            moved.append((capi.QWeight(w.Weight.ptr, z.ptr + 4, s.ptr + 2), s, z))
+        outs = p.outputs()
+        name, *args = p.args(outs)
+        if gated:
+            args[2], args[3] = moved[0][0], moved[1][0]
+        else:
+            args[0][0].weight = moved[0][0]
+        capi.call(name, *args)
+        got = outs[0].to_host().reshape(want.shape).astype(np.float64)
+        assert (np.abs(got[:tokens] - p.reference()[0][0]) <= p.reference()[0][1]).all()
+
+
 @pytest.mark.parametrize("columns", [3000, 5000, 8000, 21000, 27000])
 @pytest.mark.parametrize("tokens", [1, 16, 18, 32, 40, 64])
 @pytest.mark.parametrize("adapters", [False, True])
