@@ -111,8 +111,9 @@ __device__ __forceinline__ void put_parts(void* lows, TokenAdapter* info, size_t
 }
 
 // Few tokens: a wavefront takes a rank of a token's adapter, whose row of the adapter it sums up with the token's inputs in fp32; tokens that
-// share an adapter find it in the caches.  Nothing waits but the adapter's number for the arguments and its row for the number: ranks
-// and scales of small pools and the inputs are requested together with the number.
+// share an adapter find it in the caches.  A chain of loads bounds it, so nothing waits but the adapter's number for the arguments and its row
+// for the number: ranks and scales of small pools and the inputs are requested together with the number.  4096 inputs, one token, 16 ranks 2.8 us;
+// 5120 inputs, 64 tokens with an adapter each through two tensors 6.6 (taken in items, as below, 6.6 and 11.9).
 // WIDE: as the prompt's products take them, a block of 16 ranks per workgroup.
 constexpr int kRankLoads = 8;
 constexpr int rank_waves(bool wide) { return wide ? 16 : 8; }
@@ -198,8 +199,10 @@ __global__ __launch_bounds__(rank_waves(WIDE) * 64) void batch_ranks_kernel(LowA
     }
 }
 
-// Many tokens: a workgroup takes items of a block of 64 tokens, so that an adapter is read once for up to 16 tokens that use it, and ranks by 16; its
-// wavefronts split the inputs.  Ranks and scales of small pools are requested together with the tokens' adapters.
+// Many tokens, for whom adapters would be looked up too often that way: a workgroup takes items of a block of 64 tokens, so that an adapter is
+// read once for up to 16 tokens that use it, and ranks by 16; its wavefronts split the inputs.  Ranks and scales of small pools are
+// requested together with the tokens' adapters.  1100 tokens of 4096 inputs through three tensors of 64 ranks 19.6 us: look-ups of the adapters and
+// their turn through LDS, 5 us each, behind the chain of tokens, items and rows.
 // CHUNKS of 128 inputs that a wavefront has requested; KEEP: they are all that there are, and the inputs stay for all ranks.
 constexpr int kLowWaves = 8, kLowTable = kLowWaves * 64;
 
@@ -357,7 +360,14 @@ struct __attribute__((packed, aligned(4))) AnyWords {
 constexpr int kScaleBytes = 20480; // of LDS for the scales and zero points of a workgroup's rows
 
 // A workgroup takes R tiles of 16 outputs (GATED: half of them of the gate, half of the up projection) and T tiles of 16
-// tokens; its W wavefronts take the groups of 128 inputs in turn, D of them requested ahead, and add up through LDS.
+// tokens; its W wavefronts take the groups of 128 inputs in turn, D of them requested ahead, and add up through LDS.  Every weight is read
+// once and unpacked once for all tokens of a tile.
+//
+// What bounds it: a group's inputs are T / R * 4 times the bytes of its weights, and a CU looks up 64 bytes per cycle, so higher tiles read
+// less and leave CUs without a workgroup; in front and behind stand the arguments, the adapters' chain of loads, scales through LDS and the sums, about
+// 5 us.  48 tokens, 12288 columns of 4096 inputs with adapters 18.6 us (2.4 TB/s of weights and adapters), 64 tokens, gated 2 * 13824
+// columns of 5120 with an adapter each 50 (35 without: 432 workgroups are two rounds), 24 tokens, 5120 columns of 13824 20.5.  K cut
+// over several workgroups won 7 % on long rows and is not here.
 template <int W, int R, int T, int D, bool GATED, bool ADAPTERS>
 __global__ __launch_bounds__(W * 64, 2) void batch_product_kernel(ProductArgs)
 {

@@ -630,6 +630,9 @@ __global__ __launch_bounds__(512, 2) void prefill_gemm_kernel(GemmArgs a)
     gemm_block<MT, WN, WK, EPI>(a, lds, unit, mb);
 }
 
+// Products of many tokens for their own sake: the same blocks, any number of rows per tensor, adapters onto the sums in LDS by the wavefront whose
+// outputs they are.  The matrix cores and what unpacks for them bound it: 1100 tokens, 6144 columns of 4096 inputs with adapters of 64
+// ranks 85 us, 650 TFLOP/s; 700 tokens, gated 2 * 11008 columns 170, 740.
 template <int MT, int MT2, int WN, int WK, int EPI>
 __global__ __launch_bounds__(512, 2) void batch_gemm_kernel(BatchGemmArgs b)
 {
