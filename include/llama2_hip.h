@@ -448,8 +448,8 @@ typedef struct llama2_batch_matrix {
 /* Products of all tokens of a step with up to LLAMA2_MAX_BATCH_MATRICES int4 tensors that read the same input (q, k and
  * v; or one):
  *   output[t][n] = half(residual[t][n] + sum_k input[t][k] * (w - z) * s + adapter's part),
- * sums in fp32, one rounding at the end; what an adapter's ranks receive of the input is fp32 too, and above 64 tokens keeps
- * 22 bits of the largest of them.
+ * sums in fp32, one rounding at the end; what an adapter's ranks receive of the input is fp32 too, and above 64 tokens may keep
+ * no more than 22 bits of the largest of 16 of them.
  * rows % 8 == 0, up to 65536; cols up to 2^20, input_stride up to 2^24; scales are finite; tensors are laid out as above (ceil(rows/32)*4 words, ceil(rows/128) scales per output).
  * Token t uses adapter token_adapters[t] of every matrix that has adapters; a value that is not one of 0 .. n_adapters - 1:
  * none.  What one token or one adapter holds has no influence on the rows of other tokens.  token_adapters may be null where no

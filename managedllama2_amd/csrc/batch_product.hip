@@ -4,8 +4,8 @@
 //   y[t][n] = sum_g s[n][g] sum_{k in g} x[t][k] (w[n][k] - z[n][g])  +  f_a sum_r up_a[n][r] h[t][r],   h[t][r] = sum_k down_a[r][k] x[t][k]
 //
 // w - z is an exact fp16 integer, its products with x are summed in fp32 over a group of 128 and scaled in fp32.  h is summed in
-// fp32; up to 64 tokens it meets the adapter's halfs in fp32 too, beyond that it leaves as two fp16 numbers and a power of two (22 bits of the
-// token's largest of 16), which the matrix cores take as 16 ranks a product.
+// fp32; in the tiles here it meets the adapter's halfs in fp32 too, for the prompt's kernels it leaves as two fp16 numbers and a power of two (22
+// bits of the token's largest of 16), which the matrix cores take as 16 ranks a product.
 #include "batch_product.hpp"
 #include "prefill.hpp"
 
@@ -739,18 +739,27 @@ static int run_product(const char* fn, Product& p)
     ProductArgs& a = p.a;
     LowArgs& l = p.low;
     const int all = a.n_tokens, groups = weight_groups(a.K);
-    int columns = 0;
+    int columns = 0, max_rank = 0;
     bool fits = true, adapters = false; // the prompt's products hold a tensor's offsets in 31 bits
     for (int i = 0; i < p.n_matrices; ++i) {
         columns += a.t[i].cols; // at most 2^22
         fits = fits && static_cast<long long>(a.t[i].cols) * weight_words(a.K) * 4 <= 0x7FFFFFFFLL;
-        adapters = adapters || l.t[i].down;
+        if (!l.t[i].down)
+            continue;
+        adapters = true;
+        max_rank = l.t[i].max_rank > max_rank ? l.t[i].max_rank : max_rank;
+        a.most_adapters = l.t[i].n_adapters > a.most_adapters ? l.t[i].n_adapters : a.most_adapters;
     }
+    const int per_cu = columns / ctx().num_cus;
     // More than 64 tokens go through the kernels of the prompt's products, and more than 16 where these have tiles for every CU and no
     // adapters, of which each tile reads those of all its tokens one after the other (gated 2 * 11008 columns of 4096 inputs, 32 tokens
     // 23.2 -> 18.6 us, 64 29.5 -> 24.2; with an adapter each 49 against 122; 2 * 8192 columns, 64 tokens 18.4 against 20.7).
-    const bool wide = fits && (all > 64 || (all > 16 && !adapters && columns >= 80 * ctx().num_cus));
-    const int per_cu = columns / ctx().num_cus;
+    // For the same reason up to 192 tokens with many adapters of few ranks do not (in us, prompt's kernels against these tiles: 128 tokens through
+    // q, k and v of 4096 with 128 adapters of 16 ranks 53.8, 40.2, 4 of 16 36.1, 35.4, 32 of 32 55.6, 47.8, 4 of 64 46.0, 71.5; 192 with 64 of 16
+    // 80.0, 56.7; gated 2 * 11008, 100 with 16 of 32 82.3, 62.6; 256 through one of 4096 with 64 of 16 33.9, 39.9), nor up to 128 for a few columns
+    // (2048 of 2048 inputs 10.5, 6.0; 128 tokens through 4096 of 4096 15.4, 16.1).
+    const int tile_tokens = adapters ? (max_rank <= 32 && 2 * a.most_adapters >= max_rank ? 192 : 64) : per_cu <= 8 ? 128 : 64;
+    const bool wide = fits && (all > tile_tokens || (all > 16 && !adapters && per_cu >= 80));
     const bool packed = !wide && all > 32 && per_cu > kFewColumns && groups <= kMostGroups;
     const int step = groups <= kMostGroups ? kMostTokens : kMostTokens / 8; // threads of a launch in 32 bits
     const int most = all < step ? all : step;
@@ -768,10 +777,8 @@ static int run_product(const char* fn, Product& p)
     p.adapters = adapters;
     size_t bytes = fragments;
     for (int i = 0; i < p.n_matrices; ++i)
-        if (l.t[i].down) {
+        if (l.t[i].down)
             bytes += static_cast<size_t>(most) * ceil_div(l.t[i].max_rank, 16) * (64 + sizeof(TokenAdapter));
-            a.most_adapters = l.t[i].n_adapters > a.most_adapters ? l.t[i].n_adapters : a.most_adapters;
-        }
     if (bytes)
         if (int rc = ensure_attn_partials(bytes))
             return rc;
@@ -802,9 +809,6 @@ static int run_product(const char* fn, Product& p)
             l.most_adapters = a.most_adapters;
             l.n_matrices = p.n_matrices;
             l.packed = packed || wide ? reinterpret_cast<uint16_t*>(base) : nullptr;
-            int max_rank = 0;
-            for (int i = 0; i < p.n_matrices; ++i)
-                max_rank = l.t[i].down && l.t[i].max_rank > max_rank ? l.t[i].max_rank : max_rank;
             const hipStream_t st = ctx().stream;
             const int tensors = p.n_matrices + (l.packed ? 1 : 0);
             if (!wide) {

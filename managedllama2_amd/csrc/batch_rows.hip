@@ -181,7 +181,6 @@ struct __attribute__((packed, aligned(2))) AnyHalfs { // 16 bytes of halfs
 };
 
 constexpr int kLogProbWaves = 8, kLogProbThreads = kLogProbWaves * 64, kCandidates = 2048, kQuads = kLogProbThreads / 4;
-constexpr int kLongestSegment = 8 * 8 * kLogProbThreads;
 
 struct LogProbLds {
     float sums[2][kLogProbWaves], largest[kLogProbWaves];

@@ -96,6 +96,14 @@ def test_tiles_of_few_and_many_columns(columns, tokens, adapters):
     pu.Product(rng(21, columns, tokens, adapters), tokens, 392, [columns // 16 * 8], True, ranks, max_rank, pad=1).upload().check()
 
 
+@pytest.mark.parametrize("columns", [3000, 5000, 8000])
+@pytest.mark.parametrize("tokens", [65, 130, 192, 193])
+def test_several_blocks_of_tokens_with_many_adapters(columns, tokens):
+    ranks = [8, 3, 0, 16, 7, 16, 1, 15, 4, 2]
+    pu.Product(rng(32, columns, tokens), tokens, 392, [columns - 1000, 1000], False, ranks, 16, residual=True, pad=1).upload().check()
+    pu.Product(rng(33, columns, tokens), tokens, 392, [columns // 16 * 8], True, ranks, 16, pad=1).upload().check()
+
+
 @pytest.mark.parametrize("K,cols,tokens", [(16520, 104, 3), (16520, 24, 40), (16520, 6400, 40), (32768, 40, 1), (32768, 40, 50), (32776, 40, 1),
                                            (32776, 24, 40), (40000, 24, 100), (65536, 40, 2), (65536, 24, 20)])
 def test_long_rows(K, cols, tokens):
