@@ -176,6 +176,8 @@ __device__ __forceinline__ unsigned long long key_of(unsigned order, int i) { re
 
 __device__ __forceinline__ uint16_t element(const u32x4& v, int k) { return static_cast<uint16_t>(v[k >> 1] >> (16 * (k & 1))); }
 
+constexpr int kNotThere = -1;
+
 struct __attribute__((packed, aligned(2))) AnyHalfs { // 16 bytes of halfs
     u32x4 v;
 };
@@ -195,8 +197,9 @@ struct LogProbSums {
     float top, total, moment; // sum of e = exp((x - top) / T), and of e (x - top)
 };
 
-// What a row answers: by all threads, from its sums and its likeliest tokens in `found` (`have` of them, in any order).
-__device__ __forceinline__ void answer_row(const LogProbArgs& a, int row, const LogProbSums& s, const unsigned long long* found, int have)
+// What a row answers: by all threads, from its sums and its likeliest tokens in `found` (`have` of them, in any order).  given: the logit of the
+// thread's first given token, kNotThere of one that is not.
+__device__ __forceinline__ void answer_row(const LogProbArgs& a, int row, const LogProbSums& s, const unsigned long long* found, int have, int given)
 {
     const uint16_t* const x = a.logits + static_cast<size_t>(row) * a.stride;
     const bool wrong = s.top == INFINITY || s.total != s.total;
@@ -204,9 +207,11 @@ __device__ __forceinline__ void answer_row(const LogProbArgs& a, int row, const 
     auto log_prob = [&](float v) { return wrong ? NAN : v == -INFINITY ? -INFINITY : (v - s.top) * a.inverse - log_total; };
     if (a.log_probs)
         for (int i = threadIdx.x; i < a.n_tokens; i += kLogProbThreads) {
-            const int token = a.tokens[static_cast<size_t>(row) * a.n_tokens + i];
-            const bool there = token >= 0 && token < a.vocab;
-            a.log_probs[static_cast<size_t>(row) * a.n_tokens + i] = there ? log_prob(half_bits_to_float(x[token])) : -INFINITY;
+            if (i >= kLogProbThreads) {
+                const int token = a.tokens[static_cast<size_t>(row) * a.n_tokens + i];
+                given = token >= 0 && token < a.vocab ? x[token] : kNotThere;
+            }
+            a.log_probs[static_cast<size_t>(row) * a.n_tokens + i] = given == kNotThere ? -INFINITY : log_prob(half_bits_to_float(static_cast<uint16_t>(given)));
         }
     if (a.entropies && threadIdx.x == 0)
         a.entropies[row] = wrong ? NAN : s.top == -INFINITY ? 0.0f : log_total - s.moment * a.inverse / s.total;
@@ -345,6 +350,9 @@ __global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogPro
         return;
     const int begin = segment * a.length, end = min(begin + a.length, a.vocab);
     const uint16_t* const row_at = a.logits + static_cast<size_t>(row) * a.stride;
+    int token = -1; // of those given: its logit is looked up while the row is
+    if (tid < a.n_tokens)
+        token = a.tokens[static_cast<size_t>(row) * a.n_tokens + tid];
     u32x4 x[PIECES];
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
@@ -355,6 +363,7 @@ __global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogPro
 #pragma unroll
     for (int p = 0; p < PIECES; ++p)
         m2 = max_h2(m2, max_h2(max_h2(as_h2(x[p][0]), as_h2(x[p][1])), max_h2(as_h2(x[p][2]), as_h2(x[p][3]))));
+    const int given = token >= 0 && token < a.vocab ? row_at[token] : kNotThere;
     const float most = fmaxf(static_cast<float>(m2[0]), static_cast<float>(m2[1]));
     float quad = fmaxf(most, dpp_f32<DPP_QUAD_XOR1>(most));
     quad = fmaxf(quad, dpp_f32<DPP_QUAD_XOR2>(quad));
@@ -437,7 +446,7 @@ __global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogPro
             have = likeliest_one_by_one(lds, row_at, begin, end, want, bound > kOrderOfNothing ? 0xFFFFu : kOrderOfNothing);
     }
     if (a.segments == 1) {
-        answer_row(a, row, s, lds.found, have);
+        answer_row(a, row, s, lds.found, have, given);
         return;
     }
     // Several segments: sums and the likeliest of each go through memory that every XCD sees.
@@ -487,7 +496,7 @@ __global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogPro
     all.total = wave_sum(nothing ? own.total * 0.0f : own.total * w);
     all.moment = wave_sum(nothing ? 0.0f : w * __builtin_fmaf(own.total, d, own.moment));
     __syncthreads();
-    answer_row(a, row, all, lds.found, n);
+    answer_row(a, row, all, lds.found, n, given);
 }
 
 } // namespace l2
