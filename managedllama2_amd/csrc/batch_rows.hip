@@ -339,8 +339,8 @@ __device__ __noinline__ int likeliest_one_by_one(LogProbLds& lds, const uint16_t
 // A workgroup per segment of a row, which stays in registers.  One reading, packed maxima, one exponential per logit; with few
 // rows a row is cut into segments, which the last one to arrive puts together.
 //
-// Instructions per logit bound many rows (2000 rows of 32000 with four given and twenty likeliest 37.8 us, 3.4 TB/s; the reading alone would be 25), a chain of
-// loads, sums, search and hand-over few (48 rows 7.8 us, one row of 128000 in 32 segments 8.5; in one workgroup 97).
+// Instructions per logit bound many rows (2000 rows of 32000 with four given and twenty likeliest 37.1 us, 3.5 TB/s; the reading alone would be 25), a chain of
+// loads, sums, search and hand-over few (48 rows 7.7 us, one row of 128000 in 32 segments 7.4; in one workgroup 97).
 template <int PIECES>
 __global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogProbArgs a)
 {
@@ -485,10 +485,30 @@ __global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogPro
     LogProbSums own = {-INFINITY, 0.0f, 0.0f};
     if (lane < a.segments)
         own = {load_agent(sums + lane * 4), load_agent(sums + lane * 4 + 1), load_agent(sums + lane * 4 + 2)};
-    const int n = a.segments * a.n_top;
-    for (int i = tid; i < n; i += kLogProbThreads) {
+    auto key_at = [&](int i) {
         const unsigned lo = load_agent(keys + i * 2), hi = load_agent(keys + i * 2 + 1);
-        lds.found[i] = static_cast<unsigned long long>(hi) << 32 | lo;
+        return static_cast<unsigned long long>(hi) << 32 | lo;
+    };
+    const int n = a.segments * a.n_top;
+    const unsigned long long first = tid < n ? key_at(tid) : 0;
+    if (n <= 64) {
+        if (tid < n)
+            lds.found[tid] = first;
+    } else {
+        // Each segment's keys are in order, so the largest of their last ones bounds the n_top-th of all from below: what does not reach it
+        // need not be ranked (one row of 128000, five of each of 32 segments 8.4 -> 7.4 us; 48 rows of 25 keys would take 0.3 longer).
+        unsigned last = 0;
+        if (lane < a.segments)
+            last = load_agent(keys + ((lane + 1) * a.n_top - 1) * 2 + 1);
+        const unsigned least = static_cast<unsigned>(wave_max(static_cast<float>(last))); // 16 bits
+        if (tid == 0)
+            lds.count = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kLogProbThreads) {
+            const unsigned long long key = i == tid ? first : key_at(i);
+            if (key >> 32 >= least)
+                lds.found[atomicAdd(&lds.count, 1)] = key;
+        }
     }
     LogProbSums all = {wave_max(own.top), 0.0f, 0.0f};
     const float d = own.top - all.top, w = __builtin_amdgcn_exp2f(d * a.per_e);
@@ -496,7 +516,7 @@ __global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogPro
     all.total = wave_sum(nothing ? own.total * 0.0f : own.total * w);
     all.moment = wave_sum(nothing ? 0.0f : w * __builtin_fmaf(own.total, d, own.moment));
     __syncthreads();
-    answer_row(a, row, all, lds.found, n, given);
+    answer_row(a, row, all, lds.found, n <= 64 ? n : lds.count, given);
 }
 
 } // namespace l2
