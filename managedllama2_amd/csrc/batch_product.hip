@@ -115,7 +115,7 @@ __device__ __forceinline__ void put_parts(void* lows, TokenAdapter* info, size_t
 // for the number: ranks and scales of small pools and the inputs are requested together with the number.  4096 inputs, one token, 16 ranks 2.8 us;
 // 5120 inputs, 64 tokens with an adapter each through two tensors 6.6 (taken in items, as below, 6.6 and 11.9).
 // WIDE: as the prompt's products take them, a block of 16 ranks per workgroup.
-constexpr int kRankLoads = 8;
+constexpr int kRankLoads = 4; // at a time, which leaves room for 32 wavefronts on a CU (8: 1 .. 2 % longer steps)
 constexpr int rank_waves(bool wide) { return wide ? 16 : 8; }
 
 template <bool WIDE>
