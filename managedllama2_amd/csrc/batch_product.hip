@@ -843,7 +843,7 @@ static int run_product(const char* fn, Product& p)
         if (wide) {
             if (int rc = launch_batch_gemm(fn, a, p.n_matrices, GATED, p.adapters, p.adapters, base))
                 return rc;
-        } else if (a.n_tokens > 1 || !launch_one_token(a, p.n_matrices, GATED)) {
+        } else if (all > 1 || !launch_one_token(a, p.n_matrices, GATED)) {
             launch_shape<GATED>(p, packed, per_cu, groups);
             L2_LAUNCH_CHECK(fn);
         }

@@ -112,6 +112,27 @@ def test_long_rows(K, cols, tokens):
         pu.Product(rng(23, K, cols, tokens), tokens, K, [cols], True, [16, 5], 16).upload().check()
 
 
+def test_a_tensor_of_more_than_two_gibibytes():
+    """65 and more tokens of it, in launches of up to 4096; w - z is -1 and 1 in turn, so that all outputs of a token are equal."""
+    K, N, tokens = 32768, 131080, 4097
+    w, z, s = pu.DeviceVariable.zeros(np.uint32, N * K // 8), pu.DeviceVariable.zeros(np.uint32, N * 32), pu.DeviceVariable.zeros(np.float16, N * 256)
+    for v, byte in ((w, 0x53), (z, 0x44), (s, 0x1C)):
+        capi.call("llama2_memset", v.ptr, byte, v.nbytes)
+    base = rng(34).standard_normal((61, K)).astype(np.float16)
+    x = pu.up(base[np.arange(tokens) % 61])
+    out, positions = pu.DeviceVariable.zeros(np.float16, tokens * N), pu.up(np.zeros(tokens, np.int32))
+    m = (capi.BatchMatrix * 1)(capi.BatchMatrix(weight=capi.QWeight(w.ptr, z.ptr, s.ptr), output=out.ptr, cols=N, output_stride=N))
+    batch = capi.Batch(positions=positions.ptr, n_requests=1, n_tokens=tokens, max_length=1)
+    capi.call("llama2_batch_mat_mul_int4", m, 1, x.ptr, K, K, None, batch)
+    scale = float(np.full(1, 0x1C1C, np.uint16).view(np.float16)[0])
+    for t in (0, 31, 63, 64, 1000, 4095, 4096):
+        v = base[t % 61].astype(np.float64)
+        want, size = scale * (v[1::2].sum() - v[::2].sum()), scale * np.abs(v).sum()
+        got = pu.DeviceVariable.window(out, t * N * 2, np.float16, N).to_host().astype(np.float64)
+        # as in product_util.product and rounded
+        assert (np.abs(got - want) <= pu.rounded(np.float64(want), (128 + K // 128 + 16) * 2.0 ** -23 * size)).all(), (t, got, want)
+
+
 def test_more_tokens_than_a_launch_takes():
     pu.Product(rng(24), 4133, 264, [40, 24], False, RANKS, 32, residual=True, pad=7).upload().check()
     pu.Product(rng(25), 4133, 264, [24], True, RANKS, 32, pad=7).upload().check()
@@ -156,6 +177,16 @@ def test_only_some_matrices_have_adapters():
         s = pu.Product(rng(10, keep), 37, 256, [64], True, [8, 16], 16)
         s.pools[1 - keep] = None
         s.upload().check()
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 50, 130, 1700])
+def test_pools_of_different_sizes(tokens):
+    """An adapter that one tensor has and another does not, and ranks of different widths."""
+    for gated in (False, True):
+        for ids in (np.arange(tokens) % 7 - 1, 2):
+            p = pu.Product(rng(35, tokens, gated), tokens, 512, [64] if gated else [64, 64, 64], gated, [8, 24, 3, 31, 16], 32, ids=ids)
+            p.pools[1] = pu.Pool(rng(36, tokens, gated), [40, 7], 64, 512, 64)
+            p.upload().check(str(gated))
 
 
 @pytest.mark.parametrize("tokens", [5, 60, 300])
