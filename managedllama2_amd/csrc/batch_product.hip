@@ -693,11 +693,12 @@ constexpr int kMostGroups = 256; // of rows whose inputs are packed; of more one
 // reads the inputs of its tokens, and as many wavefronts in them as the CU has room for.  Measured in us with 256 CUs (W wavefronts, R
 // tiles of outputs; 4096 inputs and no adapters where nothing else is said):
 //   tokens  columns          chosen          others
-//   1       4096             W 8, R 1  5.7   W 12, R 2 6.6;  W 4, R 2  7.5
-//   1       5120 of 13824    W 12, R 2 14.2  W 8, R 1 16.9;  W 4, R 2 18.9
-//   16      12288            W 4, R 2 11.2   W 8, R 1 12.2
-//   16      32000            W 4, R 4 17.2   W 4, R 2 18.6;  W 8, R 1 25.4
-//   1       gated 2 * 11008  W 4, R 2 15.2   W 8, R 2 17.0;  W 4, R 4 16.4
+//   4       4096             W 8, R 1  5.7   W 12, R 2 6.6;  W 4, R 2  7.5
+//   4       5120 of 13824    W 12, R 2 14.2  W 8, R 1 16.9;  W 4, R 2 18.9
+//   16      12288            W 4, R 2 10.4   W 8, R 1 12.2;  W 4, R 2 with two groups requested ahead (D 2) 10.8
+//   16      32000            W 4, R 4 16.8   W 4, R 2 17.5;  W 8, R 1 25.4
+//   8       gated 2 * 11008  W 4, R 2 15.6   D 2 16.0;  W 8, R 2 17.0;  W 4, R 4 16.4
+//   8       gated 2 * 13824 of 5120   W 4, R 4 20.0   W 4, R 2 22.1
 //   32      4096             W 8, R 1  7.3   W 12, R 2 8.3;  W 8, R 4 11.7
 //   32      6144             W 12, R 2 9.1   W 8, R 1 11.1;  W 8, R 4 12.2
 //   32      12288            W 8, R 4 13.5   W 4, R 4 14.8;  W 8, R 1 15.6
@@ -726,7 +727,7 @@ static void launch_shape(Product& p, bool packed, int per_cu, int groups)
     if (n <= 16 && per_cu <= 32)
         launch_product<12, 2, 1, 1, GATED>(p);
     else if (n <= 16)
-        per_cu >= 100 && high ? launch_product<4, 4, 1, 1, GATED>(p) : launch_product<4, 2, 1, 2, GATED>(p);
+        per_cu >= 100 && high ? launch_product<4, 4, 1, 1, GATED>(p) : launch_product<4, 2, 1, 1, GATED>(p);
     else if (per_cu <= 24 || !high)
         launch_product<12, 2, 2, 1, GATED>(p);
     else
