@@ -112,8 +112,8 @@ __device__ __forceinline__ void put_parts(void* lows, TokenAdapter* info, size_t
 
 // Few tokens: a wavefront takes a rank of a token's adapter, whose row of the adapter it sums up with the token's inputs in fp32; tokens that
 // share an adapter find it in the caches.  A chain of loads bounds it, so nothing waits but the adapter's number for the arguments and its row
-// for the number: ranks and scales of small pools and the inputs are requested together with the number.  4096 inputs, one token, 16 ranks 2.8 us;
-// 5120 inputs, 64 tokens with an adapter each through two tensors 6.6 (taken in items, as below, 6.6 and 11.9).
+// for the number: ranks and scales of small pools and the inputs are requested together with the number.  4096 inputs, one token, 16 ranks 2.7 us;
+// 5120 inputs, 64 tokens with an adapter each through two tensors 6.0 (taken in items, as below, 6.6 and 11.9).
 // WIDE: as the prompt's products take them, a block of 16 ranks per workgroup.
 constexpr int kRankLoads = 4; // at a time, which leaves room for 32 wavefronts on a CU (8: 1 .. 2 % longer steps)
 constexpr int rank_waves(bool wide) { return wide ? 16 : 8; }
