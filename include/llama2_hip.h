@@ -450,7 +450,8 @@ typedef struct llama2_batch_matrix {
  *   output[t][n] = half(residual[t][n] + sum_k input[t][k] * (w - z) * s + adapter's part),
  * sums in fp32, one rounding at the end; what an adapter's ranks receive of the input is fp32 too, and above 64 tokens may keep
  * no more than 22 bits of the largest of 16 of them.
- * rows % 8 == 0, up to 65536; cols up to 2^20, input_stride up to 2^24; scales are finite; tensors are laid out as above (ceil(rows/32)*4 words, ceil(rows/128) scales per output).
+ * rows % 8 == 0, up to 65536; cols up to 2^20, input_stride up to 2^24; scales are finite; tensors are laid out as above
+ * (ceil(rows/32)*4 words, ceil(rows/128) scales per output).
  * Token t uses adapter token_adapters[t] of every matrix that has adapters; a value that is not one of 0 .. n_adapters - 1:
  * none.  What one token or one adapter holds has no influence on the rows of other tokens.  token_adapters may be null where no
  * matrix has adapters.  Rows of tokens without a position are left as they were.  Reads n_tokens and positions of
@@ -488,11 +489,11 @@ int llama2_batch_residual_rmsnorm(llama2_half* output, llama2_half* residual_out
  *   entropies[r]     -sum p log p
  *   top_tokens[r][j], top_log_probs[r][j]  for j < n_top: the most likely tokens in order, equal ones by their index; behind the
  *                    last of a vocabulary smaller than n_top: -1 and -infinity
- * Any of the four may be null (n_tokens / n_top 0 where theirs are; top_log_probs needs top_tokens).  A logit of -infinity has probability 0; of a row that holds
- * nothing else all log probabilities are -infinity and the entropy is 0.  A row with NaN or +infinity has NaN for its log probabilities
+ * Any of the four may be null (n_tokens / n_top 0 where theirs are; top_log_probs needs top_tokens).  A logit of -infinity has
+ * probability 0; of a row that holds nothing else all log probabilities are -infinity and the entropy is 0.  A row with NaN or +infinity has NaN for its log probabilities
  * and its entropy; its top tokens are in the order of the logits, NaN last.  Rows whose position is negative are left as they
- * were (positions null: none is).  n_tokens <= 1024, n_top <= LLAMA2_MAX_TOP_TOKENS, vocab_size <= 2^20, 0 < temperature; logits
- * need no alignment beyond their 2 bytes.  Scratch: as llama2_multi_head_attention (call once before capturing).  Asynchronous,
+ * were (positions null: none is).  n_tokens <= 1024, n_top <= LLAMA2_MAX_TOP_TOKENS, vocab_size <= 2^20, 1e-30 < temperature <= 1e30;
+ * logits need no alignment beyond their 2 bytes.  Scratch: as llama2_multi_head_attention (call once before capturing).  Asynchronous,
  * may be captured. */
 #define LLAMA2_MAX_TOP_TOKENS 64
 int llama2_batch_log_probs(float* log_probs, float* entropies, int* top_tokens, float* top_log_probs,

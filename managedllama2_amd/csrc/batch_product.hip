@@ -71,8 +71,8 @@ __device__ __forceinline__ h8_t tile_operand(const char* lds, int m)
 
 // ---------------------------------------------------------------- rows as operands
 // 16 tokens and a group of 128 inputs are the four operands of 16 x 16 x 32 products, 1 KB each: lane group c of operand m holds elements
-// 32 c + 8 m on of token lane % 16, in the order of a word's nibbles, zeros behind the end of a row.  Tokens behind the last one repeat it.  `worker` of `workers` pairs of
-// such tiles at a time, 512 threads.
+// 32 c + 8 m on of token lane % 16, in the order of a word's nibbles, zeros behind the end of a row.  Tokens behind the last one repeat it.
+// `worker` of `workers` takes pairs of such tiles with 512 threads.
 __device__ __forceinline__ void pack_rows(uint16_t* packed, const uint16_t* x, int K, int x_stride, int n_tokens, int worker, int workers)
 {
     const int groups = (K + 127) / 128, units = (n_tokens + 15) / 16 * groups, lane = threadIdx.x & 63, part = threadIdx.x >> 6;

@@ -16,7 +16,6 @@ struct TokenAdapter {
     float factor;
     int rank;
 };
-constexpr int kRankBlocks = kMaxRank / 16;
 
 // An int4 tensor of a product.  Arguments lie in memory, and a kernel that asks for them one after the other waits for each: a tensor's
 // are neighbours.

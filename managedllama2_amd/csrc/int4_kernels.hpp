@@ -1,5 +1,5 @@
 // AWQ-v1 int4 (group 128) mat-vec kernels for gfx950, shared by the module entry
-// points (int4_matvec.hip) and the fused decode step (decode.hip).
+// points (int4_matvec.hip), the fused decode step (decode.hip) and steps of one token (batch_one.hip).
 // Replaces native/mat_vec_kernel.cu:83-234 of the reference.
 //
 // Shape of the computation (batch-1 GEMV, HBM-bound, no MFMA):
