@@ -844,8 +844,9 @@ static int run_product(const char* fn, Product& p)
         if (wide) {
             if (int rc = launch_batch_gemm(fn, a, p.n_matrices, GATED, p.adapters, p.adapters, base))
                 return rc;
-        } else if (all > 1 || !launch_one_token(a, p.n_matrices, GATED)) {
-            launch_shape<GATED>(p, packed, per_cu, groups);
+        } else {
+            if (all > 1 || !launch_one_token(a, p.n_matrices, GATED))
+                launch_shape<GATED>(p, packed, per_cu, groups);
             L2_LAUNCH_CHECK(fn);
         }
         a.x = rows + static_cast<size_t>(a.n_tokens) * a.x_stride;
