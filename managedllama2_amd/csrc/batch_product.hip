@@ -210,7 +210,7 @@ template <int CHUNKS, bool KEEP>
 __global__ __launch_bounds__(kLowWaves * 64) void batch_low_kernel(LowArgs)
 {
     constexpr int kStride = 16 + 4;
-    __shared__ __align__(16) Items items;
+    __shared__ Items items;
     __shared__ int table[kLowTable];
     __shared__ float scale_table[kLowTable];
     __shared__ __align__(16) char tiles[kLowWaves * kTileBytes];

@@ -88,13 +88,14 @@ __device__ __forceinline__ int adapter_of(const int* positions, const int* token
 }
 
 // Tokens of a block of up to 64 that use the same adapter, by up to 16 of them: an item.  Items are numbered in the order of their
-// first tokens.
-struct Items {
+// first tokens.  Tokens are stored, and what stands behind several blocks' items is read, 16 bytes at a time.
+struct alignas(16) Items {
     int ids[64];            // adapter of a token, kNoAdapter, kNoToken
     int adapter[64];        // of an item
     uint8_t tokens[64][16]; // of an item, kNobody behind the last
     int count;
 };
+static_assert(sizeof(Items) % 16 == 0 && offsetof(Items, tokens) % 16 == 0, "16 bytes at a time");
 constexpr uint8_t kNobody = 255;
 
 // By one wavefront, from the first `tokens` of items.ids, which are below `most`; everyone may read the items after the next barrier.

@@ -221,6 +221,7 @@ struct GemmLds {
     static constexpr int kTurnAt = kRed + MT * static_cast<int>(sizeof(Items)), kItems = kTurnAt + 8 * 1024; // EPI_ROWS, EPI_GATED
     static constexpr int kRowsBytes = kAll > kItems ? kAll : kItems;
     static_assert(kRowsBytes <= 160 * 1024, "LDS of a compute unit");
+    static_assert(kRed % 16 == 0 && kTurnAt % 16 == 0, "items and turn buffers are read 16 bytes at a time");
     static_assert(kBytes <= 160 * 1024, "LDS of a compute unit");
 };
 
