@@ -740,7 +740,7 @@ static int run_product(const char* fn, Product& p)
     ProductArgs& a = p.a;
     LowArgs& l = p.low;
     const int all = a.n_tokens, groups = weight_groups(a.K);
-    int columns = 0, max_rank = 0;
+    int columns = 0, max_rank = 0, max_ranks[LLAMA2_MAX_BATCH_MATRICES] = {};
     bool fits = true, adapters = false; // the prompt's products hold a tensor's offsets in 31 bits
     for (int i = 0; i < p.n_matrices; ++i) {
         columns += a.t[i].cols; // at most 2^22
@@ -748,6 +748,7 @@ static int run_product(const char* fn, Product& p)
         if (!l.t[i].down)
             continue;
         adapters = true;
+        max_ranks[i] = l.t[i].max_rank;
         max_rank = l.t[i].max_rank > max_rank ? l.t[i].max_rank : max_rank;
         a.most_adapters = l.t[i].n_adapters > a.most_adapters ? l.t[i].n_adapters : a.most_adapters;
     }
@@ -776,23 +777,17 @@ static int run_product(const char* fn, Product& p)
     const bool each = looked_up <= (keeps ? 2e8 : 5e8);
     const size_t fragments = wide ? batch_gemm_bytes(most, a.K) : packed ? static_cast<size_t>(ceil_div(most, 16)) * groups * 4096 : 0;
     p.adapters = adapters;
-    size_t bytes = fragments;
-    for (int i = 0; i < p.n_matrices; ++i)
-        if (l.t[i].down)
-            bytes += static_cast<size_t>(most) * ceil_div(l.t[i].max_rank, 16) * (64 + sizeof(TokenAdapter));
-    if (bytes)
-        if (int rc = ensure_attn_partials(bytes))
+    const LowScratch scratch = low_scratch(fragments, most, max_ranks, p.n_matrices);
+    if (scratch.bytes)
+        if (int rc = ensure_attn_partials(scratch.bytes))
             return rc;
     char* const base = reinterpret_cast<char*>(ctx().attn_partials);
-    char* at = base + fragments;
     for (int i = 0; i < p.n_matrices; ++i) {
         LowTensor& t = l.t[i];
         if (!t.down)
             continue;
-        t.low = at;
-        at += static_cast<size_t>(most) * ceil_div(t.max_rank, 16) * 64;
-        t.info = reinterpret_cast<TokenAdapter*>(at);
-        at += static_cast<size_t>(most) * ceil_div(t.max_rank, 16) * sizeof(TokenAdapter);
+        t.low = base + scratch.low[i];
+        t.info = reinterpret_cast<TokenAdapter*>(base + scratch.info[i]);
         a.t[i].low = t.low;
         a.t[i].info = t.info;
         a.t[i].n_adapters = t.n_adapters;

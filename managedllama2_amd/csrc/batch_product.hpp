@@ -10,13 +10,6 @@ namespace l2 {
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-// What a tensor's adapters leave for its product, per token and 16 ranks (a block): the scale of the adapter with the block's power of
-// two, and the adapter's rank.
-struct TokenAdapter {
-    float factor;
-    int rank;
-};
-
 // An int4 tensor of a product.  Arguments lie in memory, and a kernel that asks for them one after the other waits for each: a tensor's
 // are neighbours.
 struct alignas(64) ProductTensor {

@@ -254,6 +254,38 @@ inline int check_batch_log_probs(const float* log_probs, const float* entropies,
     return LLAMA2_OK;
 }
 
+// ---------------------------------------------------------------- scratch of the products
+// What a tensor's adapters leave for its product, per token and 16 ranks (a block): the scale of the adapter with the block's power of
+// two, and the adapter's rank.
+struct TokenAdapter {
+    float factor;
+    int rank;
+};
+
+constexpr size_t kLowBytes = 64; // what 16 ranks of a token receive: looked up as one piece, on its multiples
+
+// Where that lies behind the operands: what the ranks of all tensors receive first, which stays on multiples of kLowBytes whatever the
+// number of tokens, then the factors.
+struct LowScratch {
+    size_t low[LLAMA2_MAX_BATCH_MATRICES], info[LLAMA2_MAX_BATCH_MATRICES], bytes;
+};
+
+// operands: bytes, a multiple of kLowBytes; max_ranks: of a tensor's adapters, 0 without.
+inline LowScratch low_scratch(size_t operands, int tokens, const int* max_ranks, int n_matrices)
+{
+    LowScratch s = {};
+    s.bytes = operands;
+    for (int i = 0; i < n_matrices; ++i) {
+        s.low[i] = s.bytes;
+        s.bytes += static_cast<size_t>(tokens) * ceil_div(max_ranks[i], 16) * kLowBytes;
+    }
+    for (int i = 0; i < n_matrices; ++i) {
+        s.info[i] = s.bytes;
+        s.bytes += static_cast<size_t>(tokens) * ceil_div(max_ranks[i], 16) * sizeof(TokenAdapter);
+    }
+    return s;
+}
+
 // ---------------------------------------------------------------- how rows of logits are cut
 constexpr int kLogProbRows = 1 << 15; // of a launch
 
