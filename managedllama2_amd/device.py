@@ -164,9 +164,12 @@ class Adapters:
     @classmethod
     def from_host(cls, down, up, ranks, scales):
         """down: [numAdapters][maxRank][rows], up: [numAdapters][cols][maxRank]."""
+        down, up, ranks, scales = np.asarray(down, np.float16), np.asarray(up, np.float16), np.asarray(ranks, np.int32), np.asarray(scales, np.float32)
+        if down.ndim != 3 or up.ndim != 3 or up.shape[::2] != down.shape[:2] or ranks.shape != down.shape[:1] or scales.shape != ranks.shape:
+            raise ValueError("adapters: down %s, up %s, ranks %s and scales %s must be [n][maxRank][rows], [n][cols][maxRank], [n] and [n]"
+                             % (down.shape, up.shape, ranks.shape, scales.shape))
         f = DeviceVariable.from_host
-        return cls(f(np.asarray(down, np.float16)), f(np.asarray(up, np.float16)), f(np.asarray(ranks, np.int32)),
-                   f(np.asarray(scales, np.float32)), down.shape[1])
+        return cls(f(down), f(up), f(ranks), f(scales), down.shape[1])
 
     def pointer(self):
         return C.pointer(capi.Adapters(self.down.ptr, self.up.ptr, self.scales.ptr, self.ranks.ptr, 0, 0, self.ranks.size, self.maxRank))
