@@ -449,7 +449,10 @@ typedef struct llama2_batch_matrix {
  * v; or one):
  *   output[t][n] = half(residual[t][n] + sum_k input[t][k] * (w - z) * s + adapter's part),
  * sums in fp32, one rounding at the end; what an adapter's ranks receive of the input is fp32 too, and above 64 tokens may keep
- * no more than 22 bits of the largest of 16 of them.
+ * no more than 22 bits of the largest of 16 of them.  A step of one token may go through the decode step's kernels, which sum up input * w and
+ * z * input apart for every 32 inputs: the error of its sums is then one of |input| (w + z) s, where that of more tokens is one of
+ * |input| |w - z| s (it shows where all inputs have an offset in common that is large beside their differences).  Where an input, or a number of
+ * the token's adapter, is infinite or NaN, the results that it contributes to are infinite or NaN; which of the two may differ with the number of tokens.
  * rows % 8 == 0, up to 65536; cols up to 2^20, input_stride up to 2^24; scales are finite; tensors are laid out as above
  * (ceil(rows/32)*4 words, ceil(rows/128) scales per output).
  * Token t uses adapter token_adapters[t] of every matrix that has adapters; a value that is not one of 0 .. n_adapters - 1:
@@ -473,7 +476,8 @@ int llama2_batch_mat_mul_swiglu(llama2_half* output, const llama2_half* input, c
  *   y = input, or norm(input) * input_gamma if input_gamma; y *= gate if gate
  *   r = residual + residual_scale * y   (r = residual if input is null)
  *   residual_output = half(r);  output = half(norm(r) * gamma)
- * with norm(v) = v / sqrt(mean(v^2) + eps), everything in fp32, r not rounded in front of its norm.  gammas and gate:
+ * with norm(v) = v / sqrt(mean(v^2) + eps), everything in fp32 (the squares too: from about 10^17 on a row's norm is 0), r not rounded in front of
+ * its norm.  gammas and gate:
  * `size` halfs.  output (with gamma) or residual_output may be null; residual_output may be residual with the same stride,
  * output may be input with the same stride; otherwise outputs must not overlap anything.
  * size: a multiple of 8 up to 65536; strides are multiples of 8, pointers 16-byte aligned.  Rows of tokens without a position

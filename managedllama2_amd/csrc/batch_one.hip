@@ -4,7 +4,10 @@
 // HBM and latency bound them.  Against the tiles of batch_product.hip, of whose 16 rows one token uses one: 4096 columns of 4096 inputs 5.7 -> 3.6 us,
 // with an adapter of 16 ranks 9.0 -> 6.9; three of them 10.7 -> 7.3, with 64 ranks 15.5 -> 10.9; gated 2 * 11008 14.7 -> 9.9, with 16 ranks 18.9 -> 13.2;
 // 5120 columns of 13824 inputs 13.8 -> 11.0; 32000 columns the same.  Tensors of different widths stay with the tiles, which take them in one
-// launch (4096 + 1024 + 1024 columns 7.0 us).
+// launch (4096 + 1024 + 1024 columns 7.0 us).  Three tensors of 8193 .. 10240 inputs are short of 4 registers (20 bytes of scratch per lane).
+//
+// The kernel sums up x w and z x apart for every 32 inputs, in fp32: exact integers of up to 15 where the tiles have differences, so that
+// its error grows with |x| (w + z) s.
 #include "batch_product.hpp"
 #include "int4_kernels.hpp"
 

@@ -758,7 +758,10 @@ static int run_product(const char* fn, Product& p)
     // 23.2 -> 18.6 us, 64 29.5 -> 24.2; with an adapter each 49 against 122; 2 * 8192 columns, 64 tokens 18.4 against 20.7).
     // For the same reason up to 192 tokens with many adapters of few ranks do not (in us, prompt's kernels against these tiles: 128 tokens through
     // q, k and v of 4096 with 128 adapters of 16 ranks 53.8, 40.2, 4 of 16 36.1, 35.4, 32 of 32 55.6, 47.8, 4 of 64 46.0, 71.5; 192 with 64 of 16
-    // 80.0, 56.7; gated 2 * 11008, 100 with 16 of 32 82.3, 62.6; 256 through one of 4096 with 64 of 16 33.9, 39.9), nor up to 128 for a few columns
+    // 80.0, 56.7; gated 2 * 11008, 100 with 16 of 32 82.3, 62.6; 256 through one of 4096 with 64 of 16 33.9, 39.9).  The pool's size stands for the
+    // adapters in use, which only the device knows: one prompt with one adapter out of a large pool is 0 .. 6 % slower that way at 16 ranks up to 128
+    // tokens (of 64: 100 tokens through q, k and v 32.4, 33.3, gated 46.0, 49.0) and up to 46 % at the rule's end (192 gated with one of 16 of 32 ranks
+    // 68.0, 99.1), where all 64 in use would cost twice the time the other way (100 tokens 62.9, 36.0; gated 107, 52.5).  Nor do up to 128 for a few columns
     // (2048 of 2048 inputs 10.5, 6.0; 128 tokens through 4096 of 4096 15.4, 16.1).
     const int tile_tokens = adapters ? (max_rank <= 32 && 2 * a.most_adapters >= max_rank ? 192 : 64) : per_cu <= 8 ? 128 : 64;
     const bool wide = fits && (all > tile_tokens || (all > 16 && !adapters && per_cu >= 80));

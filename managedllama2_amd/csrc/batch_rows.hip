@@ -339,8 +339,10 @@ __device__ __noinline__ int likeliest_one_by_one(LogProbLds& lds, const uint16_t
 // A workgroup per segment of a row, which stays in registers.  One reading, packed maxima, one exponential per logit; with few
 // rows a row is cut into segments, which the last one to arrive puts together.
 //
-// Instructions per logit bound many rows (2000 rows of 32000 with four given and twenty likeliest 37.1 us, 3.5 TB/s; the reading alone would be 25), a chain of
-// loads, sums, search and hand-over few (48 rows 7.7 us, one row of 128000 in 32 segments 7.4; in one workgroup 97).
+// Instructions per logit bound many rows: 2000 rows of 32000 with four given and twenty likeliest 36.8 us, 3.5 TB/s (the reading alone would be 25).  14.9
+// vector instructions per logit keep the vector units busy for 72 % of the time in which their CU has work; 73 registers leave room for three
+// workgroups on a CU, 20 wavefronts on average, to fill the rest.  A chain of loads, sums, search and hand-over bounds few (48 rows 7.7 us, one
+// row of 128000 in 32 segments 7.5; in one workgroup 97).
 template <int PIECES>
 __global__ __launch_bounds__(kLogProbThreads) void batch_log_probs_kernel(LogProbArgs a)
 {
